@@ -209,4 +209,32 @@ extern "C" {
     pub(crate) fn pxg_mixture_generate_device(count: u64, dim: u32, clusters: u64, centre_scale: f32, sigma: f32,
         queries: u64, drawn_clusters: c_int, seed: u64, d_vectors: *mut f32, d_queries: *mut f32) -> c_int;
     pub(crate) fn pxg_uniform_generate_device(count: u64, dim: u32, lo: f32, hi: f32, seed: u64, d_out: *mut f32) -> c_int;
+    pub(crate) fn pxg_block8_code_stride(cols: u64) -> u64;
+    pub(crate) fn pxg_block8_scale_stride(cols: u64) -> u64;
+    pub(crate) fn pxg_block8_pack_device(kind: c_int, d_x: *const c_void, rows: u64, cols: u64, x_stride: u64,
+        d_codes: *mut c_void, d_scales: *mut c_void, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_block8_unpack_device(kind: c_int, d_codes: *const c_void, d_scales: *const c_void, rows: u64,
+        cols: u64, d_out: *mut c_void, out_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_block8_matmul_device(d_codes: *const c_void, d_scales: *const c_void, rows: u64, k: u64,
+        d_w_codes: *const c_void, d_w_scales: *const c_void, groups: u64, n: u64, d_offsets: *const i64,
+        out_type: c_int, d_y: *mut c_void, y_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_matmul_device(kind: c_int, d_x: *const c_void, rows: u64, k: u64, x_stride: u64,
+        d_w: *const c_void, groups: u64, n: u64, w_stride: u64, w_group_stride: u64, d_offsets: *const i64,
+        out_type: c_int, d_y: *mut c_void, y_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_matmul_grad_input_device(kind: c_int, d_grad: *const c_void, rows: u64, n: u64,
+        grad_stride: u64, d_w: *const c_void, groups: u64, k: u64, w_stride: u64, w_group_stride: u64,
+        d_offsets: *const i64, out_type: c_int, d_dx: *mut c_void, dx_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_matmul_grad_weight_device(kind: c_int, d_grad: *const c_void, rows: u64, n: u64,
+        grad_stride: u64, d_x: *const c_void, k: u64, x_stride: u64, d_offsets: *const i64, groups: u64,
+        out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_matmul_grad_weight_block8_device(d_grad: *const c_void, rows: u64, n: u64,
+        grad_stride: u64, d_codes: *const c_void, d_scales: *const c_void, k: u64, d_offsets: *const i64,
+        groups: u64, out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64,
+        stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_activation_pack_device(activation: c_int, kind: c_int, d_h: *const c_void, rows: u64,
+        cols: u64, h_stride: u64, d_a: *mut c_void, a_stride: u64, d_codes: *mut c_void, d_scales: *mut c_void,
+        stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_activation_grad_device(activation: c_int, kind: c_int, d_grad: *const c_void, rows: u64,
+        cols: u64, grad_stride: u64, d_codes: *const c_void, d_scales: *const c_void, d_out: *mut c_void,
+        out_stride: u64, stream: *mut c_void) -> c_int;
 }

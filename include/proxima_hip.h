@@ -417,6 +417,80 @@ int pxg_mixture_generate_device(uint64_t count, uint32_t dim, uint64_t clusters,
  * reference counterpart; the uniform configuration's inputs). */
 int pxg_uniform_generate_device(uint64_t count, uint32_t dim, float lo, float hi, uint64_t seed, float* d_out);
 
+/* ------------------------------------------------------------------------ */
+/* Products of expert layers, and rows packed in 8 bits. No reference         */
+/* counterpart: the layers whose outputs an index stores or is queried with.  */
+/*                                                                            */
+/* Conventions of this section: device pointers; matrices are row-major with  */
+/* strides in elements, rows any stride apart that is at least the columns;   */
+/* `type` is a pxg_type. Work is ordered on `stream` (a hipStream_t; NULL =   */
+/* the null stream) and the calls return without waiting for it; they         */
+/* allocate nothing and can be captured in a graph. Outputs may not overlap   */
+/* inputs. Sums are held in f32 and rounded once, to the output's type.       */
+/* Results are the same bit for bit from call to call.                        */
+/*                                                                            */
+/* Groups: `offsets` are groups + 1 values in device memory, and group g is   */
+/* the rows from offsets[g] to offsets[g + 1] (none when they are equal).     */
+/* Values are clamped, each to [0, rows] and to no less than those before     */
+/* it. Rows before the first group and after the last get zeros.              */
+typedef enum pxg_type { PXG_F32 = 0, PXG_F16 = 1, PXG_BF16 = 2 } pxg_type;
+/* silu(h) = h / (1 + exp(-h)); gelu(h) = h (1 + erf(h / sqrt(2))) / 2. */
+typedef enum pxg_activation { PXG_SILU = 0, PXG_GELU = 1 } pxg_activation;
+
+/* Packed rows: for each block of 128 columns of a row, e the smallest integer
+ * in [-126, 127] with max |x| <= 448 * 2^e over the block's finite x; codes
+ * are x * 2^-e rounded to e4m3 (nearest, ties to even; a non-finite x gives
+ * NaN) and the scale byte is e + 127. A code's value times 2^e is exact in
+ * f32 and bf16. Codes are rows of code_stride(cols) bytes (cols rounded up to
+ * 128, zero past cols), 16-byte aligned; scales are rows of
+ * scale_stride(cols) bytes (blocks rounded up to 4, 127 past the blocks),
+ * 4-byte aligned. */
+uint64_t pxg_block8_code_stride(uint64_t cols);
+uint64_t pxg_block8_scale_stride(uint64_t cols);
+/* rows x cols values (f32, f16 or bf16) to packed rows, and back. */
+int pxg_block8_pack_device(int type, const void* d_x, uint64_t rows, uint64_t cols, uint64_t x_stride, void* d_codes,
+                           void* d_scales, void* stream);
+int pxg_block8_unpack_device(int type, const void* d_codes, const void* d_scales, uint64_t rows, uint64_t cols,
+                             void* d_out, uint64_t out_stride, void* stream);
+/* y = x w_g^T for the rows of each group: x rows x k and w (groups * n) x k,
+ * both packed, y rows x n of out_type (f32, f16 or bf16). offsets NULL: one
+ * group of all rows. */
+int pxg_block8_matmul_device(const void* d_codes, const void* d_scales, uint64_t rows, uint64_t k,
+                             const void* d_w_codes, const void* d_w_scales, uint64_t groups, uint64_t n,
+                             const int64_t* d_offsets, int out_type, void* d_y, uint64_t y_stride, void* stream);
+
+/* y = x w_g^T: x rows x k, w_g n x k (w_group_stride elements apart), y rows
+ * x n. type f16 or bf16; out_type the same or f32. offsets NULL: one group of
+ * all rows. */
+int pxg_grouped_matmul_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride, const void* d_w,
+                              uint64_t groups, uint64_t n, uint64_t w_stride, uint64_t w_group_stride,
+                              const int64_t* d_offsets, int out_type, void* d_y, uint64_t y_stride, void* stream);
+/* Its gradients, grad being y's: dx = grad w_g, and dw_g = the sum over the
+ * group's rows t of grad[t]^T x[t] (zeros for an empty group). */
+int pxg_grouped_matmul_grad_input_device(int type, const void* d_grad, uint64_t rows, uint64_t n, uint64_t grad_stride,
+                                         const void* d_w, uint64_t groups, uint64_t k, uint64_t w_stride,
+                                         uint64_t w_group_stride, const int64_t* d_offsets, int out_type, void* d_dx,
+                                         uint64_t dx_stride, void* stream);
+int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t rows, uint64_t n,
+                                          uint64_t grad_stride, const void* d_x, uint64_t k, uint64_t x_stride,
+                                          const int64_t* d_offsets, uint64_t groups, int out_type, void* d_dw,
+                                          uint64_t dw_stride, uint64_t dw_group_stride, void* stream);
+/* The weight gradient from a packed x: grad is bf16 (in which packed values
+ * are exact), out_type bf16 or f32. */
+int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t rows, uint64_t n, uint64_t grad_stride,
+                                                 const void* d_codes, const void* d_scales, uint64_t k,
+                                                 const int64_t* d_offsets, uint64_t groups, int out_type, void* d_dw,
+                                                 uint64_t dw_stride, uint64_t dw_group_stride, void* stream);
+
+/* a = f(h), computed from h itself, and h packed, to be kept for the backward
+ * pass; and that pass: dh = grad * f'(unpacked h). f32, f16 or bf16. */
+int pxg_activation_pack_device(int activation, int type, const void* d_h, uint64_t rows, uint64_t cols,
+                               uint64_t h_stride, void* d_a, uint64_t a_stride, void* d_codes, void* d_scales,
+                               void* stream);
+int pxg_activation_grad_device(int activation, int type, const void* d_grad, uint64_t rows, uint64_t cols,
+                               uint64_t grad_stride, const void* d_codes, const void* d_scales, void* d_out,
+                               uint64_t out_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

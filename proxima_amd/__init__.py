@@ -1200,3 +1200,12 @@ def uniform_generate_device(count, dim, lo, hi, seed, out):
 
 
 __all__ += ["fixture_generate", "fixture_generate_device", "mixture_generate_device", "uniform_generate_device"]
+
+
+# ---------------------------------------------------------------------------
+# packed rows and the products of expert layers
+# ---------------------------------------------------------------------------
+from .experts import *  # noqa: E402,F401,F403
+from .experts import __all__ as _experts_all  # noqa: E402
+
+__all__ += _experts_all

@@ -160,6 +160,22 @@ SIGNATURES = {
     "pxg_sq8_search_device": (_i32, [_vp, _vp, _u64, _u64, _u64, _vp, _vp, _vp, _vp, _vp]),
     "pxg_sq8_last_fallbacks": (_u64, []),
     "pxg_sq8_set_search_mode": (_i32, [_vp, _i32]),
+    # packed rows and the products of expert layers
+    "pxg_block8_code_stride": (_u64, [_u64]),
+    "pxg_block8_scale_stride": (_u64, [_u64]),
+    "pxg_block8_pack_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _vp, _vp]),
+    "pxg_block8_unpack_device": (_i32, [_i32, _vp, _vp, _u64, _u64, _vp, _u64, _vp]),
+    "pxg_block8_matmul_device": (_i32, [_vp, _vp, _u64, _u64, _vp, _vp, _u64, _u64, _vp, _i32, _vp, _u64, _vp]),
+    "pxg_grouped_matmul_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp, _i32, _vp,
+                                         _u64, _vp]),
+    "pxg_grouped_matmul_grad_input_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp,
+                                                    _i32, _vp, _u64, _vp]),
+    "pxg_grouped_matmul_grad_weight_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _i32,
+                                                     _vp, _u64, _u64, _vp]),
+    "pxg_grouped_matmul_grad_weight_block8_device": (_i32, [_vp, _u64, _u64, _u64, _vp, _vp, _u64, _vp, _u64, _i32,
+                                                            _vp, _u64, _u64, _vp]),
+    "pxg_activation_pack_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp]),
+    "pxg_activation_grad_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _vp, _vp, _u64, _vp]),
 }
 
 

@@ -1,0 +1,107 @@
+// Ragged groups of rows, from offsets that stay on the device.
+//
+// Group g is the rows from offsets[g] to offsets[g + 1]. The offsets are
+// clamped: each to [0, rows], then to no less than those before it, so that
+// any values give disjoint ranges inside the matrix. Rows before the first
+// group and after the last belong to none.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "device.hpp"
+
+namespace pxg {
+
+__device__ __forceinline__ int clamp_offset(int64_t o, int rows) {
+  return o < 0 ? 0 : o > rows ? rows : (int)o;
+}
+
+__device__ __forceinline__ int wave_max_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < WAVE; o <<= 1) {
+    const int u = __shfl_up(v, o, WAVE);
+    v = lane >= o && u > v ? u : v;
+  }
+  return v;
+}
+__device__ __forceinline__ int wave_sum_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < WAVE; o <<= 1) {
+    const int u = __shfl_up(v, o, WAVE);
+    v += lane >= o ? u : 0;
+  }
+  return v;
+}
+
+// The rows of group g, by a wavefront whose lanes all call it.
+__device__ __forceinline__ void group_range(const int64_t* __restrict__ offsets, int g, int rows, int& lo, int& hi) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  int m = 0;
+  for (int i = lane; i <= g; i += WAVE) {
+    const int o = clamp_offset(offsets[i], rows);
+    m = o > m ? o : m;
+  }
+#pragma unroll
+  for (int o = WAVE / 2; o > 0; o >>= 1) {
+    const int u = __shfl_xor(m, o, WAVE);
+    m = u > m ? u : m;
+  }
+  lo = __builtin_amdgcn_readfirstlane(m);
+  const int h = __builtin_amdgcn_readfirstlane(clamp_offset(offsets[g + 1], rows));
+  hi = h > lo ? h : lo;
+}
+
+// One tile of at most `size` rows: its group (-1: rows of no group, whose
+// results are zero), its first row and the end of its segment.
+struct RowTile {
+  int group, row, end;
+};
+
+// Tile `index` of the tiles of `size` rows that the groups, and the rows of
+// none at either end, are cut into; false past the last. `offsets` NULL is
+// one group of all rows. A wavefront's lanes all call it and get the same.
+__device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offsets, int groups, int rows, int size,
+                                              int index, RowTile& t) {
+  if (!offsets) {
+    t = {0, index * size, rows};
+    return (int64_t)index * size < rows;
+  }
+  const int lane = threadIdx.x & (WAVE - 1);
+  int begin = 0, before = 0;  // rows and tiles before the segments of this round
+  // segment s ends at offsets[s]; segment 0 and segment groups + 1 are the rows of no group
+  for (int s0 = 0; s0 < groups + 2; s0 += WAVE) {
+    const int s = s0 + lane;
+    int end = s <= groups ? clamp_offset(offsets[s], rows) : rows;
+    end = wave_max_scan(end > begin ? end : begin, lane);
+    int first = __shfl_up(end, 1, WAVE);
+    if (lane == 0) first = begin;
+    const int tiles = (end - first + size - 1) / size;
+    const int last = before + wave_sum_scan(tiles, lane);
+    const uint64_t hit = __ballot(index < last);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      const int f = __builtin_amdgcn_readlane(first, l), n = __builtin_amdgcn_readlane(tiles, l);
+      const int k = index - (__builtin_amdgcn_readlane(last, l) - n);
+      t.group = s0 + l == 0 || s0 + l > groups ? -1 : s0 + l - 1;
+      t.row = f + k * size;
+      t.end = __builtin_amdgcn_readlane(end, l);
+      return true;
+    }
+    begin = __builtin_amdgcn_readlane(end, WAVE - 1);
+    before = __builtin_amdgcn_readlane(last, WAVE - 1);
+  }
+  return false;
+}
+
+// No more tiles than this come out of `rows` rows in `groups` groups, the
+// rows of no group at either end counted as two more.
+inline uint64_t row_tiles_max(uint64_t rows, uint64_t groups, uint64_t size, bool ragged) {
+  const uint64_t full = (rows + size - 1) / size;
+  if (!ragged) return full;
+  const uint64_t parts = groups + 2 < rows ? groups + 2 : rows;
+  return rows / size + parts < full ? full : rows / size + parts;
+}
+
+}  // namespace pxg

@@ -19,6 +19,7 @@
 namespace pxg {
 namespace {
 
+typedef int i8v __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
 typedef _Float16 hf8v __attribute__((ext_vector_type(8)));
@@ -40,6 +41,7 @@ struct Product {
   uint64_t ss;
   int rows, groups;     // rows of x and dy
   int m, n, k;
+  bool c_vec;           // four adjacent elements of C, from a multiple of four on, can be stored at once
 };
 
 template <class T>
@@ -184,6 +186,353 @@ __global__ void __launch_bounds__(256) product_any(Product p) {
 }
 
 // ---------------------------------------------------------------------------
+// The tiled product: operands go to LDS by direct copies, 128 bytes of each
+// row (or 64 rows, where the summed index runs across them) at a time, into
+// one of two stages while the other is multiplied.
+// ---------------------------------------------------------------------------
+// How an operand lies in memory:
+//   ROWS    the summed index along its rows
+//   COLS    the summed index across its rows; fragments come out of LDS by
+//           transposing reads
+//   PACKED  COLS of packed rows; codes are decoded on their way to LDS
+enum Layout { ROWS, COLS, PACKED };
+
+struct Fp8 {};  // packed operands multiplied as they are
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// A raw buffer resource over [p, p + bytes), from wave-uniform scalars;
+// accesses at offsets outside it read zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* p, uint64_t bytes) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
+  const int n = __builtin_amdgcn_readfirstlane((int)(uint32_t)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)(((uint64_t)hi << 32) | lo), 0, n, 0x00020000);
+}
+
+// Copies of 16 (and 4) bytes a lane straight into LDS: lane i's land at
+// lds + 16 i (4 i), zeros for offsets outside the resource. Inline asm, so
+// that the compiler does not wait for them before every LDS read; nothing
+// else in these kernels uses m0. wait_copies() waits for all of them.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t rs, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rs)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(__amdgpu_buffer_rsrc_t rs, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rs)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+constexpr uint32_t NOWHERE = 0xFFFFFF00u;  // an offset outside every resource
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+
+// Tile `i` of n for this workgroup: workgroups go to the 8 dies in turn, so
+// each die takes an eighth of the tiles, in order, and tiles that share
+// operands meet in one L2.
+__device__ __forceinline__ int die_order(int block, int n) {
+  const int die = block & 7, at = block >> 3, each = n >> 3, more = n & 7;
+  if (at >= each + (die < more ? 1 : 0)) return -1;
+  return die * each + (die < more ? die : more) + at;
+}
+#endif
+
+// WM x WN wavefronts, each with MT x NT tiles of 16 x 16. T is the type
+// multiplied (bf16, f16 or Fp8), O the result's.
+template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
+struct Tiled {
+  static constexpr int THREADS = 64 * WM * WN, WAVES = WM * WN;
+  static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT;
+  static constexpr bool FP8 = std::is_same_v<T, Fp8>;
+  static constexpr int BYTES = FP8 ? 1 : 2;       // of an element
+  static constexpr int STEP = 128 / BYTES;        // summed elements a stage holds
+  static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
+  static constexpr int SCALES = FP8 ? (TM + TN) * 4 : 0;  // four blocks' scale bytes of each row
+  static constexpr int LDS = 2 * (STAGE + SCALES);
+};
+
+template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
+__global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  using K = Tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>;
+  constexpr int TM = K::TM, TN = K::TN, WAVES = K::WAVES;
+  __shared__ __align__(1024) char lds[K::LDS];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // this workgroup's tile
+  const int tiles_n = (p.n + TN - 1) / TN;
+  int m0, n0, rows, cols, steps, group, tail;
+  uint64_t a0, b0;  // first bytes of the operands' tiles
+  uint64_t first = 0;
+  if constexpr (FORM == GRAD_WEIGHT) {
+    const int tiles_m = (p.m + TM - 1) / TM, each = tiles_m * tiles_n;
+    // a die takes an eighth of every group's tiles: groups differ in length
+    const int per = (each + 7) / 8;
+    group = (int)(blockIdx.x / (8 * per));
+    const int in = (int)(blockIdx.x % (8 * per)), t = (in & 7) * per + (in >> 3);
+    if (t >= each) return;
+    m0 = t / tiles_n * TM;
+    n0 = t % tiles_n * TN;
+    int lo, hi;
+    group_range(p.offsets, group, p.rows, lo, hi);
+    rows = p.m - m0;
+    tail = hi - lo;
+    steps = (tail + K::STEP - 1) / K::STEP;
+    first = lo;
+    a0 = ((uint64_t)lo * p.as + m0) * 2;
+    b0 = LB == PACKED ? 0 : ((uint64_t)lo * p.bs + n0) * 2;
+  } else {
+    const int total = count_row_tiles(p.offsets, p.groups, p.rows, TM);
+    const int index = die_order(blockIdx.x, total * tiles_n);
+    RowTile t;
+    if (index < 0 || !find_row_tile(p.offsets, p.groups, p.rows, TM, index / tiles_n, t)) return;
+    m0 = t.row;
+    n0 = index % tiles_n * TN;
+    group = t.group < 0 ? 0 : t.group;
+    rows = t.end - m0;
+    tail = t.group < 0 ? 0 : p.k;
+    steps = (tail + K::STEP - 1) / K::STEP;
+    a0 = (uint64_t)m0 * p.as * K::BYTES;
+    b0 = (group * p.bg + (LB == ROWS ? (uint64_t)n0 * p.bs : (uint64_t)n0)) * K::BYTES;
+  }
+  rows = rows < TM ? rows : TM;
+  cols = p.n - n0 < TN ? p.n - n0 : TN;
+
+  // Copies. ROWS: a copy of one wavefront fills 8 rows of 128 bytes, 16-byte
+  // piece c of row r at place c ^ (r & 7), so that 8 lanes reading piece c of
+  // 8 rows meet every bank. COLS: it fills 1024 bytes of rows of 2 TM (2 TN)
+  // bytes, piece c of row k at c ^ 2 (k & 7): the four rows of a transposing
+  // read lie in different banks.
+  const char* pa = (const char*)p.a + a0;
+  const char* pb = (const char*)p.b + b0;
+  constexpr int CA = TM / 8 / WAVES, CB = TN / 8 / WAVES;  // copies a wavefront makes of a stage
+  uint32_t oa[CA], ob[LB == PACKED ? 1 : CB];
+  const uint64_t as = p.as * K::BYTES, bs = p.bs * K::BYTES;
+  auto offsets = [&](auto layout, int width, int limit, uint64_t stride, auto& o) {
+    constexpr int L = decltype(layout)::value;
+    constexpr int N = sizeof(o) / sizeof(o[0]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = wave * N + i;
+      if constexpr (L == ROWS) {
+        const int r = at * 8 + (lane >> 3);
+        o[i] = (uint32_t)(r * stride) + (((lane & 7) ^ (lane >> 3)) << 4);
+      } else {
+        const int per = width / 8;  // pieces in a row
+        const int k = at * (64 / per) + lane / per, c = (lane % per) ^ ((k & 7) << 1);
+        o[i] = c * 8 < limit ? (uint32_t)(k * stride) + c * 16 : NOWHERE;
+      }
+    }
+  };
+  offsets(std::integral_constant<int, LA>{}, TM, rows, as, oa);
+  if constexpr (LB != PACKED) offsets(std::integral_constant<int, LB>{}, TN, cols, bs, ob);
+
+  const uint32_t lds0 = lds_address(lds);
+  // bytes of the operand from the step's first element on
+  auto stage_copies = [&](auto layout, const char* base, uint64_t stride, int limit, auto& o, uint32_t to, int step) {
+    constexpr int L = decltype(layout)::value;
+    constexpr int N = sizeof(o) / sizeof(o[0]);
+    const int left = tail - step * K::STEP;  // summed elements from here on
+    if constexpr (L == ROWS) {
+      const auto rs = tile_rsrc(base + (uint64_t)step * 128, (uint64_t)(limit - 1) * stride + (uint64_t)left * K::BYTES);
+      if (left >= K::STEP) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) copy16(rs, o[i], to + (wave * N + i) * 1024);
+      } else {
+        // the last step: pieces past the row's end are zeros
+        const bool in = (((lane & 7) ^ (lane >> 3)) << 4) < left * K::BYTES;
+#pragma unroll
+        for (int i = 0; i < N; ++i) copy16(rs, in ? o[i] : NOWHERE, to + (wave * N + i) * 1024);
+      }
+    } else {
+      const auto rs = tile_rsrc(base + (uint64_t)step * K::STEP * stride, (uint64_t)(left - 1) * stride + limit * 2);
+#pragma unroll
+      for (int i = 0; i < N; ++i) copy16(rs, o[i], to + (wave * N + i) * 1024);
+    }
+  };
+  // PACKED: thread t decodes 8 columns of rows t / (TN / 8) + i * THREADS / (TN / 8)
+  constexpr int PR = K::THREADS / (TN / 8), PN = K::STEP / PR;
+  [[maybe_unused]] uint2 codes[PN];
+  [[maybe_unused]] uint32_t bytes[PN];
+  auto load_packed = [&](int step) {
+    const int c = (threadIdx.x % (TN / 8)) * 8, left = tail - step * K::STEP;
+#pragma unroll
+    for (int i = 0; i < PN; ++i) {
+      const int k = threadIdx.x / (TN / 8) + i * PR;
+      const bool in = k < left && c < cols;
+      const uint64_t row = first + (uint64_t)step * K::STEP + k;
+      codes[i] = in ? *reinterpret_cast<const uint2*>((const char*)p.b + row * p.bs + n0 + c) : make_uint2(0, 0);
+      bytes[i] = in ? p.b_scales[row * p.ss + (n0 + c) / 128] : 127;
+    }
+  };
+  auto store_packed = [&](uint32_t to) {
+    const int c = threadIdx.x % (TN / 8);
+#pragma unroll
+    for (int i = 0; i < PN; ++i) {
+      const int k = threadIdx.x / (TN / 8) + i * PR;
+      const float s = block8_scale(bytes[i]);
+      typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+      bf2v v[4];
+      v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].x, s, false);
+      v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].x, s, true);
+      v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].y, s, false);
+      v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].y, s, true);
+      *reinterpret_cast<uint4*>(lds + to + k * (TN * 2) + ((c ^ ((k & 7) << 1)) << 4)) =
+          make_uint4(__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]),
+                     __builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3]));
+    }
+  };
+  // Fp8: four blocks' scale bytes of every row of the tiles, one word a lane
+  auto scale_copies = [&](int step) {
+    const uint32_t to = lds0 + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
+#pragma unroll
+    for (int i = 0; i < (TM + TN) / 64 / WAVES; ++i) {
+      const int at = wave * ((TM + TN) / 64 / WAVES) + i;  // the first TM / 64 are A's
+      const bool of_a = at < TM / 64;
+      const uint64_t row = of_a ? (uint64_t)m0 : (uint64_t)group * p.n + n0;
+      const int r = (of_a ? at : at - TM / 64) * 64 + lane, limit = of_a ? rows : cols;
+      const auto rs = tile_rsrc((of_a ? p.a_scales : p.b_scales) + row * p.ss + step, (uint64_t)limit * p.ss - step);
+      copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
+    }
+  };
+  auto fetch = [&](int step) {
+    const uint32_t to = (step & 1) * K::STAGE;
+    stage_copies(std::integral_constant<int, LA>{}, pa, as, rows, oa, lds0 + to, step);
+    if constexpr (LB != PACKED)
+      stage_copies(std::integral_constant<int, LB>{}, pb, bs, cols, ob, lds0 + to + K::A_BYTES, step);
+    if constexpr (K::FP8)
+      if ((step & 3) == 0) scale_copies(step);
+  };
+
+  // Fragments. A lane holds row (lane & 15) of a 16-row tile and 8 summed
+  // elements from 8 (lane >> 4) on, of every 32 (Fp8: 16 from 16 (lane >> 4)
+  // on and 16 from 64 past those, of 128: any order does that A and B share,
+  // a block having one scale).
+  const int r16 = lane & 15, q = lane >> 4;
+  auto rows_at = [&](int wtile, int half) {  // of tile 0 of this wavefront
+    return (uint32_t)((wtile * 16 + r16) * 128 + (((half * 4 + q) ^ (r16 & 7)) << 4));
+  };
+  auto cols_at = [&](int wtile, int half, int width) {
+    const int x = half * 4 + (r16 >> 2);  // k & 7
+    return (uint32_t)((8 * q + x) * (width * 2) + ((wtile ^ x) << 5) + (r16 & 3) * 8);
+  };
+  const uint32_t fa0 = LA == ROWS ? rows_at(wm * MT, 0) : cols_at(wm * MT, 0, TM);
+  const uint32_t fa1 = LA == ROWS ? rows_at(wm * MT, 1) : cols_at(wm * MT, 1, TM);
+  const uint32_t fb0 = LB == ROWS ? rows_at(wn * NT, 0) : cols_at(wn * NT, 0, TN);
+  const uint32_t fb1 = LB == ROWS ? rows_at(wn * NT, 1) : cols_at(wn * NT, 1, TN);
+  // tile j of the wavefront, summed elements 32 h to 32 h + 31 (16-bit types)
+  auto fragment = [&](auto layout, const char* base, uint32_t at0, uint32_t at1, int j, int h, int width) -> uint4 {
+    constexpr int L = decltype(layout)::value;
+    if constexpr (L == ROWS) {
+      return *reinterpret_cast<const uint4*>(base + (h ? at1 : at0) + j * 2048);
+    } else {
+      typedef short s4v __attribute__((ext_vector_type(4)));
+      typedef __attribute__((address_space(3))) s4v* lds_s4;
+      const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + (at0 ^ (j << 5)) + h * 64 * width));
+      const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + (at1 ^ (j << 5)) + h * 64 * width));
+      const uint2 lo = __builtin_bit_cast(uint2, x), hi = __builtin_bit_cast(uint2, y);
+      return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    }
+  };
+
+  f4v acc[MT][NT] = {};
+  if (steps > 0) {
+    fetch(0);
+    if constexpr (LB == PACKED) load_packed(0);
+  }
+  [[maybe_unused]] uint32_t sa[MT], sb[NT];
+  for (int step = 0; step < steps; ++step) {
+    const char* base = lds + (step & 1) * K::STAGE;
+    if constexpr (LB == PACKED) store_packed((step & 1) * K::STAGE + K::A_BYTES);
+    wait_copies();
+    __syncthreads();
+    if (step + 1 < steps) {
+      fetch(step + 1);
+      if constexpr (LB == PACKED) load_packed(step + 1);
+    }
+    if constexpr (K::FP8) {
+      const char* sc = lds + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
+      if ((step & 3) == 0) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(sc + (wm * MT * 16 + i * 16 + r16) * 4);
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          sb[j] = *reinterpret_cast<const uint32_t*>(sc + TM * 4 + (wn * NT * 16 + j * 16 + r16) * 4);
+      } else {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sa[i] >>= 8;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sb[j] >>= 8;
+      }
+      i8v fb[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4*>(base + K::A_BYTES + fb0 + j * 2048);
+        const uint4 y = *reinterpret_cast<const uint4*>(base + K::A_BYTES + fb1 + j * 2048);
+        fb[j] = i8v{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(base + fa0 + i * 2048);
+        const uint4 y = *reinterpret_cast<const uint4*>(base + fa1 + i * 2048);
+        const i8v fa = {(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], 0, 0, 0, (int)sb[j], 0,
+                                                                       (int)sa[i]);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 fb[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+          fb[j] = fragment(std::integral_constant<int, LB>{}, base + K::A_BYTES, fb0, fb1, j, h, TN);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const uint4 fa = fragment(std::integral_constant<int, LA>{}, base, fa0, fa1, i, h, TM);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<T>(fb[j], fa, acc[i][j]);
+        }
+      }
+    }
+  }
+
+  // a lane holds columns 4 q to 4 q + 3 of row r16 of each tile
+  O* c = (O*)p.c + group * p.cg + (uint64_t)m0 * p.cs + n0;
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int r = (wm * MT + i) * 16 + r16;
+    if (r >= rows) continue;
+    O* row = c + (uint64_t)r * p.cs;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int at = (wn * NT + j) * 16 + 4 * q;
+      if (p.c_vec && at + 4 <= cols) {
+        typedef O o4v __attribute__((ext_vector_type(4)));
+        o4v v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (O)acc[i][j][e];
+        *reinterpret_cast<o4v*>(row + at) = v;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (at + e < cols) row[at + e] = (O)acc[i][j][e];
+      }
+    }
+  }
+#endif
+}
+
+// ---------------------------------------------------------------------------
 template <class F>
 void by_types(int type, int out_type, F f) {
   auto g = [&](auto t) {
@@ -210,12 +559,47 @@ void check_out_type(int type, int out_type) {
 }
 
 template <int FORM, class T, class O, bool PACKED>
-void launch_product(const Product& p, hipStream_t s) {
+void launch_any(const Product& p, hipStream_t s) {
   const uint64_t tm = FORM == GRAD_WEIGHT ? (uint64_t)p.groups * ((p.m + ANY_TILE - 1) / ANY_TILE)
                                           : row_tiles_max(p.rows, p.groups, ANY_TILE, p.offsets != nullptr);
   const uint64_t tn = (p.n + ANY_TILE - 1) / ANY_TILE;
   hipLaunchKernelGGL((product_any<T, O, FORM, PACKED>), dim3(grid_size(tm * tn)), dim3(256), 0, s, p);
   PXG_HIP(hipGetLastError());
+}
+
+template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
+void launch_tiled(const Product& p, hipStream_t s) {
+  using K = Tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>;
+  const uint64_t tn = (p.n + K::TN - 1) / K::TN;
+  uint64_t tiles;
+  if (FORM == GRAD_WEIGHT) tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * p.groups;
+  else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn + 7) / 8 * 8;
+  hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), dim3(grid_size(tiles)), dim3(K::THREADS), 0, s,
+                     p);
+  PXG_HIP(hipGetLastError());
+}
+
+// Whether the tiled product can copy an operand: 16-byte pieces that all
+// belong to one row, and a tile's offsets in 31 bits.
+bool copies(int bytes, const void* d, uint64_t cols, uint64_t stride, uint64_t group_stride) {
+  return ((uint64_t)(uintptr_t)d | cols * bytes | stride * bytes | group_stride * bytes) % 16 == 0 &&
+         stride * bytes <= (1u << 22);
+}
+
+template <int FORM, class T, class O, bool PACKED>
+void launch_product(Product p, hipStream_t s) {
+  p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % (4 * sizeof(O)) == 0;
+  constexpr int LA = FORM == GRAD_WEIGHT ? COLS : ROWS;
+  constexpr int LB = FORM == FORWARD ? ROWS : FORM == GRAD_INPUT ? COLS : PACKED ? Layout::PACKED : COLS;
+  if constexpr (FORM == FORWARD && PACKED) {
+    if (!std::is_same_v<O, float> && p.as <= (1u << 22) && p.rows >= 256 * p.groups)
+      return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
+  } else {
+    const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
+    if (copies(2, p.a, acols, p.as, 0) && (PACKED || copies(2, p.b, bcols, p.bs, p.bg)))
+      return launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+  }
+  launch_any<FORM, T, O, PACKED>(p, s);
 }
 
 template <int FORM>
@@ -251,7 +635,7 @@ int pxg_grouped_matmul_device(int type, const void* d_x, uint64_t rows, uint64_t
     check_rows(out_type, "y", d_y, rows, n, y_stride);
     if (rows == 0) return;
     Product p{d_x, d_w, d_y, d_offsets, x_stride, w_stride, y_stride, w_group_stride, 0, nullptr, nullptr, 0, (int)rows, (int)groups,
-              (int)rows, (int)n, (int)k};
+              (int)rows, (int)n, (int)k, false};
     run_product<FORWARD>(type, out_type, p, (hipStream_t)stream);
   });
 }
@@ -271,7 +655,7 @@ int pxg_grouped_matmul_grad_input_device(int type, const void* d_grad, uint64_t 
     check_rows(out_type, "dx", d_dx, rows, k, dx_stride);
     if (rows == 0) return;
     Product p{d_grad, d_w, d_dx, d_offsets, grad_stride, w_stride, dx_stride, w_group_stride, 0, nullptr, nullptr, 0, (int)rows,
-              (int)groups, (int)rows, (int)k, (int)n};
+              (int)groups, (int)rows, (int)k, (int)n, false};
     run_product<GRAD_INPUT>(type, out_type, p, (hipStream_t)stream);
   });
 }
@@ -291,7 +675,7 @@ int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t
     check_rows(type, "x", d_x, rows, k, x_stride);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
     Product p{d_grad, d_x, d_dw, d_offsets, grad_stride, x_stride, dw_stride, 0, dw_group_stride, nullptr, nullptr, 0, (int)rows,
-              (int)groups, (int)n, (int)k, 0};
+              (int)groups, (int)n, (int)k, 0, false};
     run_product<GRAD_WEIGHT>(type, out_type, p, (hipStream_t)stream);
   });
 }
@@ -310,7 +694,7 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
     check_packed_rows("codes", d_codes, "scales", d_scales, rows);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
     Product p{d_grad, d_codes, d_dw, d_offsets, grad_stride, block8_code_stride(k), dw_stride, 0, dw_group_stride,
-              nullptr, (const uint8_t*)d_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)n, (int)k, 0};
+              nullptr, (const uint8_t*)d_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)n, (int)k, 0, false};
     run_product<GRAD_WEIGHT>(PXG_BF16, out_type, p, (hipStream_t)stream);
   });
 }
@@ -328,9 +712,9 @@ int pxg_block8_matmul_device(const void* d_codes, const void* d_scales, uint64_t
     check_rows(out_type, "y", d_y, rows, n, y_stride);
     if (rows == 0) return;
     const uint64_t wide = block8_code_stride(k);
-    Product p{d_codes, d_w_codes, d_y, d_offsets, wide, wide, y_stride, 0, 0, (const uint8_t*)d_scales,
+    Product p{d_codes, d_w_codes, d_y, d_offsets, wide, wide, y_stride, n * wide, 0, (const uint8_t*)d_scales,
               (const uint8_t*)d_w_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)rows, (int)n,
-              (int)wide};
+              (int)wide, false};
     const hipStream_t s = (hipStream_t)stream;
     if (out_type == PXG_F32) launch_product<FORWARD, __bf16, float, true>(p, s);
     else if (out_type == PXG_F16) launch_product<FORWARD, __bf16, _Float16, true>(p, s);

@@ -95,6 +95,24 @@ __device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offset
   return false;
 }
 
+// How many tiles find_row_tile has.
+__device__ __forceinline__ int count_row_tiles(const int64_t* __restrict__ offsets, int groups, int rows, int size) {
+  if (!offsets) return (rows + size - 1) / size;
+  const int lane = threadIdx.x & (WAVE - 1);
+  int begin = 0, total = 0;
+  for (int s0 = 0; s0 < groups + 2; s0 += WAVE) {
+    const int s = s0 + lane;
+    int end = s <= groups ? clamp_offset(offsets[s], rows) : rows;
+    end = wave_max_scan(end > begin ? end : begin, lane);
+    int first = __shfl_up(end, 1, WAVE);
+    if (lane == 0) first = begin;
+    const int sum = wave_sum_scan((end - first + size - 1) / size, lane);
+    total += __builtin_amdgcn_readlane(sum, WAVE - 1);
+    begin = __builtin_amdgcn_readlane(end, WAVE - 1);
+  }
+  return total;
+}
+
 // No more tiles than this come out of `rows` rows in `groups` groups, the
 // rows of no group at either end counted as two more.
 inline uint64_t row_tiles_max(uint64_t rows, uint64_t groups, uint64_t size, bool ragged) {

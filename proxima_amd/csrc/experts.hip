@@ -233,6 +233,10 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
 
+// By how many 16-byte pieces row k of a stage is moved: a transposing read
+// takes 32 bytes of rows 8 q + {0..3} (or {4..7}) for each 16 lanes q.
+__device__ __forceinline__ int cols_swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) << 1; }
+
 // Tile `i` of n for this workgroup: workgroups go to the 8 dies in turn, so
 // each die takes an eighth of the tiles, in order, and tiles that share
 // operands meet in one L2.
@@ -309,8 +313,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   // Copies. ROWS: a copy of one wavefront fills 8 rows of 128 bytes, 16-byte
   // piece c of row r at place c ^ (r & 7), so that 8 lanes reading piece c of
   // 8 rows meet every bank. COLS: it fills 1024 bytes of rows of 2 TM (2 TN)
-  // bytes, piece c of row k at c ^ 2 (k & 7): the four rows of a transposing
-  // read lie in different banks.
+  // bytes, piece c of row k at c ^ cols_swizzle(k): of the two quarters of a
+  // transposing read that go together, the eight rows lie in different banks.
   const char* pa = (const char*)p.a + a0;
   const char* pb = (const char*)p.b + b0;
   constexpr int CA = TM / 8 / WAVES, CB = TN / 8 / WAVES;  // copies a wavefront makes of a stage
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
         o[i] = (uint32_t)(r * stride) + (((lane & 7) ^ (lane >> 3)) << 4);
       } else {
         const int per = width / 8;  // pieces in a row
-        const int k = at * (64 / per) + lane / per, c = (lane % per) ^ ((k & 7) << 1);
+        const int k = at * (64 / per) + lane / per, c = (lane % per) ^ cols_swizzle(k);
         o[i] = c * 8 < limit ? (uint32_t)(k * stride) + c * 16 : NOWHERE;
       }
     }
@@ -336,24 +340,19 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   if constexpr (LB != PACKED) offsets(std::integral_constant<int, LB>{}, TN, cols, bs, ob);
 
   const uint32_t lds0 = lds_address(lds);
-  // bytes of the operand from the step's first element on
+  // Steps past the last one copy zeros.
   auto stage_copies = [&](auto layout, const char* base, uint64_t stride, int limit, auto& o, uint32_t to, int step) {
     constexpr int L = decltype(layout)::value;
     constexpr int N = sizeof(o) / sizeof(o[0]);
     const int left = tail - step * K::STEP;  // summed elements from here on
     if constexpr (L == ROWS) {
-      const auto rs = tile_rsrc(base + (uint64_t)step * 128, (uint64_t)(limit - 1) * stride + (uint64_t)left * K::BYTES);
-      if (left >= K::STEP) {
+      const auto rs = tile_rsrc(base + (uint64_t)step * 128, (limit - 1) * stride + (uint64_t)(left * K::BYTES));
+      // pieces past the rows' end are zeros
+      const bool in = (((lane & 7) ^ (lane >> 3)) << 4) < left * K::BYTES;
 #pragma unroll
-        for (int i = 0; i < N; ++i) copy16(rs, o[i], to + (wave * N + i) * 1024);
-      } else {
-        // the last step: pieces past the row's end are zeros
-        const bool in = (((lane & 7) ^ (lane >> 3)) << 4) < left * K::BYTES;
-#pragma unroll
-        for (int i = 0; i < N; ++i) copy16(rs, in ? o[i] : NOWHERE, to + (wave * N + i) * 1024);
-      }
+      for (int i = 0; i < N; ++i) copy16(rs, in ? o[i] : NOWHERE, to + (wave * N + i) * 1024);
     } else {
-      const auto rs = tile_rsrc(base + (uint64_t)step * K::STEP * stride, (uint64_t)(left - 1) * stride + limit * 2);
+      const auto rs = tile_rsrc(base + (uint64_t)step * K::STEP * stride, left > 0 ? (left - 1) * stride + limit * 2 : 0);
 #pragma unroll
       for (int i = 0; i < N; ++i) copy16(rs, o[i], to + (wave * N + i) * 1024);
     }
@@ -364,13 +363,16 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   [[maybe_unused]] uint32_t bytes[PN];
   auto load_packed = [&](int step) {
     const int c = (threadIdx.x % (TN / 8)) * 8, left = tail - step * K::STEP;
+    const uint64_t row = first + (uint64_t)step * K::STEP;
+    const auto rc = tile_rsrc((const char*)p.b + row * p.bs + n0, left > 0 ? left * p.bs - n0 : 0);
+    const auto rb = tile_rsrc(p.b_scales + row * p.ss + n0 / 128, left > 0 ? left * p.ss - n0 / 128 : 0);
 #pragma unroll
     for (int i = 0; i < PN; ++i) {
       const int k = threadIdx.x / (TN / 8) + i * PR;
-      const bool in = k < left && c < cols;
-      const uint64_t row = first + (uint64_t)step * K::STEP + k;
-      codes[i] = in ? *reinterpret_cast<const uint2*>((const char*)p.b + row * p.bs + n0 + c) : make_uint2(0, 0);
-      bytes[i] = in ? p.b_scales[row * p.ss + (n0 + c) / 128] : 127;
+      typedef int i2v __attribute__((ext_vector_type(2)));
+      const i2v w = __builtin_amdgcn_raw_buffer_load_b64(rc, c < cols ? k * (int)p.bs + c : (int)NOWHERE, 0, 0);
+      codes[i] = __builtin_bit_cast(uint2, w);
+      bytes[i] = __builtin_amdgcn_raw_buffer_load_b8(rb, c < cols ? k * (int)p.ss + c / 128 : (int)NOWHERE, 0, 0);
     }
   };
   auto store_packed = [&](uint32_t to) {
@@ -385,7 +387,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].x, s, true);
       v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].y, s, false);
       v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].y, s, true);
-      *reinterpret_cast<uint4*>(lds + to + k * (TN * 2) + ((c ^ ((k & 7) << 1)) << 4)) =
+      *reinterpret_cast<uint4*>(lds + to + k * (TN * 2) + ((c ^ cols_swizzle(k)) << 4)) =
           make_uint4(__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]),
                      __builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3]));
     }
@@ -399,7 +401,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       const bool of_a = at < TM / 64;
       const uint64_t row = of_a ? (uint64_t)m0 : (uint64_t)group * p.n + n0;
       const int r = (of_a ? at : at - TM / 64) * 64 + lane, limit = of_a ? rows : cols;
-      const auto rs = tile_rsrc((of_a ? p.a_scales : p.b_scales) + row * p.ss + step, (uint64_t)limit * p.ss - step);
+      const auto rs = tile_rsrc((of_a ? p.a_scales : p.b_scales) + row * p.ss + step,
+                                step < p.ss ? limit * p.ss - step : 0);
       copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
     }
   };
@@ -420,45 +423,104 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   auto rows_at = [&](int wtile, int half) {  // of tile 0 of this wavefront
     return (uint32_t)((wtile * 16 + r16) * 128 + (((half * 4 + q) ^ (r16 & 7)) << 4));
   };
-  auto cols_at = [&](int wtile, int half, int width) {
-    const int x = half * 4 + (r16 >> 2);  // k & 7
-    return (uint32_t)((8 * q + x) * (width * 2) + ((wtile ^ x) << 5) + (r16 & 3) * 8);
+  auto cols_at = [&](int wtile, int width) {
+    const int k = 8 * q + (r16 >> 2);
+    return (uint32_t)(k * (width * 2) + (((wtile << 1) ^ cols_swizzle(k)) << 4) + (r16 & 3) * 8);
   };
-  const uint32_t fa0 = LA == ROWS ? rows_at(wm * MT, 0) : cols_at(wm * MT, 0, TM);
-  const uint32_t fa1 = LA == ROWS ? rows_at(wm * MT, 1) : cols_at(wm * MT, 1, TM);
-  const uint32_t fb0 = LB == ROWS ? rows_at(wn * NT, 0) : cols_at(wn * NT, 0, TN);
-  const uint32_t fb1 = LB == ROWS ? rows_at(wn * NT, 1) : cols_at(wn * NT, 1, TN);
+  const uint32_t fa0 = LA == ROWS ? rows_at(wm * MT, 0) : cols_at(wm * MT, TM);
+  const uint32_t fb0 = LB == ROWS ? rows_at(wn * NT, 0) : cols_at(wn * NT, TN);
   // tile j of the wavefront, summed elements 32 h to 32 h + 31 (16-bit types)
-  auto fragment = [&](auto layout, const char* base, uint32_t at0, uint32_t at1, int j, int h, int width) -> uint4 {
+  auto fragment = [&](auto layout, const char* base, uint32_t at, int j, int h, int width) -> uint4 {
     constexpr int L = decltype(layout)::value;
     if constexpr (L == ROWS) {
-      return *reinterpret_cast<const uint4*>(base + (h ? at1 : at0) + j * 2048);
+      return *reinterpret_cast<const uint4*>(base + (at ^ (h << 6)) + j * 2048);
     } else {
       typedef short s4v __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s4v* lds_s4;
-      const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + (at0 ^ (j << 5)) + h * 64 * width));
-      const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(base + (at1 ^ (j << 5)) + h * 64 * width));
+      const char* b = base + (at ^ (j << 5)) + h * 64 * width;
+      const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)b);
+      const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(b + 8 * width));
       const uint2 lo = __builtin_bit_cast(uint2, x), hi = __builtin_bit_cast(uint2, y);
       return make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
   };
 
   f4v acc[MT][NT] = {};
-  if (steps > 0) {
-    fetch(0);
-    if constexpr (LB == PACKED) load_packed(0);
-  }
-  [[maybe_unused]] uint32_t sa[MT], sb[NT];
-  for (int step = 0; step < steps; ++step) {
-    const char* base = lds + (step & 1) * K::STAGE;
-    if constexpr (LB == PACKED) store_packed((step & 1) * K::STAGE + K::A_BYTES);
-    wait_copies();
-    __syncthreads();
-    if (step + 1 < steps) {
-      fetch(step + 1);
-      if constexpr (LB == PACKED) load_packed(step + 1);
+  if constexpr (!K::FP8) {
+    // A step's fragments are two halves of 32 summed elements, each read while
+    // the other is multiplied; between a step's halves its stage has been read
+    // and the next one has landed, so the barrier there frees the one for the
+    // step after next and opens the other.
+    struct Half {
+      uint4 a[MT], b[NT];
+    };
+    auto read = [&](Half& f, int step, int h) {
+      const char* base = lds + (step & 1) * K::STAGE;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        f.b[j] = fragment(std::integral_constant<int, LB>{}, base + K::A_BYTES, fb0, j, h, TN);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) f.a[i] = fragment(std::integral_constant<int, LA>{}, base, fa0, i, h, TM);
+    };
+    auto multiply = [&](const Half& f) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<T>(f.b[j], f.a[i], acc[i][j]);
+    };
+    // one LDS read to every few matrix instructions
+    auto interleave = [&] {
+      constexpr int READS = (LA == ROWS ? 1 : 2) * MT + (LB == ROWS ? 1 : 2) * NT, PER = MT * NT / READS;
+#pragma unroll
+      for (int i = 0; i < READS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, MT * NT - READS * PER, 0);
+    };
+    auto next = [&](int step) {  // the copies of a step, and of PACKED its codes into registers
+      fetch(step);
+      if constexpr (LB == PACKED) load_packed(step);
+    };
+    auto decode = [&](int step) {
+      if constexpr (LB == PACKED) store_packed((step & 1) * K::STAGE + K::A_BYTES);
+    };
+    auto landed = [&] {
+      wait_copies();
+      __syncthreads();
+    };
+    if (steps > 0) {
+      Half even, odd;
+      next(0);
+      decode(0);
+      landed();
+      next(1);
+      read(even, 0, 0);
+      for (int step = 0; step < steps - 1; ++step) {
+        read(odd, step, 1);
+        multiply(even);
+        interleave();
+        decode(step + 1);
+        landed();
+        next(step + 2);
+        read(even, step + 1, 0);
+        multiply(odd);
+        interleave();
+      }
+      read(odd, steps - 1, 1);
+      multiply(even);
+      interleave();
+      multiply(odd);
+      wait_copies();  // those of the step past the last
     }
-    if constexpr (K::FP8) {
+  } else {
+    uint32_t sa[MT], sb[NT];
+    if (steps > 0) fetch(0);
+    for (int step = 0; step < steps; ++step) {
+      const char* base = lds + (step & 1) * K::STAGE;
+      wait_copies();
+      __syncthreads();
+      if (step + 1 < steps) fetch(step + 1);
       const char* sc = lds + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
       if ((step & 3) == 0) {
 #pragma unroll
@@ -472,36 +534,21 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
 #pragma unroll
         for (int j = 0; j < NT; ++j) sb[j] >>= 8;
       }
+      auto pair = [&](const char* at) {  // both halves of 64 bytes
+        const uint4 x = *reinterpret_cast<const uint4*>(at);
+        const uint4 y = *reinterpret_cast<const uint4*>((const char*)((uintptr_t)at ^ 64));
+        return i8v{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+      };
       i8v fb[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const uint4 x = *reinterpret_cast<const uint4*>(base + K::A_BYTES + fb0 + j * 2048);
-        const uint4 y = *reinterpret_cast<const uint4*>(base + K::A_BYTES + fb1 + j * 2048);
-        fb[j] = i8v{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-      }
+      for (int j = 0; j < NT; ++j) fb[j] = pair(base + K::A_BYTES + fb0 + j * 2048);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const uint4 x = *reinterpret_cast<const uint4*>(base + fa0 + i * 2048);
-        const uint4 y = *reinterpret_cast<const uint4*>(base + fa1 + i * 2048);
-        const i8v fa = {(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+        const i8v fa = pair(base + fa0 + i * 2048);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
           acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], 0, 0, 0, (int)sb[j], 0,
                                                                        (int)sa[i]);
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 fb[NT];
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          fb[j] = fragment(std::integral_constant<int, LB>{}, base + K::A_BYTES, fb0, fb1, j, h, TN);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const uint4 fa = fragment(std::integral_constant<int, LA>{}, base, fa0, fa1, i, h, TM);
-#pragma unroll
-          for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<T>(fb[j], fa, acc[i][j]);
-        }
       }
     }
   }

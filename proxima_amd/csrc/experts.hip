@@ -296,10 +296,15 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   } else {
     const int total = count_row_tiles(p.offsets, p.groups, p.rows, TM);
     const int index = die_order(blockIdx.x, total * tiles_n);
+    if (index < 0) return;
+    // the 32 workgroups that run together on a die share operands best as a
+    // block of 4 row tiles by 8
+    const int band = index / (4 * tiles_n), in = index - band * 4 * tiles_n;
+    const int high = total - band * 4 < 4 ? total - band * 4 : 4;
     RowTile t;
-    if (index < 0 || !find_row_tile(p.offsets, p.groups, p.rows, TM, index / tiles_n, t)) return;
+    if (!find_row_tile(p.offsets, p.groups, p.rows, TM, band * 4 + in % high, t)) return;
     m0 = t.row;
-    n0 = index % tiles_n * TN;
+    n0 = in / high * TN;
     group = t.group < 0 ? 0 : t.group;
     rows = t.end - m0;
     tail = t.group < 0 ? 0 : p.k;
@@ -317,44 +322,42 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   // transposing read that go together, the eight rows lie in different banks.
   const char* pa = (const char*)p.a + a0;
   const char* pb = (const char*)p.b + b0;
+  const uint32_t row_a = (lane >> 3) * (uint32_t)(p.as * K::BYTES) + (((lane & 7) ^ (lane >> 3)) << 4);
+  const uint32_t row_b = (lane >> 3) * (uint32_t)(p.bs * K::BYTES) + (((lane & 7) ^ (lane >> 3)) << 4);
   constexpr int CA = TM / 8 / WAVES, CB = TN / 8 / WAVES;  // copies a wavefront makes of a stage
-  uint32_t oa[CA], ob[LB == PACKED ? 1 : CB];
   const uint64_t as = p.as * K::BYTES, bs = p.bs * K::BYTES;
-  auto offsets = [&](auto layout, int width, int limit, uint64_t stride, auto& o) {
+  // A lane's offset in copy i of n; NOWHERE where the piece is past the matrix.
+  // `me` is its offset in copy 0 (ROWS) and hidden from the compiler inside
+  // the loop, which would otherwise keep every copy's in a register.
+  auto copy_offset = [&](auto layout, int width, int limit, uint64_t stride, int n, int i, uint32_t me) -> uint32_t {
     constexpr int L = decltype(layout)::value;
-    constexpr int N = sizeof(o) / sizeof(o[0]);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = wave * N + i;
-      if constexpr (L == ROWS) {
-        const int r = at * 8 + (lane >> 3);
-        o[i] = (uint32_t)(r * stride) + (((lane & 7) ^ (lane >> 3)) << 4);
-      } else {
-        const int per = width / 8;  // pieces in a row
-        const int k = at * (64 / per) + lane / per, c = (lane % per) ^ cols_swizzle(k);
-        o[i] = c * 8 < limit ? (uint32_t)(k * stride) + c * 16 : NOWHERE;
-      }
+    if constexpr (L == ROWS) {
+      return (uint32_t)((wave * n + i) * 8 * stride) + me;
+    } else {
+      const int per = width / 8;  // pieces in a row
+      const int k = (wave * n + i) * (64 / per) + lane / per, c = (lane % per) ^ cols_swizzle(k);
+      return c * 8 < limit ? (uint32_t)(k * stride) + c * 16 : NOWHERE;
     }
   };
-  offsets(std::integral_constant<int, LA>{}, TM, rows, as, oa);
-  if constexpr (LB != PACKED) offsets(std::integral_constant<int, LB>{}, TN, cols, bs, ob);
 
   const uint32_t lds0 = lds_address(lds);
   // Steps past the last one copy zeros.
-  auto stage_copies = [&](auto layout, const char* base, uint64_t stride, int limit, auto& o, uint32_t to, int step) {
+  auto stage_copies = [&](auto layout, const char* base, int width, int limit, uint64_t stride, auto n, uint32_t me,
+                          uint32_t to, int step) {
     constexpr int L = decltype(layout)::value;
-    constexpr int N = sizeof(o) / sizeof(o[0]);
+    constexpr int N = decltype(n)::value;
     const int left = tail - step * K::STEP;  // summed elements from here on
-    if constexpr (L == ROWS) {
-      const auto rs = tile_rsrc(base + (uint64_t)step * 128, (limit - 1) * stride + (uint64_t)(left * K::BYTES));
-      // pieces past the rows' end are zeros
-      const bool in = (((lane & 7) ^ (lane >> 3)) << 4) < left * K::BYTES;
+    const auto rs = L == ROWS ? tile_rsrc(base + (uint64_t)step * 128,
+                                          left > 0 ? (limit - 1) * stride + (uint64_t)(left * K::BYTES) : 0)
+                              : tile_rsrc(base + (uint64_t)step * K::STEP * stride,
+                                          left > 0 ? (left - 1) * stride + limit * 2 : 0);
+    if constexpr (L == ROWS) asm volatile("" : "+v"(me));
+    // pieces past the rows' end are zeros (packed rows are whole blocks)
+    const bool in = L != ROWS || K::FP8 || (((lane & 7) ^ (lane >> 3)) << 4) < left * K::BYTES;
 #pragma unroll
-      for (int i = 0; i < N; ++i) copy16(rs, in ? o[i] : NOWHERE, to + (wave * N + i) * 1024);
-    } else {
-      const auto rs = tile_rsrc(base + (uint64_t)step * K::STEP * stride, left > 0 ? (left - 1) * stride + limit * 2 : 0);
-#pragma unroll
-      for (int i = 0; i < N; ++i) copy16(rs, o[i], to + (wave * N + i) * 1024);
+    for (int i = 0; i < N; ++i) {
+      const uint32_t o = copy_offset(layout, width, limit, stride, N, i, me);
+      copy16(rs, in ? o : NOWHERE, to + (wave * N + i) * 1024);
     }
   };
   // PACKED: thread t decodes 8 columns of rows t / (TN / 8) + i * THREADS / (TN / 8)
@@ -393,26 +396,24 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     }
   };
   // Fp8: four blocks' scale bytes of every row of the tiles, one word a lane
-  auto scale_copies = [&](int step) {
+  auto scale_copies = [&](int step, int at) {  // part `at` of (TM + TN) / 64, the first TM / 64 A's
     const uint32_t to = lds0 + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
-#pragma unroll
-    for (int i = 0; i < (TM + TN) / 64 / WAVES; ++i) {
-      const int at = wave * ((TM + TN) / 64 / WAVES) + i;  // the first TM / 64 are A's
-      const bool of_a = at < TM / 64;
-      const uint64_t row = of_a ? (uint64_t)m0 : (uint64_t)group * p.n + n0;
-      const int r = (of_a ? at : at - TM / 64) * 64 + lane, limit = of_a ? rows : cols;
-      const auto rs = tile_rsrc((of_a ? p.a_scales : p.b_scales) + row * p.ss + step,
-                                step < p.ss ? limit * p.ss - step : 0);
-      copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
-    }
+    const bool of_a = at < TM / 64;
+    const uint64_t row = of_a ? (uint64_t)m0 : (uint64_t)group * p.n + n0;
+    const int r = (of_a ? at : at - TM / 64) * 64 + lane, limit = of_a ? rows : cols;
+    const auto rs = tile_rsrc((of_a ? p.a_scales : p.b_scales) + row * p.ss + step,
+                              step < p.ss ? limit * p.ss - step : 0);
+    copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
   };
   auto fetch = [&](int step) {
     const uint32_t to = (step & 1) * K::STAGE;
-    stage_copies(std::integral_constant<int, LA>{}, pa, as, rows, oa, lds0 + to, step);
+    stage_copies(std::integral_constant<int, LA>{}, pa, TM, rows, as, std::integral_constant<int, CA>{}, row_a,
+                 lds0 + to, step);
     if constexpr (LB != PACKED)
-      stage_copies(std::integral_constant<int, LB>{}, pb, bs, cols, ob, lds0 + to + K::A_BYTES, step);
+      stage_copies(std::integral_constant<int, LB>{}, pb, TN, cols, bs, std::integral_constant<int, CB>{}, row_b,
+                   lds0 + to + K::A_BYTES, step);
     if constexpr (K::FP8)
-      if ((step & 3) == 0) scale_copies(step);
+      if ((step & 3) == 0 && step < steps) scale_copies(step, wave);
   };
 
   // Fragments. A lane holds row (lane & 15) of a 16-row tile and 8 summed
@@ -427,8 +428,9 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     const int k = 8 * q + (r16 >> 2);
     return (uint32_t)(k * (width * 2) + (((wtile << 1) ^ cols_swizzle(k)) << 4) + (r16 & 3) * 8);
   };
-  const uint32_t fa0 = LA == ROWS ? rows_at(wm * MT, 0) : cols_at(wm * MT, TM);
-  const uint32_t fb0 = LB == ROWS ? rows_at(wn * NT, 0) : cols_at(wn * NT, TN);
+  [[maybe_unused]] const uint32_t rows_half0 = rows_at(0, 0), rows_half1 = rows_at(0, 1);
+  [[maybe_unused]] const uint32_t fa0 = LA == ROWS ? rows_at(wm * MT, 0) : cols_at(wm * MT, TM);
+  [[maybe_unused]] const uint32_t fb0 = LB == ROWS ? rows_at(wn * NT, 0) : cols_at(wn * NT, TN);
   // tile j of the wavefront, summed elements 32 h to 32 h + 31 (16-bit types)
   auto fragment = [&](auto layout, const char* base, uint32_t at, int j, int h, int width) -> uint4 {
     constexpr int L = decltype(layout)::value;
@@ -514,41 +516,110 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       wait_copies();  // those of the step past the last
     }
   } else {
-    uint32_t sa[MT], sb[NT];
-    if (steps > 0) fetch(0);
-    for (int step = 0; step < steps; ++step) {
+    // Wavefronts 0 to 3 and 4 to 7, one of each on every SIMD, take turns: one
+    // half reads a step's fragments while the other multiplies, with a barrier
+    // between the turns. The first half reads step s in turn 2 s and
+    // multiplies it in turn 2 s + 1, the second half is a turn behind. Step
+    // s's stage has then been read by the end of turn 2 s + 1, is filled for
+    // step s + 2 by copies issued in turn 2 s + 2, and has landed by the end of
+    // turn 2 s + 3.
+    static_assert(K::WAVES == 8, "two wavefronts on a SIMD");
+    struct Fragment {
+      i8v v;
+      int scale;
+    };
+    auto read = [&](const char* at, int step, int row) {
+      Fragment f;
+      const uint4 x = *reinterpret_cast<const uint4*>(at + rows_half0);
+      const uint4 y = *reinterpret_cast<const uint4*>(at + rows_half1);
+      f.v = i8v{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+      f.scale = (uint8_t)lds[2 * K::STAGE + ((step >> 2) & 1) * K::SCALES + (row + r16) * 4 + (step & 3)];
+      return f;
+    };
+    const bool second = wave >= 4;
+    Fragment fa[MT], fb[NT];
+    auto read_step = [&](int step) {
       const char* base = lds + (step & 1) * K::STAGE;
-      wait_copies();
-      __syncthreads();
-      if (step + 1 < steps) fetch(step + 1);
-      const char* sc = lds + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
-      if ((step & 3) == 0) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) sa[i] = *reinterpret_cast<const uint32_t*>(sc + (wm * MT * 16 + i * 16 + r16) * 4);
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          sb[j] = *reinterpret_cast<const uint32_t*>(sc + TM * 4 + (wn * NT * 16 + j * 16 + r16) * 4);
-      } else {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) sa[i] >>= 8;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) sb[j] >>= 8;
+      for (int j = 0; j < NT; ++j) {
+        const int row = (wn * NT + j) * 16;
+        fb[j] = read(base + K::A_BYTES + row * 128, step, TM + row);
       }
-      auto pair = [&](const char* at) {  // both halves of 64 bytes
-        const uint4 x = *reinterpret_cast<const uint4*>(at);
-        const uint4 y = *reinterpret_cast<const uint4*>((const char*)((uintptr_t)at ^ 64));
-        return i8v{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
-      };
-      i8v fb[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) fb[j] = pair(base + K::A_BYTES + fb0 + j * 2048);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const i8v fa = pair(base + fa0 + i * 2048);
+        const int row = (wm * MT + i) * 16;
+        fa[i] = read(base + row * 128, step, row);
+      }
+    };
+    auto multiply_row = [&](int i) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], 0, 0, 0, (int)sb[j], 0,
-                                                                       (int)sa[i]);
+      for (int j = 0; j < NT; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i].v, acc[i][j], 0, 0, 0,
+                                                                     fb[j].scale, 0, fa[i].scale);
+    };
+    auto turn = [&] {  // LDS reads have returned
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    // the second half's share of a step's copies: all of them, MT parts
+    const uint32_t row_off = (lane >> 3) * (uint32_t)p.as + (((lane & 7) ^ (lane >> 3)) << 4);
+    auto copy_part = [&](__amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int step, int i) {
+      uint32_t me = row_off;
+      asm volatile("" : "+v"(me));
+      const int at = (wave & 3) * MT + i;
+      const uint32_t to = lds0 + (step & 1) * K::STAGE + at * 1024;
+      static_assert(TM == 32 * MT && TN == TM);
+      copy16(ra, (uint32_t)(at * 8 * as) + me, to);
+      copy16(rb, (uint32_t)(at * 8 * as) + me, to + K::A_BYTES);
+    };
+    if (steps > 0) {
+      fetch(0);
+      wait_copies();
+      turn();
+      if (second) {
+        auto copies_of = [&](const char* base, int limit, int step) {
+          return tile_rsrc(base + (uint64_t)step * 128, step < steps ? (limit - 1) * as + (tail - step * 128) : 0);
+        };
+        {
+          const auto ra = copies_of(pa, rows, 1), rb = copies_of(pb, cols, 1);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) copy_part(ra, rb, 1, i);
+        }
+        turn();
+        for (int step = 0; step < steps; ++step) {
+          read_step(step);
+          wait_copies();
+          turn();
+          const auto ra = copies_of(pa, rows, step + 2), rb = copies_of(pb, cols, step + 2);
+          if (((step + 2) & 3) == 0 && step + 2 < steps) {
+            scale_copies(step + 2, (wave & 3) * 2);
+            scale_copies(step + 2, (wave & 3) * 2 + 1);
+          }
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            multiply_row(i);
+            __builtin_amdgcn_sched_barrier(0);
+            copy_part(ra, rb, step + 2, i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          __builtin_amdgcn_s_setprio(0);
+          turn();
+        }
+        wait_copies();  // those of the steps past the last
+      } else {
+        for (int step = 0; step < steps; ++step) {
+          read_step(step);
+          turn();
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) multiply_row(i);
+          __builtin_amdgcn_s_setprio(0);
+          turn();
+        }
+        turn();
       }
     }
   }

@@ -233,6 +233,17 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
 }
 
+// 8 codes times their scale, in bf16.
+__device__ __forceinline__ uint4 decode_bf16(uint32_t x, uint32_t y, float s) {
+  typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+  const bf2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, s, false);
+  const bf2v b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, s, true);
+  const bf2v c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, s, false);
+  const bf2v d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, s, true);
+  return make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
+                    __builtin_bit_cast(uint32_t, d));
+}
+
 // By how many 16-byte pieces row k of a stage is moved: a transposing read
 // takes 32 bytes of rows 8 q + {0..3} (or {4..7}) for each 16 lanes q.
 __device__ __forceinline__ int cols_swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) << 1; }
@@ -383,16 +394,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
 #pragma unroll
     for (int i = 0; i < PN; ++i) {
       const int k = threadIdx.x / (TN / 8) + i * PR;
-      const float s = block8_scale(bytes[i]);
-      typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
-      bf2v v[4];
-      v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].x, s, false);
-      v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].x, s, true);
-      v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].y, s, false);
-      v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes[i].y, s, true);
       *reinterpret_cast<uint4*>(lds + to + k * (TN * 2) + ((c ^ cols_swizzle(k)) << 4)) =
-          make_uint4(__builtin_bit_cast(uint32_t, v[0]), __builtin_bit_cast(uint32_t, v[1]),
-                     __builtin_bit_cast(uint32_t, v[2]), __builtin_bit_cast(uint32_t, v[3]));
+          decode_bf16(codes[i].x, codes[i].y, block8_scale(bytes[i]));
     }
   };
   // Fp8: four blocks' scale bytes of every row of the tiles, one word a lane
@@ -651,6 +654,146 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
 }
 
 // ---------------------------------------------------------------------------
+// Few rows in a group: the time is that of reading the matrices. A workgroup
+// takes 16 MT rows and 16 rows of a matrix (COLS: 128 of its columns); its
+// eight wavefronts read 128 bytes of each row (COLS: 32 rows) in turn, straight
+// into the registers that the matrix cores take, and their partial sums are
+// added in LDS, in order.
+// ---------------------------------------------------------------------------
+template <class T, class O, int LB, bool IS_PACKED, int MT>
+__global__ void __launch_bounds__(512) product_few(Product p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int WAVES = 8, N16 = LB == ROWS ? 1 : 8;     // tiles of 16 columns of C
+  constexpr int TN = 16 * N16, PIECES = LB == ROWS ? 2 : 1;  // loads of a row (ROWS) in a round
+  constexpr int ROUND = LB == ROWS ? (IS_PACKED ? 128 : 64) : 32;  // summed elements of a wavefront's round
+  constexpr int AHEAD = LB == ROWS ? (IS_PACKED || MT > 1 ? (MT > 2 ? 2 : 4) : 8) : 1;  // rounds loaded before they are multiplied
+  __shared__ f4v part[WAVES][N16 * MT][64];
+  const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles_n = (p.n + TN - 1) / TN;
+  RowTile t;
+  if (!find_row_tile(p.offsets, p.groups, p.rows, 16 * MT, (int)(blockIdx.x / tiles_n), t)) return;
+  const int n0 = (int)(blockIdx.x % tiles_n) * TN;
+  const int rows = t.end - t.row < 16 * MT ? t.end - t.row : 16 * MT, cols = p.n - n0 < TN ? p.n - n0 : TN;
+  const int k_end = t.group < 0 ? 0 : p.k, group = t.group < 0 ? 0 : t.group;
+  constexpr int BYTES = IS_PACKED ? 1 : 2;
+  const auto ra = tile_rsrc((const char*)p.a + (uint64_t)t.row * p.as * BYTES,
+                            ((uint64_t)(rows - 1) * p.as + p.k) * BYTES);
+  uint32_t oa[MT];  // this lane's rows of A
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+    oa[i] = 16 * i + r16 < rows ? (uint32_t)((16 * i + r16) * p.as * BYTES) + q * 16 : NOWHERE;
+  f4v acc[N16][MT] = {};
+  typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+  auto load = [&](__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
+    return __builtin_bit_cast(uint4, (u4v)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)offset, 0, 0));
+  };
+  if constexpr (LB == ROWS) {
+    const uint64_t row = (uint64_t)group * p.n + n0;  // packed: of the codes
+    const auto rb = tile_rsrc(IS_PACKED ? (const char*)p.b + row * p.bs : (const char*)p.b + (group * p.bg + n0 * p.bs) * 2,
+                              ((uint64_t)(cols - 1) * p.bs + p.k) * BYTES);
+    const uint32_t ob = r16 < cols ? (uint32_t)(r16 * p.bs * BYTES) + q * 16 : NOWHERE;
+    [[maybe_unused]] __amdgpu_buffer_rsrc_t rsa, rsb;
+    if constexpr (IS_PACKED) {
+      rsa = tile_rsrc(p.a_scales + (uint64_t)t.row * p.ss, (uint64_t)rows * p.ss);
+      rsb = tile_rsrc(p.b_scales + row * p.ss, (uint64_t)cols * p.ss);
+    }
+    for (int k0 = wave * ROUND; k0 < k_end; k0 += WAVES * ROUND * AHEAD) {
+      uint4 b[AHEAD][PIECES], a[AHEAD][PIECES][MT];
+      [[maybe_unused]] uint32_t xb[AHEAD], xa[AHEAD][MT];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int k = k0 + u * WAVES * ROUND;
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+          // past the rows' end: zeros
+          const bool in = (k * BYTES + h * 64 + q * 16) < k_end * BYTES;
+          b[u][h] = load(rb, in && ob != NOWHERE ? ob + k * BYTES + h * 64 : NOWHERE);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+            a[u][h][i] = load(ra, in && oa[i] != NOWHERE ? oa[i] + k * BYTES + h * 64 : NOWHERE);
+        }
+        if constexpr (IS_PACKED) {
+          const bool in = k < k_end;
+          xb[u] = __builtin_amdgcn_raw_buffer_load_b8(rsb, in && r16 < cols ? r16 * (int)p.ss + k / 128 : (int)NOWHERE, 0, 0);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+            xa[u][i] = __builtin_amdgcn_raw_buffer_load_b8(
+                rsa, in && 16 * i + r16 < rows ? (16 * i + r16) * (int)p.ss + k / 128 : (int)NOWHERE, 0, 0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first is waited for
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int h = 0; h < PIECES; ++h) {
+          if constexpr (IS_PACKED) {
+            // 16 codes a lane: 8 for each of two instructions, of A as of B
+            const float sb = block8_scale(xb[u]);
+            const uint4 b0 = decode_bf16(b[u][h].x, b[u][h].y, sb), b1 = decode_bf16(b[u][h].z, b[u][h].w, sb);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              const float sa = block8_scale(xa[u][i]);
+              acc[0][i] = mfma16<T>(b0, decode_bf16(a[u][h][i].x, a[u][h][i].y, sa), acc[0][i]);
+              acc[0][i] = mfma16<T>(b1, decode_bf16(a[u][h][i].z, a[u][h][i].w, sa), acc[0][i]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[0][i] = mfma16<T>(b[u][h], a[u][h][i], acc[0][i]);
+          }
+        }
+    }
+  } else {
+    const auto rb = tile_rsrc((const char*)p.b + (group * p.bg + n0) * 2, ((uint64_t)(p.k - 1) * p.bs + cols) * 2);
+    // 8 columns from 8 r16 on of rows 8 q to 8 q + 7
+    const uint32_t ob = 8 * r16 < cols ? (uint32_t)(8 * q * p.bs * 2) + r16 * 16 : NOWHERE;
+    for (int k0 = wave * ROUND; k0 < k_end; k0 += WAVES * ROUND) {
+      uint4 b[8], a[MT];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        b[j] = load(rb, ob != NOWHERE && k0 + 8 * q + j < k_end ? ob + (uint32_t)((k0 + j) * p.bs * 2) : NOWHERE);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        a[i] = load(ra, oa[i] != NOWHERE && k0 + 8 * q < k_end ? oa[i] + k0 * 2 : NOWHERE);
+      __builtin_amdgcn_sched_barrier(0);
+      // column c of the eight rows, c even and odd: the low and the high halves of word c / 2
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(b);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[j] = __builtin_amdgcn_perm(w[(2 * j + 1) * 4 + c / 2], w[2 * j * 4 + c / 2], c & 1 ? 0x07060302 : 0x05040100);
+        const uint4 f = make_uint4(v[0], v[1], v[2], v[3]);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[c][i] = mfma16<T>(f, a[i], acc[c][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < N16; ++c)
+#pragma unroll
+    for (int i = 0; i < MT; ++i) part[wave][c * MT + i][lane] = acc[c][i];
+  __syncthreads();
+  O* out = (O*)p.c + (uint64_t)t.row * p.cs + n0;
+  for (int j = wave; j < N16 * MT; j += WAVES) {
+    const int c = j / MT, i = j % MT;
+    f4v s = part[0][j][lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) s += part[w][j][lane];
+    const int r = 16 * i + r16;
+    if (r >= rows) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      // tile c holds columns 4 q to 4 q + 3 (COLS: every eighth column from c on)
+      const int at = LB == ROWS ? 4 * q + e : 8 * (4 * q + e) + c;
+      if (at < cols) out[(uint64_t)r * p.cs + at] = (O)s[e];
+    }
+  }
+#endif
+}
+
+// ---------------------------------------------------------------------------
 template <class F>
 void by_types(int type, int out_type, F f) {
   auto g = [&](auto t) {
@@ -704,20 +847,40 @@ bool copies(int bytes, const void* d, uint64_t cols, uint64_t stride, uint64_t g
          stride * bytes <= (1u << 22);
 }
 
-template <int FORM, class T, class O, bool PACKED>
+template <class T, class O, int LB, bool IS_PACKED, int MT>
+void launch_few(const Product& p, hipStream_t s) {
+  constexpr uint64_t TN = LB == ROWS ? 16 : 128;
+  const uint64_t tiles = row_tiles_max(p.rows, p.groups, 16 * MT, p.offsets != nullptr) * ((p.n + TN - 1) / TN);
+  hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED, MT>), dim3(grid_size(tiles)), dim3(512), 0, s, p);
+  PXG_HIP(hipGetLastError());
+}
+
+template <int FORM, class T, class O, bool IS_PACKED>
 void launch_product(Product p, hipStream_t s) {
   p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % (4 * sizeof(O)) == 0;
   constexpr int LA = FORM == GRAD_WEIGHT ? COLS : ROWS;
-  constexpr int LB = FORM == FORWARD ? ROWS : FORM == GRAD_INPUT ? COLS : PACKED ? Layout::PACKED : COLS;
-  if constexpr (FORM == FORWARD && PACKED) {
-    if (!std::is_same_v<O, float> && p.as <= (1u << 22) && p.rows >= 256 * p.groups)
-      return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
-  } else {
-    const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
-    if (copies(2, p.a, acols, p.as, 0) && (PACKED || copies(2, p.b, bcols, p.bs, p.bg)))
-      return launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+  constexpr int LB = FORM == FORWARD ? ROWS : FORM == GRAD_INPUT ? COLS : IS_PACKED ? PACKED : COLS;
+  constexpr int bytes = FORM == FORWARD && IS_PACKED ? 1 : 2;
+  const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
+  if (!copies(bytes, p.a, acols, p.as, 0) || (LB != PACKED && !copies(bytes, p.b, bcols, p.bs, p.bg)))
+    return launch_any<FORM, T, O, IS_PACKED>(p, s);
+  const uint64_t each = ((uint64_t)p.rows + p.groups - 1) / p.groups;  // rows of a group, on average
+  if constexpr (FORM != GRAD_WEIGHT) {
+    // COLS spans a matrix' rows with one resource
+    if (LB == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF) {
+      if (each <= 16) return launch_few<T, O, LB, IS_PACKED, 1>(p, s);
+      if (each <= 32) return launch_few<T, O, LB, IS_PACKED, 2>(p, s);
+      if constexpr (LB == ROWS)
+        if (each <= 64) return launch_few<T, O, LB, IS_PACKED, 4>(p, s);
+    }
   }
-  launch_any<FORM, T, O, PACKED>(p, s);
+  if constexpr (FORM == FORWARD && IS_PACKED) {
+    if constexpr (!std::is_same_v<O, float>)
+      if (each >= 256) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
+    return launch_any<FORM, T, O, IS_PACKED>(p, s);
+  } else {
+    launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+  }
 }
 
 template <int FORM>

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) product_any(Product p) {
     c = (O*)p.c + group * p.cg;
   } else {
     RowTile t;
-    if (!find_row_tile(p.offsets, p.groups, p.rows, ANY_TILE, index, t)) return;
+    if (!find_row_tile<ALL_TILES>(p.offsets, p.groups, p.rows, ANY_TILE, index, t)) return;
     m0 = t.row;
     m_end = t.end;
     k_end = t.group < 0 ? 0 : p.k;
@@ -194,8 +194,11 @@ __global__ void __launch_bounds__(256) product_any(Product p) {
 //   ROWS    the summed index along its rows
 //   COLS    the summed index across its rows; fragments come out of LDS by
 //           transposing reads
-//   PACKED  COLS of packed rows; codes are decoded on their way to LDS
-enum Layout { ROWS, COLS, PACKED };
+//   PACKED_ROWS, PACKED_COLS  the same of packed rows; codes are decoded on
+//           their way to LDS
+enum Layout { ROWS, COLS, PACKED_ROWS, PACKED_COLS };
+constexpr bool is_packed(int l) { return l == PACKED_ROWS || l == PACKED_COLS; }
+constexpr bool is_rows(int l) { return l == ROWS || l == PACKED_ROWS; }
 
 struct Fp8 {};  // packed operands multiplied as they are
 
@@ -248,13 +251,11 @@ __device__ __forceinline__ uint4 decode_bf16(uint32_t x, uint32_t y, float s) {
 // takes 32 bytes of rows 8 q + {0..3} (or {4..7}) for each 16 lanes q.
 __device__ __forceinline__ int cols_swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) << 1; }
 
-// Tile `i` of n for this workgroup: workgroups go to the 8 dies in turn, so
-// each die takes an eighth of the tiles, in order, and tiles that share
-// operands meet in one L2.
-__device__ __forceinline__ int die_order(int block, int n) {
-  const int die = block & 7, at = block >> 3, each = n >> 3, more = n & 7;
-  if (at >= each + (die < more ? 1 : 0)) return -1;
-  return die * each + (die < more ? die : more) + at;
+// Part `die` of n cut into eight, the larger parts first: its first and size.
+__device__ __forceinline__ void eighth(int n, int die, int& first, int& size) {
+  const int each = n >> 3, more = n & 7;
+  first = die * each + (die < more ? die : more);
+  size = each + (die < more ? 1 : 0);
 }
 #endif
 
@@ -282,47 +283,61 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
 
-  // this workgroup's tile
+  // This workgroup's tile. Workgroups go to the eight dies in turn. Each die
+  // takes an eighth of the tiles, in order, so that tiles that share operands
+  // meet in one L2; the longest come first.
   const int tiles_n = (p.n + TN - 1) / TN;
+  const int die = blockIdx.x & 7, at = blockIdx.x >> 3;
   int m0, n0, rows, cols, steps, group, tail;
-  uint64_t a0, b0;  // first bytes of the operands' tiles
-  uint64_t first = 0;
+  uint64_t a0, b0;  // first elements of the operands' tiles
+  [[maybe_unused]] uint64_t sa0 = 0, sb0 = 0;  // and their rows, packed
   if constexpr (FORM == GRAD_WEIGHT) {
-    const int tiles_m = (p.m + TM - 1) / TM, each = tiles_m * tiles_n;
-    // a die takes an eighth of every group's tiles: groups differ in length
-    const int per = (each + 7) / 8;
-    group = (int)(blockIdx.x / (8 * per));
-    const int in = (int)(blockIdx.x % (8 * per)), t = (in & 7) * per + (in >> 3);
-    if (t >= each) return;
+    // an eighth of every group's tiles, the longest group first
+    const int tiles_m = (p.m + TM - 1) / TM, each = tiles_m * tiles_n, per = (each + 7) / 8;
+    const int t = die * per + at % per;
+    if (t >= each || at % per >= per) return;
+    group = group_by_size(p.offsets, p.groups, p.rows, at / per);
     m0 = t / tiles_n * TM;
     n0 = t % tiles_n * TN;
     int lo, hi;
     group_range(p.offsets, group, p.rows, lo, hi);
     rows = p.m - m0;
     tail = hi - lo;
-    steps = (tail + K::STEP - 1) / K::STEP;
-    first = lo;
-    a0 = ((uint64_t)lo * p.as + m0) * 2;
-    b0 = LB == PACKED ? 0 : ((uint64_t)lo * p.bs + n0) * 2;
+    a0 = (uint64_t)lo * p.as + m0;
+    b0 = (uint64_t)lo * p.bs + n0;
+    sb0 = (uint64_t)lo * p.ss + n0 / 128;
   } else {
-    const int total = count_row_tiles(p.offsets, p.groups, p.rows, TM);
-    const int index = die_order(blockIdx.x, total * tiles_n);
-    if (index < 0) return;
-    // the 32 workgroups that run together on a die share operands best as a
-    // block of 4 row tiles by 8
+    // an eighth of the whole row tiles, then of the partial ones. The 32
+    // workgroups that run together on a die share operands best as a block of
+    // 4 row tiles by 8.
+    int whole, partial, first, size;
+    count_row_tiles(p.offsets, p.groups, p.rows, TM, whole, partial);
+    eighth(whole * tiles_n, die, first, size);
+    const bool is_whole = at < size;
+    int index = first + at, count = whole;
+    if (!is_whole) {
+      index = at - size;
+      eighth(partial * tiles_n, 7 - die, first, size);
+      if (index >= size) return;
+      index += first;
+      count = partial;
+    }
     const int band = index / (4 * tiles_n), in = index - band * 4 * tiles_n;
-    const int high = total - band * 4 < 4 ? total - band * 4 : 4;
+    const int high = count - band * 4 < 4 ? count - band * 4 : 4;
     RowTile t;
-    if (!find_row_tile(p.offsets, p.groups, p.rows, TM, band * 4 + in % high, t)) return;
+    if (is_whole) find_row_tile<WHOLE_TILES>(p.offsets, p.groups, p.rows, TM, band * 4 + in % high, t);
+    else find_row_tile<PARTIAL_TILES>(p.offsets, p.groups, p.rows, TM, band * 4 + in % high, t);
     m0 = t.row;
     n0 = in / high * TN;
     group = t.group < 0 ? 0 : t.group;
     rows = t.end - m0;
     tail = t.group < 0 ? 0 : p.k;
-    steps = (tail + K::STEP - 1) / K::STEP;
-    a0 = (uint64_t)m0 * p.as * K::BYTES;
-    b0 = (group * p.bg + (LB == ROWS ? (uint64_t)n0 * p.bs : (uint64_t)n0)) * K::BYTES;
+    a0 = (uint64_t)m0 * p.as;
+    b0 = group * p.bg + (is_rows(LB) ? (uint64_t)n0 * p.bs : (uint64_t)n0);
+    sa0 = (uint64_t)m0 * p.ss;
+    sb0 = ((uint64_t)group * p.n + n0) * p.ss;
   }
+  steps = (tail + K::STEP - 1) / K::STEP;
   rows = rows < TM ? rows : TM;
   cols = p.n - n0 < TN ? p.n - n0 : TN;
 
@@ -331,216 +346,237 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   // 8 rows meet every bank. COLS: it fills 1024 bytes of rows of 2 TM (2 TN)
   // bytes, piece c of row k at c ^ cols_swizzle(k): of the two quarters of a
   // transposing read that go together, the eight rows lie in different banks.
-  const char* pa = (const char*)p.a + a0;
-  const char* pb = (const char*)p.b + b0;
-  const uint32_t row_a = (lane >> 3) * (uint32_t)(p.as * K::BYTES) + (((lane & 7) ^ (lane >> 3)) << 4);
-  const uint32_t row_b = (lane >> 3) * (uint32_t)(p.bs * K::BYTES) + (((lane & 7) ^ (lane >> 3)) << 4);
-  constexpr int CA = TM / 8 / WAVES, CB = TN / 8 / WAVES;  // copies a wavefront makes of a stage
-  const uint64_t as = p.as * K::BYTES, bs = p.bs * K::BYTES;
-  // A lane's offset in copy i of n; NOWHERE where the piece is past the matrix.
-  // `me` is its offset in copy 0 (ROWS) and hidden from the compiler inside
-  // the loop, which would otherwise keep every copy's in a register.
-  auto copy_offset = [&](auto layout, int width, int limit, uint64_t stride, int n, int i, uint32_t me) -> uint32_t {
-    constexpr int L = decltype(layout)::value;
-    if constexpr (L == ROWS) {
-      return (uint32_t)((wave * n + i) * 8 * stride) + me;
-    } else {
-      const int per = width / 8;  // pieces in a row
-      const int k = (wave * n + i) * (64 / per) + lane / per, c = (lane % per) ^ cols_swizzle(k);
-      return c * 8 < limit ? (uint32_t)(k * stride) + c * 16 : NOWHERE;
-    }
+  struct Operand {
+    const char* base;  // the tile's first element
+    const uint8_t* scales;
+    uint64_t stride;  // bytes from row to row
+    int limit;        // rows (COLS: columns) of the tile inside the matrix
+    uint32_t place;   // of the tile in a stage
+    uint32_t row;     // ROWS: this lane's offset in copy 0
   };
-
+  auto operand = [&](const void* base, uint64_t first, const uint8_t* scales, uint64_t row, uint64_t stride, int limit,
+                     uint32_t place, int bytes) {
+    return Operand{(const char*)base + first * bytes, scales + row, stride * bytes, limit, place,
+                   (lane >> 3) * (uint32_t)(stride * bytes) + (((lane & 7) ^ (lane >> 3)) << 4)};
+  };
+  const Operand A = operand(p.a, a0, p.a_scales, sa0, p.as, rows, 0, is_packed(LA) ? 1 : K::BYTES);
+  const Operand B = operand(p.b, b0, p.b_scales, sb0, p.bs, cols, K::A_BYTES, is_packed(LB) ? 1 : K::BYTES);
   const uint32_t lds0 = lds_address(lds);
-  // Steps past the last one copy zeros.
-  auto stage_copies = [&](auto layout, const char* base, int width, int limit, uint64_t stride, auto n, uint32_t me,
-                          uint32_t to, int step) {
-    constexpr int L = decltype(layout)::value;
-    constexpr int N = decltype(n)::value;
+  // Part i of n of a step's copies of an operand, by one wavefront, in order
+  // `who`. Steps past the last one copy zeros.
+  auto stage_resource = [&](auto layout, const Operand& o, int step) {
     const int left = tail - step * K::STEP;  // summed elements from here on
-    const auto rs = L == ROWS ? tile_rsrc(base + (uint64_t)step * 128,
-                                          left > 0 ? (limit - 1) * stride + (uint64_t)(left * K::BYTES) : 0)
-                              : tile_rsrc(base + (uint64_t)step * K::STEP * stride,
-                                          left > 0 ? (left - 1) * stride + limit * 2 : 0);
-    if constexpr (L == ROWS) asm volatile("" : "+v"(me));
-    // pieces past the rows' end are zeros (packed rows are whole blocks)
-    const bool in = L != ROWS || K::FP8 || (((lane & 7) ^ (lane >> 3)) << 4) < left * K::BYTES;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t o = copy_offset(layout, width, limit, stride, N, i, me);
-      copy16(rs, in ? o : NOWHERE, to + (wave * N + i) * 1024);
+    return decltype(layout)::value == ROWS
+               ? tile_rsrc(o.base + (uint64_t)step * 128,
+                           left > 0 ? (o.limit - 1) * o.stride + (uint64_t)(left * K::BYTES) : 0)
+               : tile_rsrc(o.base + (uint64_t)step * K::STEP * o.stride,
+                           left > 0 ? (left - 1) * o.stride + o.limit * 2 : 0);
+  };
+  auto stage_copy = [&](auto layout, auto width, const Operand& o, __amdgpu_buffer_rsrc_t rs, int step, int part) {
+    const uint32_t to = lds0 + (step & 1) * K::STAGE + o.place + part * 1024;
+    if constexpr (decltype(layout)::value == ROWS) {
+      uint32_t at = o.row;
+      asm volatile("" : "+v"(at));  // keeps one register for all parts, not one for each
+      // pieces past the rows' end are zeros (packed rows are whole blocks)
+      const bool in = K::FP8 || (((lane & 7) ^ (lane >> 3)) << 4) < (tail - step * K::STEP) * K::BYTES;
+      copy16(rs, in ? (uint32_t)(part * 8 * o.stride) + at : NOWHERE, to);
+    } else {
+      constexpr int PER = decltype(width)::value / 8;  // pieces in a row
+      int me = lane;
+      if constexpr (is_packed(LB)) asm volatile("" : "+v"(me));  // registers are short there
+      const int k = part * (64 / PER) + me / PER, c = (me % PER) ^ cols_swizzle(k);
+      copy16(rs, c * 8 < o.limit ? (uint32_t)(k * (int)o.stride) + c * 16 : NOWHERE, to);
     }
   };
-  // PACKED: thread t decodes 8 columns of rows t / (TN / 8) + i * THREADS / (TN / 8)
-  constexpr int PR = K::THREADS / (TN / 8), PN = K::STEP / PR;
-  [[maybe_unused]] uint2 codes[PN];
-  [[maybe_unused]] uint32_t bytes[PN];
-  auto load_packed = [&](int step) {
-    const int c = (threadIdx.x % (TN / 8)) * 8, left = tail - step * K::STEP;
-    const uint64_t row = first + (uint64_t)step * K::STEP;
-    const auto rc = tile_rsrc((const char*)p.b + row * p.bs + n0, left > 0 ? left * p.bs - n0 : 0);
-    const auto rb = tile_rsrc(p.b_scales + row * p.ss + n0 / 128, left > 0 ? left * p.ss - n0 / 128 : 0);
+  using LayoutA = std::integral_constant<int, LA>;
+  using LayoutB = std::integral_constant<int, LB>;
+  using WidthA = std::integral_constant<int, TM>;
+  using WidthB = std::integral_constant<int, TN>;
+  auto stage_copies = [&](auto layout, auto width, const Operand& o, int step) {
+    if constexpr (!is_packed(decltype(layout)::value)) {
+      constexpr int N = decltype(width)::value / 8 / WAVES;
+      const auto rs = stage_resource(layout, o, step);
 #pragma unroll
-    for (int i = 0; i < PN; ++i) {
-      const int k = threadIdx.x / (TN / 8) + i * PR;
+      for (int i = 0; i < N; ++i) stage_copy(layout, width, o, rs, step, wave * N + i);
+    }
+  };
+  // Packed: a thread takes 8 codes at a time, of row (COLS: summed element)
+  // `line` from `piece` eights on, reads them a step ahead and decodes them.
+  struct Codes {
+    uint2 codes[8];
+    uint32_t bytes[8];
+  };
+  auto packed_pieces = [&](auto layout, auto width, auto f) {
+    constexpr int W = decltype(width)::value;
+    constexpr int PER = decltype(layout)::value == PACKED_ROWS ? 8 : W / 8;  // pieces in a line
+    constexpr int N = W * 8 / K::THREADS;
+    static_assert(N <= 8);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f(i, (int)threadIdx.x / PER + i * (K::THREADS / PER), (int)threadIdx.x % PER);
+  };
+  auto load_packed = [&](auto layout, auto width, const Operand& o, int step, Codes& x) {
+    constexpr int L = decltype(layout)::value;
+    if constexpr (is_packed(L)) {
       typedef int i2v __attribute__((ext_vector_type(2)));
-      const i2v w = __builtin_amdgcn_raw_buffer_load_b64(rc, c < cols ? k * (int)p.bs + c : (int)NOWHERE, 0, 0);
-      codes[i] = __builtin_bit_cast(uint2, w);
-      bytes[i] = __builtin_amdgcn_raw_buffer_load_b8(rb, c < cols ? k * (int)p.ss + c / 128 : (int)NOWHERE, 0, 0);
+      const int left = tail - step * K::STEP;
+      const uint64_t lines = L == PACKED_ROWS ? (left > 0 ? o.limit : 0) : left > 0 ? left : 0;
+      // resources end with the last line that counts; a line's own end is a multiple of 128 columns
+      const uint64_t codes0 = L == PACKED_ROWS ? (uint64_t)step * 64 : (uint64_t)step * K::STEP * o.stride;
+      const uint64_t scales0 = L == PACKED_ROWS ? (uint64_t)step / 2 : (uint64_t)step * K::STEP * p.ss;
+      const uint64_t skip = L == PACKED_ROWS ? codes0 : n0, skip_s = L == PACKED_ROWS ? scales0 : n0 / 128;
+      const auto rc = tile_rsrc(o.base + codes0, lines ? lines * o.stride - skip : 0);
+      const auto rb = tile_rsrc(o.scales + scales0, lines ? lines * p.ss - skip_s : 0);
+      packed_pieces(layout, width, [&](int i, int line, int piece) {
+        const bool in = L == PACKED_ROWS ? line < o.limit : piece * 8 < o.limit;
+        const i2v w = __builtin_amdgcn_raw_buffer_load_b64(rc, in ? line * (int)o.stride + piece * 8 : (int)NOWHERE, 0, 0);
+        x.codes[i] = __builtin_bit_cast(uint2, w);
+        x.bytes[i] = __builtin_amdgcn_raw_buffer_load_b8(
+            rb, in ? line * (int)p.ss + (L == PACKED_ROWS ? 0 : piece / 16) : (int)NOWHERE, 0, 0);
+      });
     }
   };
-  auto store_packed = [&](uint32_t to) {
-    const int c = threadIdx.x % (TN / 8);
-#pragma unroll
-    for (int i = 0; i < PN; ++i) {
-      const int k = threadIdx.x / (TN / 8) + i * PR;
-      *reinterpret_cast<uint4*>(lds + to + k * (TN * 2) + ((c ^ cols_swizzle(k)) << 4)) =
-          decode_bf16(codes[i].x, codes[i].y, block8_scale(bytes[i]));
+  auto store_packed = [&](auto layout, auto width, const Operand& o, int step, const Codes& x) {
+    constexpr int L = decltype(layout)::value;
+    if constexpr (is_packed(L)) {
+      char* to = lds + (step & 1) * K::STAGE + o.place;
+      packed_pieces(layout, width, [&](int i, int line, int piece) {
+        const int at = L == PACKED_ROWS ? line * 128 + ((piece ^ (line & 7)) << 4)
+                                        : line * (decltype(width)::value * 2) + ((piece ^ cols_swizzle(line)) << 4);
+        *reinterpret_cast<uint4*>(to + at) = decode_bf16(x.codes[i].x, x.codes[i].y, block8_scale(x.bytes[i]));
+      });
     }
-  };
-  // Fp8: four blocks' scale bytes of every row of the tiles, one word a lane
-  auto scale_copies = [&](int step, int at) {  // part `at` of (TM + TN) / 64, the first TM / 64 A's
-    const uint32_t to = lds0 + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
-    const bool of_a = at < TM / 64;
-    const uint64_t row = of_a ? (uint64_t)m0 : (uint64_t)group * p.n + n0;
-    const int r = (of_a ? at : at - TM / 64) * 64 + lane, limit = of_a ? rows : cols;
-    const auto rs = tile_rsrc((of_a ? p.a_scales : p.b_scales) + row * p.ss + step,
-                              step < p.ss ? limit * p.ss - step : 0);
-    copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
-  };
-  auto fetch = [&](int step) {
-    const uint32_t to = (step & 1) * K::STAGE;
-    stage_copies(std::integral_constant<int, LA>{}, pa, TM, rows, as, std::integral_constant<int, CA>{}, row_a,
-                 lds0 + to, step);
-    if constexpr (LB != PACKED)
-      stage_copies(std::integral_constant<int, LB>{}, pb, TN, cols, bs, std::integral_constant<int, CB>{}, row_b,
-                   lds0 + to + K::A_BYTES, step);
-    if constexpr (K::FP8)
-      if ((step & 3) == 0 && step < steps) scale_copies(step, wave);
   };
 
   // Fragments. A lane holds row (lane & 15) of a 16-row tile and 8 summed
   // elements from 8 (lane >> 4) on, of every 32 (Fp8: 16 from 16 (lane >> 4)
   // on and 16 from 64 past those, of 128: any order does that A and B share,
-  // a block having one scale).
+  // a block having one scale). Tile i of wavefront row wm is tile i WM + wm of
+  // A's, so that a partial tile's rows are spread over all wavefronts; B's
+  // tiles of a wavefront are adjacent.
   const int r16 = lane & 15, q = lane >> 4;
-  auto rows_at = [&](int wtile, int half) {  // of tile 0 of this wavefront
-    return (uint32_t)((wtile * 16 + r16) * 128 + (((half * 4 + q) ^ (r16 & 7)) << 4));
+  auto rows_at = [&](int tile, int half) {
+    return (uint32_t)((tile * 16 + r16) * 128 + (((half * 4 + q) ^ (r16 & 7)) << 4));
   };
-  auto cols_at = [&](int wtile, int width) {
+  auto cols_at = [&](int tile, int width) {
     const int k = 8 * q + (r16 >> 2);
-    return (uint32_t)(k * (width * 2) + (((wtile << 1) ^ cols_swizzle(k)) << 4) + (r16 & 3) * 8);
-  };
-  [[maybe_unused]] const uint32_t rows_half0 = rows_at(0, 0), rows_half1 = rows_at(0, 1);
-  [[maybe_unused]] const uint32_t fa0 = LA == ROWS ? rows_at(wm * MT, 0) : cols_at(wm * MT, TM);
-  [[maybe_unused]] const uint32_t fb0 = LB == ROWS ? rows_at(wn * NT, 0) : cols_at(wn * NT, TN);
-  // tile j of the wavefront, summed elements 32 h to 32 h + 31 (16-bit types)
-  auto fragment = [&](auto layout, const char* base, uint32_t at, int j, int h, int width) -> uint4 {
-    constexpr int L = decltype(layout)::value;
-    if constexpr (L == ROWS) {
-      return *reinterpret_cast<const uint4*>(base + (at ^ (h << 6)) + j * 2048);
-    } else {
-      typedef short s4v __attribute__((ext_vector_type(4)));
-      typedef __attribute__((address_space(3))) s4v* lds_s4;
-      const char* b = base + (at ^ (j << 5)) + h * 64 * width;
-      const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)b);
-      const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(b + 8 * width));
-      const uint2 lo = __builtin_bit_cast(uint2, x), hi = __builtin_bit_cast(uint2, y);
-      return make_uint4(lo.x, lo.y, hi.x, hi.y);
-    }
+    return (uint32_t)(k * (width * 2) + (((tile << 1) ^ cols_swizzle(k)) << 4) + (r16 & 3) * 8);
   };
 
   f4v acc[MT][NT] = {};
-  if constexpr (!K::FP8) {
+  // LIVE of a wavefront's MT row tiles are inside the matrix.
+  [[maybe_unused]] auto run16 = [&](auto live) {
     // A step's fragments are two halves of 32 summed elements, each read while
     // the other is multiplied; between a step's halves its stage has been read
     // and the next one has landed, so the barrier there frees the one for the
     // step after next and opens the other.
+    constexpr int LIVE = decltype(live)::value;
+    const uint32_t fa0 = is_rows(LA) ? rows_at(wm, 0) : cols_at(wm, TM);
+    const uint32_t fb0 = is_rows(LB) ? rows_at(wn * NT, 0) : cols_at(wn * NT, TN);
+    // the tile j tiles on, summed elements 32 h to 32 h + 31
+    auto fragment = [&](auto layout, auto width, const char* base, uint32_t at, int j, int h) -> uint4 {
+      if constexpr (is_rows(decltype(layout)::value)) {
+        return *reinterpret_cast<const uint4*>(base + (at ^ (h << 6)) + j * 2048);
+      } else {
+        constexpr int W = decltype(width)::value;
+        typedef short s4v __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s4v* lds_s4;
+        const char* b = base + (at ^ (j << 5)) + h * 64 * W;
+        const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)b);
+        const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(b + 8 * W));
+        const uint2 lo = __builtin_bit_cast(uint2, x), hi = __builtin_bit_cast(uint2, y);
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+    };
     struct Half {
-      uint4 a[MT], b[NT];
+      uint4 a[LIVE], b[NT];
     };
     auto read = [&](Half& f, int step, int h) {
       const char* base = lds + (step & 1) * K::STAGE;
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        f.b[j] = fragment(std::integral_constant<int, LB>{}, base + K::A_BYTES, fb0, j, h, TN);
+      for (int j = 0; j < NT; ++j) f.b[j] = fragment(LayoutB{}, WidthB{}, base + K::A_BYTES, fb0, j, h);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) f.a[i] = fragment(std::integral_constant<int, LA>{}, base, fa0, i, h, TM);
+      for (int i = 0; i < LIVE; ++i) f.a[i] = fragment(LayoutA{}, WidthA{}, base, fa0, i * WM, h);
     };
     auto multiply = [&](const Half& f) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int i = 0; i < LIVE; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = mfma16<T>(f.b[j], f.a[i], acc[i][j]);
     };
     // one LDS read to every few matrix instructions
     auto interleave = [&] {
-      constexpr int READS = (LA == ROWS ? 1 : 2) * MT + (LB == ROWS ? 1 : 2) * NT, PER = MT * NT / READS;
+      constexpr int READS = (is_rows(LA) ? 1 : 2) * LIVE + (is_rows(LB) ? 1 : 2) * NT, PER = LIVE * NT / READS;
+      if constexpr (PER > 0) {
 #pragma unroll
-      for (int i = 0; i < READS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+        for (int i = 0; i < READS; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, LIVE * NT - READS * PER, 0);
       }
-      __builtin_amdgcn_sched_group_barrier(0x008, MT * NT - READS * PER, 0);
     };
-    auto next = [&](int step) {  // the copies of a step, and of PACKED its codes into registers
-      fetch(step);
-      if constexpr (LB == PACKED) load_packed(step);
+    Codes xa, xb;
+    auto next = [&](int step) {  // a step's copies, and its codes into registers
+      stage_copies(LayoutA{}, WidthA{}, A, step);
+      stage_copies(LayoutB{}, WidthB{}, B, step);
+      load_packed(LayoutA{}, WidthA{}, A, step, xa);
+      load_packed(LayoutB{}, WidthB{}, B, step, xb);
     };
     auto decode = [&](int step) {
-      if constexpr (LB == PACKED) store_packed((step & 1) * K::STAGE + K::A_BYTES);
+      store_packed(LayoutA{}, WidthA{}, A, step, xa);
+      store_packed(LayoutB{}, WidthB{}, B, step, xb);
     };
     auto landed = [&] {
       wait_copies();
       __syncthreads();
     };
-    if (steps > 0) {
-      Half even, odd;
-      next(0);
-      decode(0);
-      landed();
-      next(1);
-      read(even, 0, 0);
-      for (int step = 0; step < steps - 1; ++step) {
-        read(odd, step, 1);
-        multiply(even);
-        interleave();
-        decode(step + 1);
-        landed();
-        next(step + 2);
-        read(even, step + 1, 0);
-        multiply(odd);
-        interleave();
-      }
-      read(odd, steps - 1, 1);
+    Half even, odd;
+    next(0);
+    decode(0);
+    landed();
+    next(1);
+    read(even, 0, 0);
+    for (int step = 0; step < steps - 1; ++step) {
+      read(odd, step, 1);
       multiply(even);
       interleave();
+      decode(step + 1);
+      landed();
+      next(step + 2);
+      read(even, step + 1, 0);
       multiply(odd);
-      wait_copies();  // those of the step past the last
+      interleave();
     }
-  } else {
+    read(odd, steps - 1, 1);
+    multiply(even);
+    interleave();
+    multiply(odd);
+    wait_copies();  // those of the step past the last
+  };
+  [[maybe_unused]] auto run8 = [&](auto live) {
     // Wavefronts 0 to 3 and 4 to 7, one of each on every SIMD, take turns: one
     // half reads a step's fragments while the other multiplies, with a barrier
     // between the turns. The first half reads step s in turn 2 s and
-    // multiplies it in turn 2 s + 1, the second half is a turn behind. Step
-    // s's stage has then been read by the end of turn 2 s + 1, is filled for
-    // step s + 2 by copies issued in turn 2 s + 2, and has landed by the end of
-    // turn 2 s + 3.
-    static_assert(K::WAVES == 8, "two wavefronts on a SIMD");
+    // multiplies it in turn 2 s + 1, the second half is a turn behind and makes
+    // the copies, between its matrix instructions. Step s's stage has been
+    // read by the end of turn 2 s + 1, is filled for step s + 2 by copies
+    // issued in turn 2 s + 2, and has landed by the end of turn 2 s + 3.
+    constexpr int LIVE = decltype(live)::value;
+    static_assert(WAVES == 8 && TM == 32 * MT && TN == TM);
     struct Fragment {
       i8v v;
       int scale;
     };
+    Fragment fa[LIVE], fb[NT];
+    const uint32_t half0 = rows_at(0, 0), half1 = rows_at(0, 1);
     auto read = [&](const char* at, int step, int row) {
       Fragment f;
-      const uint4 x = *reinterpret_cast<const uint4*>(at + rows_half0);
-      const uint4 y = *reinterpret_cast<const uint4*>(at + rows_half1);
+      const uint4 x = *reinterpret_cast<const uint4*>(at + half0);
+      const uint4 y = *reinterpret_cast<const uint4*>(at + half1);
       f.v = i8v{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
       f.scale = (uint8_t)lds[2 * K::STAGE + ((step >> 2) & 1) * K::SCALES + (row + r16) * 4 + (step & 3)];
       return f;
     };
-    const bool second = wave >= 4;
-    Fragment fa[MT], fb[NT];
     auto read_step = [&](int step) {
       const char* base = lds + (step & 1) * K::STAGE;
 #pragma unroll
@@ -549,16 +585,17 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
         fb[j] = read(base + K::A_BYTES + row * 128, step, TM + row);
       }
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int row = (wm * MT + i) * 16;
+      for (int i = 0; i < LIVE; ++i) {
+        const int row = (i * WM + wm) * 16;
         fa[i] = read(base + row * 128, step, row);
       }
     };
     auto multiply_row = [&](int i) {
+      if (i < LIVE)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i].v, acc[i][j], 0, 0, 0,
-                                                                     fb[j].scale, 0, fa[i].scale);
+        for (int j = 0; j < NT; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j].v, fa[i].v, acc[i][j], 0, 0, 0,
+                                                                       fb[j].scale, 0, fa[i].scale);
     };
     auto turn = [&] {  // LDS reads have returned
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -566,72 +603,80 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
     };
-    // the second half's share of a step's copies: all of them, MT parts
-    const uint32_t row_off = (lane >> 3) * (uint32_t)p.as + (((lane & 7) ^ (lane >> 3)) << 4);
-    auto copy_part = [&](__amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int step, int i) {
-      uint32_t me = row_off;
-      asm volatile("" : "+v"(me));
-      const int at = (wave & 3) * MT + i;
-      const uint32_t to = lds0 + (step & 1) * K::STAGE + at * 1024;
-      static_assert(TM == 32 * MT && TN == TM);
-      copy16(ra, (uint32_t)(at * 8 * as) + me, to);
-      copy16(rb, (uint32_t)(at * 8 * as) + me, to + K::A_BYTES);
+    // four blocks' scale bytes of every row of the tiles, one word a lane:
+    // part `at` of (TM + TN) / 64, the first TM / 64 A's
+    auto scale_copies = [&](int step, int at) {
+      const uint32_t to = lds0 + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
+      const bool of_a = at < TM / 64;
+      const int r = (of_a ? at : at - TM / 64) * 64 + lane, limit = of_a ? rows : cols;
+      const auto rs = tile_rsrc((of_a ? A.scales : B.scales) + step, step < (int)p.ss ? limit * p.ss - step : 0);
+      copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
     };
-    if (steps > 0) {
-      fetch(0);
-      wait_copies();
+    stage_copies(LayoutA{}, WidthA{}, A, 0);
+    stage_copies(LayoutB{}, WidthB{}, B, 0);
+    scale_copies(0, wave);
+    wait_copies();
+    turn();
+    if (wave >= 4) {
+      auto part = [&](__amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int step, int i) {
+        stage_copy(LayoutA{}, WidthA{}, A, ra, step, (wave & 3) * MT + i);
+        stage_copy(LayoutB{}, WidthB{}, B, rb, step, (wave & 3) * MT + i);
+      };
+      {
+        const auto ra = stage_resource(LayoutA{}, A, 1), rb = stage_resource(LayoutB{}, B, 1);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) part(ra, rb, 1, i);
+      }
       turn();
-      if (second) {
-        auto copies_of = [&](const char* base, int limit, int step) {
-          return tile_rsrc(base + (uint64_t)step * 128, step < steps ? (limit - 1) * as + (tail - step * 128) : 0);
-        };
-        {
-          const auto ra = copies_of(pa, rows, 1), rb = copies_of(pb, cols, 1);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) copy_part(ra, rb, 1, i);
-        }
+      for (int step = 0; step < steps; ++step) {
+        read_step(step);
+        wait_copies();
         turn();
-        for (int step = 0; step < steps; ++step) {
-          read_step(step);
-          wait_copies();
-          turn();
-          const auto ra = copies_of(pa, rows, step + 2), rb = copies_of(pb, cols, step + 2);
-          if (((step + 2) & 3) == 0 && step + 2 < steps) {
-            scale_copies(step + 2, (wave & 3) * 2);
-            scale_copies(step + 2, (wave & 3) * 2 + 1);
-          }
-          __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            multiply_row(i);
-            __builtin_amdgcn_sched_barrier(0);
-            copy_part(ra, rb, step + 2, i);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          __builtin_amdgcn_s_setprio(0);
-          turn();
+        const auto ra = stage_resource(LayoutA{}, A, step + 2), rb = stage_resource(LayoutB{}, B, step + 2);
+        if (((step + 2) & 3) == 0) {
+          scale_copies(step + 2, (wave & 3) * 2);
+          scale_copies(step + 2, (wave & 3) * 2 + 1);
         }
-        wait_copies();  // those of the steps past the last
-      } else {
-        for (int step = 0; step < steps; ++step) {
-          read_step(step);
-          turn();
-          __builtin_amdgcn_s_setprio(1);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-          for (int i = 0; i < MT; ++i) multiply_row(i);
-          __builtin_amdgcn_s_setprio(0);
-          turn();
+        for (int i = 0; i < MT; ++i) {
+          multiply_row(i);
+          __builtin_amdgcn_sched_barrier(0);
+          part(ra, rb, step + 2, i);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         turn();
       }
+      wait_copies();  // those of the steps past the last
+    } else {
+      for (int step = 0; step < steps; ++step) {
+        read_step(step);
+        turn();
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) multiply_row(i);
+        __builtin_amdgcn_s_setprio(0);
+        turn();
+      }
+      turn();
     }
+  };
+  auto run = [&](auto live) {
+    if constexpr (K::FP8) run8(live);
+    else run16(live);
+  };
+  if (steps > 0) {
+    if (rows <= TM / 4) run(std::integral_constant<int, MT / 4>{});
+    else if (rows <= TM / 2) run(std::integral_constant<int, MT / 2>{});
+    else run(std::integral_constant<int, MT>{});
   }
 
   // a lane holds columns 4 q to 4 q + 3 of row r16 of each tile
   O* c = (O*)p.c + group * p.cg + (uint64_t)m0 * p.cs + n0;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int r = (wm * MT + i) * 16 + r16;
+    const int r = (i * WM + wm) * 16 + r16;
     if (r >= rows) continue;
     O* row = c + (uint64_t)r * p.cs;
 #pragma unroll
@@ -672,7 +717,7 @@ __global__ void __launch_bounds__(512) product_few(Product p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_n = (p.n + TN - 1) / TN;
   RowTile t;
-  if (!find_row_tile(p.offsets, p.groups, p.rows, 16 * MT, (int)(blockIdx.x / tiles_n), t)) return;
+  if (!find_row_tile<ALL_TILES>(p.offsets, p.groups, p.rows, 16 * MT, (int)(blockIdx.x / tiles_n), t)) return;
   const int n0 = (int)(blockIdx.x % tiles_n) * TN;
   const int rows = t.end - t.row < 16 * MT ? t.end - t.row : 16 * MT, cols = p.n - n0 < TN ? p.n - n0 : TN;
   const int k_end = t.group < 0 ? 0 : p.k, group = t.group < 0 ? 0 : t.group;
@@ -834,7 +879,7 @@ void launch_tiled(const Product& p, hipStream_t s) {
   const uint64_t tn = (p.n + K::TN - 1) / K::TN;
   uint64_t tiles;
   if (FORM == GRAD_WEIGHT) tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * p.groups;
-  else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn + 7) / 8 * 8;
+  else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn / 8 + 2) * 8;  // both kinds' eighths
   hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), dim3(grid_size(tiles)), dim3(K::THREADS), 0, s,
                      p);
   PXG_HIP(hipGetLastError());
@@ -859,27 +904,31 @@ template <int FORM, class T, class O, bool IS_PACKED>
 void launch_product(Product p, hipStream_t s) {
   p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % (4 * sizeof(O)) == 0;
   constexpr int LA = FORM == GRAD_WEIGHT ? COLS : ROWS;
-  constexpr int LB = FORM == FORWARD ? ROWS : FORM == GRAD_INPUT ? COLS : IS_PACKED ? PACKED : COLS;
+  constexpr int LB = FORM == FORWARD ? ROWS : FORM == GRAD_INPUT ? COLS : IS_PACKED ? PACKED_COLS : COLS;
   constexpr int bytes = FORM == FORWARD && IS_PACKED ? 1 : 2;
   const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
-  if (!copies(bytes, p.a, acols, p.as, 0) || (LB != PACKED && !copies(bytes, p.b, bcols, p.bs, p.bg)))
+  if (!copies(bytes, p.a, acols, p.as, 0) || (!is_packed(LB) && !copies(bytes, p.b, bcols, p.bs, p.bg)))
     return launch_any<FORM, T, O, IS_PACKED>(p, s);
   const uint64_t each = ((uint64_t)p.rows + p.groups - 1) / p.groups;  // rows of a group, on average
   if constexpr (FORM != GRAD_WEIGHT) {
     // COLS spans a matrix' rows with one resource
-    if (LB == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF) {
-      if (each <= 16) return launch_few<T, O, LB, IS_PACKED, 1>(p, s);
-      if (each <= 32) return launch_few<T, O, LB, IS_PACKED, 2>(p, s);
-      if constexpr (LB == ROWS)
-        if (each <= 64) return launch_few<T, O, LB, IS_PACKED, 4>(p, s);
-    }
+    if (each <= 16 && (LB == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF)) return launch_few<T, O, LB, IS_PACKED, 1>(p, s);
   }
   if constexpr (FORM == FORWARD && IS_PACKED) {
     if constexpr (!std::is_same_v<O, float>)
-      if (each >= 256) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
-    return launch_any<FORM, T, O, IS_PACKED>(p, s);
+      if (each >= 192) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
+    launch_tiled<T, O, FORM, PACKED_ROWS, PACKED_ROWS, 2, 2, 4, 4>(p, s);
   } else {
-    launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+    // 256 x 256 tiles take about 1.75 us for 64 summed elements, one on a CU;
+    // 128 x 128 tiles 1.17 us, two on a CU. Groups end inside a tile.
+    auto rounds = [&](uint64_t tile, uint64_t slots) {
+      const uint64_t tn = (p.n + tile - 1) / tile;
+      const uint64_t tiles = FORM == GRAD_WEIGHT ? p.groups * ((p.m + tile - 1) / tile) * tn
+                                                 : (p.rows + p.groups * tile / 2 + tile - 1) / tile * tn;
+      return (double)((tiles + slots - 1) / slots);
+    };
+    if (rounds(256, 256) * 1.75 <= rounds(128, 512) * 1.17) launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+    else launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
   }
 }
 

@@ -59,14 +59,24 @@ struct RowTile {
   int group, row, end;
 };
 
-// Tile `index` of the tiles of `size` rows that the groups, and the rows of
-// none at either end, are cut into; false past the last. `offsets` NULL is
-// one group of all rows. A wavefront's lanes all call it and get the same.
+// The tiles of `size` rows that the groups, and the rows of none at either
+// end, are cut into: all of them in order, only the whole ones, or only the
+// last, partial ones of each.
+enum RowTileKind { ALL_TILES, WHOLE_TILES, PARTIAL_TILES };
+
+template <int KIND>
+__device__ __forceinline__ int row_tiles_of(int rows, int size) {
+  return KIND == ALL_TILES ? (rows + size - 1) / size : KIND == WHOLE_TILES ? rows / size : rows % size ? 1 : 0;
+}
+
+// Tile `index` of its kind; false past the last. `offsets` NULL is one group
+// of all rows. A wavefront's lanes all call it and get the same.
+template <int KIND>
 __device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offsets, int groups, int rows, int size,
                                               int index, RowTile& t) {
   if (!offsets) {
-    t = {0, index * size, rows};
-    return (int64_t)index * size < rows;
+    t = {0, (KIND == PARTIAL_TILES ? rows / size + index : index) * size, rows};
+    return index < row_tiles_of<KIND>(rows, size);
   }
   const int lane = threadIdx.x & (WAVE - 1);
   int begin = 0, before = 0;  // rows and tiles before the segments of this round
@@ -77,7 +87,7 @@ __device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offset
     end = wave_max_scan(end > begin ? end : begin, lane);
     int first = __shfl_up(end, 1, WAVE);
     if (lane == 0) first = begin;
-    const int tiles = (end - first + size - 1) / size;
+    const int tiles = row_tiles_of<KIND>(end - first, size);
     const int last = before + wave_sum_scan(tiles, lane);
     const uint64_t hit = __ballot(index < last);
     if (hit) {
@@ -85,8 +95,8 @@ __device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offset
       const int f = __builtin_amdgcn_readlane(first, l), n = __builtin_amdgcn_readlane(tiles, l);
       const int k = index - (__builtin_amdgcn_readlane(last, l) - n);
       t.group = s0 + l == 0 || s0 + l > groups ? -1 : s0 + l - 1;
-      t.row = f + k * size;
       t.end = __builtin_amdgcn_readlane(end, l);
+      t.row = KIND == PARTIAL_TILES ? f + (t.end - f) / size * size : f + k * size;
       return true;
     }
     begin = __builtin_amdgcn_readlane(end, WAVE - 1);
@@ -95,22 +105,47 @@ __device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offset
   return false;
 }
 
-// How many tiles find_row_tile has.
-__device__ __forceinline__ int count_row_tiles(const int64_t* __restrict__ offsets, int groups, int rows, int size) {
-  if (!offsets) return (rows + size - 1) / size;
+// How many whole and partial tiles there are.
+__device__ __forceinline__ void count_row_tiles(const int64_t* __restrict__ offsets, int groups, int rows, int size,
+                                                int& whole, int& partial) {
+  if (!offsets) {
+    whole = row_tiles_of<WHOLE_TILES>(rows, size);
+    partial = row_tiles_of<PARTIAL_TILES>(rows, size);
+    return;
+  }
   const int lane = threadIdx.x & (WAVE - 1);
-  int begin = 0, total = 0;
+  int begin = 0;
+  whole = partial = 0;
   for (int s0 = 0; s0 < groups + 2; s0 += WAVE) {
     const int s = s0 + lane;
     int end = s <= groups ? clamp_offset(offsets[s], rows) : rows;
     end = wave_max_scan(end > begin ? end : begin, lane);
     int first = __shfl_up(end, 1, WAVE);
     if (lane == 0) first = begin;
-    const int sum = wave_sum_scan((end - first + size - 1) / size, lane);
-    total += __builtin_amdgcn_readlane(sum, WAVE - 1);
+    partial += __popcll(__ballot(row_tiles_of<PARTIAL_TILES>(end - first, size)));
+    whole += __builtin_amdgcn_readlane(wave_sum_scan(row_tiles_of<WHOLE_TILES>(end - first, size), lane), WAVE - 1);
     begin = __builtin_amdgcn_readlane(end, WAVE - 1);
   }
-  return total;
+}
+
+// Which group a place in the order of falling sizes belongs to (ties by
+// index), by a wavefront whose lanes all call it; above 64 groups the order
+// is the groups' own.
+__device__ __forceinline__ int group_by_size(const int64_t* __restrict__ offsets, int groups, int rows, int place) {
+  if (groups > WAVE) return place;
+  const int lane = threadIdx.x & (WAVE - 1);
+  int end = lane < groups ? clamp_offset(offsets[lane + 1], rows) : rows;
+  int begin = clamp_offset(offsets[0], rows);
+  end = wave_max_scan(end > begin ? end : begin, lane);
+  int first = __shfl_up(end, 1, WAVE);
+  if (lane == 0) first = begin;
+  const int size = lane < groups ? end - first : -1;
+  int rank = 0;
+  for (int g = 0; g < groups; ++g) {
+    const int o = __builtin_amdgcn_readlane(size, g);
+    rank += o > size || (o == size && g < lane) ? 1 : 0;
+  }
+  return __builtin_ctzll(__ballot(lane < groups && rank == place));
 }
 
 // No more tiles than this come out of `rows` rows in `groups` groups, the

@@ -53,139 +53,6 @@ __device__ __forceinline__ f4v mfma16(uint4 a, uint4 b, f4v c) {
 }
 
 // ---------------------------------------------------------------------------
-// Any stride and alignment: 64 x 64 tiles, 32 summed at a time, staged in LDS
-// element by element with zeros outside the operands.
-// ---------------------------------------------------------------------------
-constexpr int ANY_TILE = 64, ANY_K = 32;
-constexpr int ANY_LD = ANY_K + 8;  // LDS rows of 80 bytes: 16-byte aligned, and 8 rows meet every bank
-
-// 64 rows of an operand whose summed index runs along its rows: row r, then
-// elements k0 .. k0 + 31 of it.
-template <class T>
-__device__ __forceinline__ void any_stage_rows(T* lds, const T* __restrict__ p, uint64_t stride, int rows, int k0,
-                                               int k) {
-  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
-  T v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = r < rows && k0 + c + i < k ? p[(uint64_t)r * stride + (k0 + c + i)] : (T)0.0f;
-  *reinterpret_cast<uint4*>(&lds[r * ANY_LD + c]) = *reinterpret_cast<uint4*>(v);
-}
-// The same of one whose summed index runs across its rows.
-template <class T>
-__device__ __forceinline__ void any_stage_cols(T* lds, const T* __restrict__ p, uint64_t stride, int cols, int k0,
-                                               int k) {
-  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    lds[(c + i) * ANY_LD + r] = k0 + r < k && c + i < cols ? p[(uint64_t)(k0 + r) * stride + (c + i)] : (T)0.0f;
-}
-
-// Rows, and columns, of packed operands: codes times scales, exact in bf16.
-__device__ __forceinline__ void any_stage_packed_rows(__bf16* lds, const uint8_t* __restrict__ codes,
-                                                      const uint8_t* __restrict__ scales, uint64_t stride,
-                                                      uint64_t sstride, int rows, int k0) {
-  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 8;
-  float v[8] = {};
-  if (r < rows) {  // k0 + c is inside the codes' row, whose columns are a multiple of 128
-    const uint2 w = *reinterpret_cast<const uint2*>(codes + (uint64_t)r * stride + k0 + c);
-    const uint32_t code[2] = {w.x, w.y};
-    block8_decode(code, block8_scale(scales[(uint64_t)r * sstride + k0 / 128]), v);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) lds[r * ANY_LD + c + i] = (__bf16)v[i];
-}
-__device__ __forceinline__ void any_stage_packed_cols(__bf16* lds, const uint8_t* __restrict__ codes,
-                                                 const uint8_t* __restrict__ scales, uint64_t stride, uint64_t sstride,
-                                                 int n0, int cols, int k0, int k) {
-  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 8;
-  float v[8] = {};
-  if (k0 + r < k && c < cols) {  // whole columns past `cols` stay zero, and codes past a row's columns are
-    const uint2 w = *reinterpret_cast<const uint2*>(codes + (uint64_t)(k0 + r) * stride + n0 + c);
-    const uint32_t code[2] = {w.x, w.y};
-    block8_decode(code, block8_scale(scales[(uint64_t)(k0 + r) * sstride + n0 / 128]), v);
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) lds[(c + i) * ANY_LD + r] = (__bf16)v[i];
-}
-
-template <class T, class O, int FORM, bool PACKED>
-__global__ void __launch_bounds__(256) product_any(Product p) {
-  __shared__ __align__(16) T as[ANY_TILE * ANY_LD], bs[ANY_TILE * ANY_LD];
-  const int tiles_n = (p.n + ANY_TILE - 1) / ANY_TILE;
-  const int n0 = (int)(blockIdx.x % tiles_n) * ANY_TILE;
-  int index = (int)(blockIdx.x / tiles_n);
-  int m0, m_end, k_end, group;
-  [[maybe_unused]] uint64_t lo = 0;  // B's first row (grad weight, packed)
-  const T *a, *b;
-  O* c;
-  if constexpr (FORM == GRAD_WEIGHT) {
-    const int tiles_m = (p.m + ANY_TILE - 1) / ANY_TILE;
-    group = index / tiles_m;
-    m0 = (index - group * tiles_m) * ANY_TILE;
-    m_end = p.m;
-    int first, end;
-    group_range(p.offsets, group, p.rows, first, end);
-    lo = first;
-    k_end = end - first;
-    a = (const T*)p.a + lo * p.as + m0;
-    b = (const T*)p.b + lo * p.bs + n0;
-    c = (O*)p.c + group * p.cg;
-  } else {
-    RowTile t;
-    if (!find_row_tile<ALL_TILES>(p.offsets, p.groups, p.rows, ANY_TILE, index, t)) return;
-    m0 = t.row;
-    m_end = t.end;
-    k_end = t.group < 0 ? 0 : p.k;
-    group = t.group < 0 ? 0 : t.group;
-    lo = (uint64_t)group * p.n + n0;
-    a = (const T*)p.a + (uint64_t)m0 * p.as;
-    b = (const T*)p.b + group * p.bg + (FORM == FORWARD ? (uint64_t)n0 * p.bs : (uint64_t)n0);
-    c = (O*)p.c;
-  }
-  const int rows = m_end - m0 < ANY_TILE ? m_end - m0 : ANY_TILE;
-  const int cols = p.n - n0 < ANY_TILE ? p.n - n0 : ANY_TILE;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-  f4v acc[2][2] = {};
-  for (int k0 = 0; k0 < k_end; k0 += ANY_K) {
-    __syncthreads();
-    if constexpr (FORM == GRAD_WEIGHT) any_stage_cols(as, a, p.as, rows, k0, k_end);
-    else if constexpr (PACKED)
-      any_stage_packed_rows(as, (const uint8_t*)p.a + (uint64_t)m0 * p.as, p.a_scales + (uint64_t)m0 * p.ss, p.as, p.ss, rows, k0);
-    else any_stage_rows(as, a, p.as, rows, k0, k_end);
-    if constexpr (FORM == GRAD_WEIGHT && PACKED)
-      any_stage_packed_cols(bs, (const uint8_t*)p.b + lo * p.bs, p.b_scales + lo * p.ss, p.bs, p.ss, n0, cols, k0,
-                            k_end);
-    else if constexpr (PACKED)
-      any_stage_packed_rows(bs, (const uint8_t*)p.b + lo * p.bs, p.b_scales + lo * p.ss, p.bs, p.ss, cols, k0);
-    else if constexpr (FORM == FORWARD) any_stage_rows(bs, b, p.bs, cols, k0, k_end);
-    else any_stage_cols(bs, b, p.bs, cols, k0, k_end);
-    __syncthreads();
-    uint4 fa[2], fb[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      fa[i] = *reinterpret_cast<const uint4*>(&as[(wm + 16 * i + (lane & 15)) * ANY_LD + (lane >> 4) * 8]);
-      fb[i] = *reinterpret_cast<const uint4*>(&bs[(wn + 16 * i + (lane & 15)) * ANY_LD + (lane >> 4) * 8]);
-    }
-    // B first: a lane then holds four adjacent columns of one row of C
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<T>(fb[j], fa[i], acc[i][j]);
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = wm + 16 * i + (lane & 15), q = wn + 16 * j + (lane >> 4) * 4;
-      if (r >= rows) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (q + e < cols) c[(uint64_t)(m0 + r) * p.cs + (n0 + q + e)] = (O)acc[i][j][e];
-    }
-}
-
-// ---------------------------------------------------------------------------
 // The tiled product: operands go to LDS by direct copies, 128 bytes of each
 // row (or 64 rows, where the summed index runs across them) at a time, into
 // one of two stages while the other is multiplied.
@@ -196,9 +63,13 @@ __global__ void __launch_bounds__(256) product_any(Product p) {
 //           transposing reads
 //   PACKED_ROWS, PACKED_COLS  the same of packed rows; codes are decoded on
 //           their way to LDS
-enum Layout { ROWS, COLS, PACKED_ROWS, PACKED_COLS };
+//   ANY_ROWS, ANY_COLS  the same of rows that are not whole 16-byte pieces;
+//           they are shifted into place on their way to LDS
+enum Layout { ROWS, COLS, PACKED_ROWS, PACKED_COLS, ANY_ROWS, ANY_COLS };
 constexpr bool is_packed(int l) { return l == PACKED_ROWS || l == PACKED_COLS; }
-constexpr bool is_rows(int l) { return l == ROWS || l == PACKED_ROWS; }
+constexpr bool is_any(int l) { return l == ANY_ROWS || l == ANY_COLS; }
+constexpr bool is_rows(int l) { return l == ROWS || l == PACKED_ROWS || l == ANY_ROWS; }
+constexpr bool is_copied(int l) { return l == ROWS || l == COLS; }
 
 struct Fp8 {};  // packed operands multiplied as they are
 
@@ -248,8 +119,12 @@ __device__ __forceinline__ uint4 decode_bf16(uint32_t x, uint32_t y, float s) {
 }
 
 // By how many 16-byte pieces row k of a stage is moved: a transposing read
-// takes 32 bytes of rows 8 q + {0..3} (or {4..7}) for each 16 lanes q.
-__device__ __forceinline__ int cols_swizzle(int k) { return ((k & 3) | ((k >> 1) & 4)) << 1; }
+// takes 32 bytes of rows 8 q + {0..3} (or {4..7}) for each 16 lanes q. Rows of
+// 64 elements have four such pieces only.
+template <int WIDTH>
+__device__ __forceinline__ int cols_swizzle(int k) {
+  return (WIDTH == 64 ? k & 3 : (k & 3) | ((k >> 1) & 4)) << 1;
+}
 
 // Part `die` of n cut into eight, the larger parts first: its first and size.
 __device__ __forceinline__ void eighth(int n, int die, int& first, int& size) {
@@ -384,7 +259,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       constexpr int PER = decltype(width)::value / 8;  // pieces in a row
       int me = lane;
       if constexpr (is_packed(LB)) asm volatile("" : "+v"(me));  // registers are short there
-      const int k = part * (64 / PER) + me / PER, c = (me % PER) ^ cols_swizzle(k);
+      const int k = part * (64 / PER) + me / PER, c = (me % PER) ^ cols_swizzle<decltype(width)::value>(k);
       copy16(rs, c * 8 < o.limit ? (uint32_t)(k * (int)o.stride) + c * 16 : NOWHERE, to);
     }
   };
@@ -393,7 +268,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   using WidthA = std::integral_constant<int, TM>;
   using WidthB = std::integral_constant<int, TN>;
   auto stage_copies = [&](auto layout, auto width, const Operand& o, int step) {
-    if constexpr (!is_packed(decltype(layout)::value)) {
+    if constexpr (is_copied(decltype(layout)::value)) {
       constexpr int N = decltype(width)::value / 8 / WAVES;
       const auto rs = stage_resource(layout, o, step);
 #pragma unroll
@@ -401,24 +276,32 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     }
   };
   // Packed: a thread takes 8 codes at a time, of row (COLS: summed element)
-  // `line` from `piece` eights on, reads them a step ahead and decodes them.
-  struct Codes {
-    uint2 codes[8];
-    uint32_t bytes[8];
+  // `line`, piece `c` of 8, reads them a step ahead and decodes them.
+  // ANY: the same with 16 elements. Rows begin at any multiple of two bytes,
+  // so the nine words that the elements touch are read and shifted. A word
+  // that the row shares with a neighbour is read whole; elements of other rows
+  // are set to zero.
+  struct Staged {
+    uint4 lo[4], hi[2];
+    uint32_t last[4];  // ANY: the ninth word; packed: the scale byte
   };
-  auto packed_pieces = [&](auto layout, auto width, auto f) {
-    constexpr int W = decltype(width)::value;
-    constexpr int PER = decltype(layout)::value == PACKED_ROWS ? 8 : W / 8;  // pieces in a line
-    constexpr int N = W * 8 / K::THREADS;
-    static_assert(N <= 8);
+  auto pieces = [&](auto layout, auto width, auto f) {
+    constexpr int L = decltype(layout)::value, W = decltype(width)::value, SIZE = is_any(L) ? 16 : 8;
+    constexpr int PER = (is_rows(L) ? K::STEP : W) / SIZE;  // pieces in a line
+    constexpr int N = W * K::STEP / SIZE / K::THREADS;
+    static_assert(N <= (is_any(L) ? 2 : 4));
 #pragma unroll
     for (int i = 0; i < N; ++i) f(i, (int)threadIdx.x / PER + i * (K::THREADS / PER), (int)threadIdx.x % PER);
   };
-  auto load_packed = [&](auto layout, auto width, const Operand& o, int step, Codes& x) {
+  auto load_staged = [&](auto layout, auto width, const Operand& o, int step, Staged& x) {
     constexpr int L = decltype(layout)::value;
+    const int left = tail - step * K::STEP;
+    [[maybe_unused]] auto load = [](__amdgpu_buffer_rsrc_t rs, uint32_t at) {
+      typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+      return __builtin_bit_cast(uint4, (u4v)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)at, 0, 0));
+    };
     if constexpr (is_packed(L)) {
       typedef int i2v __attribute__((ext_vector_type(2)));
-      const int left = tail - step * K::STEP;
       const uint64_t lines = L == PACKED_ROWS ? (left > 0 ? o.limit : 0) : left > 0 ? left : 0;
       // resources end with the last line that counts; a line's own end is a multiple of 128 columns
       const uint64_t codes0 = L == PACKED_ROWS ? (uint64_t)step * 64 : (uint64_t)step * K::STEP * o.stride;
@@ -426,23 +309,57 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       const uint64_t skip = L == PACKED_ROWS ? codes0 : n0, skip_s = L == PACKED_ROWS ? scales0 : n0 / 128;
       const auto rc = tile_rsrc(o.base + codes0, lines ? lines * o.stride - skip : 0);
       const auto rb = tile_rsrc(o.scales + scales0, lines ? lines * p.ss - skip_s : 0);
-      packed_pieces(layout, width, [&](int i, int line, int piece) {
-        const bool in = L == PACKED_ROWS ? line < o.limit : piece * 8 < o.limit;
-        const i2v w = __builtin_amdgcn_raw_buffer_load_b64(rc, in ? line * (int)o.stride + piece * 8 : (int)NOWHERE, 0, 0);
-        x.codes[i] = __builtin_bit_cast(uint2, w);
-        x.bytes[i] = __builtin_amdgcn_raw_buffer_load_b8(
-            rb, in ? line * (int)p.ss + (L == PACKED_ROWS ? 0 : piece / 16) : (int)NOWHERE, 0, 0);
+      // of a block, the columns before the tile's first
+      const int before = L == PACKED_ROWS ? 0 : n0 % 128;
+      pieces(layout, width, [&](int i, int line, int c) {
+        const bool in = L == PACKED_ROWS ? line < o.limit : c * 8 < o.limit;
+        const i2v w = __builtin_amdgcn_raw_buffer_load_b64(rc, in ? line * (int)o.stride + c * 8 : (int)NOWHERE, 0, 0);
+        x.lo[i].x = w[0];
+        x.lo[i].y = w[1];
+        x.last[i] = __builtin_amdgcn_raw_buffer_load_b8(
+            rb, in ? line * (int)p.ss + (L == PACKED_ROWS ? 0 : (before + c * 8) / 128) : (int)NOWHERE, 0, 0);
+      });
+    } else if constexpr (is_any(L)) {
+      const int odd = (int)((uintptr_t)o.base & 2);
+      const uint64_t end = L == ANY_ROWS ? (o.limit - 1) * o.stride + (uint64_t)left * 2
+                                         : (uint64_t)(left - 1) * o.stride + o.limit * 2;
+      const auto rs = tile_rsrc(o.base - odd + (L == ANY_ROWS ? (uint64_t)step * 128 : (uint64_t)step * K::STEP * o.stride),
+                                left > 0 ? (end + odd + 3) & ~3ull : 0);
+      pieces(layout, width, [&](int i, int line, int c) {
+        const bool in = L == ANY_ROWS ? line < o.limit && c * 16 < left : line < left && c * 16 < o.limit;
+        const uint32_t at = in ? (odd + line * (uint32_t)o.stride + c * 32) & ~3u : NOWHERE;
+        x.lo[i] = load(rs, at);
+        x.hi[i] = load(rs, in ? at + 16 : NOWHERE);
+        x.last[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, in ? (int)at + 32 : (int)NOWHERE, 0, 0);
       });
     }
   };
-  auto store_packed = [&](auto layout, auto width, const Operand& o, int step, const Codes& x) {
-    constexpr int L = decltype(layout)::value;
+  auto store_staged = [&](auto layout, auto width, const Operand& o, int step, const Staged& x) {
+    constexpr int L = decltype(layout)::value, W = decltype(width)::value;
+    char* to = lds + (step & 1) * K::STAGE + o.place;
+    auto place = [&](int line, int c) {
+      return reinterpret_cast<uint4*>(
+          to + (is_rows(L) ? line * 128 + ((c ^ (line & 7)) << 4) : line * (W * 2) + ((c ^ cols_swizzle<W>(line)) << 4)));
+    };
     if constexpr (is_packed(L)) {
-      char* to = lds + (step & 1) * K::STAGE + o.place;
-      packed_pieces(layout, width, [&](int i, int line, int piece) {
-        const int at = L == PACKED_ROWS ? line * 128 + ((piece ^ (line & 7)) << 4)
-                                        : line * (decltype(width)::value * 2) + ((piece ^ cols_swizzle(line)) << 4);
-        *reinterpret_cast<uint4*>(to + at) = decode_bf16(x.codes[i].x, x.codes[i].y, block8_scale(x.bytes[i]));
+      pieces(layout, width, [&](int i, int line, int c) {
+        *place(line, c) = decode_bf16(x.lo[i].x, x.lo[i].y, block8_scale(x.last[i]));
+      });
+    } else if constexpr (is_any(L)) {
+      const int left = tail - step * K::STEP;
+      pieces(layout, width, [&](int i, int line, int c) {
+        const uint32_t shift = (((uint32_t)(uintptr_t)o.base + line * (uint32_t)o.stride) & 2) * 8;
+        const int valid = (L == ANY_ROWS ? left : o.limit) - c * 16;
+        const uint32_t w[9] = {x.lo[i].x, x.lo[i].y, x.lo[i].z, x.lo[i].w, x.hi[i].x,
+                               x.hi[i].y, x.hi[i].z, x.hi[i].w, x.last[i]};
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t both = __builtin_amdgcn_alignbit(w[e + 1], w[e], shift);
+          v[e] = valid > 2 * e + 1 ? both : valid > 2 * e ? both & 0xFFFF : 0;
+        }
+        *place(line, 2 * c) = make_uint4(v[0], v[1], v[2], v[3]);
+        *place(line, 2 * c + 1) = make_uint4(v[4], v[5], v[6], v[7]);
       });
     }
   };
@@ -457,9 +374,10 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   auto rows_at = [&](int tile, int half) {
     return (uint32_t)((tile * 16 + r16) * 128 + (((half * 4 + q) ^ (r16 & 7)) << 4));
   };
-  auto cols_at = [&](int tile, int width) {
+  auto cols_at = [&](int tile, auto width) {
+    constexpr int W = decltype(width)::value;
     const int k = 8 * q + (r16 >> 2);
-    return (uint32_t)(k * (width * 2) + (((tile << 1) ^ cols_swizzle(k)) << 4) + (r16 & 3) * 8);
+    return (uint32_t)(k * (W * 2) + (((tile << 1) ^ cols_swizzle<W>(k)) << 4) + (r16 & 3) * 8);
   };
 
   f4v acc[MT][NT] = {};
@@ -470,8 +388,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     // and the next one has landed, so the barrier there frees the one for the
     // step after next and opens the other.
     constexpr int LIVE = decltype(live)::value;
-    const uint32_t fa0 = is_rows(LA) ? rows_at(wm, 0) : cols_at(wm, TM);
-    const uint32_t fb0 = is_rows(LB) ? rows_at(wn * NT, 0) : cols_at(wn * NT, TN);
+    const uint32_t fa0 = is_rows(LA) ? rows_at(wm, 0) : cols_at(wm, WidthA{});
+    const uint32_t fb0 = is_rows(LB) ? rows_at(wn * NT, 0) : cols_at(wn * NT, WidthB{});
     // the tile j tiles on, summed elements 32 h to 32 h + 31
     auto fragment = [&](auto layout, auto width, const char* base, uint32_t at, int j, int h) -> uint4 {
       if constexpr (is_rows(decltype(layout)::value)) {
@@ -515,16 +433,16 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
         __builtin_amdgcn_sched_group_barrier(0x008, LIVE * NT - READS * PER, 0);
       }
     };
-    Codes xa, xb;
-    auto next = [&](int step) {  // a step's copies, and its codes into registers
+    Staged xa, xb;
+    auto next = [&](int step) {  // a step's copies, and what goes through registers
       stage_copies(LayoutA{}, WidthA{}, A, step);
       stage_copies(LayoutB{}, WidthB{}, B, step);
-      load_packed(LayoutA{}, WidthA{}, A, step, xa);
-      load_packed(LayoutB{}, WidthB{}, B, step, xb);
+      load_staged(LayoutA{}, WidthA{}, A, step, xa);
+      load_staged(LayoutB{}, WidthB{}, B, step, xb);
     };
-    auto decode = [&](int step) {
-      store_packed(LayoutA{}, WidthA{}, A, step, xa);
-      store_packed(LayoutB{}, WidthB{}, B, step, xb);
+    auto stage = [&](int step) {
+      store_staged(LayoutA{}, WidthA{}, A, step, xa);
+      store_staged(LayoutB{}, WidthB{}, B, step, xb);
     };
     auto landed = [&] {
       wait_copies();
@@ -532,7 +450,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     };
     Half even, odd;
     next(0);
-    decode(0);
+    stage(0);
     landed();
     next(1);
     read(even, 0, 0);
@@ -540,7 +458,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       read(odd, step, 1);
       multiply(even);
       interleave();
-      decode(step + 1);
+      stage(step + 1);
       landed();
       next(step + 2);
       read(even, step + 1, 0);
@@ -667,7 +585,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     else run16(live);
   };
   if (steps > 0) {
-    if (rows <= TM / 4) run(std::integral_constant<int, MT / 4>{});
+    if (MT >= 4 && rows <= TM / 4) run(std::integral_constant<int, (MT + 3) / 4>{});
     else if (rows <= TM / 2) run(std::integral_constant<int, MT / 2>{});
     else run(std::integral_constant<int, MT>{});
   }
@@ -864,15 +782,6 @@ void check_out_type(int type, int out_type) {
     config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
 }
 
-template <int FORM, class T, class O, bool PACKED>
-void launch_any(const Product& p, hipStream_t s) {
-  const uint64_t tm = FORM == GRAD_WEIGHT ? (uint64_t)p.groups * ((p.m + ANY_TILE - 1) / ANY_TILE)
-                                          : row_tiles_max(p.rows, p.groups, ANY_TILE, p.offsets != nullptr);
-  const uint64_t tn = (p.n + ANY_TILE - 1) / ANY_TILE;
-  hipLaunchKernelGGL((product_any<T, O, FORM, PACKED>), dim3(grid_size(tm * tn)), dim3(256), 0, s, p);
-  PXG_HIP(hipGetLastError());
-}
-
 template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
 void launch_tiled(const Product& p, hipStream_t s) {
   using K = Tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>;
@@ -885,11 +794,9 @@ void launch_tiled(const Product& p, hipStream_t s) {
   PXG_HIP(hipGetLastError());
 }
 
-// Whether the tiled product can copy an operand: 16-byte pieces that all
-// belong to one row, and a tile's offsets in 31 bits.
+// Whether an operand can be copied: 16-byte pieces that all belong to one row.
 bool copies(int bytes, const void* d, uint64_t cols, uint64_t stride, uint64_t group_stride) {
-  return ((uint64_t)(uintptr_t)d | cols * bytes | stride * bytes | group_stride * bytes) % 16 == 0 &&
-         stride * bytes <= (1u << 22);
+  return ((uint64_t)(uintptr_t)d | cols * bytes | stride * bytes | group_stride * bytes) % 16 == 0;
 }
 
 template <class T, class O, int LB, bool IS_PACKED, int MT>
@@ -903,32 +810,39 @@ void launch_few(const Product& p, hipStream_t s) {
 template <int FORM, class T, class O, bool IS_PACKED>
 void launch_product(Product p, hipStream_t s) {
   p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % (4 * sizeof(O)) == 0;
-  constexpr int LA = FORM == GRAD_WEIGHT ? COLS : ROWS;
-  constexpr int LB = FORM == FORWARD ? ROWS : FORM == GRAD_INPUT ? COLS : IS_PACKED ? PACKED_COLS : COLS;
-  constexpr int bytes = FORM == FORWARD && IS_PACKED ? 1 : 2;
+  constexpr int LA = FORM == GRAD_WEIGHT ? COLS : FORM == FORWARD && IS_PACKED ? PACKED_ROWS : ROWS;
+  constexpr int LB = FORM == GRAD_INPUT ? COLS : FORM == GRAD_WEIGHT ? (IS_PACKED ? PACKED_COLS : COLS) : LA;
   const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
-  if (!copies(bytes, p.a, acols, p.as, 0) || (!is_packed(LB) && !copies(bytes, p.b, bcols, p.bs, p.bg)))
-    return launch_any<FORM, T, O, IS_PACKED>(p, s);
+  const bool copied = (is_packed(LA) || copies(2, p.a, acols, p.as, 0)) &&
+                      (is_packed(LB) || copies(2, p.b, bcols, p.bs, p.bg));
   const uint64_t each = ((uint64_t)p.rows + p.groups - 1) / p.groups;  // rows of a group, on average
   if constexpr (FORM != GRAD_WEIGHT) {
     // COLS spans a matrix' rows with one resource
-    if (each <= 16 && (LB == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF)) return launch_few<T, O, LB, IS_PACKED, 1>(p, s);
+    if (copied && each <= 16 && (FORM == FORWARD || p.k * p.bs * 2 <= 0x7FFFFFFF))
+      return launch_few<T, O, FORM == FORWARD ? ROWS : COLS, IS_PACKED, 1>(p, s);
   }
-  if constexpr (FORM == FORWARD && IS_PACKED) {
-    if constexpr (!std::is_same_v<O, float>)
-      if (each >= 192) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
-    launch_tiled<T, O, FORM, PACKED_ROWS, PACKED_ROWS, 2, 2, 4, 4>(p, s);
-  } else {
-    // 256 x 256 tiles take about 1.75 us for 64 summed elements, one on a CU;
-    // 128 x 128 tiles 1.17 us, two on a CU. Groups end inside a tile.
-    auto rounds = [&](uint64_t tile, uint64_t slots) {
-      const uint64_t tn = (p.n + tile - 1) / tile;
-      const uint64_t tiles = FORM == GRAD_WEIGHT ? p.groups * ((p.m + tile - 1) / tile) * tn
-                                                 : (p.rows + p.groups * tile / 2 + tile - 1) / tile * tn;
-      return (double)((tiles + slots - 1) / slots);
-    };
-    if (rounds(256, 256) * 1.75 <= rounds(128, 512) * 1.17) launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
-    else launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
+  if constexpr (FORM == FORWARD && IS_PACKED && !std::is_same_v<O, float>)
+    if (each >= 192) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
+  // What 64 summed elements cost a tile, in us, times the rounds of tiles that
+  // the chip takes: 256 x 256 tiles 1.75, one on a CU; 128 x 128 tiles 1.17,
+  // two on a CU; 64 x 64 tiles 0.75, four on a CU. Groups end inside a tile.
+  auto cost = [&](uint64_t tile, uint64_t slots, double step) {
+    const uint64_t tn = (p.n + tile - 1) / tile;
+    const uint64_t tiles = FORM == GRAD_WEIGHT ? p.groups * ((p.m + tile - 1) / tile) * tn
+                                               : (p.rows + p.groups * tile / 2 + tile - 1) / tile * tn;
+    return (double)((tiles + slots - 1) / slots) * step;
+  };
+  const double c256 = cost(256, 256, 1.75), c128 = cost(128, 512, 1.17), c64 = cost(64, 1024, 0.75);
+  if (copied) {
+    if constexpr (LA != PACKED_ROWS)
+      if (c256 <= c128 && c256 <= c64) return launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+    if (c128 <= c64) launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
+    else launch_tiled<T, O, FORM, LA, LB, 2, 2, 2, 2>(p, s);
+  } else if constexpr (!is_packed(LA)) {
+    constexpr int AA = FORM == GRAD_WEIGHT ? ANY_COLS : ANY_ROWS;
+    constexpr int AB = is_packed(LB) ? LB : FORM == FORWARD ? ANY_ROWS : ANY_COLS;
+    if (c128 <= c64) launch_tiled<T, O, FORM, AA, AB, 2, 2, 4, 4>(p, s);
+    else launch_tiled<T, O, FORM, AA, AB, 2, 2, 2, 2>(p, s);
   }
 }
 
@@ -963,6 +877,8 @@ int pxg_grouped_matmul_device(int type, const void* d_x, uint64_t rows, uint64_t
     check_rows(type, "x", d_x, rows, k, x_stride);
     check_rows(type, "w", d_w, n, k, w_stride);
     check_rows(out_type, "y", d_y, rows, n, y_stride);
+    x_stride = check_stride(rows, k, x_stride);
+    w_stride = check_stride(n, k, w_stride);
     if (rows == 0) return;
     Product p{d_x, d_w, d_y, d_offsets, x_stride, w_stride, y_stride, w_group_stride, 0, nullptr, nullptr, 0, (int)rows, (int)groups,
               (int)rows, (int)n, (int)k, false};
@@ -983,6 +899,8 @@ int pxg_grouped_matmul_grad_input_device(int type, const void* d_grad, uint64_t 
     check_rows(type, "grad", d_grad, rows, n, grad_stride);
     check_rows(type, "w", d_w, n, k, w_stride);
     check_rows(out_type, "dx", d_dx, rows, k, dx_stride);
+    grad_stride = check_stride(rows, n, grad_stride);
+    w_stride = check_stride(n, k, w_stride);
     if (rows == 0) return;
     Product p{d_grad, d_w, d_dx, d_offsets, grad_stride, w_stride, dx_stride, w_group_stride, 0, nullptr, nullptr, 0, (int)rows,
               (int)groups, (int)rows, (int)k, (int)n, false};
@@ -1004,6 +922,8 @@ int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t
     check_rows(type, "grad", d_grad, rows, n, grad_stride);
     check_rows(type, "x", d_x, rows, k, x_stride);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
+    grad_stride = check_stride(rows, n, grad_stride);
+    x_stride = check_stride(rows, k, x_stride);
     Product p{d_grad, d_x, d_dw, d_offsets, grad_stride, x_stride, dw_stride, 0, dw_group_stride, nullptr, nullptr, 0, (int)rows,
               (int)groups, (int)n, (int)k, 0, false};
     run_product<GRAD_WEIGHT>(type, out_type, p, (hipStream_t)stream);
@@ -1023,6 +943,8 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
     check_rows(PXG_BF16, "grad", d_grad, rows, n, grad_stride);
     check_packed_rows("codes", d_codes, "scales", d_scales, rows);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
+    grad_stride = check_stride(rows, n, grad_stride);
+    check_stride(2, k, block8_code_stride(k));
     Product p{d_grad, d_codes, d_dw, d_offsets, grad_stride, block8_code_stride(k), dw_stride, 0, dw_group_stride,
               nullptr, (const uint8_t*)d_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)n, (int)k, 0, false};
     run_product<GRAD_WEIGHT>(PXG_BF16, out_type, p, (hipStream_t)stream);
@@ -1041,7 +963,7 @@ int pxg_block8_matmul_device(const void* d_codes, const void* d_scales, uint64_t
     check_packed_rows("w_codes", d_w_codes, "w_scales", d_w_scales, n);
     check_rows(out_type, "y", d_y, rows, n, y_stride);
     if (rows == 0) return;
-    const uint64_t wide = block8_code_stride(k);
+    const uint64_t wide = check_stride(2, k, block8_code_stride(k));
     Product p{d_codes, d_w_codes, d_y, d_offsets, wide, wide, y_stride, n * wide, 0, (const uint8_t*)d_scales,
               (const uint8_t*)d_w_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)rows, (int)n,
               (int)wide, false};

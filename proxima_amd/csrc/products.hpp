@@ -22,6 +22,13 @@ inline void check_size(const char* name, uint64_t size) {
 inline void check_aligned(const char* name, const void* p, uint64_t bytes) {
   if ((uint64_t)(uintptr_t)p % bytes) config_error(name, (uint64_t)(uintptr_t)p, "must be aligned: codes to 16 bytes, offsets to 8, scales to 4");
 }
+// A product's operand: a tile's offsets count in 31 bits. The distance of a
+// single row to the next means nothing and is the columns.
+inline uint64_t check_stride(uint64_t rows, uint64_t cols, uint64_t stride) {
+  if (rows <= 1) stride = cols;
+  if (stride > (1ull << 22)) config_error("stride", stride, "must be at most 4194304 elements");
+  return stride;
+}
 // A row-major matrix: rows may be 0 (the pointer is then not looked at).
 inline void check_rows(int type, const char* name, const void* p, uint64_t rows, uint64_t cols, uint64_t stride) {
   if (rows > PRODUCT_SIZE_MAX) config_error("rows", rows, "must be at most 2147482624");

@@ -226,11 +226,13 @@ extern "C" {
         d_offsets: *const i64, out_type: c_int, d_dx: *mut c_void, dx_stride: u64, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_grouped_matmul_grad_weight_device(kind: c_int, d_grad: *const c_void, rows: u64, n: u64,
         grad_stride: u64, d_x: *const c_void, k: u64, x_stride: u64, d_offsets: *const i64, groups: u64,
-        out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64, stream: *mut c_void) -> c_int;
+        out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64, d_workspace: *mut c_void,
+        workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_matmul_grad_weight_workspace(rows: u64, n: u64, k: u64, groups: u64) -> u64;
     pub(crate) fn pxg_grouped_matmul_grad_weight_block8_device(d_grad: *const c_void, rows: u64, n: u64,
         grad_stride: u64, d_codes: *const c_void, d_scales: *const c_void, k: u64, d_offsets: *const i64,
         groups: u64, out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64,
-        stream: *mut c_void) -> c_int;
+        d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_activation_pack_device(activation: c_int, kind: c_int, d_h: *const c_void, rows: u64,
         cols: u64, h_stride: u64, d_a: *mut c_void, a_stride: u64, d_codes: *mut c_void, d_scales: *mut c_void,
         stream: *mut c_void) -> c_int;

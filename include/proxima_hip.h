@@ -466,7 +466,11 @@ int pxg_grouped_matmul_device(int type, const void* d_x, uint64_t rows, uint64_t
                               uint64_t groups, uint64_t n, uint64_t w_stride, uint64_t w_group_stride,
                               const int64_t* d_offsets, int out_type, void* d_y, uint64_t y_stride, void* stream);
 /* Its gradients, grad being y's: dx = grad w_g, and dw_g = the sum over the
- * group's rows t of grad[t]^T x[t] (zeros for an empty group). */
+ * group's rows t of grad[t]^T x[t] (zeros for an empty group). Long sums into
+ * small matrices are faster with a workspace (16-byte aligned device memory,
+ * not kept after the work is done): workspace() says how many bytes, 0 where
+ * none helps; with less, or NULL, the sums are taken in one part. */
+uint64_t pxg_grouped_matmul_grad_weight_workspace(uint64_t rows, uint64_t n, uint64_t k, uint64_t groups);
 int pxg_grouped_matmul_grad_input_device(int type, const void* d_grad, uint64_t rows, uint64_t n, uint64_t grad_stride,
                                          const void* d_w, uint64_t groups, uint64_t k, uint64_t w_stride,
                                          uint64_t w_group_stride, const int64_t* d_offsets, int out_type, void* d_dx,
@@ -474,13 +478,15 @@ int pxg_grouped_matmul_grad_input_device(int type, const void* d_grad, uint64_t 
 int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t rows, uint64_t n,
                                           uint64_t grad_stride, const void* d_x, uint64_t k, uint64_t x_stride,
                                           const int64_t* d_offsets, uint64_t groups, int out_type, void* d_dw,
-                                          uint64_t dw_stride, uint64_t dw_group_stride, void* stream);
+                                          uint64_t dw_stride, uint64_t dw_group_stride, void* d_workspace,
+                                          uint64_t workspace_bytes, void* stream);
 /* The weight gradient from a packed x: grad is bf16 (in which packed values
  * are exact), out_type bf16 or f32. */
 int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t rows, uint64_t n, uint64_t grad_stride,
                                                  const void* d_codes, const void* d_scales, uint64_t k,
                                                  const int64_t* d_offsets, uint64_t groups, int out_type, void* d_dw,
-                                                 uint64_t dw_stride, uint64_t dw_group_stride, void* stream);
+                                                 uint64_t dw_stride, uint64_t dw_group_stride, void* d_workspace,
+                                          uint64_t workspace_bytes, void* stream);
 
 /* a = f(h), computed from h itself, and h packed, to be kept for the backward
  * pass; and that pass: dh = grad * f'(unpacked h). f32, f16 or bf16. */

@@ -171,9 +171,10 @@ SIGNATURES = {
     "pxg_grouped_matmul_grad_input_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp,
                                                     _i32, _vp, _u64, _vp]),
     "pxg_grouped_matmul_grad_weight_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _i32,
-                                                     _vp, _u64, _u64, _vp]),
+                                                     _vp, _u64, _u64, _vp, _u64, _vp]),
     "pxg_grouped_matmul_grad_weight_block8_device": (_i32, [_vp, _u64, _u64, _u64, _vp, _vp, _u64, _vp, _u64, _i32,
-                                                            _vp, _u64, _u64, _vp]),
+                                                            _vp, _u64, _u64, _vp, _u64, _vp]),
+    "pxg_grouped_matmul_grad_weight_workspace": (_u64, [_u64, _u64, _u64, _u64]),
     "pxg_activation_pack_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp]),
     "pxg_activation_grad_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _vp, _vp, _u64, _vp]),
 }

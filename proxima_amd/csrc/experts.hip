@@ -8,6 +8,8 @@
 //
 // Every sum is held in f32 on the matrix cores and rounded once, to the
 // output's type.
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "block8.hpp"
@@ -41,7 +43,9 @@ struct Product {
   uint64_t ss;
   int rows, groups;     // rows of x and dy
   int m, n, k;
-  bool c_vec;           // four adjacent elements of C, from a multiple of four on, can be stored at once
+  bool c_vec;           // C's rows are 16-byte aligned
+  int splits = 1;       // grad weight: parts of a group's rows, c then m x n of each group of each part
+  int tile = 0;         // and the tiles chosen with them
 };
 
 template <class T>
@@ -118,6 +122,13 @@ __device__ __forceinline__ uint4 decode_bf16(uint32_t x, uint32_t y, float s) {
                     __builtin_bit_cast(uint32_t, d));
 }
 
+// A barrier after the wavefront's LDS accesses; copies stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // By how many 16-byte pieces row k of a stage is moved: a transposing read
 // takes 32 bytes of rows 8 q + {0..3} (or {4..7}) for each 16 lanes q. Rows of
 // 64 elements have four such pieces only.
@@ -166,17 +177,26 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   int m0, n0, rows, cols, steps, group, tail;
   uint64_t a0, b0;  // first elements of the operands' tiles
   [[maybe_unused]] uint64_t sa0 = 0, sb0 = 0;  // and their rows, packed
+  uint64_t c_first = 0;                        // of the result's part
   if constexpr (FORM == GRAD_WEIGHT) {
     // an eighth of every group's tiles, the longest group first
     const int tiles_m = (p.m + TM - 1) / TM, each = tiles_m * tiles_n, per = (each + 7) / 8;
-    const int t = die * per + at % per;
-    if (t >= each || at % per >= per) return;
-    group = group_by_size(p.offsets, p.groups, p.rows, at / per);
+    const int t = die * per + at % per, part = at / per;
+    if (t >= each) return;
+    group = group_by_size(p.offsets, p.groups, p.rows, part / p.splits);
     m0 = t / tiles_n * TM;
     n0 = t % tiles_n * TN;
     int lo, hi;
     group_range(p.offsets, group, p.rows, lo, hi);
     rows = p.m - m0;
+    if (p.splits > 1) {  // whole steps a part
+      const int split = part % p.splits;
+      const int64_t size = (hi - lo + p.splits * K::STEP - 1) / (p.splits * K::STEP) * K::STEP;
+      const int64_t from = lo + size * split;
+      lo = from < hi ? (int)from : hi;
+      hi = from + size < hi ? (int)(from + size) : hi;
+      c_first = (uint64_t)split * p.groups * p.cg;
+    }
     tail = hi - lo;
     a0 = (uint64_t)lo * p.as + m0;
     b0 = (uint64_t)lo * p.bs + n0;
@@ -216,6 +236,13 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   rows = rows < TM ? rows : TM;
   cols = p.n - n0 < TN ? p.n - n0 : TN;
 
+  // Dies begin at different places of the sum: rows a power of two apart
+  // otherwise have all of them read the same memory channels. Four steps share
+  // a word of scale bytes.
+  const int spin = !K::FP8 ? steps / 8 * die : steps % 4 == 0 ? steps / 32 * 4 * die : 0;
+  int source = spin;  // of the step copied last: its place in the sum
+  auto advance = [&] { source = source + 1 < steps ? source + 1 : 0; };
+
   // Copies. ROWS: a copy of one wavefront fills 8 rows of 128 bytes, 16-byte
   // piece c of row r at place c ^ (r & 7), so that 8 lanes reading piece c of
   // 8 rows meet every bank. COLS: it fills 1024 bytes of rows of 2 TM (2 TN)
@@ -240,12 +267,12 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   // Part i of n of a step's copies of an operand, by one wavefront, in order
   // `who`. Steps past the last one copy zeros.
   auto stage_resource = [&](auto layout, const Operand& o, int step) {
-    const int left = tail - step * K::STEP;  // summed elements from here on
+    const int left = tail - source * K::STEP;  // summed elements from here on
     return decltype(layout)::value == ROWS
-               ? tile_rsrc(o.base + (uint64_t)step * 128,
-                           left > 0 ? (o.limit - 1) * o.stride + (uint64_t)(left * K::BYTES) : 0)
-               : tile_rsrc(o.base + (uint64_t)step * K::STEP * o.stride,
-                           left > 0 ? (left - 1) * o.stride + o.limit * 2 : 0);
+               ? tile_rsrc(o.base + (uint64_t)source * 128,
+                           step < steps ? (o.limit - 1) * o.stride + (uint64_t)(left * K::BYTES) : 0)
+               : tile_rsrc(o.base + (uint64_t)source * K::STEP * o.stride,
+                           step < steps ? (left - 1) * o.stride + o.limit * 2 : 0);
   };
   auto stage_copy = [&](auto layout, auto width, const Operand& o, __amdgpu_buffer_rsrc_t rs, int step, int part) {
     const uint32_t to = lds0 + (step & 1) * K::STAGE + o.place + part * 1024;
@@ -253,7 +280,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       uint32_t at = o.row;
       asm volatile("" : "+v"(at));  // keeps one register for all parts, not one for each
       // pieces past the rows' end are zeros (packed rows are whole blocks)
-      const bool in = K::FP8 || (((lane & 7) ^ (lane >> 3)) << 4) < (tail - step * K::STEP) * K::BYTES;
+      const bool in = K::FP8 || (((lane & 7) ^ (lane >> 3)) << 4) < (tail - source * K::STEP) * K::BYTES;
       copy16(rs, in ? (uint32_t)(part * 8 * o.stride) + at : NOWHERE, to);
     } else {
       constexpr int PER = decltype(width)::value / 8;  // pieces in a row
@@ -295,7 +322,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   };
   auto load_staged = [&](auto layout, auto width, const Operand& o, int step, Staged& x) {
     constexpr int L = decltype(layout)::value;
-    const int left = tail - step * K::STEP;
+    const int left = step < steps ? tail - source * K::STEP : 0;
     [[maybe_unused]] auto load = [](__amdgpu_buffer_rsrc_t rs, uint32_t at) {
       typedef uint32_t u4v __attribute__((ext_vector_type(4)));
       return __builtin_bit_cast(uint4, (u4v)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)at, 0, 0));
@@ -304,8 +331,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       typedef int i2v __attribute__((ext_vector_type(2)));
       const uint64_t lines = L == PACKED_ROWS ? (left > 0 ? o.limit : 0) : left > 0 ? left : 0;
       // resources end with the last line that counts; a line's own end is a multiple of 128 columns
-      const uint64_t codes0 = L == PACKED_ROWS ? (uint64_t)step * 64 : (uint64_t)step * K::STEP * o.stride;
-      const uint64_t scales0 = L == PACKED_ROWS ? (uint64_t)step / 2 : (uint64_t)step * K::STEP * p.ss;
+      const uint64_t codes0 = L == PACKED_ROWS ? (uint64_t)source * 64 : (uint64_t)source * K::STEP * o.stride;
+      const uint64_t scales0 = L == PACKED_ROWS ? (uint64_t)source / 2 : (uint64_t)source * K::STEP * p.ss;
       const uint64_t skip = L == PACKED_ROWS ? codes0 : n0, skip_s = L == PACKED_ROWS ? scales0 : n0 / 128;
       const auto rc = tile_rsrc(o.base + codes0, lines ? lines * o.stride - skip : 0);
       const auto rb = tile_rsrc(o.scales + scales0, lines ? lines * p.ss - skip_s : 0);
@@ -323,7 +350,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       const int odd = (int)((uintptr_t)o.base & 2);
       const uint64_t end = L == ANY_ROWS ? (o.limit - 1) * o.stride + (uint64_t)left * 2
                                          : (uint64_t)(left - 1) * o.stride + o.limit * 2;
-      const auto rs = tile_rsrc(o.base - odd + (L == ANY_ROWS ? (uint64_t)step * 128 : (uint64_t)step * K::STEP * o.stride),
+      const auto rs = tile_rsrc(o.base - odd + (L == ANY_ROWS ? (uint64_t)source * 128 : (uint64_t)source * K::STEP * o.stride),
                                 left > 0 ? (end + odd + 3) & ~3ull : 0);
       pieces(layout, width, [&](int i, int line, int c) {
         const bool in = L == ANY_ROWS ? line < o.limit && c * 16 < left : line < left && c * 16 < o.limit;
@@ -346,7 +373,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
         *place(line, c) = decode_bf16(x.lo[i].x, x.lo[i].y, block8_scale(x.last[i]));
       });
     } else if constexpr (is_any(L)) {
-      const int left = tail - step * K::STEP;
+      const int left = tail - source * K::STEP;
       pieces(layout, width, [&](int i, int line, int c) {
         const uint32_t shift = (((uint32_t)(uintptr_t)o.base + line * (uint32_t)o.stride) & 2) * 8;
         const int valid = (L == ANY_ROWS ? left : o.limit) - c * 16;
@@ -435,6 +462,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     };
     Staged xa, xb;
     auto next = [&](int step) {  // a step's copies, and what goes through registers
+      if (step > 0) advance();
       stage_copies(LayoutA{}, WidthA{}, A, step);
       stage_copies(LayoutB{}, WidthB{}, B, step);
       load_staged(LayoutA{}, WidthA{}, A, step, xa);
@@ -527,7 +555,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       const uint32_t to = lds0 + 2 * K::STAGE + ((step >> 2) & 1) * K::SCALES;
       const bool of_a = at < TM / 64;
       const int r = (of_a ? at : at - TM / 64) * 64 + lane, limit = of_a ? rows : cols;
-      const auto rs = tile_rsrc((of_a ? A.scales : B.scales) + step, step < (int)p.ss ? limit * p.ss - step : 0);
+      const auto rs = tile_rsrc((of_a ? A.scales : B.scales) + source, step < steps ? limit * p.ss - source : 0);
       copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
     };
     stage_copies(LayoutA{}, WidthA{}, A, 0);
@@ -541,6 +569,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
         stage_copy(LayoutB{}, WidthB{}, B, rb, step, (wave & 3) * MT + i);
       };
       {
+        advance();
         const auto ra = stage_resource(LayoutA{}, A, 1), rb = stage_resource(LayoutB{}, B, 1);
 #pragma unroll
         for (int i = 0; i < MT; ++i) part(ra, rb, 1, i);
@@ -550,6 +579,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
         read_step(step);
         wait_copies();
         turn();
+        advance();
         const auto ra = stage_resource(LayoutA{}, A, step + 2), rb = stage_resource(LayoutB{}, B, step + 2);
         if (((step + 2) & 3) == 0) {
           scale_copies(step + 2, (wave & 3) * 2);
@@ -590,26 +620,40 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     else run(std::integral_constant<int, MT>{});
   }
 
-  // a lane holds columns 4 q to 4 q + 3 of row r16 of each tile
-  O* c = (O*)p.c + group * p.cg + (uint64_t)m0 * p.cs + n0;
+  // A lane holds columns 4 q to 4 q + 3 of row r16 of each tile. Through LDS,
+  // 16 rows of the wavefront's columns at a time, so that what is stored
+  // together is whole rows of them.
+  constexpr int EACH = 16 / sizeof(O), PER = NT * 16 / EACH;  // a lane's elements, lanes to a row
+  constexpr int PITCH = NT * 16 * sizeof(O) + 16;             // 16 bytes more spread the rows over the banks
+  static_assert(WAVES * 16 * PITCH <= K::LDS);
+  lds_barrier();
+  char* mine = lds + wave * (16 * PITCH);
+  O* c = (O*)p.c + c_first + group * p.cg + (uint64_t)m0 * p.cs + n0;
+  const int col = wn * NT * 16 + lane % PER * EACH;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int r = (i * WM + wm) * 16 + r16;
-    if (r >= rows) continue;
-    O* row = c + (uint64_t)r * p.cs;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const int at = (wn * NT + j) * 16 + 4 * q;
-      if (p.c_vec && at + 4 <= cols) {
-        typedef O o4v __attribute__((ext_vector_type(4)));
-        o4v v;
+      typedef O o4v __attribute__((ext_vector_type(4)));
+      o4v v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (O)acc[i][j][e];
-        *reinterpret_cast<o4v*>(row + at) = v;
+      for (int e = 0; e < 4; ++e) v[e] = (O)acc[i][j][e];
+      *reinterpret_cast<o4v*>(mine + r16 * PITCH + (j * 16 + 4 * q) * sizeof(O)) = v;
+    }
+#pragma unroll
+    for (int h = 0; h < 16 * PER / 64; ++h) {
+      const int r = lane / PER + h * (64 / PER), row = (i * WM + wm) * 16 + r;
+      const uint4 v = *reinterpret_cast<const uint4*>(mine + r * PITCH + lane % PER * 16);
+      if (row >= rows) continue;
+      O* to = c + (uint64_t)row * p.cs + col;
+      if (p.c_vec && col + EACH <= cols) {
+        *reinterpret_cast<uint4*>(to) = v;
       } else {
+        O x[EACH];
+        *reinterpret_cast<uint4*>(x) = v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (at + e < cols) row[at + e] = (O)acc[i][j][e];
+        for (int e = 0; e < EACH; ++e)
+          if (col + e < cols) to[e] = x[e];
       }
     }
   }
@@ -782,12 +826,36 @@ void check_out_type(int type, int out_type) {
     config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
 }
 
+// The parts of each element, in order: a grid of rows of dw by 256 columns.
+template <class O>
+__global__ void __launch_bounds__(256)
+join_parts(const float* __restrict__ parts, int splits, uint64_t part, int n, int k, O* __restrict__ out, uint64_t os,
+           uint64_t og) {
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (c >= k) return;
+  const uint64_t row = blockIdx.x;
+  const float* from = parts + row * k + c;
+  O* to = out + row / n * og + row % n * os + c;
+  if (c + 4 <= k && k % 4 == 0) {
+    f4v x = *reinterpret_cast<const f4v*>(from);
+    for (int s = 1; s < splits; ++s) x += *reinterpret_cast<const f4v*>(from + s * part);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = (O)x[e];
+  } else {
+    for (int e = 0; e < 4 && c + e < k; ++e) {
+      float x = from[e];
+      for (int s = 1; s < splits; ++s) x += from[s * part + e];
+      to[e] = (O)x;
+    }
+  }
+}
+
 template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
 void launch_tiled(const Product& p, hipStream_t s) {
   using K = Tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>;
   const uint64_t tn = (p.n + K::TN - 1) / K::TN;
   uint64_t tiles;
-  if (FORM == GRAD_WEIGHT) tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * p.groups;
+  if (FORM == GRAD_WEIGHT) tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * p.groups * p.splits;
   else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn / 8 + 2) * 8;  // both kinds' eighths
   hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), dim3(grid_size(tiles)), dim3(K::THREADS), 0, s,
                      p);
@@ -807,9 +875,56 @@ void launch_few(const Product& p, hipStream_t s) {
   PXG_HIP(hipGetLastError());
 }
 
+// Which tiles a product takes: the cheapest by what was measured, in us. A
+// tile takes `fixed` and then `step` for 64 summed elements, `least` of it
+// alone on its CU and `more` where the chip is full (256 x 256 tiles one on a
+// CU, 128 x 128 two, 64 x 64 four). Groups end inside a tile. Measured at
+// 16384 rows, 2048 -> 2048, one group (256, 128, 64): forward 115, 150, 211 us;
+// at 4096 rows, 768 -> 768: 23, 14, 12 us.
+struct Tile {
+  int size, slots;
+  double fixed, least, more;
+};
+constexpr Tile TILES[3] = {{256, 256, 6, 1.15, 0.45}, {128, 512, 4, 0.7, 0.35}, {64, 1024, 3, 0.42, 0.3}};
+constexpr Tile PACKED_TILES[3] = {{256, 256, 6, 0.6, 0.25}, {128, 512, 4, 0.95, 0.45}, {64, 1024, 3, 0.6, 0.4}};
+constexpr double JOIN_BYTES_PER_US = 4e6, JOIN_US = 4;
+constexpr int SPLITS_MAX = 32;
+
+struct Cost {
+  double best = 1e30, fp8 = 1e30;
+  int tile = 64, splits = 1;
+};
+// packed: the first of PACKED_TILES is the fp8 product's, not among the choice
+Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0) {
+  Cost best;
+  const double summed = form == GRAD_WEIGHT ? (double)p.rows / p.groups : p.k;
+  for (int i = 0; i < 3; ++i) {
+    const Tile& t = packed ? PACKED_TILES[i] : TILES[i];
+    const uint64_t tn = ((uint64_t)p.n + t.size - 1) / t.size;
+    const uint64_t tiles = form == GRAD_WEIGHT ? p.groups * (((uint64_t)p.m + t.size - 1) / t.size) * tn
+                                               : (p.rows + (uint64_t)p.groups * t.size / 2 + t.size - 1) / t.size * tn;
+    for (int splits = 1; splits <= SPLITS_MAX; splits *= 2) {
+      const double bytes = splits > 1 ? 4.0 * splits * p.groups * p.m * p.n : 0;
+      if (splits > 1 && (form != GRAD_WEIGHT || bytes > (double)room || summed < 128.0 * splits)) break;
+      const double full = std::min(1.0, (double)tiles * splits / t.slots);
+      const double each = t.fixed + std::ceil(summed / splits / 64) * (t.least + t.more * full);
+      const double us = (double)((tiles * splits + t.slots - 1) / t.slots) * each +
+                        (splits > 1 ? JOIN_US + 2 * bytes / JOIN_BYTES_PER_US : 0);
+      if (packed && i == 0) {
+        best.fp8 = us;
+      } else if (us < best.best) {
+        best.best = us;
+        best.tile = t.size;
+        best.splits = splits;
+      }
+    }
+  }
+  return best;
+}
+
 template <int FORM, class T, class O, bool IS_PACKED>
 void launch_product(Product p, hipStream_t s) {
-  p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % (4 * sizeof(O)) == 0;
+  p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % 16 == 0;
   constexpr int LA = FORM == GRAD_WEIGHT ? COLS : FORM == FORWARD && IS_PACKED ? PACKED_ROWS : ROWS;
   constexpr int LB = FORM == GRAD_INPUT ? COLS : FORM == GRAD_WEIGHT ? (IS_PACKED ? PACKED_COLS : COLS) : LA;
   const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
@@ -821,27 +936,19 @@ void launch_product(Product p, hipStream_t s) {
     if (copied && each <= 16 && (FORM == FORWARD || p.k * p.bs * 2 <= 0x7FFFFFFF))
       return launch_few<T, O, FORM == FORWARD ? ROWS : COLS, IS_PACKED, 1>(p, s);
   }
+  Cost cost = product_cost(FORM, p, FORM == FORWARD && IS_PACKED);
+  if (p.splits > 1) cost.tile = p.tile;
   if constexpr (FORM == FORWARD && IS_PACKED && !std::is_same_v<O, float>)
-    if (each >= 192) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
-  // What 64 summed elements cost a tile, in us, times the rounds of tiles that
-  // the chip takes: 256 x 256 tiles 1.75, one on a CU; 128 x 128 tiles 1.17,
-  // two on a CU; 64 x 64 tiles 0.75, four on a CU. Groups end inside a tile.
-  auto cost = [&](uint64_t tile, uint64_t slots, double step) {
-    const uint64_t tn = (p.n + tile - 1) / tile;
-    const uint64_t tiles = FORM == GRAD_WEIGHT ? p.groups * ((p.m + tile - 1) / tile) * tn
-                                               : (p.rows + p.groups * tile / 2 + tile - 1) / tile * tn;
-    return (double)((tiles + slots - 1) / slots) * step;
-  };
-  const double c256 = cost(256, 256, 1.75), c128 = cost(128, 512, 1.17), c64 = cost(64, 1024, 0.75);
+    if (each >= 192 && cost.fp8 <= cost.best) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
   if (copied) {
     if constexpr (LA != PACKED_ROWS)
-      if (c256 <= c128 && c256 <= c64) return launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
-    if (c128 <= c64) launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
+      if (cost.tile == 256) return launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+    if (cost.tile >= 128) launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
     else launch_tiled<T, O, FORM, LA, LB, 2, 2, 2, 2>(p, s);
   } else if constexpr (!is_packed(LA)) {
     constexpr int AA = FORM == GRAD_WEIGHT ? ANY_COLS : ANY_ROWS;
     constexpr int AB = is_packed(LB) ? LB : FORM == FORWARD ? ANY_ROWS : ANY_COLS;
-    if (c128 <= c64) launch_tiled<T, O, FORM, AA, AB, 2, 2, 4, 4>(p, s);
+    if (cost.tile >= 128) launch_tiled<T, O, FORM, AA, AB, 2, 2, 4, 4>(p, s);
     else launch_tiled<T, O, FORM, AA, AB, 2, 2, 2, 2>(p, s);
   }
 }
@@ -855,6 +962,28 @@ void run_product(int type, int out_type, const Product& p, hipStream_t s) {
       if (p.b_scales) return launch_product<FORM, T, O, true>(p, s);
     }
     launch_product<FORM, T, O, false>(p, s);
+  });
+}
+
+// A weight gradient whose groups are long and whose matrices are few tiles:
+// parts of each group's rows go to workgroups of their own, their sums to the
+// workspace, and are joined in order.
+void run_grad_weight(int type, int out_type, const Product& whole, void* workspace, uint64_t bytes, hipStream_t s) {
+  const Cost cost = product_cost(GRAD_WEIGHT, whole, false, workspace ? bytes : 0);
+  if (cost.splits == 1) return run_product<GRAD_WEIGHT>(type, out_type, whole, s);
+  Product p = whole;
+  p.splits = cost.splits;
+  p.tile = cost.tile;
+  p.c = workspace;
+  p.cs = p.n;
+  p.cg = (uint64_t)p.m * p.n;
+  run_product<GRAD_WEIGHT>(type, PXG_F32, p, s);
+  by_types(type, out_type, [&](auto, auto o) {
+    using O = decltype(o);
+    const dim3 grid(grid_size((uint64_t)p.groups * p.m), (unsigned)((p.n + 1023) / 1024));
+    hipLaunchKernelGGL(join_parts<O>, grid, dim3(256), 0, s, (const float*)workspace, p.splits, p.groups * p.cg, p.m,
+                       p.n, (O*)whole.c, whole.cs, whole.cg);
+    PXG_HIP(hipGetLastError());
   });
 }
 
@@ -908,10 +1037,25 @@ int pxg_grouped_matmul_grad_input_device(int type, const void* d_grad, uint64_t 
   });
 }
 
+uint64_t pxg_grouped_matmul_grad_weight_workspace(uint64_t rows, uint64_t n, uint64_t k, uint64_t groups) {
+  if (rows > PRODUCT_SIZE_MAX || n == 0 || n > PRODUCT_SIZE_MAX || k == 0 || k > PRODUCT_SIZE_MAX || groups == 0 ||
+      groups > (1u << 20))
+    return 0;
+  Product p{};
+  p.rows = (int)rows;
+  p.groups = (int)groups;
+  p.m = (int)n;
+  p.n = (int)k;
+  p.splits = 1;
+  const Cost cost = product_cost(GRAD_WEIGHT, p, false, UINT64_MAX);
+  return cost.splits == 1 ? 0 : 4 * cost.splits * groups * n * k;
+}
+
 int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t rows, uint64_t n,
                                           uint64_t grad_stride, const void* d_x, uint64_t k, uint64_t x_stride,
                                           const int64_t* d_offsets, uint64_t groups, int out_type, void* d_dw,
-                                          uint64_t dw_stride, uint64_t dw_group_stride, void* stream) {
+                                          uint64_t dw_stride, uint64_t dw_group_stride, void* d_workspace,
+                                          uint64_t workspace_bytes, void* stream) {
   return guard([&] {
     check_type(type, false);
     check_out_type(type, out_type);
@@ -922,18 +1066,20 @@ int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t
     check_rows(type, "grad", d_grad, rows, n, grad_stride);
     check_rows(type, "x", d_x, rows, k, x_stride);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
+    check_aligned("workspace", d_workspace, 16);
     grad_stride = check_stride(rows, n, grad_stride);
     x_stride = check_stride(rows, k, x_stride);
     Product p{d_grad, d_x, d_dw, d_offsets, grad_stride, x_stride, dw_stride, 0, dw_group_stride, nullptr, nullptr, 0, (int)rows,
               (int)groups, (int)n, (int)k, 0, false};
-    run_product<GRAD_WEIGHT>(type, out_type, p, (hipStream_t)stream);
+    run_grad_weight(type, out_type, p, d_workspace, workspace_bytes, (hipStream_t)stream);
   });
 }
 
 int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t rows, uint64_t n, uint64_t grad_stride,
                                                  const void* d_codes, const void* d_scales, uint64_t k,
                                                  const int64_t* d_offsets, uint64_t groups, int out_type, void* d_dw,
-                                                 uint64_t dw_stride, uint64_t dw_group_stride, void* stream) {
+                                                 uint64_t dw_stride, uint64_t dw_group_stride, void* d_workspace,
+                                                 uint64_t workspace_bytes, void* stream) {
   return guard([&] {
     check_out_type(PXG_BF16, out_type);
     check_size("k", k);
@@ -943,11 +1089,12 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
     check_rows(PXG_BF16, "grad", d_grad, rows, n, grad_stride);
     check_packed_rows("codes", d_codes, "scales", d_scales, rows);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
+    check_aligned("workspace", d_workspace, 16);
     grad_stride = check_stride(rows, n, grad_stride);
     check_stride(2, k, block8_code_stride(k));
     Product p{d_grad, d_codes, d_dw, d_offsets, grad_stride, block8_code_stride(k), dw_stride, 0, dw_group_stride,
               nullptr, (const uint8_t*)d_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)n, (int)k, 0, false};
-    run_product<GRAD_WEIGHT>(PXG_BF16, out_type, p, (hipStream_t)stream);
+    run_grad_weight(PXG_BF16, out_type, p, d_workspace, workspace_bytes, (hipStream_t)stream);
   });
 }
 

@@ -20,7 +20,7 @@ inline void check_size(const char* name, uint64_t size) {
   if (size == 0 || size > PRODUCT_SIZE_MAX) config_error(name, size, "must be between 1 and 2147482624");
 }
 inline void check_aligned(const char* name, const void* p, uint64_t bytes) {
-  if ((uint64_t)(uintptr_t)p % bytes) config_error(name, (uint64_t)(uintptr_t)p, "must be aligned: codes to 16 bytes, offsets to 8, scales to 4");
+  if ((uint64_t)(uintptr_t)p % bytes) config_error(name, (uint64_t)(uintptr_t)p, "must be aligned: codes and workspace to 16 bytes, offsets to 8, scales to 4");
 }
 // A product's operand: a tile's offsets count in 31 bits. The distance of a
 // single row to the next means nothing and is the columns.

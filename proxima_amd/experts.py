@@ -273,13 +273,17 @@ def grouped_matmul_grad_weight(grad, x, offsets, out_dtype=None, out=None):
     if xrows != rows:
         _mismatch(xrows, rows, "x's rows")
     out, stride = _out(out, (groups, n, k), dtype, grad)
+    size = _lib.pxg_grouped_matmul_grad_weight_workspace(rows, n, k, groups)
+    space = grad.new_empty(size, dtype=_torch.uint8) if size else None
+    at = space.data_ptr() if size else None
     if isinstance(x, Block8):
         _run(_lib.pxg_grouped_matmul_grad_weight_block8_device, (grad, codes, scales, offsets, out), grad.data_ptr(),
              rows, n, _stride(grad), codes.data_ptr(), scales.data_ptr(), k, ptr, groups, out_kind, out.data_ptr(),
-             stride, out.stride(0))
+             stride, out.stride(0), at, size)
     else:
         _run(_lib.pxg_grouped_matmul_grad_weight_device, (grad, x, offsets, out), kind, grad.data_ptr(), rows, n,
-             _stride(grad), x.data_ptr(), k, _stride(x), ptr, groups, out_kind, out.data_ptr(), stride, out.stride(0))
+             _stride(grad), x.data_ptr(), k, _stride(x), ptr, groups, out_kind, out.data_ptr(), stride, out.stride(0),
+             at, size)
     return out
 
 

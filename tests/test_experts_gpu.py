@@ -250,6 +250,28 @@ def test_larger_products(gpu, sizes, n, k):
     _check(gpu.grouped_matmul_grad_weight(grad, px, offsets, out_dtype=torch.float32), want, size, max(sizes))
 
 
+@pytest.mark.parametrize("sizes,n,k", [([9000], 128, 72), ([5000, 0, 130, 4000], 64, 200), ([20000], 33, 17),
+                                       ([3, 8000], 256, 256)])
+def test_weight_gradients_of_long_groups(gpu, sizes, n, k):
+    # long sums into small matrices: parts of a group's rows, joined
+    import torch
+    for dtype in (torch.bfloat16, torch.float16):
+        x, w, grad, offsets = _make(torch, sizes, n, k, dtype, 14, 2, 9)
+        assert gpu._lib.pxg_grouped_matmul_grad_weight_workspace(x.shape[0], n, k, len(sizes)) > 0
+        ends = offsets.tolist()
+        want, size = _per_group(torch, grad, x, ends)
+        for out_dtype in (dtype, torch.float32):
+            hold = torch.full((len(sizes), n, k + 5), 3.0, dtype=out_dtype, device="cuda")
+            got = gpu.grouped_matmul_grad_weight(grad, x, offsets, out=hold[..., :k])
+            _check(got, want, size, max(sizes))
+            assert bool((hold[..., k:] == 3.0).all())
+            assert torch.equal(got, gpu.grouped_matmul_grad_weight(grad, x, offsets, out_dtype=out_dtype))
+    packed = gpu.block8_pack(x)
+    grad = grad.bfloat16()
+    want, size = _per_group(torch, grad, gpu.block8_unpack(packed, torch.float32), ends)
+    _check(gpu.grouped_matmul_grad_weight(grad, packed, offsets, out_dtype=torch.float32), want, size, max(sizes))
+
+
 def test_one_group_without_offsets(gpu):
     import torch
     x, w, grad, offsets = _make(torch, [190], 96, 160, torch.float16, 4)

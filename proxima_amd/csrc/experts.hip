@@ -183,11 +183,10 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     const int tiles_m = (p.m + TM - 1) / TM, each = tiles_m * tiles_n, per = (each + 7) / 8;
     const int t = die * per + at % per, part = at / per;
     if (t >= each) return;
-    group = group_by_size(p.offsets, p.groups, p.rows, part / p.splits);
+    int lo, hi;
+    group = group_by_size(p.offsets, p.groups, p.rows, part / p.splits, lo, hi);
     m0 = t / tiles_n * TM;
     n0 = t % tiles_n * TN;
-    int lo, hi;
-    group_range(p.offsets, group, p.rows, lo, hi);
     rows = p.m - m0;
     if (p.splits > 1) {  // whole steps a part
       const int split = part % p.splits;
@@ -206,7 +205,14 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     // workgroups that run together on a die share operands best as a block of
     // 4 row tiles by 8.
     int whole, partial, first, size;
-    count_row_tiles(p.offsets, p.groups, p.rows, TM, whole, partial);
+    const bool few = p.offsets && p.groups <= SEGMENT_GROUPS;  // one load of the offsets
+    Segments segments{};
+    if (few) {
+      segments = load_segments(p.offsets, p.groups, p.rows);
+      count_segments(segments, TM, whole, partial);
+    } else {
+      count_row_tiles(p.offsets, p.groups, p.rows, TM, whole, partial);
+    }
     eighth(whole * tiles_n, die, first, size);
     const bool is_whole = at < size;
     int index = first + at, count = whole;
@@ -220,8 +226,14 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     const int band = index / (4 * tiles_n), in = index - band * 4 * tiles_n;
     const int high = count - band * 4 < 4 ? count - band * 4 : 4;
     RowTile t;
-    if (is_whole) find_row_tile<WHOLE_TILES>(p.offsets, p.groups, p.rows, TM, band * 4 + in % high, t);
-    else find_row_tile<PARTIAL_TILES>(p.offsets, p.groups, p.rows, TM, band * 4 + in % high, t);
+    const int nth = band * 4 + in % high;
+    if (few) {
+      if (is_whole) pick_row_tile<WHOLE_TILES>(segments, p.groups, TM, nth, t);
+      else pick_row_tile<PARTIAL_TILES>(segments, p.groups, TM, nth, t);
+    } else {
+      if (is_whole) find_row_tile<WHOLE_TILES>(p.offsets, p.groups, p.rows, TM, nth, t);
+      else find_row_tile<PARTIAL_TILES>(p.offsets, p.groups, p.rows, TM, nth, t);
+    }
     m0 = t.row;
     n0 = in / high * TN;
     group = t.group < 0 ? 0 : t.group;
@@ -908,7 +920,9 @@ Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0) {
       if (splits > 1 && (form != GRAD_WEIGHT || bytes > (double)room || summed < 128.0 * splits)) break;
       const double full = std::min(1.0, (double)tiles * splits / t.slots);
       const double each = t.fixed + std::ceil(summed / splits / 64) * (t.least + t.more * full);
-      const double us = (double)((tiles * splits + t.slots - 1) / t.slots) * each +
+      // one group's half tile of padding does not begin a round
+      const double rounds = std::ceil((double)tiles * splits / t.slots - (p.groups == 1 ? 0.12 : 0.0));
+      const double us = std::max(1.0, rounds) * each +
                         (splits > 1 ? JOIN_US + 2 * bytes / JOIN_BYTES_PER_US : 0);
       if (packed && i == 0) {
         best.fp8 = us;

@@ -128,24 +128,64 @@ __device__ __forceinline__ void count_row_tiles(const int64_t* __restrict__ offs
   }
 }
 
-// Which group a place in the order of falling sizes belongs to (ties by
-// index), by a wavefront whose lanes all call it; above 64 groups the order
-// is the groups' own.
-__device__ __forceinline__ int group_by_size(const int64_t* __restrict__ offsets, int groups, int rows, int place) {
-  if (groups > WAVE) return place;
+// The segments of up to 62 groups, one a lane: segment s is rows first to end,
+// segments 0 and groups + 1 (and the empty ones past it) those of no group.
+struct Segments {
+  int first, end;
+};
+constexpr int SEGMENT_GROUPS = WAVE - 2;
+__device__ __forceinline__ Segments load_segments(const int64_t* __restrict__ offsets, int groups, int rows) {
   const int lane = threadIdx.x & (WAVE - 1);
-  int end = lane < groups ? clamp_offset(offsets[lane + 1], rows) : rows;
-  int begin = clamp_offset(offsets[0], rows);
-  end = wave_max_scan(end > begin ? end : begin, lane);
-  int first = __shfl_up(end, 1, WAVE);
-  if (lane == 0) first = begin;
-  const int size = lane < groups ? end - first : -1;
+  Segments s;
+  s.end = wave_max_scan(lane <= groups ? clamp_offset(offsets[lane], rows) : rows, lane);
+  s.first = __shfl_up(s.end, 1, WAVE);
+  if (lane == 0) s.first = 0;
+  return s;
+}
+
+// Tile `index` of its kind, as find_row_tile.
+template <int KIND>
+__device__ __forceinline__ bool pick_row_tile(const Segments& s, int groups, int size, int index, RowTile& t) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  const int tiles = row_tiles_of<KIND>(s.end - s.first, size);
+  const int last = wave_sum_scan(tiles, lane);
+  const uint64_t hit = __ballot(index < last);
+  if (!hit) return false;
+  const int l = __builtin_ctzll(hit);
+  const int f = __builtin_amdgcn_readlane(s.first, l), n = __builtin_amdgcn_readlane(tiles, l);
+  const int k = index - (__builtin_amdgcn_readlane(last, l) - n);
+  t.group = l == 0 || l > groups ? -1 : l - 1;
+  t.end = __builtin_amdgcn_readlane(s.end, l);
+  t.row = KIND == PARTIAL_TILES ? f + (t.end - f) / size * size : f + k * size;
+  return true;
+}
+__device__ __forceinline__ void count_segments(const Segments& s, int size, int& whole, int& partial) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  partial = __popcll(__ballot(row_tiles_of<PARTIAL_TILES>(s.end - s.first, size)));
+  whole = __builtin_amdgcn_readlane(wave_sum_scan(row_tiles_of<WHOLE_TILES>(s.end - s.first, size), lane), WAVE - 1);
+}
+
+// The group, and its rows, at a place in the order of falling sizes (ties by
+// index), by a wavefront whose lanes all call it; above 62 groups the order is
+// the groups' own.
+__device__ __forceinline__ int group_by_size(const int64_t* __restrict__ offsets, int groups, int rows, int place,
+                                             int& lo, int& hi) {
+  if (groups > SEGMENT_GROUPS) {
+    group_range(offsets, place, rows, lo, hi);
+    return place;
+  }
+  const int lane = threadIdx.x & (WAVE - 1);
+  const Segments s = load_segments(offsets, groups, rows);
+  const int size = lane >= 1 && lane <= groups ? s.end - s.first : -1;
   int rank = 0;
-  for (int g = 0; g < groups; ++g) {
+  for (int g = 1; g <= groups; ++g) {
     const int o = __builtin_amdgcn_readlane(size, g);
     rank += o > size || (o == size && g < lane) ? 1 : 0;
   }
-  return __builtin_ctzll(__ballot(lane < groups && rank == place));
+  const int l = __builtin_ctzll(__ballot(size >= 0 && rank == place));
+  lo = __builtin_amdgcn_readlane(s.first, l);
+  hi = __builtin_amdgcn_readlane(s.end, l);
+  return l - 1;
 }
 
 // No more tiles than this come out of `rows` rows in `groups` groups, the

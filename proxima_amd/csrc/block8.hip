@@ -62,58 +62,61 @@ __device__ __forceinline__ void store8(T* __restrict__ row, uint64_t c, uint64_t
 }
 
 // The codes of 8 columns and their block's scale byte; all 16 threads of a
-// block call it together.
+// block call it together. The maximum passes NaN over, and NaN times a scale
+// becomes the NaN code by itself; infinities, which neither does, take the
+// branch.
 __device__ __forceinline__ uint32_t pack8(const float (&x)[8], uint32_t (&code)[2]) {
-  uint32_t m = 0;  // magnitudes order as their bits; infinities and NaN are left out
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu;
-    const uint32_t f = b < 0x7F800000u ? b : 0u;
-    m = f > m ? f : m;
-  }
-  uint32_t o;
-  o = xor_lane<1>(m), m = o > m ? o : m;
-  o = xor_lane<2>(m), m = o > m ? o : m;
-  o = xor_lane<4>(m), m = o > m ? o : m;
-  o = xor_lane<8>(m), m = o > m ? o : m;
-  const uint32_t byte = block8_scale_byte(__builtin_bit_cast(float, m));
-  const float inv = block8_inverse(byte);
+  constexpr float INF = __builtin_inff();
   float y[8];
+  float m = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu;
-    y[i] = b < 0x7F800000u ? x[i] * inv : __builtin_bit_cast(float, 0x7FC00000u);
+    y[i] = x[i];
+    m = fmaxf(m, fabsf(x[i]));
   }
+  if (m == INF) {
+    m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (fabsf(y[i]) == INF) y[i] = __builtin_nanf("");
+      m = fmaxf(m, fabsf(y[i]));
+    }
+  }
+  auto other = [&](uint32_t o) { m = fmaxf(m, __builtin_bit_cast(float, o)); };
+  other(xor_lane<1>(__builtin_bit_cast(uint32_t, m)));
+  other(xor_lane<2>(__builtin_bit_cast(uint32_t, m)));
+  other(xor_lane<4>(__builtin_bit_cast(uint32_t, m)));
+  other(xor_lane<8>(__builtin_bit_cast(uint32_t, m)));
+  const uint32_t byte = block8_scale_byte(m);
+  const float inv = block8_inverse(byte);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i], y[4 * i + 1], 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2], y[4 * i + 3], w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * inv, y[4 * i + 1] * inv, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * inv, y[4 * i + 3] * inv, w, true);
     code[i] = (uint32_t)w;
   }
   return byte;
 }
 
-// Where thread `item` of a launch over rows of `wide` (a multiple of 128)
-// columns is.
+// Where a thread begins: threads of a workgroup are blockDim.x / 16 blocks of
+// 128 columns by blockDim.y rows. The rows are the grid's x; its y are column
+// parts.
 struct Place {
   uint64_t row;
-  uint32_t col;
-  bool live;
-  __device__ Place(uint32_t rows, uint32_t wide) {
-    const uint32_t item = blockIdx.x * ROW_THREADS + threadIdx.x, per = wide / 8;
-    const uint32_t r = item / per;
-    row = r;
-    col = (item - r * per) * 8;
-    live = r < rows;  // uniform over the 16 threads of a block: per is a multiple of 16
+  uint32_t col, step;
+  __device__ Place() {
+    row = (uint64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+    step = gridDim.y * blockDim.x * 8;
   }
 };
 
 // The scale byte of a block, and 127 in the bytes past the row's last block.
 __device__ __forceinline__ void store_scale(uint8_t* __restrict__ scales, const Place& at, uint32_t wide,
-                                            uint32_t sstride, uint32_t byte) {
-  if (at.col % 128) return;
+                                            uint32_t sstride, uint32_t col, uint32_t byte) {
+  if (col % 128) return;
   uint8_t* s = scales + at.row * sstride;
-  const uint32_t b = at.col / 128;
+  const uint32_t b = col / 128;
   s[b] = (uint8_t)byte;
   if (b == wide / 128 - 1)
     for (uint32_t i = b + 1; i < sstride; ++i) s[i] = 127;
@@ -123,42 +126,90 @@ template <class T, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS)
 block8_pack_rows(const T* __restrict__ x, uint64_t xs, uint32_t rows, uint32_t cols, uint32_t wide, uint32_t sstride,
                  uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-  const Place at(rows, wide);
-  if (!at.live) return;
-  float v[8];
-  load8<T, VEC>(x + at.row * xs, at.col, cols, v);
-  uint32_t code[2];
-  const uint32_t byte = pack8(v, code);
-  *reinterpret_cast<uint2*>(codes + at.row * wide + at.col) = make_uint2(code[0], code[1]);
-  store_scale(scales, at, wide, sstride, byte);
+  const Place at;
+  if (at.row >= rows) return;
+  for (uint32_t col = at.col; col < wide; col += at.step) {
+    float v[8];
+    load8<T, VEC>(x + at.row * xs, col, cols, v);
+    uint32_t code[2];
+    const uint32_t byte = pack8(v, code);
+    *reinterpret_cast<uint2*>(codes + at.row * wide + col) = make_uint2(code[0], code[1]);
+    store_scale(scales, at, wide, sstride, col, byte);
+  }
 }
 
 template <class T, bool VEC>
 __global__ void __launch_bounds__(ROW_THREADS)
 block8_unpack_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, uint32_t rows, uint32_t cols,
                    uint32_t wide, uint32_t sstride, T* __restrict__ out, uint64_t os) {
-  const Place at(rows, wide);
-  if (!at.live) return;
-  const uint2 w = *reinterpret_cast<const uint2*>(codes + at.row * wide + at.col);
-  const uint32_t code[2] = {w.x, w.y};
-  float v[8];
-  block8_decode(code, block8_scale(scales[at.row * sstride + at.col / 128]), v);
-  store8<T, VEC>(out + at.row * os, at.col, cols, v);
+  const Place at;
+  if (at.row >= rows) return;
+  for (uint32_t col = at.col; col < wide; col += at.step) {
+    const uint2 w = *reinterpret_cast<const uint2*>(codes + at.row * wide + col);
+    const uint32_t code[2] = {w.x, w.y};
+    float v[8];
+    block8_decode(code, block8_scale(scales[at.row * sstride + col / 128]), v);
+    store8<T, VEC>(out + at.row * os, col, cols, v);
+  }
 }
 
 // f(h) and f'(h) of the activations:
 //   silu: h s, s = 1 / (1 + exp(-h));  s (1 + h (1 - s))
 //   gelu: h P, P = (1 + erf(h / sqrt 2)) / 2;  P + h exp(-h^2 / 2) / sqrt(2 pi)
-template <int ACT>
+//
+// f32 takes the math library's functions. For 16-bit types these would cost
+// more than the memory (gelu's backward pass, 16384 x 4096 in bf16: 90 us with
+// them), so they take the hardware's exp2 and reciprocal, and for gelu one
+// polynomial: 1 - P(|h|) = exp(-h^2 / 2) t R(t), t = 1 / (1 + 0.28 |h|), with R
+// the polynomial of degree 8 of least largest relative error over all h
+// (1.7e-7; 6e-7 evaluated in f32, 2^-11 being half of f16's last place). Its
+// exp is the slope's second term's too.
+template <class T>
+constexpr bool fast_activation = sizeof(T) == 2;
+
+__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// 1 - P(|h|), and exp(-h^2 / 2).
+__device__ __forceinline__ float gelu_tail(float h, float& e) {
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.28f, fabsf(h), 1.0f));
+  float r = 0.0247248504f;
+  r = __builtin_fmaf(r, t, -0.0936122835f);
+  r = __builtin_fmaf(r, t, 0.0924588069f);
+  r = __builtin_fmaf(r, t, -0.00647497689f);
+  r = __builtin_fmaf(r, t, 0.0727872029f);
+  r = __builtin_fmaf(r, t, 0.0836275741f);
+  r = __builtin_fmaf(r, t, 0.103085108f);
+  r = __builtin_fmaf(r, t, 0.111699775f);
+  r = __builtin_fmaf(r, t, 0.111703858f);
+  e = __builtin_amdgcn_exp2f(h * h * -0.72134752f);
+  return e * (t * r);
+}
+
+template <class T, int ACT>
 __device__ __forceinline__ float act_value(float h) {
-  if constexpr (ACT == PXG_SILU) return h / (1.0f + expf(-h));
+  if constexpr (ACT == PXG_SILU) {
+    if constexpr (fast_activation<T>) return h * __builtin_amdgcn_rcpf(1.0f + fast_exp(-h));
+    return h / (1.0f + expf(-h));
+  }
+  if constexpr (fast_activation<T>) {
+    float e;
+    const float q = gelu_tail(h, e);
+    return h * (h < 0.0f ? q : 1.0f - q);
+  }
   return h * (0.5f * (1.0f + erff(h * 0.70710678f)));
 }
-template <int ACT>
+template <class T, int ACT>
 __device__ __forceinline__ float act_slope(float h) {
   if constexpr (ACT == PXG_SILU) {
-    const float s = 1.0f / (1.0f + expf(-h));
+    float s;
+    if constexpr (fast_activation<T>) s = __builtin_amdgcn_rcpf(1.0f + fast_exp(-h));
+    else s = 1.0f / (1.0f + expf(-h));
     return s * (1.0f + h * (1.0f - s));
+  }
+  if constexpr (fast_activation<T>) {
+    float e;
+    const float q = gelu_tail(h, e);
+    return __builtin_fmaf(h * 0.39894228f, e, h < 0.0f ? q : 1.0f - q);
   }
   const float p = 0.5f * (1.0f + erff(h * 0.70710678f));
   return p + h * (0.39894228f * expf(-0.5f * h * h));
@@ -169,17 +220,19 @@ __global__ void __launch_bounds__(ROW_THREADS)
 activation_pack_rows(const T* __restrict__ h, uint64_t hs, uint32_t rows, uint32_t cols, uint32_t wide,
                      uint32_t sstride, T* __restrict__ a, uint64_t as, uint8_t* __restrict__ codes,
                      uint8_t* __restrict__ scales) {
-  const Place at(rows, wide);
-  if (!at.live) return;
-  float v[8], f[8];
-  load8<T, VEC>(h + at.row * hs, at.col, cols, v);
+  const Place at;
+  if (at.row >= rows) return;
+  for (uint32_t col = at.col; col < wide; col += at.step) {
+    float v[8], f[8];
+    load8<T, VEC>(h + at.row * hs, col, cols, v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = act_value<ACT>(v[i]);
-  store8<T, VEC>(a + at.row * as, at.col, cols, f);
-  uint32_t code[2];
-  const uint32_t byte = pack8(v, code);
-  *reinterpret_cast<uint2*>(codes + at.row * wide + at.col) = make_uint2(code[0], code[1]);
-  store_scale(scales, at, wide, sstride, byte);
+    for (int i = 0; i < 8; ++i) f[i] = act_value<T, ACT>(v[i]);
+    store8<T, VEC>(a + at.row * as, col, cols, f);
+    uint32_t code[2];
+    const uint32_t byte = pack8(v, code);
+    *reinterpret_cast<uint2*>(codes + at.row * wide + col) = make_uint2(code[0], code[1]);
+    store_scale(scales, at, wide, sstride, col, byte);
+  }
 }
 
 template <class T, bool VEC, int ACT>
@@ -187,27 +240,30 @@ __global__ void __launch_bounds__(ROW_THREADS)
 activation_grad_rows(const T* __restrict__ g, uint64_t gs, uint32_t rows, uint32_t cols, uint32_t wide,
                      uint32_t sstride, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
                      T* __restrict__ out, uint64_t os) {
-  const Place at(rows, wide);
-  if (!at.live) return;
-  float v[8], d[8];
-  load8<T, VEC>(g + at.row * gs, at.col, cols, d);
-  const uint2 w = *reinterpret_cast<const uint2*>(codes + at.row * wide + at.col);
-  const uint32_t code[2] = {w.x, w.y};
-  block8_decode(code, block8_scale(scales[at.row * sstride + at.col / 128]), v);
+  const Place at;
+  if (at.row >= rows) return;
+  for (uint32_t col = at.col; col < wide; col += at.step) {
+    float v[8], d[8];
+    load8<T, VEC>(g + at.row * gs, col, cols, d);
+    const uint2 w = *reinterpret_cast<const uint2*>(codes + at.row * wide + col);
+    const uint32_t code[2] = {w.x, w.y};
+    block8_decode(code, block8_scale(scales[at.row * sstride + col / 128]), v);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) d[i] *= act_slope<ACT>(v[i]);
-  store8<T, VEC>(out + at.row * os, at.col, cols, d);
+    for (int i = 0; i < 8; ++i) d[i] *= act_slope<T, ACT>(v[i]);
+    store8<T, VEC>(out + at.row * os, col, cols, d);
+  }
 }
 
-// A launch's rows are bounded so that its threads count in 31 bits.
+// Calls launch(grid, block) with a thread for 8 columns: workgroups of one
+// row's 2048 columns, or of several rows of fewer.
 template <class F>
 void by_rows(uint64_t rows, uint64_t wide, F launch) {
-  const uint64_t per = wide / 8, most = ((1ull << 31) - 1) / per;
-  for (uint64_t r = 0; r < rows; r += most) {
-    const uint64_t m = rows - r < most ? rows - r : most;
-    launch(r, (uint32_t)m, dim3((unsigned)((m * per + ROW_THREADS - 1) / ROW_THREADS)));
-    PXG_HIP(hipGetLastError());
-  }
+  uint64_t x = 16;
+  while (x < ROW_THREADS && x * 8 < wide) x *= 2;
+  const uint64_t y = ROW_THREADS / x, parts = (wide / 8 + x - 1) / x;
+  launch(dim3((unsigned)((rows + y - 1) / y), (unsigned)(parts < 1024 ? parts : 1024)),
+         dim3((unsigned)x, (unsigned)y));
+  PXG_HIP(hipGetLastError());
 }
 
 // Calls f with a value of the element type and whether 16-byte accesses are
@@ -252,10 +308,10 @@ int pxg_block8_pack_device(int type, const void* d_x, uint64_t rows, uint64_t co
     const uint64_t wide = block8_code_stride(cols), ss = block8_scale_stride(cols);
     by_type(type, rows_aligned(type, d_x, x_stride), [&](auto t, auto vec) {
       using T = decltype(t);
-      by_rows(rows, wide, [&](uint64_t r, uint32_t m, dim3 grid) {
-        hipLaunchKernelGGL((block8_pack_rows<T, decltype(vec)::value>), grid, dim3(ROW_THREADS), 0,
-                           (hipStream_t)stream, (const T*)d_x + r * x_stride, x_stride, m, (uint32_t)cols,
-                           (uint32_t)wide, (uint32_t)ss, (uint8_t*)d_codes + r * wide, (uint8_t*)d_scales + r * ss);
+      by_rows(rows, wide, [&](dim3 grid, dim3 block) {
+        hipLaunchKernelGGL((block8_pack_rows<T, decltype(vec)::value>), grid, block, 0,
+                           (hipStream_t)stream, (const T*)d_x, x_stride, (uint32_t)rows, (uint32_t)cols,
+                           (uint32_t)wide, (uint32_t)ss, (uint8_t*)d_codes, (uint8_t*)d_scales);
       });
     });
   });
@@ -271,11 +327,11 @@ int pxg_block8_unpack_device(int type, const void* d_codes, const void* d_scales
     const uint64_t wide = block8_code_stride(cols), ss = block8_scale_stride(cols);
     by_type(type, rows_aligned(type, d_out, out_stride), [&](auto t, auto vec) {
       using T = decltype(t);
-      by_rows(rows, wide, [&](uint64_t r, uint32_t m, dim3 grid) {
-        hipLaunchKernelGGL((block8_unpack_rows<T, decltype(vec)::value>), grid, dim3(ROW_THREADS), 0,
-                           (hipStream_t)stream, (const uint8_t*)d_codes + r * wide,
-                           (const uint8_t*)d_scales + r * ss, m, (uint32_t)cols, (uint32_t)wide, (uint32_t)ss,
-                           (T*)d_out + r * out_stride, out_stride);
+      by_rows(rows, wide, [&](dim3 grid, dim3 block) {
+        hipLaunchKernelGGL((block8_unpack_rows<T, decltype(vec)::value>), grid, block, 0,
+                           (hipStream_t)stream, (const uint8_t*)d_codes,
+                           (const uint8_t*)d_scales, (uint32_t)rows, (uint32_t)cols, (uint32_t)wide, (uint32_t)ss,
+                           (T*)d_out, out_stride);
       });
     });
   });
@@ -296,12 +352,12 @@ int pxg_activation_pack_device(int activation, int type, const void* d_h, uint64
     by_type(type, vec, [&](auto t, auto v) {
       using T = decltype(t);
       constexpr bool V = decltype(v)::value;
-      by_rows(rows, wide, [&](uint64_t r, uint32_t m, dim3 grid) {
+      by_rows(rows, wide, [&](dim3 grid, dim3 block) {
         auto kernel = activation == PXG_SILU ? activation_pack_rows<T, V, PXG_SILU>
                                              : activation_pack_rows<T, V, PXG_GELU>;
-        hipLaunchKernelGGL(kernel, grid, dim3(ROW_THREADS), 0, (hipStream_t)stream, (const T*)d_h + r * h_stride,
-                           h_stride, m, (uint32_t)cols, (uint32_t)wide, (uint32_t)ss, (T*)d_a + r * a_stride,
-                           a_stride, (uint8_t*)d_codes + r * wide, (uint8_t*)d_scales + r * ss);
+        hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream, (const T*)d_h,
+                           h_stride, (uint32_t)rows, (uint32_t)cols, (uint32_t)wide, (uint32_t)ss, (T*)d_a,
+                           a_stride, (uint8_t*)d_codes, (uint8_t*)d_scales);
       });
     });
   });
@@ -322,13 +378,13 @@ int pxg_activation_grad_device(int activation, int type, const void* d_grad, uin
     by_type(type, vec, [&](auto t, auto v) {
       using T = decltype(t);
       constexpr bool V = decltype(v)::value;
-      by_rows(rows, wide, [&](uint64_t r, uint32_t m, dim3 grid) {
+      by_rows(rows, wide, [&](dim3 grid, dim3 block) {
         auto kernel = activation == PXG_SILU ? activation_grad_rows<T, V, PXG_SILU>
                                              : activation_grad_rows<T, V, PXG_GELU>;
-        hipLaunchKernelGGL(kernel, grid, dim3(ROW_THREADS), 0, (hipStream_t)stream,
-                           (const T*)d_grad + r * grad_stride, grad_stride, m, (uint32_t)cols, (uint32_t)wide,
-                           (uint32_t)ss, (const uint8_t*)d_codes + r * wide, (const uint8_t*)d_scales + r * ss,
-                           (T*)d_out + r * out_stride, out_stride);
+        hipLaunchKernelGGL(kernel, grid, block, 0, (hipStream_t)stream,
+                           (const T*)d_grad, grad_stride, (uint32_t)rows, (uint32_t)cols, (uint32_t)wide,
+                           (uint32_t)ss, (const uint8_t*)d_codes, (const uint8_t*)d_scales,
+                           (T*)d_out, out_stride);
       });
     });
   });

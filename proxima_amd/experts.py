@@ -12,7 +12,6 @@ groups + 1 values: group g is the rows offsets[g] to offsets[g + 1], and rows
 of no group get zeros.
 """
 import sys
-from collections import namedtuple
 
 from . import DimensionMismatch, _check
 from ._capi import lib as _lib
@@ -25,29 +24,50 @@ __all__ = [
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
-class Block8(namedtuple("Block8", ["codes", "scales", "cols"])):
-    """Rows packed in 8 bits: e4m3 codes (uint8 [rows, cols rounded up to 128])
-    and one power-of-two scale per block of 128 columns (uint8 [rows, blocks
-    rounded up to 4]), as block8_pack lays them out."""
+class Block8:
+    """Rows packed in 8 bits, as block8_pack lays them out: e4m3 codes (uint8
+    [rows, cols rounded up to 128], contiguous) and one power-of-two scale per
+    block of 128 columns (uint8 [rows, blocks rounded up to 4])."""
 
-    __slots__ = ()
+    __slots__ = ("_codes", "_scales", "_cols")
 
-    @property
-    def rows(self):
-        return self.codes.shape[0]
+    def __init__(self, codes, scales, cols):
+        if _torch is None:
+            _setup()
+        for t, what in ((codes, "codes"), (scales, "scales")):
+            if not t.is_cuda or t.dtype is not _torch.uint8 or not t.is_contiguous():
+                raise ValueError(f"{what} must be a contiguous uint8 GPU tensor")
+        if cols < 1:
+            raise ValueError("cols must be at least 1")
+        wide, few = _strides(cols)
+        rows = codes.shape[0]
+        if codes.shape != (rows, wide):
+            _mismatch(tuple(codes.shape), (rows, wide), "codes' shape")
+        if scales.shape != (rows, few):
+            _mismatch(tuple(scales.shape), (rows, few), "scales' shape")
+        self._codes, self._scales, self._cols = codes, scales, cols
+
+    codes = property(lambda self: self._codes)
+    scales = property(lambda self: self._scales)
+    cols = property(lambda self: self._cols)
+    rows = property(lambda self: self._codes.shape[0])
 
     def nbytes(self):
-        return self.codes.numel() + self.scales.numel()
+        return self._codes.numel() + self._scales.numel()
+
+    def __repr__(self):
+        return f"Block8({self.rows} x {self.cols})"
 
 
 # torch is the caller's: this package does not import it by itself. Filled on the first call with a tensor.
 _KINDS = {}  # torch dtype -> pxg_type
-_torch = None
+_torch = _current_device = _current_stream = None
 
 
 def _setup():
-    global _torch
+    global _torch, _current_device, _current_stream
     _torch = sys.modules["torch"]
+    _current_device, _current_stream = _torch._C._cuda_getDevice, _torch._C._cuda_getCurrentRawStream
     _KINDS.update({_torch.float32: 0, _torch.float16: 1, _torch.bfloat16: 2})
 
 
@@ -67,7 +87,7 @@ def _matrix(t, name, dims=2):
     shape = t.shape
     if len(shape) != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got {len(shape)}")
-    if t.stride(-1) != 1 and shape[-1] > 1:
+    if shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have contiguous rows")
     return shape
 
@@ -83,22 +103,11 @@ def _strides(cols):
 
 
 def _packed(p, name):
-    """Checks a Block8; its rows."""
-    if not isinstance(p, Block8):
+    """(codes, scales, rows, cols) of a Block8."""
+    if type(p) is not Block8:
         raise ValueError(f"{name} must be a Block8")
-    codes, scales, cols = p
-    if _torch is None:
-        _setup()
-    for t, what in ((codes, "codes"), (scales, "scales")):
-        if not t.is_cuda or t.dtype is not _torch.uint8 or not t.is_contiguous():
-            raise ValueError(f"{name}.{what} must be a contiguous uint8 GPU tensor")
-    wide, few = _strides(cols)
-    rows = codes.shape[0]
-    if codes.shape != (rows, wide):
-        _mismatch(tuple(codes.shape), (rows, wide), f"{name}.codes' shape")
-    if scales.shape != (rows, few):
-        _mismatch(tuple(scales.shape), (rows, few), f"{name}.scales' shape")
-    return rows
+    codes = p._codes
+    return codes, p._scales, codes.shape[0], p._cols
 
 
 def _groups(offsets):
@@ -137,20 +146,22 @@ def _run(fn, tensors, *args):
     for t in tensors:
         if t is not None and t.get_device() != device:
             raise ValueError("operands must be on one device")
-    stream = _torch._C._cuda_getCurrentRawStream(device)
-    if _torch._C._cuda_getDevice() == device:
-        status = fn(*args, stream)
+    if _current_device() == device:
+        status = fn(*args, _current_stream(device))
     else:
         with _torch.cuda.device(device):
-            status = fn(*args, stream)
+            status = fn(*args, _current_stream(device))
     if status:
         _check(status)
 
 
 def _new_packed(like, rows, cols):
     wide, few = _strides(cols)
-    return Block8(like.new_empty((rows, wide), dtype=_torch.uint8), like.new_empty((rows, few), dtype=_torch.uint8),
-                  cols)
+    p = Block8.__new__(Block8)
+    p._codes = like.new_empty((rows, wide), dtype=_torch.uint8)
+    p._scales = like.new_empty((rows, few), dtype=_torch.uint8)
+    p._cols = cols
+    return p
 
 
 def block8_pack(x, out=None):
@@ -159,9 +170,9 @@ def block8_pack(x, out=None):
     kind = _type(x.dtype, "x")
     if out is None:
         out = _new_packed(x, rows, cols)
-    elif (_packed(out, "out"), out.cols) != (rows, cols):
-        _mismatch((out.rows, out.cols), (rows, cols), "out's shape")
-    codes, scales, _ = out
+    codes, scales, prows, pcols = _packed(out, "out")
+    if prows != rows or pcols != cols:
+        _mismatch((prows, pcols), (rows, cols), "out's shape")
     _run(_lib.pxg_block8_pack_device, (x, codes, scales), kind, x.data_ptr(), rows, cols, _stride(x),
          codes.data_ptr(), scales.data_ptr())
     return out
@@ -169,8 +180,7 @@ def block8_pack(x, out=None):
 
 def block8_unpack(packed, dtype=None, out=None):
     """The values of packed rows as [rows, cols] of `dtype` (bf16 by default; exact there and in f32)."""
-    rows = _packed(packed, "packed")
-    codes, scales, cols = packed
+    codes, scales, rows, cols = _packed(packed, "packed")
     dtype = dtype or (out.dtype if out is not None else _torch.bfloat16)
     kind = _type(dtype, "dtype")
     out, stride = _out(out, (rows, cols), dtype, codes)
@@ -187,9 +197,8 @@ def block8_matmul(x, w, offsets=None, out_dtype=None, out=None):
     Large products into 16 bits are multiplied in 8 bits on the matrix cores,
     which align the eight products of a group to their largest and drop what
     is below about 2^-13 of it; all others are exact up to f32 sums."""
-    rows, wrows = _packed(x, "x"), _packed(w, "w")
-    codes, scales, k = x
-    wcodes, wscales, wk = w
+    codes, scales, rows, k = _packed(x, "x")
+    wcodes, wscales, wrows, wk = _packed(w, "w")
     if wk != k:
         _mismatch(wk, k, "w's columns")
     ptr, groups = _groups(offsets)
@@ -262,10 +271,9 @@ def grouped_matmul_grad_weight(grad, x, offsets, out_dtype=None, out=None):
     dtype = out_dtype or (out.dtype if out is not None else grad.dtype)
     out_kind = _type(dtype, "out_dtype")
     if isinstance(x, Block8):
-        xrows = _packed(x, "x")
+        codes, scales, xrows, k = _packed(x, "x")
         if kind != 2:
             raise ValueError("grad must be bfloat16 with a packed x")
-        codes, scales, k = x
     else:
         xrows, k = _matrix(x, "x")
         if x.dtype is not grad.dtype:
@@ -301,7 +309,7 @@ def activation_pack(h, activation, out=None):
     kind = _type(h.dtype, "h")
     out, stride = _out(out, (rows, cols), h.dtype, h)
     packed = _new_packed(h, rows, cols)
-    codes, scales, _ = packed
+    codes, scales = packed._codes, packed._scales
     _run(_lib.pxg_activation_pack_device, (h, out), which, kind, h.data_ptr(), rows, cols, _stride(h), out.data_ptr(),
          stride, codes.data_ptr(), scales.data_ptr())
     return out, packed
@@ -312,9 +320,9 @@ def activation_grad(grad, packed, activation, out=None):
     which = _activation(activation)
     rows, cols = _matrix(grad, "grad")
     kind = _type(grad.dtype, "grad")
-    if (_packed(packed, "packed"), packed.cols) != (rows, cols):
-        _mismatch((packed.rows, packed.cols), (rows, cols), "packed's shape")
-    codes, scales, _ = packed
+    codes, scales, prows, pcols = _packed(packed, "packed")
+    if prows != rows or pcols != cols:
+        _mismatch((prows, pcols), (rows, cols), "packed's shape")
     out, stride = _out(out, (rows, cols), grad.dtype, grad)
     _run(_lib.pxg_activation_grad_device, (grad, codes, scales, out), which, kind, grad.data_ptr(), rows, cols,
          _stride(grad), codes.data_ptr(), scales.data_ptr(), out.data_ptr(), stride)

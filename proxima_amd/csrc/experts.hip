@@ -91,7 +91,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* p, uint6
 // Copies of 16 (and 4) bytes a lane straight into LDS: lane i's land at
 // lds + 16 i (4 i), zeros for offsets outside the resource. Inline asm, so
 // that the compiler does not wait for them before every LDS read; nothing
-// else in these kernels uses m0. wait_copies() waits for all of them.
+// else in these kernels uses m0. wait_copies() waits for all of them,
+// wait_copies_but<N>() for all but the last N.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t rs, uint32_t offset, uint32_t lds) {
@@ -103,7 +104,11 @@ __device__ __forceinline__ void copy4(__amdgpu_buffer_rsrc_t rs, uint32_t offset
                : "memory", "m0");
 }
 #pragma clang diagnostic pop
-__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies_but() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { wait_copies_but<0>(); }
 
 constexpr uint32_t NOWHERE = 0xFFFFFF00u;  // an offset outside every resource
 
@@ -489,10 +494,17 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       __syncthreads();
     };
     Half even, odd;
-    next(0);
-    stage(0);
-    landed();
-    next(1);
+    if constexpr (is_copied(LA) && is_copied(LB)) {  // the second step's copies fly with the first's
+      next(0);
+      next(1);
+      wait_copies_but<(TM + TN) / 8 / WAVES>();
+      lds_barrier();
+    } else {
+      next(0);
+      stage(0);
+      landed();
+      next(1);
+    }
     read(even, 0, 0);
     for (int step = 0; step < steps - 1; ++step) {
       read(odd, step, 1);
@@ -573,8 +585,6 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     stage_copies(LayoutA{}, WidthA{}, A, 0);
     stage_copies(LayoutB{}, WidthB{}, B, 0);
     scale_copies(0, wave);
-    wait_copies();
-    turn();
     if (wave >= 4) {
       auto part = [&](__amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int step, int i) {
         stage_copy(LayoutA{}, WidthA{}, A, ra, step, (wave & 3) * MT + i);
@@ -586,6 +596,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) part(ra, rb, 1, i);
       }
+      wait_copies_but<2 * MT>();
+      turn();
       turn();
       for (int step = 0; step < steps; ++step) {
         read_step(step);
@@ -610,6 +622,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       }
       wait_copies();  // those of the steps past the last
     } else {
+      wait_copies();
+      turn();
       for (int step = 0; step < steps; ++step) {
         read_step(step);
         turn();

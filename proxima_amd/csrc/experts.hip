@@ -161,7 +161,8 @@ struct Tiled {
   static constexpr int STEP = 128 / BYTES;        // summed elements a stage holds
   static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int SCALES = FP8 ? (TM + TN) * 4 : 0;  // four blocks' scale bytes of each row
-  static constexpr int LDS = 2 * (STAGE + SCALES);
+  // a large tile's stages, or three of half its rows
+  static constexpr int LDS = std::max(2 * (STAGE + SCALES), THREADS == 512 && !FP8 ? 3 * (STAGE - A_BYTES / 2) : 0);
 };
 
 template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
@@ -270,19 +271,18 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     const uint8_t* scales;
     uint64_t stride;  // bytes from row to row
     int limit;        // rows (COLS: columns) of the tile inside the matrix
-    uint32_t place;   // of the tile in a stage
     uint32_t row;     // ROWS: this lane's offset in copy 0
   };
   auto operand = [&](const void* base, uint64_t first, const uint8_t* scales, uint64_t row, uint64_t stride, int limit,
-                     uint32_t place, int bytes) {
-    return Operand{(const char*)base + first * bytes, scales + row, stride * bytes, limit, place,
+                     int bytes) {
+    return Operand{(const char*)base + first * bytes, scales + row, stride * bytes, limit,
                    (lane >> 3) * (uint32_t)(stride * bytes) + (((lane & 7) ^ (lane >> 3)) << 4)};
   };
-  const Operand A = operand(p.a, a0, p.a_scales, sa0, p.as, rows, 0, is_packed(LA) ? 1 : K::BYTES);
-  const Operand B = operand(p.b, b0, p.b_scales, sb0, p.bs, cols, K::A_BYTES, is_packed(LB) ? 1 : K::BYTES);
+  const Operand A = operand(p.a, a0, p.a_scales, sa0, p.as, rows, is_packed(LA) ? 1 : K::BYTES);
+  const Operand B = operand(p.b, b0, p.b_scales, sb0, p.bs, cols, is_packed(LB) ? 1 : K::BYTES);
   const uint32_t lds0 = lds_address(lds);
-  // Part i of n of a step's copies of an operand, by one wavefront, in order
-  // `who`. Steps past the last one copy zeros.
+  // A step's elements of an operand from the tile's first on; none past the
+  // last step, whose copies then write zeros without reading.
   auto stage_resource = [&](auto layout, const Operand& o, int step) {
     const int left = tail - source * K::STEP;  // summed elements from here on
     return decltype(layout)::value == ROWS
@@ -291,8 +291,9 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
                : tile_rsrc(o.base + (uint64_t)source * K::STEP * o.stride,
                            step < steps ? (left - 1) * o.stride + o.limit * 2 : 0);
   };
-  auto stage_copy = [&](auto layout, auto width, const Operand& o, __amdgpu_buffer_rsrc_t rs, int step, int part) {
-    const uint32_t to = lds0 + (step & 1) * K::STAGE + o.place + part * 1024;
+  // one wavefront's part of its copies, to an operand's place in a stage
+  auto stage_copy = [&](auto layout, auto width, const Operand& o, __amdgpu_buffer_rsrc_t rs, int place, int part) {
+    const uint32_t to = lds0 + place + part * 1024;
     if constexpr (decltype(layout)::value == ROWS) {
       uint32_t at = o.row;
       asm volatile("" : "+v"(at));  // keeps one register for all parts, not one for each
@@ -311,12 +312,12 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   using LayoutB = std::integral_constant<int, LB>;
   using WidthA = std::integral_constant<int, TM>;
   using WidthB = std::integral_constant<int, TN>;
-  auto stage_copies = [&](auto layout, auto width, const Operand& o, int step) {
+  auto stage_copies = [&](auto layout, auto width, const Operand& o, int step, int place) {
     if constexpr (is_copied(decltype(layout)::value)) {
       constexpr int N = decltype(width)::value / 8 / WAVES;
       const auto rs = stage_resource(layout, o, step);
 #pragma unroll
-      for (int i = 0; i < N; ++i) stage_copy(layout, width, o, rs, step, wave * N + i);
+      for (int i = 0; i < N; ++i) stage_copy(layout, width, o, rs, place, wave * N + i);
     }
   };
   // Packed: a thread takes 8 codes at a time, of row (COLS: summed element)
@@ -378,9 +379,9 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       });
     }
   };
-  auto store_staged = [&](auto layout, auto width, const Operand& o, int step, const Staged& x) {
+  auto store_staged = [&](auto layout, auto width, const Operand& o, int at, const Staged& x) {
     constexpr int L = decltype(layout)::value, W = decltype(width)::value;
-    char* to = lds + (step & 1) * K::STAGE + o.place;
+    char* to = lds + at;
     auto place = [&](int line, int c) {
       return reinterpret_cast<uint4*>(
           to + (is_rows(L) ? line * 128 + ((c ^ (line & 7)) << 4) : line * (W * 2) + ((c ^ cols_swizzle<W>(line)) << 4)));
@@ -432,6 +433,13 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     // and the next one has landed, so the barrier there frees the one for the
     // step after next and opens the other.
     constexpr int LIVE = decltype(live)::value;
+    // A partial row tile of at most half the rows has room for a third stage,
+    // which its little work needs to hide the copies' latency.
+    constexpr bool DEEP = FORM != GRAD_WEIGHT && is_copied(LB) && K::THREADS == 512 && 2 * LIVE <= MT;
+    constexpr int STAGES = DEEP ? 3 : 2, AW = DEEP ? TM / 2 : TM, STAGE = AW * 128 + K::B_BYTES;
+    constexpr int COPIES = (AW + TN) / 8 / WAVES;  // of a wavefront in a step
+    static_assert(STAGES * STAGE <= K::LDS);
+    using WideA = std::integral_constant<int, AW>;
     const uint32_t fa0 = is_rows(LA) ? rows_at(wm, 0) : cols_at(wm, WidthA{});
     const uint32_t fb0 = is_rows(LB) ? rows_at(wn * NT, 0) : cols_at(wn * NT, WidthB{});
     // the tile j tiles on, summed elements 32 h to 32 h + 31
@@ -452,10 +460,12 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     struct Half {
       uint4 a[LIVE], b[NT];
     };
-    auto read = [&](Half& f, int step, int h) {
-      const char* base = lds + (step & 1) * K::STAGE;
+    int slot = 0;  // the stage of the step being multiplied
+    auto later = [&](int by) { return slot + by < STAGES ? slot + by : slot + by - STAGES; };
+    auto read = [&](Half& f, int at, int h) {
+      const char* base = lds + at * STAGE;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) f.b[j] = fragment(LayoutB{}, WidthB{}, base + K::A_BYTES, fb0, j, h);
+      for (int j = 0; j < NT; ++j) f.b[j] = fragment(LayoutB{}, WidthB{}, base + AW * 128, fb0, j, h);
 #pragma unroll
       for (int i = 0; i < LIVE; ++i) f.a[i] = fragment(LayoutA{}, WidthA{}, base, fa0, i * WM, h);
     };
@@ -478,50 +488,50 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       }
     };
     Staged xa, xb;
-    auto next = [&](int step) {  // a step's copies, and what goes through registers
+    auto next = [&](int step, int at) {  // a step's copies, and what goes through registers
       if (step > 0) advance();
-      stage_copies(LayoutA{}, WidthA{}, A, step);
-      stage_copies(LayoutB{}, WidthB{}, B, step);
+      stage_copies(LayoutA{}, WideA{}, A, step, at * STAGE);
+      stage_copies(LayoutB{}, WidthB{}, B, step, at * STAGE + AW * 128);
       load_staged(LayoutA{}, WidthA{}, A, step, xa);
       load_staged(LayoutB{}, WidthB{}, B, step, xb);
     };
-    auto stage = [&](int step) {
-      store_staged(LayoutA{}, WidthA{}, A, step, xa);
-      store_staged(LayoutB{}, WidthB{}, B, step, xb);
-    };
-    auto landed = [&] {
-      wait_copies();
-      __syncthreads();
+    auto stage = [&](int at) {
+      store_staged(LayoutA{}, WidthA{}, A, at * STAGE, xa);
+      store_staged(LayoutB{}, WidthB{}, B, at * STAGE + AW * 128, xb);
     };
     Half even, odd;
-    if constexpr (is_copied(LA) && is_copied(LB)) {  // the second step's copies fly with the first's
-      next(0);
-      next(1);
-      wait_copies_but<(TM + TN) / 8 / WAVES>();
+    if constexpr (is_copied(LA) && is_copied(LB)) {  // all stages' copies fly together
+#pragma unroll
+      for (int step = 0; step < STAGES; ++step) next(step, step);
+      wait_copies_but<(STAGES - 1) * COPIES>();
       lds_barrier();
     } else {
-      next(0);
+      next(0, 0);
       stage(0);
-      landed();
-      next(1);
+      wait_copies();
+      lds_barrier();
+      next(1, 1);
     }
     read(even, 0, 0);
     for (int step = 0; step < steps - 1; ++step) {
-      read(odd, step, 1);
+      read(odd, slot, 1);
       multiply(even);
       interleave();
-      stage(step + 1);
-      landed();
-      next(step + 2);
-      read(even, step + 1, 0);
+      stage(later(1));
+      if constexpr (is_copied(LA) && is_copied(LB)) wait_copies_but<(STAGES - 2) * COPIES>();
+      else wait_copies();
+      lds_barrier();
+      next(step + STAGES, slot);
+      slot = later(1);
+      read(even, slot, 0);
       multiply(odd);
       interleave();
     }
-    read(odd, steps - 1, 1);
+    read(odd, slot, 1);
     multiply(even);
     interleave();
     multiply(odd);
-    wait_copies();  // those of the step past the last
+    wait_copies();  // those of the steps past the last
   };
   [[maybe_unused]] auto run8 = [&](auto live) {
     // Wavefronts 0 to 3 and 4 to 7, one of each on every SIMD, take turns: one
@@ -582,13 +592,13 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
       const auto rs = tile_rsrc((of_a ? A.scales : B.scales) + source, step < steps ? limit * p.ss - source : 0);
       copy4(rs, r < limit ? (uint32_t)(r * p.ss) : NOWHERE, to + at * 256);
     };
-    stage_copies(LayoutA{}, WidthA{}, A, 0);
-    stage_copies(LayoutB{}, WidthB{}, B, 0);
+    stage_copies(LayoutA{}, WidthA{}, A, 0, 0);
+    stage_copies(LayoutB{}, WidthB{}, B, 0, K::A_BYTES);
     scale_copies(0, wave);
     if (wave >= 4) {
       auto part = [&](__amdgpu_buffer_rsrc_t ra, __amdgpu_buffer_rsrc_t rb, int step, int i) {
-        stage_copy(LayoutA{}, WidthA{}, A, ra, step, (wave & 3) * MT + i);
-        stage_copy(LayoutB{}, WidthB{}, B, rb, step, (wave & 3) * MT + i);
+        stage_copy(LayoutA{}, WidthA{}, A, ra, (step & 1) * K::STAGE, (wave & 3) * MT + i);
+        stage_copy(LayoutB{}, WidthB{}, B, rb, (step & 1) * K::STAGE + K::A_BYTES, (wave & 3) * MT + i);
       };
       {
         advance();

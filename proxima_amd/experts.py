@@ -195,8 +195,8 @@ def block8_matmul(x, w, offsets=None, out_dtype=None, out=None):
     out_dtype (bf16 by default, f16 or f32). Without offsets, one group.
 
     Large products into 16 bits are multiplied in 8 bits on the matrix cores,
-    which align the eight products of a group to their largest and drop what
-    is below about 2^-13 of it; all others are exact up to f32 sums."""
+    which align the products that they sum together to the largest and cut
+    each below 2^-11 of it; all others are exact up to f32 sums."""
     codes, scales, rows, k = _packed(x, "x")
     wcodes, wscales, wrows, wk = _packed(w, "w")
     if wk != k:

@@ -405,6 +405,71 @@ def test_products_in_a_graph(gpu):
             assert torch.equal(a, b)
 
 
+# --- the 8-bit matrix cores ------------------------------------------------------------
+# Products into 16 bits of many rows a group are multiplied in 8 bits. The cores
+# align the products that they sum together to the largest of them and cut each
+# below 2^-11 of it (two products of the type's extremes are off by 2^-10.9 of
+# the larger, never more in 10^5 trials), so products whose magnitudes are
+# within 2^5 of each other are summed exactly, and others within
+# 2^-11 of their block's largest product each.
+LARGE = [([600], 256, 512), ([300, 700], 512, 1024), ([0, 900, 40], 264, 384), ([2500, 3, 1200, 900], 1024, 640),
+         ([4096], 2048, 2048)]
+
+
+def _runs_in_8_bits(px, torch, sizes, n, k):
+    """Whether the result differs from the exactly summed one on values that the cores cut."""
+    x, w, _, offsets = _make(torch, sizes, n, k, torch.bfloat16, 15)
+    p, q = px.block8_pack(x), px.block8_pack(w.reshape(-1, k))
+    return not torch.equal(px.block8_matmul(p, q, offsets),
+                           px.block8_matmul(p, q, offsets, out_dtype=torch.float32).bfloat16())
+
+
+@pytest.mark.parametrize("sizes,n,k", LARGE)
+def test_products_in_8_bits_of_exact_sums(gpu, sizes, n, k):
+    # values of +-1, +-1.5, +-2 and +-4 with a power of two for every block: sums are exact, to the last bit
+    import torch
+    if sizes == [4096]:
+        assert _runs_in_8_bits(gpu, torch, sizes, n, k)
+    g = _dev(torch, n + k)
+    rows = sum(sizes) + 7
+    values = torch.tensor([1.0, 1.5, 2.0, 4.0, -1.0, -1.5, -2.0, -4.0], device="cuda")
+
+    def draw(r):
+        v = values[torch.randint(0, 8, (r, k), generator=g, device="cuda")]
+        scale = torch.exp2(torch.randint(-2, 3, (r, (k + 127) // 128), generator=g, device="cuda").float())
+        return v * scale.repeat_interleave(128, 1)[:, :k]
+
+    x, w = draw(rows), draw(len(sizes) * n)
+    offsets = _offsets(torch, sizes, 3)
+    ends = offsets.tolist()
+    p, q = gpu.block8_pack(x), gpu.block8_pack(w)
+    assert torch.equal(gpu.block8_unpack(p, torch.float32), x)
+    want, _ = _per_row(torch, x, w.view(len(sizes), n, k), ends, True)
+    for dtype in (torch.bfloat16, torch.float16):
+        assert torch.equal(gpu.block8_matmul(p, q, offsets, out_dtype=dtype), want.float().to(dtype))
+
+
+@pytest.mark.parametrize("sizes,n,k", LARGE)
+def test_products_in_8_bits(gpu, sizes, n, k):
+    import torch
+    x, w, _, offsets = _make(torch, sizes, n, k, torch.bfloat16, 16, 5, 11)
+    ends = offsets.tolist()
+    p, q = gpu.block8_pack(x), gpu.block8_pack(w.reshape(-1, k))
+    xv, wv = gpu.block8_unpack(p, torch.float32), gpu.block8_unpack(q, torch.float32).view(w.shape)
+    want, size = _per_row(torch, xv, wv, ends, True)
+    cut = torch.zeros_like(want)  # 128 products of a block, each within 2^-11 of the largest of them at most
+    for b in range(0, k, 128):
+        top, _ = _per_row(torch, xv[:, b:b + 128].abs().amax(1, keepdim=True),
+                          wv[:, :, b:b + 128].abs().amax(2, keepdim=True), ends, True)
+        cut += 128 * 2.0 ** -11 * top
+    for dtype in (torch.bfloat16, torch.float16):
+        got = gpu.block8_matmul(p, q, offsets, out_dtype=dtype).double()
+        bound = cut + 1.25 * k * 2.0 ** -24 * size
+        assert bool(((got - want).abs() <= bound + _unit(dtype) * (want.abs() + bound)).all())
+        # and as a whole: the cuts are of either sign, so far below the sum of their bounds
+        assert float((got - want).norm() / want.norm()) < 2 * _unit(dtype)
+
+
 # --- activations --------------------------------------------------------------------
 def _act64(torch, h, act):
     """(f, f', the magnitudes of their terms) in 64 bits."""
@@ -502,6 +567,20 @@ def test_layer_gradients_against_differences(gpu):
         hi, lo = w.clone(), w.clone()
         hi[e, 7, 9], lo[e, 7, 9] = 16.0, -16.0
         assert abs((loss(x, hi) - loss(x, lo)) / 32.0 - float(dw[e, 7, 9])) <= tol
+
+
+# --- all of them together ---------------------------------------------------------------
+def test_the_adapter_example_learns(gpu, capsys):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "expert_adapters.py")
+    spec = importlib.util.spec_from_file_location("expert_adapters", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    before, after = module.main(docs=20_000, train=16_384, steps=150)
+    with capsys.disabled():
+        print(f"recall {before:.3f} -> {after:.3f} ", end="")
+    assert after > before + 0.3
 
 
 # --- refusals ------------------------------------------------------------------------

@@ -44,8 +44,8 @@ struct Product {
   int rows, groups;     // rows of x and dy
   int m, n, k;
   bool c_vec;           // C's rows are 16-byte aligned
-  int splits = 1;       // grad weight: parts of a group's rows, c then m x n of each group of each part
-  int tile = 0;         // and the tiles chosen with them
+  int limit = 0;              // grad weight: longer groups are summed in parts (groups.hpp)
+  float* workspace = nullptr;  // whose slots are m x n each
 };
 
 template <class T>
@@ -183,25 +183,19 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   int m0, n0, rows, cols, steps, group, tail;
   uint64_t a0, b0;  // first elements of the operands' tiles
   [[maybe_unused]] uint64_t sa0 = 0, sb0 = 0;  // and their rows, packed
-  uint64_t c_first = 0;                        // of the result's part
+  [[maybe_unused]] int slot = -1;              // of the workspace, for a group summed in parts
   if constexpr (FORM == GRAD_WEIGHT) {
-    // an eighth of every group's tiles, the longest group first
+    // an eighth of every part's tiles, the longest part first
     const int tiles_m = (p.m + TM - 1) / TM, each = tiles_m * tiles_n, per = (each + 7) / 8;
-    const int t = die * per + at % per, part = at / per;
-    if (t >= each) return;
-    int lo, hi;
-    group = group_by_size(p.offsets, p.groups, p.rows, part / p.splits, lo, hi);
+    const int t = die * per + at % per;
+    GroupPart part;
+    if (t >= each || !find_group_part(p.offsets, p.groups, p.rows, p.limit, at / per, part)) return;
+    group = part.group;
+    slot = part.parts > 1 ? part.slot : -1;
+    const int lo = part.lo, hi = part.hi;
     m0 = t / tiles_n * TM;
     n0 = t % tiles_n * TN;
     rows = p.m - m0;
-    if (p.splits > 1) {  // whole steps a part
-      const int split = part % p.splits;
-      const int64_t size = (hi - lo + p.splits * K::STEP - 1) / (p.splits * K::STEP) * K::STEP;
-      const int64_t from = lo + size * split;
-      lo = from < hi ? (int)from : hi;
-      hi = from + size < hi ? (int)(from + size) : hi;
-      c_first = (uint64_t)split * p.groups * p.cg;
-    }
     tail = hi - lo;
     a0 = (uint64_t)lo * p.as + m0;
     b0 = (uint64_t)lo * p.bs + n0;
@@ -659,40 +653,47 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   // A lane holds columns 4 q to 4 q + 3 of row r16 of each tile. Through LDS,
   // 16 rows of the wavefront's columns at a time, so that what is stored
   // together is whole rows of them.
-  constexpr int EACH = 16 / sizeof(O), PER = NT * 16 / EACH;  // a lane's elements, lanes to a row
-  constexpr int PITCH = NT * 16 * sizeof(O) + 16;             // 16 bytes more spread the rows over the banks
-  static_assert(WAVES * 16 * PITCH <= K::LDS);
-  lds_barrier();
-  char* mine = lds + wave * (16 * PITCH);
-  O* c = (O*)p.c + c_first + group * p.cg + (uint64_t)m0 * p.cs + n0;
-  const int col = wn * NT * 16 + lane % PER * EACH;
+  auto store = [&](auto type, void* result, uint64_t stride, bool whole) {
+    using R = decltype(type);
+    constexpr int EACH = 16 / sizeof(R), PER = NT * 16 / EACH;  // a lane's elements, lanes to a row
+    constexpr int PITCH = NT * 16 * sizeof(R) + 16;             // 16 bytes more spread the rows over the banks
+    static_assert(WAVES * 16 * PITCH <= K::LDS);
+    char* mine = lds + wave * (16 * PITCH);
+    R* c = (R*)result + (uint64_t)m0 * stride + n0;
+    const int col = wn * NT * 16 + lane % PER * EACH;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
+    for (int i = 0; i < MT; ++i) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      typedef O o4v __attribute__((ext_vector_type(4)));
-      o4v v;
+      for (int j = 0; j < NT; ++j) {
+        typedef R r4v __attribute__((ext_vector_type(4)));
+        r4v v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (O)acc[i][j][e];
-      *reinterpret_cast<o4v*>(mine + r16 * PITCH + (j * 16 + 4 * q) * sizeof(O)) = v;
-    }
+        for (int e = 0; e < 4; ++e) v[e] = (R)acc[i][j][e];
+        *reinterpret_cast<r4v*>(mine + r16 * PITCH + (j * 16 + 4 * q) * sizeof(R)) = v;
+      }
 #pragma unroll
-    for (int h = 0; h < 16 * PER / 64; ++h) {
-      const int r = lane / PER + h * (64 / PER), row = (i * WM + wm) * 16 + r;
-      const uint4 v = *reinterpret_cast<const uint4*>(mine + r * PITCH + lane % PER * 16);
-      if (row >= rows) continue;
-      O* to = c + (uint64_t)row * p.cs + col;
-      if (p.c_vec && col + EACH <= cols) {
-        *reinterpret_cast<uint4*>(to) = v;
-      } else {
-        O x[EACH];
-        *reinterpret_cast<uint4*>(x) = v;
+      for (int h = 0; h < 16 * PER / 64; ++h) {
+        const int r = lane / PER + h * (64 / PER), row = (i * WM + wm) * 16 + r;
+        const uint4 v = *reinterpret_cast<const uint4*>(mine + r * PITCH + lane % PER * 16);
+        if (row >= rows) continue;
+        R* to = c + (uint64_t)row * stride + col;
+        if (whole && col + EACH <= cols) {
+          *reinterpret_cast<uint4*>(to) = v;
+        } else {
+          R x[EACH];
+          *reinterpret_cast<uint4*>(x) = v;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e)
-          if (col + e < cols) to[e] = x[e];
+          for (int e = 0; e < EACH; ++e)
+            if (col + e < cols) to[e] = x[e];
+        }
       }
     }
-  }
+  };
+  lds_barrier();
+  if (FORM == GRAD_WEIGHT && slot >= 0)
+    store(float{}, p.workspace + (uint64_t)slot * p.m * p.n, p.n, p.n % 4 == 0);
+  else
+    store(O{}, (O*)p.c + group * p.cg, p.cs, p.c_vec);
 #endif
 }
 
@@ -862,25 +863,26 @@ void check_out_type(int type, int out_type) {
     config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
 }
 
-// The parts of each element, in order: a grid of rows of dw by 256 columns.
+// The sums of divided groups: a grid of (such group, row of dw) by 1024
+// columns adds the parts of each element in order.
 template <class O>
-__global__ void __launch_bounds__(256)
-join_parts(const float* __restrict__ parts, int splits, uint64_t part, int n, int k, O* __restrict__ out, uint64_t os,
-           uint64_t og) {
-  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
-  if (c >= k) return;
-  const uint64_t row = blockIdx.x;
-  const float* from = parts + row * k + c;
-  O* to = out + row / n * og + row % n * os + c;
-  if (c + 4 <= k && k % 4 == 0) {
+__global__ void __launch_bounds__(256) join_parts(Product p) {
+  GroupPart g;
+  if (!find_divided_group(p.offsets, p.groups, p.rows, p.limit, (int)(blockIdx.x / p.m), g)) return;
+  const int row = (int)(blockIdx.x % p.m), c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (c >= p.n) return;
+  const uint64_t part = (uint64_t)p.m * p.n;
+  const float* from = p.workspace + g.slot * part + (uint64_t)row * p.n + c;
+  O* to = (O*)p.c + g.group * p.cg + row * p.cs + c;
+  if (p.n % 4 == 0) {
     f4v x = *reinterpret_cast<const f4v*>(from);
-    for (int s = 1; s < splits; ++s) x += *reinterpret_cast<const f4v*>(from + s * part);
+    for (int s = 1; s < g.parts; ++s) x += *reinterpret_cast<const f4v*>(from + s * part);
 #pragma unroll
     for (int e = 0; e < 4; ++e) to[e] = (O)x[e];
   } else {
-    for (int e = 0; e < 4 && c + e < k; ++e) {
+    for (int e = 0; e < 4 && c + e < p.n; ++e) {
       float x = from[e];
-      for (int s = 1; s < splits; ++s) x += from[s * part + e];
+      for (int s = 1; s < g.parts; ++s) x += from[s * part + e];
       to[e] = (O)x;
     }
   }
@@ -891,7 +893,8 @@ void launch_tiled(const Product& p, hipStream_t s) {
   using K = Tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>;
   const uint64_t tn = (p.n + K::TN - 1) / K::TN;
   uint64_t tiles;
-  if (FORM == GRAD_WEIGHT) tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * p.groups * p.splits;
+  if (FORM == GRAD_WEIGHT)
+    tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * group_parts_max(p.rows, p.groups, p.limit);
   else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn / 8 + 2) * 8;  // both kinds' eighths
   hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), dim3(grid_size(tiles)), dim3(K::THREADS), 0, s,
                      p);
@@ -923,45 +926,63 @@ struct Tile {
 };
 constexpr Tile TILES[3] = {{256, 256, 6, 1.15, 0.45}, {128, 512, 4, 0.7, 0.35}, {64, 1024, 3, 0.42, 0.3}};
 constexpr Tile PACKED_TILES[3] = {{256, 256, 6, 0.6, 0.25}, {128, 512, 4, 0.95, 0.45}, {64, 1024, 3, 0.6, 0.4}};
-constexpr double JOIN_BYTES_PER_US = 4e6, JOIN_US = 4;
-constexpr int SPLITS_MAX = 32;
+// Joining the parts of divided groups: a launch, and their bytes twice.
+constexpr double JOIN_US = 4, JOIN_BYTES_PER_US = 4e6;
 
 struct Cost {
   double best = 1e30, fp8 = 1e30;
-  int tile = 64, splits = 1;
+  int tile = 64, limit = 0;
 };
-// packed: the first of PACKED_TILES is the fp8 product's, not among the choice
+// packed: the first of PACKED_TILES is the fp8 product's, not among the choice.
+// Weight gradients: routers' groups are uneven, so the longest of g is taken as
+// sqrt(g) averages; its tiles, or its parts', are the last to end. Between one part a
+// group and many, in us at each one's best tile (a part's greatest length):
+//   1 group of 16384 rows, 2048 x 2048            188 -> 122 (4096)
+//   1 of 4096, 768 x 768                           36 ->  21 (1536)
+//   8 uneven ones, 16384 rows in all, 512 x 512    39 ->  30 (1024)
+//   8 uneven, 8192 rows, 4096 x 1024               63 ->  87 (2048): the sums' traffic
 Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0) {
   Cost best;
-  const double summed = form == GRAD_WEIGHT ? (double)p.rows / p.groups : p.k;
+  const double average = form == GRAD_WEIGHT ? (double)p.rows / p.groups : p.k;
+  const double longest = form == GRAD_WEIGHT ? average * std::sqrt((double)p.groups) : p.k;
   for (int i = 0; i < 3; ++i) {
     const Tile& t = packed ? PACKED_TILES[i] : TILES[i];
     const uint64_t tn = ((uint64_t)p.n + t.size - 1) / t.size;
-    const uint64_t tiles = form == GRAD_WEIGHT ? p.groups * (((uint64_t)p.m + t.size - 1) / t.size) * tn
+    const uint64_t tiles = form == GRAD_WEIGHT ? (((uint64_t)p.m + t.size - 1) / t.size) * tn
                                                : (p.rows + (uint64_t)p.groups * t.size / 2 + t.size - 1) / t.size * tn;
-    for (int splits = 1; splits <= SPLITS_MAX; splits *= 2) {
-      const double bytes = splits > 1 ? 4.0 * splits * p.groups * p.m * p.n : 0;
-      if (splits > 1 && (form != GRAD_WEIGHT || bytes > (double)room || summed < 128.0 * splits)) break;
-      const double full = std::min(1.0, (double)tiles * splits / t.slots);
-      const double each = t.fixed + std::ceil(summed / splits / 64) * (t.least + t.more * full);
+    for (int parts = 1; parts <= 32; parts *= 2) {
+      const uint64_t limit = parts == 1 ? 0 : ((uint64_t)(longest / parts) + 63) / 64 * 64;
+      uint64_t all = tiles, bytes = 0;
+      if (form == GRAD_WEIGHT) {
+        const uint64_t slots = group_slots_max(p.rows, p.groups, limit);
+        bytes = 4 * slots * p.m * p.n;
+        if (parts > 1 && (limit < 128 || p.groups > SEGMENT_GROUPS || bytes > room)) break;
+        all *= group_parts_max(p.rows, p.groups, limit);
+      } else if (parts > 1) {
+        break;
+      }
+      const double step = t.least + t.more * std::min(1.0, (double)all / t.slots);
+      const double summed = form == GRAD_WEIGHT ? (double)tiles * p.rows / all : p.k;
       // one group's half tile of padding does not begin a round
-      const double rounds = std::ceil((double)tiles * splits / t.slots - (p.groups == 1 ? 0.12 : 0.0));
-      const double us = std::max(1.0, rounds) * each +
-                        (splits > 1 ? JOIN_US + 2 * bytes / JOIN_BYTES_PER_US : 0);
+      const double rounds = std::ceil((double)all / t.slots - (p.groups == 1 ? 0.12 : 0.0));
+      double us = std::max(1.0, rounds) * (t.fixed + std::ceil(summed / 64) * step);
+      us = std::max(us, t.fixed + (limit ? (double)limit : longest) / 64 * step);
+      if (limit) us += JOIN_US + 2.0 * bytes / JOIN_BYTES_PER_US;
       if (packed && i == 0) {
         best.fp8 = us;
       } else if (us < best.best) {
         best.best = us;
         best.tile = t.size;
-        best.splits = splits;
+        best.limit = (int)limit;
       }
     }
   }
   return best;
 }
 
+// `room`: bytes of p.workspace.
 template <int FORM, class T, class O, bool IS_PACKED>
-void launch_product(Product p, hipStream_t s) {
+void launch_product(Product p, uint64_t room, hipStream_t s) {
   p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % 16 == 0;
   constexpr int LA = FORM == GRAD_WEIGHT ? COLS : FORM == FORWARD && IS_PACKED ? PACKED_ROWS : ROWS;
   constexpr int LB = FORM == GRAD_INPUT ? COLS : FORM == GRAD_WEIGHT ? (IS_PACKED ? PACKED_COLS : COLS) : LA;
@@ -974,54 +995,43 @@ void launch_product(Product p, hipStream_t s) {
     if (copied && each <= 16 && (FORM == FORWARD || p.k * p.bs * 2 <= 0x7FFFFFFF))
       return launch_few<T, O, FORM == FORWARD ? ROWS : COLS, IS_PACKED, 1>(p, s);
   }
-  Cost cost = product_cost(FORM, p, FORM == FORWARD && IS_PACKED);
-  if (p.splits > 1) cost.tile = p.tile;
+  const Cost cost = product_cost(FORM, p, FORM == FORWARD && IS_PACKED, room);
+  if constexpr (FORM == GRAD_WEIGHT) p.limit = cost.limit;
   if constexpr (FORM == FORWARD && IS_PACKED && !std::is_same_v<O, float>)
     if (each >= 192 && cost.fp8 <= cost.best) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
   if (copied) {
-    if constexpr (LA != PACKED_ROWS)
-      if (cost.tile == 256) return launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
-    if (cost.tile >= 128) launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
-    else launch_tiled<T, O, FORM, LA, LB, 2, 2, 2, 2>(p, s);
+    if (LA != PACKED_ROWS && cost.tile == 256) {
+      if constexpr (LA != PACKED_ROWS) launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
+    } else if (cost.tile >= 128) {
+      launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
+    } else {
+      launch_tiled<T, O, FORM, LA, LB, 2, 2, 2, 2>(p, s);
+    }
   } else if constexpr (!is_packed(LA)) {
     constexpr int AA = FORM == GRAD_WEIGHT ? ANY_COLS : ANY_ROWS;
     constexpr int AB = is_packed(LB) ? LB : FORM == FORWARD ? ANY_ROWS : ANY_COLS;
     if (cost.tile >= 128) launch_tiled<T, O, FORM, AA, AB, 2, 2, 4, 4>(p, s);
     else launch_tiled<T, O, FORM, AA, AB, 2, 2, 2, 2>(p, s);
   }
+  if (FORM == GRAD_WEIGHT && p.limit) {
+    const uint64_t divided = std::min<uint64_t>(p.groups, p.rows / p.limit);
+    if (divided) {
+      const dim3 grid(grid_size(divided * p.m), (unsigned)(((uint64_t)p.n + 1023) / 1024));
+      hipLaunchKernelGGL(join_parts<O>, grid, dim3(256), 0, s, p);
+      PXG_HIP(hipGetLastError());
+    }
+  }
 }
 
 template <int FORM>
-void run_product(int type, int out_type, const Product& p, hipStream_t s) {
+void run_product(int type, int out_type, const Product& p, hipStream_t s, uint64_t room = 0) {
   by_types(type, out_type, [&](auto t, auto o) {
     using T = decltype(t);
     using O = decltype(o);
     if constexpr (FORM == GRAD_WEIGHT && std::is_same_v<T, __bf16>) {
-      if (p.b_scales) return launch_product<FORM, T, O, true>(p, s);
+      if (p.b_scales) return launch_product<FORM, T, O, true>(p, room, s);
     }
-    launch_product<FORM, T, O, false>(p, s);
-  });
-}
-
-// A weight gradient whose groups are long and whose matrices are few tiles:
-// parts of each group's rows go to workgroups of their own, their sums to the
-// workspace, and are joined in order.
-void run_grad_weight(int type, int out_type, const Product& whole, void* workspace, uint64_t bytes, hipStream_t s) {
-  const Cost cost = product_cost(GRAD_WEIGHT, whole, false, workspace ? bytes : 0);
-  if (cost.splits == 1) return run_product<GRAD_WEIGHT>(type, out_type, whole, s);
-  Product p = whole;
-  p.splits = cost.splits;
-  p.tile = cost.tile;
-  p.c = workspace;
-  p.cs = p.n;
-  p.cg = (uint64_t)p.m * p.n;
-  run_product<GRAD_WEIGHT>(type, PXG_F32, p, s);
-  by_types(type, out_type, [&](auto, auto o) {
-    using O = decltype(o);
-    const dim3 grid(grid_size((uint64_t)p.groups * p.m), (unsigned)((p.n + 1023) / 1024));
-    hipLaunchKernelGGL(join_parts<O>, grid, dim3(256), 0, s, (const float*)workspace, p.splits, p.groups * p.cg, p.m,
-                       p.n, (O*)whole.c, whole.cs, whole.cg);
-    PXG_HIP(hipGetLastError());
+    launch_product<FORM, T, O, false>(p, room, s);
   });
 }
 
@@ -1084,9 +1094,8 @@ uint64_t pxg_grouped_matmul_grad_weight_workspace(uint64_t rows, uint64_t n, uin
   p.groups = (int)groups;
   p.m = (int)n;
   p.n = (int)k;
-  p.splits = 1;
   const Cost cost = product_cost(GRAD_WEIGHT, p, false, UINT64_MAX);
-  return cost.splits == 1 ? 0 : 4 * cost.splits * groups * n * k;
+  return 4 * group_slots_max(rows, groups, cost.limit) * n * k;
 }
 
 int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t rows, uint64_t n,
@@ -1109,7 +1118,8 @@ int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t
     x_stride = check_stride(rows, k, x_stride);
     Product p{d_grad, d_x, d_dw, d_offsets, grad_stride, x_stride, dw_stride, 0, dw_group_stride, nullptr, nullptr, 0, (int)rows,
               (int)groups, (int)n, (int)k, 0, false};
-    run_grad_weight(type, out_type, p, d_workspace, workspace_bytes, (hipStream_t)stream);
+    p.workspace = (float*)d_workspace;
+    run_product<GRAD_WEIGHT>(type, out_type, p, (hipStream_t)stream, d_workspace ? workspace_bytes : 0);
   });
 }
 
@@ -1132,7 +1142,8 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
     check_stride(2, k, block8_code_stride(k));
     Product p{d_grad, d_codes, d_dw, d_offsets, grad_stride, block8_code_stride(k), dw_stride, 0, dw_group_stride,
               nullptr, (const uint8_t*)d_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)n, (int)k, 0, false};
-    run_grad_weight(PXG_BF16, out_type, p, d_workspace, workspace_bytes, (hipStream_t)stream);
+    p.workspace = (float*)d_workspace;
+    run_product<GRAD_WEIGHT>(PXG_BF16, out_type, p, (hipStream_t)stream, d_workspace ? workspace_bytes : 0);
   });
 }
 
@@ -1153,9 +1164,9 @@ int pxg_block8_matmul_device(const void* d_codes, const void* d_scales, uint64_t
               (const uint8_t*)d_w_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)rows, (int)n,
               (int)wide, false};
     const hipStream_t s = (hipStream_t)stream;
-    if (out_type == PXG_F32) launch_product<FORWARD, __bf16, float, true>(p, s);
-    else if (out_type == PXG_F16) launch_product<FORWARD, __bf16, _Float16, true>(p, s);
-    else launch_product<FORWARD, __bf16, __bf16, true>(p, s);
+    if (out_type == PXG_F32) launch_product<FORWARD, __bf16, float, true>(p, 0, s);
+    else if (out_type == PXG_F16) launch_product<FORWARD, __bf16, _Float16, true>(p, 0, s);
+    else launch_product<FORWARD, __bf16, __bf16, true>(p, 0, s);
   });
 }
 

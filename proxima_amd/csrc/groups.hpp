@@ -165,27 +165,82 @@ __device__ __forceinline__ void count_segments(const Segments& s, int size, int&
   whole = __builtin_amdgcn_readlane(wave_sum_scan(row_tiles_of<WHOLE_TILES>(s.end - s.first, size), lane), WAVE - 1);
 }
 
-// The group, and its rows, at a place in the order of falling sizes (ties by
-// index), by a wavefront whose lanes all call it; above 62 groups the order is
-// the groups' own.
-__device__ __forceinline__ int group_by_size(const int64_t* __restrict__ offsets, int groups, int rows, int place,
-                                             int& lo, int& hi) {
+// A group's rows are summed in one part, or, longer than `limit` rows
+// (limit > 0), in as few parts as keep each within it, whole steps of 64 rows.
+// Parts of divided groups have slots of a workspace, in the groups' order.
+// Above 62 groups none is divided.
+struct GroupPart {
+  int group, lo, hi;
+  int parts, slot;  // of the group; this part's slot where there are several
+};
+__device__ __forceinline__ int group_parts(int size, int limit) {
+  return limit > 0 && size > limit ? (size + limit - 1) / limit : 1;
+}
+
+// The part at a place in the order of falling lengths (ties by index; above 62
+// groups the groups' own order), by a wavefront whose lanes all call it; false
+// past the last.
+__device__ __forceinline__ bool find_group_part(const int64_t* __restrict__ offsets, int groups, int rows, int limit,
+                                                int place, GroupPart& g) {
   if (groups > SEGMENT_GROUPS) {
-    group_range(offsets, place, rows, lo, hi);
-    return place;
+    if (place >= groups) return false;
+    group_range(offsets, place, rows, g.lo, g.hi);
+    g.group = place;
+    g.parts = 1;
+    g.slot = 0;
+    return true;
   }
   const int lane = threadIdx.x & (WAVE - 1);
   const Segments s = load_segments(offsets, groups, rows);
-  const int size = lane >= 1 && lane <= groups ? s.end - s.first : -1;
-  int rank = 0;
-  for (int g = 1; g <= groups; ++g) {
-    const int o = __builtin_amdgcn_readlane(size, g);
-    rank += o > size || (o == size && g < lane) ? 1 : 0;
+  const bool real = lane >= 1 && lane <= groups;
+  const int size = s.end - s.first, parts = real ? group_parts(size, limit) : 0;
+  const int length = parts > 1 ? ((size + parts - 1) / parts + 63) / 64 * 64 : size;
+  int before = 0;
+  for (int o = 1; o <= groups; ++o) {
+    const int l = __builtin_amdgcn_readlane(length, o), n = __builtin_amdgcn_readlane(parts, o);
+    before += l > length || (l == length && o < lane) ? n : 0;
   }
-  const int l = __builtin_ctzll(__ballot(size >= 0 && rank == place));
-  lo = __builtin_amdgcn_readlane(s.first, l);
-  hi = __builtin_amdgcn_readlane(s.end, l);
-  return l - 1;
+  const int slots = parts > 1 ? parts : 0, slot = wave_sum_scan(slots, lane) - slots;
+  const uint64_t hit = __ballot(real && place >= before && place < before + parts);
+  if (!hit) return false;
+  const int l = __builtin_ctzll(hit), k = place - __builtin_amdgcn_readlane(before, l);
+  const int first = __builtin_amdgcn_readlane(s.first, l), end = __builtin_amdgcn_readlane(s.end, l);
+  const int64_t from = first + (int64_t)k * __builtin_amdgcn_readlane(length, l);
+  const int64_t to = from + __builtin_amdgcn_readlane(length, l);
+  g.group = l - 1;
+  g.lo = from < end ? (int)from : end;
+  g.hi = to < end ? (int)to : end;
+  g.parts = __builtin_amdgcn_readlane(parts, l);
+  g.slot = __builtin_amdgcn_readlane(slot, l) + k;
+  return true;
+}
+
+// Divided group `index` in the groups' order: itself, its parts and its first
+// slot; false past the last.
+__device__ __forceinline__ bool find_divided_group(const int64_t* __restrict__ offsets, int groups, int rows, int limit,
+                                                   int index, GroupPart& g) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  const Segments s = load_segments(offsets, groups, rows);
+  const int parts = lane >= 1 && lane <= groups ? group_parts(s.end - s.first, limit) : 0;
+  const int slots = parts > 1 ? parts : 0, slot = wave_sum_scan(slots, lane) - slots;
+  const int nth = wave_sum_scan(parts > 1 ? 1 : 0, lane);
+  const uint64_t hit = __ballot(parts > 1 && nth == index + 1);
+  if (!hit) return false;
+  const int l = __builtin_ctzll(hit);
+  g = {l - 1, __builtin_amdgcn_readlane(s.first, l), __builtin_amdgcn_readlane(s.end, l),
+       __builtin_amdgcn_readlane(parts, l), __builtin_amdgcn_readlane(slot, l)};
+  return true;
+}
+
+// No more parts, and no more slots, than this.
+inline uint64_t group_parts_max(uint64_t rows, uint64_t groups, uint64_t limit) {
+  if (groups == 1 && limit) return (rows + limit - 1) / limit;
+  return limit ? groups + rows / limit : groups;
+}
+inline uint64_t group_slots_max(uint64_t rows, uint64_t groups, uint64_t limit) {
+  if (groups == 1 && limit) return (rows + limit - 1) / limit;
+  const uint64_t divided = limit ? rows / limit : 0;
+  return divided + (divided < groups ? divided : groups);
 }
 
 // No more tiles than this come out of `rows` rows in `groups` groups, the

@@ -151,8 +151,8 @@ __device__ __forceinline__ void eighth(int n, int die, int& first, int& size) {
 #endif
 
 // WM x WN wavefronts, each with MT x NT tiles of 16 x 16. T is the type
-// multiplied (bf16, f16 or Fp8), O the result's.
-template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
+// multiplied: bf16, f16 or Fp8.
+template <class T, int WM, int WN, int MT, int NT>
 struct Tiled {
   static constexpr int THREADS = 64 * WM * WN, WAVES = WM * WN;
   static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT;
@@ -168,7 +168,7 @@ struct Tiled {
 template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
 __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using K = Tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>;
+  using K = Tiled<T, WM, WN, MT, NT>;
   constexpr int TM = K::TM, TN = K::TN, WAVES = K::WAVES;
   __shared__ __align__(1024) char lds[K::LDS];
   const int lane = threadIdx.x & 63;
@@ -645,8 +645,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     else run16(live);
   };
   if (steps > 0) {
-    if (MT >= 4 && rows <= TM / 4) run(std::integral_constant<int, (MT + 3) / 4>{});
-    else if (rows <= TM / 2) run(std::integral_constant<int, MT / 2>{});
+    if (FORM != GRAD_WEIGHT && rows <= TM / 2) run(std::integral_constant<int, MT / 2>{});
     else run(std::integral_constant<int, MT>{});
   }
 
@@ -698,36 +697,33 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows in a group: the time is that of reading the matrices. A workgroup
-// takes 16 MT rows and 16 rows of a matrix (COLS: 128 of its columns); its
+// Few rows: the time is that of reading the matrices. A workgroup
+// takes 16 rows and 16 rows of a matrix (COLS: 128 of its columns); its
 // eight wavefronts read 128 bytes of each row (COLS: 32 rows) in turn, straight
 // into the registers that the matrix cores take, and their partial sums are
 // added in LDS, in order.
 // ---------------------------------------------------------------------------
-template <class T, class O, int LB, bool IS_PACKED, int MT>
-__global__ void __launch_bounds__(512) product_few(Product p) {
+template <class T, class O, int LB, bool IS_PACKED>
+__global__ void __launch_bounds__(512, 4) product_few(Product p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int WAVES = 8, N16 = LB == ROWS ? 1 : 8;     // tiles of 16 columns of C
   constexpr int TN = 16 * N16, PIECES = LB == ROWS ? 2 : 1;  // loads of a row (ROWS) in a round
   constexpr int ROUND = LB == ROWS ? (IS_PACKED ? 128 : 64) : 32;  // summed elements of a wavefront's round
-  constexpr int AHEAD = LB == ROWS ? (IS_PACKED || MT > 1 ? (MT > 2 ? 2 : 4) : 8) : 1;  // rounds loaded before they are multiplied
-  __shared__ f4v part[WAVES][N16 * MT][64];
+  constexpr int AHEAD = IS_PACKED ? 1 : 2;  // ROWS: rounds loaded before they are multiplied
+  __shared__ f4v part[WAVES][N16][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_n = (p.n + TN - 1) / TN;
   RowTile t;
-  if (!find_row_tile<ALL_TILES>(p.offsets, p.groups, p.rows, 16 * MT, (int)(blockIdx.x / tiles_n), t)) return;
+  if (!find_row_tile<ALL_TILES>(p.offsets, p.groups, p.rows, 16, (int)(blockIdx.x / tiles_n), t)) return;
   const int n0 = (int)(blockIdx.x % tiles_n) * TN;
-  const int rows = t.end - t.row < 16 * MT ? t.end - t.row : 16 * MT, cols = p.n - n0 < TN ? p.n - n0 : TN;
+  const int rows = t.end - t.row < 16 ? t.end - t.row : 16, cols = p.n - n0 < TN ? p.n - n0 : TN;
   const int k_end = t.group < 0 ? 0 : p.k, group = t.group < 0 ? 0 : t.group;
   constexpr int BYTES = IS_PACKED ? 1 : 2;
   const auto ra = tile_rsrc((const char*)p.a + (uint64_t)t.row * p.as * BYTES,
                             ((uint64_t)(rows - 1) * p.as + p.k) * BYTES);
-  uint32_t oa[MT];  // this lane's rows of A
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-    oa[i] = 16 * i + r16 < rows ? (uint32_t)((16 * i + r16) * p.as * BYTES) + q * 16 : NOWHERE;
-  f4v acc[N16][MT] = {};
+  const uint32_t oa = r16 < rows ? (uint32_t)(r16 * p.as * BYTES) + q * 16 : NOWHERE;  // this lane's row of A
+  f4v acc[N16] = {};
   typedef uint32_t u4v __attribute__((ext_vector_type(4)));
   auto load = [&](__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
     return __builtin_bit_cast(uint4, (u4v)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)offset, 0, 0));
@@ -743,8 +739,8 @@ __global__ void __launch_bounds__(512) product_few(Product p) {
       rsb = tile_rsrc(p.b_scales + row * p.ss, (uint64_t)cols * p.ss);
     }
     for (int k0 = wave * ROUND; k0 < k_end; k0 += WAVES * ROUND * AHEAD) {
-      uint4 b[AHEAD][PIECES], a[AHEAD][PIECES][MT];
-      [[maybe_unused]] uint32_t xb[AHEAD], xa[AHEAD][MT];
+      uint4 b[AHEAD][PIECES], a[AHEAD][PIECES];
+      [[maybe_unused]] uint32_t xb[AHEAD], xa[AHEAD];
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int k = k0 + u * WAVES * ROUND;
@@ -753,17 +749,12 @@ __global__ void __launch_bounds__(512) product_few(Product p) {
           // past the rows' end: zeros
           const bool in = (k * BYTES + h * 64 + q * 16) < k_end * BYTES;
           b[u][h] = load(rb, in && ob != NOWHERE ? ob + k * BYTES + h * 64 : NOWHERE);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-            a[u][h][i] = load(ra, in && oa[i] != NOWHERE ? oa[i] + k * BYTES + h * 64 : NOWHERE);
+          a[u][h] = load(ra, in && oa != NOWHERE ? oa + k * BYTES + h * 64 : NOWHERE);
         }
         if constexpr (IS_PACKED) {
           const bool in = k < k_end;
           xb[u] = __builtin_amdgcn_raw_buffer_load_b8(rsb, in && r16 < cols ? r16 * (int)p.ss + k / 128 : (int)NOWHERE, 0, 0);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-            xa[u][i] = __builtin_amdgcn_raw_buffer_load_b8(
-                rsa, in && 16 * i + r16 < rows ? (16 * i + r16) * (int)p.ss + k / 128 : (int)NOWHERE, 0, 0);
+          xa[u] = __builtin_amdgcn_raw_buffer_load_b8(rsa, in && r16 < rows ? r16 * (int)p.ss + k / 128 : (int)NOWHERE, 0, 0);
         }
       }
       __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first is waited for
@@ -773,17 +764,12 @@ __global__ void __launch_bounds__(512) product_few(Product p) {
         for (int h = 0; h < PIECES; ++h) {
           if constexpr (IS_PACKED) {
             // 16 codes a lane: 8 for each of two instructions, of A as of B
-            const float sb = block8_scale(xb[u]);
-            const uint4 b0 = decode_bf16(b[u][h].x, b[u][h].y, sb), b1 = decode_bf16(b[u][h].z, b[u][h].w, sb);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              const float sa = block8_scale(xa[u][i]);
-              acc[0][i] = mfma16<T>(b0, decode_bf16(a[u][h][i].x, a[u][h][i].y, sa), acc[0][i]);
-              acc[0][i] = mfma16<T>(b1, decode_bf16(a[u][h][i].z, a[u][h][i].w, sa), acc[0][i]);
-            }
+            const uint4 x = a[u][h], y = b[u][h];
+            const float sa = block8_scale(xa[u]), sb = block8_scale(xb[u]);
+            acc[0] = mfma16<T>(decode_bf16(y.x, y.y, sb), decode_bf16(x.x, x.y, sa), acc[0]);
+            acc[0] = mfma16<T>(decode_bf16(y.z, y.w, sb), decode_bf16(x.z, x.w, sa), acc[0]);
           } else {
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[0][i] = mfma16<T>(b[u][h], a[u][h][i], acc[0][i]);
+            acc[0] = mfma16<T>(b[u][h], a[u][h], acc[0]);
           }
         }
     }
@@ -792,13 +778,11 @@ __global__ void __launch_bounds__(512) product_few(Product p) {
     // 8 columns from 8 r16 on of rows 8 q to 8 q + 7
     const uint32_t ob = 8 * r16 < cols ? (uint32_t)(8 * q * p.bs * 2) + r16 * 16 : NOWHERE;
     for (int k0 = wave * ROUND; k0 < k_end; k0 += WAVES * ROUND) {
-      uint4 b[8], a[MT];
+      uint4 b[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         b[j] = load(rb, ob != NOWHERE && k0 + 8 * q + j < k_end ? ob + (uint32_t)((k0 + j) * p.bs * 2) : NOWHERE);
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-        a[i] = load(ra, oa[i] != NOWHERE && k0 + 8 * q < k_end ? oa[i] + k0 * 2 : NOWHERE);
+      const uint4 a = load(ra, oa != NOWHERE && k0 + 8 * q < k_end ? oa + k0 * 2 : NOWHERE);
       __builtin_amdgcn_sched_barrier(0);
       // column c of the eight rows, c even and odd: the low and the high halves of word c / 2
       const uint32_t* w = reinterpret_cast<const uint32_t*>(b);
@@ -808,30 +792,24 @@ __global__ void __launch_bounds__(512) product_few(Product p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           v[j] = __builtin_amdgcn_perm(w[(2 * j + 1) * 4 + c / 2], w[2 * j * 4 + c / 2], c & 1 ? 0x07060302 : 0x05040100);
-        const uint4 f = make_uint4(v[0], v[1], v[2], v[3]);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) acc[c][i] = mfma16<T>(f, a[i], acc[c][i]);
+        acc[c] = mfma16<T>(make_uint4(v[0], v[1], v[2], v[3]), a, acc[c]);
       }
     }
   }
 #pragma unroll
-  for (int c = 0; c < N16; ++c)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) part[wave][c * MT + i][lane] = acc[c][i];
+  for (int c = 0; c < N16; ++c) part[wave][c][lane] = acc[c];
   __syncthreads();
   O* out = (O*)p.c + (uint64_t)t.row * p.cs + n0;
-  for (int j = wave; j < N16 * MT; j += WAVES) {
-    const int c = j / MT, i = j % MT;
-    f4v s = part[0][j][lane];
+  for (int c = wave; c < N16; c += WAVES) {
+    f4v s = part[0][c][lane];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) s += part[w][j][lane];
-    const int r = 16 * i + r16;
-    if (r >= rows) continue;
+    for (int w = 1; w < WAVES; ++w) s += part[w][c][lane];
+    if (r16 >= rows) continue;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       // tile c holds columns 4 q to 4 q + 3 (COLS: every eighth column from c on)
       const int at = LB == ROWS ? 4 * q + e : 8 * (4 * q + e) + c;
-      if (at < cols) out[(uint64_t)r * p.cs + at] = (O)s[e];
+      if (at < cols) out[(uint64_t)r16 * p.cs + at] = (O)s[e];
     }
   }
 #endif
@@ -890,7 +868,7 @@ __global__ void __launch_bounds__(256) join_parts(Product p) {
 
 template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
 void launch_tiled(const Product& p, hipStream_t s) {
-  using K = Tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>;
+  using K = Tiled<T, WM, WN, MT, NT>;
   const uint64_t tn = (p.n + K::TN - 1) / K::TN;
   uint64_t tiles;
   if (FORM == GRAD_WEIGHT)
@@ -906,11 +884,11 @@ bool copies(int bytes, const void* d, uint64_t cols, uint64_t stride, uint64_t g
   return ((uint64_t)(uintptr_t)d | cols * bytes | stride * bytes | group_stride * bytes) % 16 == 0;
 }
 
-template <class T, class O, int LB, bool IS_PACKED, int MT>
+template <class T, class O, int LB, bool IS_PACKED>
 void launch_few(const Product& p, hipStream_t s) {
   constexpr uint64_t TN = LB == ROWS ? 16 : 128;
-  const uint64_t tiles = row_tiles_max(p.rows, p.groups, 16 * MT, p.offsets != nullptr) * ((p.n + TN - 1) / TN);
-  hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED, MT>), dim3(grid_size(tiles)), dim3(512), 0, s, p);
+  const uint64_t tiles = row_tiles_max(p.rows, p.groups, 16, p.offsets != nullptr) * ((p.n + TN - 1) / TN);
+  hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED>), dim3(grid_size(tiles)), dim3(512), 0, s, p);
   PXG_HIP(hipGetLastError());
 }
 
@@ -980,6 +958,26 @@ Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0) {
   return best;
 }
 
+// What product_few takes, in us: a start, and its row tiles' matrices at the
+// rate that it reads them, which falls with the rows beside them. COLS reads
+// them again out of the caches, and k rows one after another. Tiles are bound
+// by their own cost or by the matrices' bytes. Few and tiled, measured:
+//   16 rows, 4096 -> 4096              forward 11, 35; input gradient 18, 36; packed 9, 41
+//   64 rows, the same                          33, 35;                18, 36;        25, 43
+//   16 groups of 1 row, 2048 -> 2048           29, 23;                22, 23;        17, 32
+//   8 groups of 64 rows, 1024 -> 1024          19,  9;                10,  9;        14, 14
+double few_cost(int b, bool packed, const Product& p) {
+  const double used = std::min(p.rows, p.groups);
+  const double tiles = p.groups == 1 ? (p.rows + 15) / 16 : std::max(used, p.rows / 16.0 + p.groups / 2.0);
+  const double matrix = (double)p.n * p.k * (packed ? 1 : 2), full = p.rows / (16 * tiles);
+  if (b == COLS) return 2 + std::max(matrix * (used * (1 + full / 7) / 6e6 + (tiles - used) / 12e6), p.k * 0.0033);
+  return 2 + matrix * tiles * (packed ? (1 + full / 2) / 4.5e6 : (1 + full / 3) / 5e6);
+}
+double tiled_cost(const Cost& cost, bool packed, const Product& p) {
+  const double matrices = (double)std::min(p.rows, p.groups) * p.n * p.k * (packed ? 1 : 2);
+  return std::max(std::min(cost.best, cost.fp8), matrices / 5.9e6);
+}
+
 // `room`: bytes of p.workspace.
 template <int FORM, class T, class O, bool IS_PACKED>
 void launch_product(Product p, uint64_t room, hipStream_t s) {
@@ -989,16 +987,16 @@ void launch_product(Product p, uint64_t room, hipStream_t s) {
   const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
   const bool copied = (is_packed(LA) || copies(2, p.a, acols, p.as, 0)) &&
                       (is_packed(LB) || copies(2, p.b, bcols, p.bs, p.bg));
-  const uint64_t each = ((uint64_t)p.rows + p.groups - 1) / p.groups;  // rows of a group, on average
-  if constexpr (FORM != GRAD_WEIGHT) {
-    // COLS spans a matrix' rows with one resource
-    if (copied && each <= 16 && (FORM == FORWARD || p.k * p.bs * 2 <= 0x7FFFFFFF))
-      return launch_few<T, O, FORM == FORWARD ? ROWS : COLS, IS_PACKED, 1>(p, s);
-  }
   const Cost cost = product_cost(FORM, p, FORM == FORWARD && IS_PACKED, room);
+  if constexpr (FORM != GRAD_WEIGHT) {
+    constexpr int B = FORM == GRAD_INPUT ? COLS : ROWS;
+    // COLS spans a matrix' rows with one resource
+    if (copied && (B == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF) && few_cost(B, IS_PACKED, p) <= tiled_cost(cost, IS_PACKED, p))
+      return launch_few<T, O, B, IS_PACKED>(p, s);
+  }
   if constexpr (FORM == GRAD_WEIGHT) p.limit = cost.limit;
   if constexpr (FORM == FORWARD && IS_PACKED && !std::is_same_v<O, float>)
-    if (each >= 192 && cost.fp8 <= cost.best) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
+    if (cost.fp8 <= cost.best) return launch_tiled<Fp8, O, FORM, ROWS, ROWS, 2, 4, 8, 4>(p, s);
   if (copied) {
     if (LA != PACKED_ROWS && cost.tile == 256) {
       if constexpr (LA != PACKED_ROWS) launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);

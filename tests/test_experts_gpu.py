@@ -272,6 +272,85 @@ def test_weight_gradients_of_long_groups(gpu, sizes, n, k):
     _check(gpu.grouped_matmul_grad_weight(grad, packed, offsets, out_dtype=torch.float32), want, size, max(sizes))
 
 
+@pytest.mark.parametrize("sizes,n,k", [([24], 520, 2048), ([33], 2048, 1000), ([100], 256, 4096), ([20, 0, 45, 7], 1024, 1032),
+                                       ([1] * 16, 2048, 1024), ([100] * 70, 264, 200), ([1] * 62 + [129], 136, 72),
+                                       ([16] * 8, 1024, 2048)])
+def test_few_rows_and_many_groups(gpu, sizes, n, k):
+    # on either side of the products' choice for few rows, and of 62 groups
+    import torch
+    for dtype in (torch.bfloat16, torch.float16):
+        x, w, grad, offsets = _make(torch, sizes, n, k, dtype, 21, 1, 2)
+        _check_products(torch, gpu, x, w, grad, offsets, offsets.tolist(), torch.float32)
+        _check_products(torch, gpu, x, w, grad, offsets, offsets.tolist(), None)
+    x, w, grad, offsets = _make(torch, sizes, n, k, torch.bfloat16, 22, 2, 1)
+    p, q = gpu.block8_pack(x), gpu.block8_pack(w.reshape(-1, k))
+    xv, wv = gpu.block8_unpack(p, torch.float32), gpu.block8_unpack(q, torch.float32).view(w.shape)
+    want, size = _per_row(torch, xv, wv, offsets.tolist(), True)
+    _check(gpu.block8_matmul(p, q, offsets, out_dtype=torch.float32), want, size, k)
+
+
+def test_rows_millions_of_elements_apart(gpu):
+    # operands and results whose bytes pass 2^32 and whose tiles pass 2^31
+    import torch
+    sizes, n, k, far = [300, 0, 260], 264, 136, 1 << 22
+    x, w, grad, offsets = _make(torch, sizes, n, k, torch.bfloat16, 23)
+    ends = offsets.tolist()
+
+    def apart(t):
+        hold = torch.empty(t.shape[0] * far, dtype=t.dtype, device="cuda").view(t.shape[0], far)[:, :t.shape[1]]
+        return hold.copy_(t)
+
+    ws = apart(w.reshape(-1, k)).as_strided((3, n, k), (n * far, far, 1))
+    xs, gs = apart(x), apart(grad)
+    want, size = _per_row(torch, x, w, ends, True)
+    _check(gpu.grouped_matmul(xs, ws, offsets, out=apart(torch.zeros_like(grad))), want, size, k)
+    want, size = _per_row(torch, grad, w, ends, False)
+    _check(gpu.grouped_matmul_grad_input(gs, ws, offsets, out=apart(torch.zeros_like(x))), want, size, n)
+    want, size = _per_group(torch, grad, x, ends)
+    out = apart(torch.zeros_like(w.reshape(-1, k))).as_strided((3, n, k), (n * far, far, 1))
+    _check(gpu.grouped_matmul_grad_weight(gs, xs, offsets, out=out), want, size, max(sizes))
+    p = gpu.block8_pack(xs)
+    assert torch.equal(p.codes, gpu.block8_pack(x).codes)
+    assert torch.equal(gpu.block8_unpack(p, out=apart(torch.zeros_like(x))), gpu.block8_unpack(p, torch.bfloat16))
+    for act in ("silu", "gelu"):
+        a, h8 = gpu.activation_pack(gs, act)
+        b, g8 = gpu.activation_pack(grad, act)
+        assert torch.equal(a, b) and torch.equal(h8.codes, g8.codes)
+        assert torch.equal(gpu.activation_grad(gs, h8, act), gpu.activation_grad(grad, g8, act))
+
+
+def test_a_million_rows(gpu):
+    # rows, codes and gradients past 2^32 bytes; what is not zero lies at the very end
+    import torch
+    rows, n, k, tail = 1_060_000, 64, 4096, 50
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    _, w, grad, _ = _make(torch, [1, 1], n, k, torch.bfloat16, 24)
+    x[-tail:] = torch.randn(tail, k, generator=_dev(torch, 25), device="cuda").bfloat16()
+    offsets = torch.tensor([0, rows - tail, rows], device="cuda")
+    last = [0, tail]
+    want, size = _per_row(torch, x[-tail:], w[1:], last, True)
+    y = gpu.grouped_matmul(x, w, offsets)
+    _check(y[-tail:], want, size, k)
+    assert not bool(y[:-tail].any())
+    p, q = gpu.block8_pack(x), gpu.block8_pack(w.reshape(-1, k))
+    xv, wv = gpu.block8_unpack(p, torch.float32)[-tail:].clone(), gpu.block8_unpack(q, torch.float32).view(w.shape)
+    assert torch.equal(p.codes[-tail:], gpu.block8_pack(x[-tail:]).codes)
+    want, size = _per_row(torch, xv, wv[1:], last, True)
+    _check(gpu.block8_matmul(p, q, offsets, out_dtype=torch.float32)[-tail:], want, size, k)
+    grad = torch.randn(rows, n, generator=_dev(torch, 26), device="cuda").bfloat16()
+    for rhs, plain in ((x, x[-tail:].float()), (p, xv)):
+        want, size = _per_group(torch, grad[-tail:], plain, last)
+        got = gpu.grouped_matmul_grad_weight(grad, rhs, offsets, out_dtype=torch.float32)
+        _check(got[1:], want, size, tail)
+        assert not bool(got[0].any())
+    dx = gpu.grouped_matmul_grad_input(grad, w, offsets)
+    want, size = _per_row(torch, grad[-tail:], w[1:], last, False)
+    _check(dx[-tail:], want, size, n)
+    a, h8 = gpu.activation_pack(x, "gelu")
+    assert torch.equal(h8.codes, p.codes)
+    assert torch.equal(a[-tail:], gpu.activation_pack(x[-tail:], "gelu")[0])
+
+
 def test_one_group_without_offsets(gpu):
     import torch
     x, w, grad, offsets = _make(torch, [190], 96, 160, torch.float16, 4)
@@ -468,6 +547,15 @@ def test_products_in_8_bits(gpu, sizes, n, k):
         assert bool(((got - want).abs() <= bound + _unit(dtype) * (want.abs() + bound)).all())
         # and as a whole: the cuts are of either sign, so far below the sum of their bounds
         assert float((got - want).norm() / want.norm()) < 2 * _unit(dtype)
+
+
+def test_products_in_8_bits_of_short_groups(gpu):
+    # many matrices with 40 rows each: the 8-bit cores also there
+    import torch
+    sizes, n, k = [40, 0, 61, 33] * 8, 2048, 1024
+    assert _runs_in_8_bits(gpu, torch, sizes, n, k)
+    test_products_in_8_bits(gpu, sizes, n, k)
+    test_products_in_8_bits_of_exact_sums(gpu, sizes, n, k)
 
 
 # --- activations --------------------------------------------------------------------

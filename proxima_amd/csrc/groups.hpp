@@ -79,7 +79,7 @@ __device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offset
     return index < row_tiles_of<KIND>(rows, size);
   }
   const int lane = threadIdx.x & (WAVE - 1);
-  int begin = 0, before = 0;  // rows and tiles before the segments of this round
+  int begin = 0, before = 0;  // rows and tiles before the segments of this pass
   // segment s ends at offsets[s]; segment 0 and segment groups + 1 are the rows of no group
   for (int s0 = 0; s0 < groups + 2; s0 += WAVE) {
     const int s = s0 + lane;

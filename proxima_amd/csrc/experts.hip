@@ -689,29 +689,51 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
         for (int e = 0; e < 4; ++e) v[e] = (R)acc[i][j][e];
         *reinterpret_cast<r4v*>(mine + r16 * PITCH + (j * 16 + 4 * q) * sizeof(R)) = v;
       }
+      if (whole) {
 #pragma unroll
-      for (int h = 0; h < 16 * PER / 64; ++h) {
-        const int r = lane / PER + h * (64 / PER), row = (i * WM + wm) * 16 + r;
-        const uint4 v = *reinterpret_cast<const uint4*>(mine + r * PITCH + lane % PER * 16);
-        if (row >= rows) continue;
-        R* to = c + (uint64_t)row * stride + col;
-        if (whole && col + EACH <= cols) {
-          *reinterpret_cast<uint4*>(to) = v;
-        } else {
-          R x[EACH];
-          *reinterpret_cast<uint4*>(x) = v;
+        for (int h = 0; h < 16 * PER / 64; ++h) {
+          const int r = lane / PER + h * (64 / PER), row = (i * WM + wm) * 16 + r;
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + r * PITCH + lane % PER * 16);
+          if (row >= rows) continue;
+          R* to = c + (uint64_t)row * stride + col;
+          if (col + EACH <= cols) {
+            *reinterpret_cast<uint4*>(to) = v;
+          } else {
+            R x[EACH];
+            *reinterpret_cast<uint4*>(x) = v;
 #pragma unroll
-          for (int e = 0; e < EACH; ++e)
-            if (col + e < cols) to[e] = x[e];
+            for (int e = 0; e < EACH; ++e)
+              if (col + e < cols) to[e] = x[e];
+          }
+        }
+      } else {
+        // rows that are not 16-byte aligned: an element a lane, of one row or two
+        // (8192 rows packed, 2049 -> 1027: 39 us; the pieces' elements in turn 46)
+        constexpr int W = NT * 16;
+#pragma unroll
+        for (int h = 0; h < 16 * W / 64; ++h) {
+          const int r = lane / W + h * (64 / W), row = (i * WM + wm) * 16 + r, at = lane % W;
+          const R v = *reinterpret_cast<const R*>(mine + r * PITCH + at * sizeof(R));
+          if (row < rows && wn * W + at < cols) c[(uint64_t)row * stride + wn * W + at] = v;
         }
       }
     }
   };
   lds_barrier();
-  if (FORM == GRAD_WEIGHT && slot >= 0)
-    store(float{}, p.workspace + (uint64_t)slot * p.m * p.n, p.n, p.n % 4 == 0);
-  else
-    store(O{}, (O*)p.c + group * p.cg, p.cs, p.c_vec);
+  O* result = (O*)p.c + group * p.cg;
+  if constexpr (FORM == GRAD_WEIGHT) {
+    float* part = p.workspace + (uint64_t)(slot < 0 ? 0 : slot) * p.m * p.n;
+    const bool apart = slot >= 0;
+    if constexpr (std::is_same_v<O, float>) {  // one piece of code for both
+      store(O{}, apart ? part : result, apart ? p.n : p.cs, apart ? p.n % 4 == 0 : p.c_vec);
+    } else if (apart) {
+      store(float{}, part, p.n, p.n % 4 == 0);
+    } else {
+      store(O{}, result, p.cs, p.c_vec);
+    }
+  } else {
+    store(O{}, result, p.cs, p.c_vec);
+  }
 #endif
 }
 

@@ -53,8 +53,8 @@ struct Product {
   int rows, groups;     // rows of x and dy
   int m, n, k;
   bool c_vec;           // C's rows are 16-byte aligned
-  int limit = 0;              // grad weight: longer groups are summed in parts (groups.hpp)
-  float* workspace = nullptr;  // whose slots are m x n each
+  int limit = 0;        // grad weight: longer groups are summed in parts (groups.hpp),
+  float* workspace = nullptr;  // in slots of m x n
 };
 
 template <class T>

@@ -272,6 +272,27 @@ def test_weight_gradients_of_long_groups(gpu, sizes, n, k):
     _check(gpu.grouped_matmul_grad_weight(grad, packed, offsets, out_dtype=torch.float32), want, size, max(sizes))
 
 
+def test_weight_gradients_with_less_workspace(gpu):
+    import torch
+    lib = gpu._lib
+    sizes, n, k = [6000, 0, 2500, 64], 96, 136
+    x, w, grad, offsets = _make(torch, sizes, n, k, torch.bfloat16, 31)
+    want, size = _per_group(torch, grad, x, offsets.tolist())
+    rows = x.shape[0]
+    need = lib.pxg_grouped_matmul_grad_weight_workspace(rows, n, k, len(sizes))
+    slot = 4 * n * k
+    assert need > slot
+    space = torch.full((need + slot,), 255, dtype=torch.uint8, device="cuda")  # NaN in f32
+    for given in (0, slot - 4, slot, need - 4, need, need + slot):
+        out = torch.empty(len(sizes), n, k, dtype=torch.float32, device="cuda")
+        status = lib.pxg_grouped_matmul_grad_weight_device(
+            2, grad.data_ptr(), rows, n, n, x.data_ptr(), k, k, offsets.data_ptr(), len(sizes), 0, out.data_ptr(), k,
+            n * k, space.data_ptr() if given else None, given, torch.cuda.current_stream().cuda_stream)
+        assert status == 0
+        _check(out, want, size, max(sizes))
+        assert bool((space[given:] == 255).all())
+
+
 @pytest.mark.parametrize("sizes,n,k", [([24], 520, 2048), ([33], 2048, 1000), ([100], 256, 4096), ([20, 0, 45, 7], 1024, 1032),
                                        ([1] * 16, 2048, 1024), ([100] * 70, 264, 200), ([1] * 62 + [129], 136, 72),
                                        ([16] * 8, 1024, 2048)])

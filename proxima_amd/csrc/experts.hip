@@ -1028,9 +1028,8 @@ double few_cost(int b, bool packed, const Product& p) {
   if (b == COLS) return 2 + std::max(matrix * (used * (1 + full / 7) / 6e6 + (tiles - used) / 12e6), p.k * 0.0033);
   return 2 + matrix * tiles * (packed ? (1 + full / 2) / 4.5e6 : (1 + full / 3) / 5e6);
 }
-double tiled_cost(const Cost& cost, bool packed, const Product& p) {
-  const double matrices = (double)std::min(p.rows, p.groups) * p.n * p.k * (packed ? 1 : 2);
-  return std::max(std::min(cost.best, cost.fp8), matrices / 5.9e6);
+double tiled_cost(double cost, bool packed, const Product& p) {
+  return std::max(cost, (double)std::min(p.rows, p.groups) * p.n * p.k * (packed ? 1 : 2) / 5.9e6);
 }
 
 // `room`: bytes of p.workspace.
@@ -1046,7 +1045,9 @@ void launch_product(Product p, uint64_t room, hipStream_t s) {
   if constexpr (FORM != GRAD_WEIGHT) {
     constexpr int B = FORM == GRAD_INPUT ? COLS : ROWS;
     // COLS spans a matrix' rows with one resource
-    if (copied && (B == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF) && few_cost(B, IS_PACKED, p) <= tiled_cost(cost, IS_PACKED, p))
+    const bool reaches = B == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF;
+    const double tiled = std::is_same_v<O, float> ? cost.best : std::min(cost.best, cost.fp8);
+    if (copied && reaches && few_cost(B, IS_PACKED, p) <= tiled_cost(tiled, IS_PACKED, p))
       return launch_few<T, O, B, IS_PACKED>(p, s);
   }
   if constexpr (FORM == GRAD_WEIGHT) p.limit = cost.limit;

@@ -885,27 +885,31 @@ void check_out_type(int type, int out_type) {
     config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
 }
 
-// The sums of divided groups: a grid of (such group, row of dw) by 1024
+// The sums of divided groups: a grid of (such group, some rows of dw) by 1024
 // columns adds the parts of each element in order.
+constexpr int JOIN_ROWS = 512;  // workgroups to a group
 template <class O>
 __global__ void __launch_bounds__(256) join_parts(Product p) {
+  const int each = p.m < JOIN_ROWS ? p.m : JOIN_ROWS;
   GroupPart g;
-  if (!find_divided_group(p.offsets, p.groups, p.rows, p.limit, (int)(blockIdx.x / p.m), g)) return;
-  const int row = (int)(blockIdx.x % p.m), c = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (!find_divided_group(p.offsets, p.groups, p.rows, p.limit, (int)blockIdx.x / each, g)) return;
+  const int c = (blockIdx.y * 256 + threadIdx.x) * 4;
   if (c >= p.n) return;
   const uint64_t part = (uint64_t)p.m * p.n;
-  const float* from = p.workspace + g.slot * part + (uint64_t)row * p.n + c;
-  O* to = (O*)p.c + g.group * p.cg + row * p.cs + c;
-  if (p.n % 4 == 0) {
-    f4v x = *reinterpret_cast<const f4v*>(from);
-    for (int s = 1; s < g.parts; ++s) x += *reinterpret_cast<const f4v*>(from + s * part);
+  for (int row = (int)blockIdx.x % each; row < p.m; row += each) {
+    const float* from = p.workspace + g.slot * part + (uint64_t)row * p.n + c;
+    O* to = (O*)p.c + g.group * p.cg + row * p.cs + c;
+    if (p.n % 4 == 0) {
+      f4v x = *reinterpret_cast<const f4v*>(from);
+      for (int s = 1; s < g.parts; ++s) x += *reinterpret_cast<const f4v*>(from + s * part);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) to[e] = (O)x[e];
-  } else {
-    for (int e = 0; e < 4 && c + e < p.n; ++e) {
-      float x = from[e];
-      for (int s = 1; s < g.parts; ++s) x += from[s * part + e];
-      to[e] = (O)x;
+      for (int e = 0; e < 4; ++e) to[e] = (O)x[e];
+    } else {
+      for (int e = 0; e < 4 && c + e < p.n; ++e) {
+        float x = from[e];
+        for (int s = 1; s < g.parts; ++s) x += from[s * part + e];
+        to[e] = (O)x;
+      }
     }
   }
 }
@@ -973,7 +977,7 @@ struct Cost {
 //   1 group of 16384 rows, 2048 x 2048            188 -> 122 (4096)
 //   1 of 4096, 768 x 768                           36 ->  21 (1536)
 //   8 uneven ones, 16384 rows in all, 512 x 512    39 ->  30 (1024)
-//   8 uneven, 8192 rows, 4096 x 1024               63 ->  87 (2048): the sums' traffic
+//   8 uneven, 8192 rows, 4096 x 1024               63 ->  87 (2048): the parts' traffic
 Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0) {
   Cost best;
   const double average = form == GRAD_WEIGHT ? (double)p.rows / p.groups : p.k;
@@ -1009,6 +1013,19 @@ Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0) {
         best.limit = (int)limit;
       }
     }
+  }
+  // A much longer group than assumed: where it alone would take half as long
+  // again as all tiles together, and dividing it saves more than its parts'
+  // traffic costs. Packed, into f32, whole and divided, with the longest of 8
+  // groups of 8192 rows, 1024 -> 4096: 5500 rows 155, 99; 4200 rows 127, 103;
+  // none divided 92, 94. Of 16 of 16384, 2048 -> 2048: 7799 rows 269, 206 us.
+  if (form == GRAD_WEIGHT && !best.limit && p.groups > 1 && p.groups <= SEGMENT_GROUPS) {
+    const Tile& t = TILES[best.tile == 256 ? 0 : best.tile == 128 ? 1 : 2];
+    const uint64_t tiles = (((uint64_t)p.m + t.size - 1) / t.size) * (((uint64_t)p.n + t.size - 1) / t.size);
+    const uint64_t limit = (p.rows * tiles * 3 / 2 / t.slots + 63) / 64 * 64, slot = 4ull * p.m * p.n;
+    const double saved = limit / 128.0 * (t.least + t.more), join = JOIN_US + 4.0 * slot / JOIN_BYTES_PER_US;
+    if (limit < (uint64_t)p.rows && saved > join && group_slots_max(p.rows, p.groups, limit) * slot <= room)
+      best.limit = (int)limit;
   }
   return best;
 }
@@ -1070,7 +1087,7 @@ void launch_product(Product p, uint64_t room, hipStream_t s) {
   if (FORM == GRAD_WEIGHT && p.limit) {
     const uint64_t divided = std::min<uint64_t>(p.groups, p.rows / p.limit);
     if (divided) {
-      const dim3 grid(grid_size(divided * p.m), (unsigned)(((uint64_t)p.n + 1023) / 1024));
+      const dim3 grid(grid_size(divided * std::min(p.m, JOIN_ROWS)), (unsigned)(((uint64_t)p.n + 1023) / 1024));
       hipLaunchKernelGGL(join_parts<O>, grid, dim3(256), 0, s, p);
       PXG_HIP(hipGetLastError());
     }

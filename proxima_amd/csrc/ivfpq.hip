@@ -1026,11 +1026,12 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // waits with an explicit vmcnt. The asm sets m0 itself; the kernels that use
 // these copies keep no value of their own in m0 (no dynamic register
 // indexing, no LDS-DMA builtins, no messages), so the clobber of the
-// reserved register is harmless there.
+// reserved register is harmless there. A write of m0 needs one wait state
+// before a copy reads it, which the compiler does not add inside asm.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void lds_copy16(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 template <int N>

@@ -298,11 +298,12 @@ __device__ const float4 km_zero16 = {0.0f, 0.0f, 0.0f, 0.0f};
 // Global -> LDS copy of 16 bytes per lane (lane i's bytes land at m0 + 16 i),
 // 64-bit address per lane. Inline asm, so that the compiler does not count
 // it under vmcnt; km_mfma_top waits for it with km_vm_wait0 before each
-// slice's barrier and uses m0 for nothing else.
+// slice's barrier and uses m0 for nothing else. A write of m0 needs one wait
+// state before a copy reads it, which the compiler does not add inside asm.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void km_lds_copy16(const void* g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(g) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ void km_vm_wait0() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }

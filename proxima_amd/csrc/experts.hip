@@ -104,17 +104,18 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* p, uint6
 // Copies of 16 (and 4) bytes a lane straight into LDS: lane i's land at
 // lds + 16 i (4 i), zeros for offsets outside the resource. Inline asm, so
 // that the compiler does not wait for them before every LDS read; nothing
-// else in these kernels uses m0. A write of m0 needs one wait state before a
-// copy reads it, which the compiler does not add inside asm. wait_copies() waits for all of them,
+// else in these kernels uses m0. Inside asm the compiler adds no wait
+// states: a copy needs one after m0's write, and five after a vector
+// instruction (a readfirstlane) wrote part of its resource. wait_copies() waits for all of them,
 // wait_copies_but<N>() for all but the last N.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16(__amdgpu_buffer_rsrc_t rs, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rs)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rs)
                : "memory", "m0");
 }
 __device__ __forceinline__ void copy4(__amdgpu_buffer_rsrc_t rs, uint32_t offset, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rs)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(lds), "v"(offset), "s"(rs)
                : "memory", "m0");
 }
 #pragma clang diagnostic pop

@@ -86,13 +86,14 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t uniform_rsrc(const void* p, in
 // m0 + 16 i, and an offset outside the resource lands as zeros. Inline asm,
 // so that the compiler neither tracks these loads under vmcnt (it would wait
 // for them before every LDS read) nor needs m0 elsewhere: this kernel has no
-// other use of m0 (no LDS-DMA builtins, no indirect register indexing). A
-// write of m0 needs one wait state before a copy reads it, which the compiler
-// does not add inside asm. The copies' wait is vm_wait0().
+// other use of m0 (no LDS-DMA builtins, no indirect register indexing). Inside
+// asm the compiler adds no wait states: a copy needs one after m0's write, and
+// five after a vector instruction (a readfirstlane) wrote part of its
+// resource or offset. The copies' wait is vm_wait0().
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t soff, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0), "v"(voff), "s"(rs),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(m0), "v"(voff), "s"(rs),
                "s"(soff)
                : "memory", "m0");
 }

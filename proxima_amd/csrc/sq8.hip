@@ -233,16 +233,17 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t sq_rsrc(const void* p, int byt
 // that the compiler does not count these loads under vmcnt (it would wait
 // for every one in flight before each LDS read of the tile); the scan waits
 // for them itself (wait_vm_upto) before the tile barrier. The scan kernel
-// has no other use of m0. A write of m0 needs one wait state before a copy
-// reads it, which the compiler does not add inside asm.
+// has no other use of m0. Inside asm the compiler adds no wait states: a copy
+// needs one after m0's write, and five after a vector instruction (a
+// readfirstlane) wrote part of its resource.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void sq_dma16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(voff), "s"(rs)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(m0), "v"(voff), "s"(rs)
                : "memory", "m0");
 }
 __device__ __forceinline__ void sq_dma4(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t m0) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(m0), "v"(voff), "s"(rs)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(m0), "v"(voff), "s"(rs)
                : "memory", "m0");
 }
 #pragma clang diagnostic pop

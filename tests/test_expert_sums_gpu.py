@@ -1,0 +1,133 @@
+"""What the 8-bit matrix cores sum, against an emulation of their rule in 64 bits.
+
+The rule, from probes of single instructions over all pairs of codes: of each
+eight neighbouring columns, every product is cut toward zero to a multiple of
+2^(E - 13), E being the largest sum of two codes' exponents among the eight (a
+subnormal code's is -6; products of zeros do not count). The sixteen sums of
+eights of a block and the accumulator are then added in f32; where one of them
+is far larger than the accumulator, that is off by up to 2^-18 of it.
+
+So an element may differ from the emulated sum by 2^-18 of the largest eight
+of each block, and by 2^-23 of the largest partial sum (twice the largest of
+those in the order of the columns, the sum beginning anywhere) for each block;
+then it is rounded once, to 2^-8 (bf16) or 2^-11 (f16; 2^-25 below its normals).
+"""
+import numpy as np
+import pytest
+
+import test_experts_gpu as base
+
+pytestmark = pytest.mark.gpu
+
+# products into 16 bits that run on the 8-bit cores: one group, rows and columns that end inside a tile and a block,
+# groups with more than 32 steps of which one is empty and one shorter than a tile
+SHAPES = [([8192], 4096, 4096), ([4096], 1027, 2049), ([1200, 0, 90, 1500, 1210], 1500, 4500),
+          ([2000, 1500, 90, 0, 1700, 900, 1000, 1002], 4096, 1024)]
+
+
+def _inputs(torch, px, sizes, n, k, spread, seed):
+    """Packed rows, whose columns' magnitudes spread as exp(spread normal), packed matrices and offsets."""
+    g = base._dev(torch, seed)
+    rows = sum(sizes) + 12
+    x = torch.randn(rows, k, generator=g, device="cuda") * torch.exp(
+        spread * torch.randn(k, generator=g, device="cuda"))
+    w = torch.randn(len(sizes) * n, k, generator=g, device="cuda") / k ** 0.5
+    return px.block8_pack(x.bfloat16()), px.block8_pack(w.bfloat16()), base._offsets(torch, sizes, 7)
+
+
+def _parts(torch, p, rows):
+    """(values, exponents) of packed rows in 64 bits; a zero's exponent is -1000."""
+    codes, scales = p.codes[rows], p.scales[rows].int() - 127
+    values = torch.from_numpy(base._values(np.arange(256))).cuda()[codes.long()]
+    scale = scales.repeat_interleave(128, 1)[:, :codes.shape[1]]
+    e = (((codes.int() & 127) >> 3) - 7).clamp(min=-6) + scale
+    return values * torch.exp2(scale.double()), torch.where((codes & 127) == 0, torch.full_like(e, -1000), e)
+
+
+def _emulated(torch, p, q, rows, matrix_rows):
+    """(the cores' sums, exact sums, allowance) of some rows of x by some rows of a matrix."""
+    x, ex = _parts(torch, p, rows)
+    w, ew = _parts(torch, q, matrix_rows)
+    products = (x[:, None, :] * w[None]).unflatten(2, (-1, 8))
+    unit = torch.exp2(((ex[:, None, :] + ew[None]).unflatten(2, (-1, 8)).amax(3, keepdim=True).clamp(min=-900) - 13)
+                      .double())
+    eights = (torch.trunc(products / unit) * unit).sum(3)
+    blocks = eights.unflatten(2, (-1, 16))
+    sums = blocks.sum(3)
+    partial = sums.cumsum(2)
+    allowance = 2.0 ** -18 * blocks.abs().amax(3).sum(2) + sums.shape[2] * 2.0 ** -22 * partial.abs().amax(2)
+    return partial[:, :, -1], products.sum((2, 3)), allowance
+
+
+@pytest.mark.parametrize("spread", [0.0, 0.7, 2.0])
+@pytest.mark.parametrize("sizes,n,k", SHAPES)
+def test_the_cores_rule(gpu, sizes, n, k, spread):
+    import torch
+    p, q, offsets = _inputs(torch, gpu, sizes, n, k, spread, n + k)
+    ends = offsets.tolist()
+    got = {dtype: gpu.block8_matmul(p, q, offsets, out_dtype=dtype) for dtype in (torch.bfloat16, torch.float16)}
+    g = base._dev(torch, 3)
+    cut, exact_norm, changed = 0.0, 0.0, 0
+    off, own = {d: 0.0 for d in got}, {d: 0.0 for d in got}
+    for e, (lo, hi) in enumerate(zip(ends[:-1], ends[1:])):
+        if lo == hi:
+            continue
+        rows = torch.cat([torch.randint(lo, hi, (14,), generator=g, device="cuda"),
+                          torch.tensor([lo, hi - 1], device="cuda")])
+        cols = torch.cat([torch.randint(0, n, (38,), generator=g, device="cuda"),
+                          torch.tensor([0, n - 1], device="cuda")])
+        sums, exact, allowance = _emulated(torch, p, q, rows, e * n + cols)
+        cut += float((sums - exact).square().sum())
+        exact_norm += float(exact.square().sum())
+        for dtype, y in got.items():
+            y = y[rows][:, cols].double()
+            unit = base._unit(dtype)
+            bound = allowance + unit * (sums.abs() + allowance) + (2.0 ** -25 if dtype is torch.float16 else 0.0)
+            assert bool(((y - sums).abs() <= bound).all()), float(((y - sums).abs() / bound).max())
+            changed += int((y != exact.to(dtype)).sum())
+            off[dtype] += float((y - exact).square().sum())
+            own[dtype] += float((exact.to(dtype).double() - exact).square().sum())
+    assert changed > 0  # the cores did it: products of exact sums are rounded as the exact sums are
+    # what is said of the cut: below 10^-4 of the result as a whole, at a spread that makes a column of a hundred a
+    # hundred times the middle one; f16 results then lose under a tenth of their accuracy, bf16 ones under a hundredth
+    assert (cut / exact_norm) ** 0.5 < 1e-4
+    assert off[torch.float16] < 1.1 ** 2 * own[torch.float16]
+    assert off[torch.bfloat16] < 1.01 ** 2 * own[torch.bfloat16]
+
+
+@pytest.mark.parametrize("sizes,n,k", SHAPES[1:])
+def test_f32_results_are_of_exact_products(gpu, sizes, n, k):
+    import torch
+    p, q, offsets = _inputs(torch, gpu, sizes, n, k, 2.0, n + k)
+    xv = gpu.block8_unpack(p, torch.float32)
+    wv = gpu.block8_unpack(q, torch.float32).view(len(sizes), n, k)
+    want, size = base._per_row(torch, xv, wv, offsets.tolist(), True)
+    base._check(gpu.block8_matmul(p, q, offsets, out_dtype=torch.float32), want, size, k)
+
+
+def test_the_cores_keep_other_groups_out_and_repeat(gpu):
+    # NaN and infinities in one group's rows and matrix and in rows of no group; equal calls give equal bits
+    import torch
+    sizes, n, k = [700, 0, 90, 1500, 1710], 1500, 4500
+    x, w, _, offsets = base._make(torch, sizes, n, k, torch.bfloat16, 9, 10, 20)
+    ends = offsets.tolist()
+
+    def product():
+        return gpu.block8_matmul(gpu.block8_pack(x), gpu.block8_pack(w.reshape(-1, k)), offsets)
+
+    clean = product()
+    assert not torch.equal(clean, gpu.block8_matmul(gpu.block8_pack(x), gpu.block8_pack(w.reshape(-1, k)), offsets,
+                                                    out_dtype=torch.float32).bfloat16())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = product()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(clean, again)
+    x[:ends[0]], x[ends[-1]:], x[ends[2]:ends[3]] = float("nan"), float("inf"), float("nan")
+    w[1], w[2] = float("nan"), float("-inf")
+    dirty = product()
+    for lo, hi in ((0, ends[2]), (ends[3], x.shape[0])):
+        assert torch.equal(clean[lo:hi], dirty[lo:hi])
+    assert bool(torch.isnan(dirty[ends[2]:ends[3]]).all())
+    assert not bool(dirty[:ends[0]].any()) and not bool(dirty[ends[-1]:].any())

@@ -173,8 +173,12 @@ struct GroupPart {
   int group, lo, hi;
   int parts, slot;  // of the group; this part's slot where there are several
 };
-__device__ __forceinline__ int group_parts(int size, int limit) {
-  return limit > 0 && size > limit ? (size + limit - 1) / limit : 1;
+__host__ __device__ __forceinline__ int group_parts(int size, int limit) {
+  return limit > 0 && size > limit ? (size - 1) / limit + 1 : 1;  // size + limit may pass 2^31
+}
+// The rows of each of several parts but the last, which may have fewer.
+__host__ __device__ __forceinline__ int group_part_length(int size, int parts) {
+  return ((size - 1) / parts / 64 + 1) * 64;
 }
 
 // The part at a place in the order of falling lengths (ties by index; above 62
@@ -194,7 +198,7 @@ __device__ __forceinline__ bool find_group_part(const int64_t* __restrict__ offs
   const Segments s = load_segments(offsets, groups, rows);
   const bool real = lane >= 1 && lane <= groups;
   const int size = s.end - s.first, parts = real ? group_parts(size, limit) : 0;
-  const int length = parts > 1 ? ((size + parts - 1) / parts + 63) / 64 * 64 : size;
+  const int length = parts > 1 ? group_part_length(size, parts) : size;
   int before = 0;
   for (int o = 1; o <= groups; ++o) {
     const int l = __builtin_amdgcn_readlane(length, o), n = __builtin_amdgcn_readlane(parts, o);

@@ -131,3 +131,24 @@ def test_the_cores_keep_other_groups_out_and_repeat(gpu):
         assert torch.equal(clean[lo:hi], dirty[lo:hi])
     assert bool(torch.isnan(dirty[ends[2]:ends[3]]).all())
     assert not bool(dirty[:ends[0]].any()) and not bool(dirty[ends[-1]:].any())
+
+
+def test_weight_gradients_of_two_billion_rows(gpu):
+    # one group whose length and greatest part together pass 2^31
+    import torch
+    rows, n, k = 2_090_000_000, 8, 8
+    if torch.cuda.mem_get_info()[0] < 90 * 2 ** 30:
+        pytest.skip("needs 67 GB")
+    assert gpu._lib.pxg_grouped_matmul_grad_weight_workspace(rows, n, k, 1) > 4 * n * k
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    grad = torch.zeros(rows, n, dtype=torch.bfloat16, device="cuda")
+    g = base._dev(torch, 41)
+    at = torch.cat([torch.randint(0, rows, (60,), generator=g, device="cuda"),
+                    torch.tensor([0, rows // 2, rows - 1], device="cuda")])
+    x[at] = torch.randn(63, k, generator=g, device="cuda").bfloat16()
+    grad[at] = torch.randn(63, n, generator=g, device="cuda").bfloat16()
+    out = torch.full((1, n, k), 7.0, device="cuda")
+    gpu.grouped_matmul_grad_weight(grad, x, torch.tensor([0, rows], device="cuda"), out=out)
+    # all other products are zero, and adding zeros rounds nothing
+    want, size = base._per_group(torch, grad[at], x[at], [0, 63])
+    base._check(out, want, size, 63)

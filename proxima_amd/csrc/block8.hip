@@ -103,13 +103,13 @@ __device__ __forceinline__ uint32_t pack8(const float (&x)[8], uint32_t (&code)[
 }
 
 // Where a thread begins: threads of a workgroup are blockDim.x / 16 blocks of
-// 128 columns by blockDim.y rows. The rows are the grid's x; its y are column
-// parts.
+// 128 columns by blockDim.y rows. The rows are the grid's x and z; its y are
+// column parts.
 struct Place {
   uint64_t row;
   uint32_t col, step;
   __device__ Place() {
-    row = (uint64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    row = ((uint64_t)blockIdx.z * gridDim.x + blockIdx.x) * blockDim.y + threadIdx.y;
     col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
     step = gridDim.y * blockDim.x * 8;
   }
@@ -259,13 +259,17 @@ activation_grad_rows(const T* __restrict__ g, uint64_t gs, uint32_t rows, uint32
 }
 
 // Calls launch(grid, block) with a thread for 8 columns: workgroups of one
-// row's 2048 columns, or of several rows of fewer.
+// row's 2048 columns, or of several rows of fewer. A launch has less than 2^32
+// work-items along x (more wrap around silently): what is over goes along z.
 template <class F>
 void by_rows(uint64_t rows, uint64_t wide, F launch) {
   uint64_t x = 16;
   while (x < ROW_THREADS && x * 8 < wide) x *= 2;
   const uint64_t y = ROW_THREADS / x, parts = (wide / 8 + x - 1) / x;
-  launch(dim3((unsigned)((rows + y - 1) / y), (unsigned)(parts < 1024 ? parts : 1024)),
+  constexpr uint64_t ACROSS = 1u << 23;  // workgroups of at most 256 threads along x
+  const uint64_t workgroups = (rows + y - 1) / y;
+  launch(dim3((unsigned)(workgroups < ACROSS ? workgroups : ACROSS), (unsigned)(parts < 1024 ? parts : 1024),
+              (unsigned)((workgroups + ACROSS - 1) / ACROSS)),
          dim3((unsigned)x, (unsigned)y));
   PXG_HIP(hipGetLastError());
 }

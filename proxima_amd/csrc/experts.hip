@@ -57,6 +57,7 @@ struct Product {
   bool c_vec;           // C's rows are 16-byte aligned
   int limit = 0;        // grad weight: longer groups are summed in parts (groups.hpp),
   float* workspace = nullptr;  // in slots of m x n
+  unsigned across = 0;  // workgroups to a row of the grid
 };
 
 template <class T>
@@ -93,6 +94,9 @@ constexpr bool is_copied(int l) { return l == ROWS || l == COLS; }
 struct Fp8 {};  // packed operands multiplied as they are
 
 #if defined(__HIP_DEVICE_COMPILE__)
+// A workgroup's place among all of its launch.
+__device__ __forceinline__ unsigned workgroup(const Product& p) { return blockIdx.y * p.across + blockIdx.x; }
+
 // A raw buffer resource over [p, p + bytes), from wave-uniform scalars;
 // accesses at offsets outside it read zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* p, uint64_t bytes) {
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   // takes an eighth of the tiles, in order, so that tiles that share operands
   // meet in one L2; the longest come first, as what begins last ends last.
   const int tiles_n = (p.n + TN - 1) / TN;
-  const int die = blockIdx.x & 7, at = blockIdx.x >> 3;
+  const int die = workgroup(p) & 7, at = workgroup(p) >> 3;
   int m0, n0, rows, cols, steps, group, tail;
   uint64_t a0, b0;  // first elements of the operands' tiles
   [[maybe_unused]] uint64_t sa0 = 0, sb0 = 0;  // and their rows, packed
@@ -776,8 +780,8 @@ __global__ void __launch_bounds__(512, 4) product_few(Product p) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tiles_n = (p.n + TN - 1) / TN;
   RowTile t;
-  if (!find_row_tile<ALL_TILES>(p.offsets, p.groups, p.rows, 16, (int)(blockIdx.x / tiles_n), t)) return;
-  const int n0 = (int)(blockIdx.x % tiles_n) * TN;
+  if (!find_row_tile<ALL_TILES>(p.offsets, p.groups, p.rows, 16, (int)(workgroup(p) / tiles_n), t)) return;
+  const int n0 = (int)(workgroup(p) % tiles_n) * TN;
   const int rows = t.end - t.row < 16 ? t.end - t.row : 16, cols = p.n - n0 < TN ? p.n - n0 : TN;
   const int k_end = t.group < 0 ? 0 : p.k, group = t.group < 0 ? 0 : t.group;
   constexpr int BYTES = IS_PACKED ? 1 : 2;
@@ -887,9 +891,14 @@ void by_types(int type, int out_type, F f) {
   else g((__bf16)0.0f);
 }
 
-unsigned grid_size(uint64_t tiles) {
+// A launch has less than 2^32 work-items along x (more wrap around silently):
+// what is over goes along y, in rows of a multiple of eight workgroups, so that
+// the dies still take them in turn.
+dim3 grid_of(uint64_t tiles, Product& p) {
+  constexpr uint64_t ACROSS = 1u << 22;  // of at most 512 threads
   if (tiles > PRODUCT_SIZE_MAX) config_error("rows", tiles, "gives more tiles than a launch has workgroups");
-  return (unsigned)tiles;
+  p.across = (unsigned)std::min(tiles, ACROSS);
+  return dim3(p.across, (unsigned)((tiles + ACROSS - 1) / ACROSS));
 }
 
 void check_groups(uint64_t groups, const int64_t* offsets) {
@@ -932,15 +941,15 @@ __global__ void __launch_bounds__(256) join_parts(Product p) {
 }
 
 template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
-void launch_tiled(const Product& p, hipStream_t s) {
+void launch_tiled(Product p, hipStream_t s) {
   using K = Tiled<T, WM, WN, MT, NT>;
   const uint64_t tn = (p.n + K::TN - 1) / K::TN;
   uint64_t tiles;
   if (FORM == GRAD_WEIGHT)
     tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * group_parts_max(p.rows, p.groups, p.limit);
   else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn / 8 + 2) * 8;  // both kinds' eighths
-  hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), dim3(grid_size(tiles)), dim3(K::THREADS), 0, s,
-                     p);
+  const dim3 grid = grid_of(tiles, p);
+  hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), grid, dim3(K::THREADS), 0, s, p);
   PXG_HIP(hipGetLastError());
 }
 
@@ -950,10 +959,11 @@ bool copies(int bytes, const void* d, uint64_t cols, uint64_t stride, uint64_t g
 }
 
 template <class T, class O, int LB, bool IS_PACKED>
-void launch_few(const Product& p, hipStream_t s) {
+void launch_few(Product p, hipStream_t s) {
   constexpr uint64_t TN = LB == ROWS ? 16 : 128;
   const uint64_t tiles = row_tiles_max(p.rows, p.groups, 16, p.offsets != nullptr) * ((p.n + TN - 1) / TN);
-  hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED>), dim3(grid_size(tiles)), dim3(512), 0, s, p);
+  const dim3 grid = grid_of(tiles, p);
+  hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED>), grid, dim3(512), 0, s, p);
   PXG_HIP(hipGetLastError());
 }
 
@@ -1104,7 +1114,7 @@ void launch_product(Product p, uint64_t room, hipStream_t s) {
   if (FORM == GRAD_WEIGHT && p.limit) {
     const uint64_t divided = std::min<uint64_t>(p.groups, p.rows / p.limit);
     if (divided) {
-      const dim3 grid(grid_size(divided * std::min(p.m, JOIN_ROWS)), (unsigned)(((uint64_t)p.n + 1023) / 1024));
+      const dim3 grid((unsigned)(divided * std::min(p.m, JOIN_ROWS)), (unsigned)(((uint64_t)p.n + 1023) / 1024));
       hipLaunchKernelGGL(join_parts<O>, grid, dim3(256), 0, s, p);
       PXG_HIP(hipGetLastError());
     }

@@ -152,3 +152,65 @@ def test_weight_gradients_of_two_billion_rows(gpu):
     # all other products are zero, and adding zeros rounds nothing
     want, size = base._per_group(torch, grad[at], x[at], [0, 63])
     base._check(out, want, size, 63)
+
+
+def _marked(torch, rows, cols, dtype, seed, at):
+    """Zeros but for some rows."""
+    x = torch.zeros(rows, cols, dtype=dtype, device="cuda")
+    x[at] = torch.randn(len(at), cols, generator=base._dev(torch, seed), device="cuda").to(dtype)
+    return x
+
+
+def _spots(torch, rows, seed):
+    g = base._dev(torch, seed)
+    at = torch.cat([torch.randint(0, rows, (50,), generator=g, device="cuda"),
+                    torch.tensor([0, rows // 2, rows - 2, rows - 1], device="cuda")])
+    return torch.unique(at)
+
+
+def _need(torch, gigabytes):
+    if torch.cuda.mem_get_info()[0] < gigabytes * 2 ** 30:
+        pytest.skip(f"needs {gigabytes} GB")
+
+
+def test_packing_of_more_rows_than_a_grid_has_along_x(gpu):
+    # 2^24 rows and 256 threads for each: 2^32 work-items
+    import torch
+    rows, cols = 2 ** 24 + 37, 1025
+    _need(torch, 150)
+    at = _spots(torch, rows, 51)
+    x = _marked(torch, rows, cols, torch.float16, 52, at)
+    p = gpu.block8_pack(x)
+    q = gpu.block8_pack(x[at])
+    assert torch.equal(p.codes[at], q.codes) and torch.equal(p.scales[at], q.scales)
+    y = gpu.block8_unpack(p, torch.float16)
+    assert torch.equal(y[at], gpu.block8_unpack(q, torch.float16))
+    y[at] = 0
+    assert not bool(y.any())
+    del y
+    a, p = gpu.activation_pack(x, "gelu")
+    b, q = gpu.activation_pack(x[at], "gelu")
+    assert torch.equal(a[at], b) and torch.equal(p.codes[at], q.codes)
+    d = gpu.activation_grad(x, p, "gelu", out=a)
+    assert torch.equal(d[at], gpu.activation_grad(x[at], q, "gelu"))
+    d[at] = 0
+    assert not bool(d.any())
+
+
+@pytest.mark.parametrize("rows,n,k", [(140_000_000, 8, 8), (1_080_000_000, 7, 7), (1_080_000_000, 8, 8)])
+def test_products_of_more_tiles_than_a_grid_has_along_x(gpu, rows, n, k):
+    # workgroups of 512 threads for 16 rows, of 256 for 64
+    import torch
+    _need(torch, 100 if rows > 10 ** 9 else 20)
+    at = _spots(torch, rows, 61)
+    x = _marked(torch, rows, k, torch.bfloat16, 62, at)
+    w = torch.randn(2, n, k, generator=base._dev(torch, 63), device="cuda").bfloat16()
+    offsets = torch.tensor([0, rows // 2 + 1, rows], device="cuda")
+    ends = [0, int((at <= rows // 2).sum()), len(at)]
+    for call, transposed in ((gpu.grouped_matmul, True), (gpu.grouped_matmul_grad_input, False)):
+        y = call(x, w, offsets)
+        want, size = base._per_row(torch, x[at], w, ends, transposed)
+        base._check(y[at], want, size, k)
+        y[at] = 0
+        assert not bool(y.any())
+        del y

@@ -10,6 +10,11 @@ return without waiting; outputs are new tensors unless `out` is given. Rows may
 be strided; a row's columns are contiguous. `offsets` is an int64 tensor of
 groups + 1 values: group g is the rows offsets[g] to offsets[g + 1], and rows
 of no group get zeros.
+
+None of them records history for autograd: the gradients are functions of their
+own. An operand that requires grad is refused while grad mode is on, so that no
+gradient is lost unseen; inside torch.no_grad() and a torch.autograd.Function
+it is off.
 """
 import sys
 
@@ -144,8 +149,12 @@ def _run(fn, tensors, *args):
     """fn(*args, stream) on torch's current stream of the device that all tensors share."""
     device = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise ValueError("operands must be on one device")
+        if t is not None:
+            if t.get_device() != device:
+                raise ValueError("operands must be on one device")
+            if t.requires_grad and _torch.is_grad_enabled():
+                raise ValueError("an operand requires grad, but no history is recorded here: call the gradients' own "
+                                 "functions, under torch.no_grad() or from a torch.autograd.Function")
     if _current_device() == device:
         status = fn(*args, _current_stream(device))
     else:

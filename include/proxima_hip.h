@@ -474,7 +474,8 @@ int pxg_grouped_matmul_device(int type, const void* d_x, uint64_t rows, uint64_t
                               uint64_t groups, uint64_t n, uint64_t w_stride, uint64_t w_group_stride,
                               const int64_t* d_offsets, int out_type, void* d_y, uint64_t y_stride, void* stream);
 /* Its gradients, grad being y's: dx = grad w_g, and dw_g = the sum over the
- * group's rows t of grad[t]^T x[t] (zeros for an empty group). Long sums into
+ * group's rows t of grad[t]^T x[t] (zeros for an empty group); the groups' dw
+ * lie dw_group_stride apart and may not overlap. Long sums into
  * small matrices are faster with a workspace (16-byte aligned device memory,
  * not kept after the work is done): workspace() says how many bytes, 0 where
  * none helps; with less, or NULL, sums are taken in fewer parts, or one. */

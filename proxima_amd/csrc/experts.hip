@@ -1211,6 +1211,7 @@ int pxg_grouped_matmul_grad_weight_device(int type, const void* d_grad, uint64_t
     check_rows(type, "grad", d_grad, rows, n, grad_stride);
     check_rows(type, "x", d_x, rows, k, x_stride);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
+    check_matrices_apart("dw_group_stride", groups, n, k, dw_stride, dw_group_stride);
     check_aligned("workspace", d_workspace, 16);
     grad_stride = check_stride(rows, n, grad_stride);
     x_stride = check_stride(rows, k, x_stride);
@@ -1235,6 +1236,7 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
     check_rows(PXG_BF16, "grad", d_grad, rows, n, grad_stride);
     check_packed_rows("codes", d_codes, "scales", d_scales, rows);
     check_rows(out_type, "dw", d_dw, n, k, dw_stride);
+    check_matrices_apart("dw_group_stride", groups, n, k, dw_stride, dw_group_stride);
     check_aligned("workspace", d_workspace, 16);
     grad_stride = check_stride(rows, n, grad_stride);
     check_stride(2, k, block8_code_stride(k));

@@ -37,6 +37,17 @@ inline void check_rows(int type, const char* name, const void* p, uint64_t rows,
   if (rows && (uint64_t)(uintptr_t)p % type_bytes(type))
     config_error(name, (uint64_t)(uintptr_t)p, "must be aligned to its type");
 }
+// The groups' matrices of a result, each of n rows of `cols`: one after the
+// other or, row by row, between one another. Overlapping ones would be written
+// by several groups at once.
+inline void check_matrices_apart(const char* name, uint64_t groups, uint64_t n, uint64_t cols, uint64_t stride,
+                                 uint64_t group_stride) {
+  using u128 = unsigned __int128;
+  if (groups <= 1) return;
+  const bool after = group_stride >= (u128)(n - 1) * stride + cols;
+  const bool between = group_stride >= cols && stride >= (u128)(groups - 1) * group_stride + cols;
+  if (!after && !between) config_error(name, group_stride, "must keep the groups' matrices apart");
+}
 // Packed rows (block8.hpp), laid out as the packing entry point does.
 inline void check_packed_rows(const char* codes_name, const void* codes, const char* scales_name, const void* scales,
                               uint64_t rows) {

@@ -1,5 +1,6 @@
-"""Expert layers under torch's autograd: no gradient is lost unseen, and a
-torch.autograd.Function made of them is differentiated by their gradients."""
+"""Expert layers in a training program: no gradient is lost unseen under
+autograd, a torch.autograd.Function made of them is differentiated by their
+gradients, and gradients may be written among others."""
 import pytest
 
 import test_experts_gpu as base
@@ -57,3 +58,17 @@ def test_a_function_of_them_is_differentiated(gpu):
     with torch.no_grad():
         assert torch.equal(x.grad, gpu.grouped_matmul_grad_input(grad, w, offsets))
         assert torch.equal(w.grad, gpu.grouped_matmul_grad_weight(grad, x, offsets))
+
+
+def test_gradients_into_matrices_that_lie_between_one_another(gpu):
+    import torch
+    x, w, grad, offsets = base._make(torch, [70, 0, 33], 48, 64, torch.bfloat16, 3)
+    want = gpu.grouped_matmul_grad_weight(grad, x, offsets)
+    between = torch.zeros(48, 3, 64, dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    apart = torch.zeros(3, 50, 72, dtype=torch.bfloat16, device="cuda")[:, :48, :64]
+    for out in (between, apart):
+        gpu.grouped_matmul_grad_weight(grad, x, offsets, out=out)
+        assert torch.equal(out, want)
+    one = torch.zeros(1, 48, 64, dtype=torch.bfloat16, device="cuda").expand(3, 48, 64)
+    with pytest.raises(gpu.ProximaError, match="dw_group_stride"):
+        gpu.grouped_matmul_grad_weight(grad, x, offsets, out=one)

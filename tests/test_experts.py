@@ -88,3 +88,21 @@ def test_python_side_refuses_host_tensors():
                  lambda: px.activation_pack(x, "tanh")):
         with pytest.raises(ValueError):
             call()
+
+
+def test_matrices_of_a_result_may_not_overlap(lib):
+    p = C.c_void_p(4096)
+
+    def plain(groups, n, k, stride, group_stride):
+        return lib.pxg_grouped_matmul_grad_weight_device(2, p, 4, n, n, p, k, k, p, groups, 2, p, stride, group_stride,
+                                                         None, 0, None)
+
+    def packed(groups, n, k, stride, group_stride):
+        return lib.pxg_grouped_matmul_grad_weight_block8_device(p, 4, n, n, p, p, k, p, groups, 2, p, stride,
+                                                                group_stride, None, 0, None)
+
+    for call in (plain, packed):
+        # one matrix for all groups; a row, an element too near; rows of one group among another's; past 64 bits
+        for groups, n, k, stride, apart in ((2, 8, 8, 8, 0), (2, 8, 8, 8, 56), (3, 8, 8, 8, 63), (3, 8, 8, 23, 8),
+                                            (2, 8, 8, 16, 4), (2, 1, 8, 8, 7), (2, 8, 8, (1 << 63) + 8, 7)):
+            _refused(lib, call(groups, n, k, stride, apart), b"dw_group_stride")

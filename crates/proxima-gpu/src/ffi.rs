@@ -233,6 +233,8 @@ extern "C" {
         grad_stride: u64, d_codes: *const c_void, d_scales: *const c_void, k: u64, d_offsets: *const i64,
         groups: u64, out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64,
         d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_matmul_set_kernel(rows: c_int) -> c_int;
+    pub(crate) fn pxg_grouped_matmul_last_kernel() -> u32;
     pub(crate) fn pxg_activation_pack_device(activation: c_int, kind: c_int, d_h: *const c_void, rows: u64,
         cols: u64, h_stride: u64, d_a: *mut c_void, a_stride: u64, d_codes: *mut c_void, d_scales: *mut c_void,
         stream: *mut c_void) -> c_int;

@@ -497,6 +497,17 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
                                                  uint64_t dw_stride, uint64_t dw_group_stride, void* d_workspace,
                                                  uint64_t workspace_bytes, void* stream);
 
+/* Which kernel the products of this thread take (for tests and tuning): 0 =
+ * the one estimated fastest, 16 = that for few rows, 64, 128 or 256 = tiles of
+ * as many rows and columns; where it cannot take a product's operands, the
+ * estimate decides. 256 multiplies packed rows into 16 bits on the 8-bit cores. */
+int pxg_grouped_matmul_set_kernel(int rows);
+/* The kernel of the last product on this thread: its rows as above, with these
+ * bits. PARTS: groups longer than a limit, if there are any, were summed in
+ * parts. */
+enum { PXG_KERNEL_8_BIT = 1 << 16, PXG_KERNEL_UNALIGNED = 1 << 17, PXG_KERNEL_PARTS = 1 << 18 };
+uint32_t pxg_grouped_matmul_last_kernel(void);
+
 /* a = f(h), computed from h itself, and h packed, to be kept for the backward
  * pass; and that pass: dh = grad * f'(unpacked h). f32, f16 or bf16. */
 int pxg_activation_pack_device(int activation, int type, const void* d_h, uint64_t rows, uint64_t cols,

@@ -940,6 +940,10 @@ __global__ void __launch_bounds__(256) join_parts(Product p) {
   }
 }
 
+// The kernel asked for on this thread (0: the cheapest), and the last one launched.
+thread_local int g_kernel = 0;
+thread_local uint32_t g_last_kernel = 0;
+
 template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT>
 void launch_tiled(Product p, hipStream_t s) {
   using K = Tiled<T, WM, WN, MT, NT>;
@@ -951,6 +955,8 @@ void launch_tiled(Product p, hipStream_t s) {
   const dim3 grid = grid_of(tiles, p);
   hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), grid, dim3(K::THREADS), 0, s, p);
   PXG_HIP(hipGetLastError());
+  g_last_kernel = K::TM | (K::FP8 ? PXG_KERNEL_8_BIT : 0) | (is_any(LA) ? PXG_KERNEL_UNALIGNED : 0) |
+                  (p.limit ? PXG_KERNEL_PARTS : 0);
 }
 
 // Whether an operand can be copied: 16-byte pieces that all belong to one row.
@@ -965,6 +971,7 @@ void launch_few(Product p, hipStream_t s) {
   const dim3 grid = grid_of(tiles, p);
   hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED>), grid, dim3(512), 0, s, p);
   PXG_HIP(hipGetLastError());
+  g_last_kernel = 16;
 }
 
 // Which tiles a product takes: the cheapest by what was measured, in us. A
@@ -1005,12 +1012,13 @@ struct Cost {
 //   1 of 4096, 768 x 768                           36 ->  21 (1536)
 //   8 uneven ones, 16384 rows in all, 512 x 512    39 ->  30 (1024)
 //   8 uneven, 8192 rows, 4096 x 1024               63 ->  87 (2048): the parts' traffic
-Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0) {
+Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0, int tile_asked = 0) {
   Cost best;
   const double average = form == GRAD_WEIGHT ? (double)p.rows / p.groups : p.k;
   const double longest = form == GRAD_WEIGHT ? average * std::sqrt((double)p.groups) : p.k;
   for (int i = 0; i < 3; ++i) {
     const Tile& t = packed ? PACKED_TILES[i] : TILES[i];
+    if (tile_asked && tile_asked != t.size) continue;
     const uint64_t tn = ((uint64_t)p.n + t.size - 1) / t.size;
     const uint64_t tiles = form == GRAD_WEIGHT ? (((uint64_t)p.m + t.size - 1) / t.size) * tn
                                                : (p.rows + (uint64_t)p.groups * t.size / 2 + t.size - 1) / t.size * tn;
@@ -1076,6 +1084,11 @@ double tiled_cost(double cost, bool packed, const Product& p) {
   return std::max(cost, (double)std::min(p.rows, p.groups) * p.n * p.k * (packed ? 1 : 2) / 5.9e6);
 }
 
+// The tile asked for on this thread, 0 if any; packed rows into f32 have no 256.
+int asked_tile(bool packed_into_f32) {
+  return g_kernel == 16 || (packed_into_f32 && g_kernel == 256) ? 0 : g_kernel;
+}
+
 // `room`: bytes of p.workspace.
 template <int FORM, class T, class O, bool IS_PACKED>
 void launch_product(Product p, uint64_t room, hipStream_t s) {
@@ -1085,14 +1098,15 @@ void launch_product(Product p, uint64_t room, hipStream_t s) {
   const uint64_t acols = FORM == GRAD_WEIGHT ? p.m : p.k, bcols = FORM == FORWARD ? p.k : p.n;
   const bool copied = (is_packed(LA) || copies(2, p.a, acols, p.as, 0)) &&
                       (is_packed(LB) || copies(2, p.b, bcols, p.bs, p.bg));
-  const Cost cost = product_cost(FORM, p, FORM == FORWARD && IS_PACKED, room);
+  constexpr bool PACKED_FORWARD = FORM == FORWARD && IS_PACKED;
+  const Cost cost = product_cost(FORM, p, PACKED_FORWARD, room, asked_tile(PACKED_FORWARD && std::is_same_v<O, float>));
   if constexpr (FORM != GRAD_WEIGHT) {
     constexpr int B = FORM == GRAD_INPUT ? COLS : ROWS;
     // COLS spans a matrix' rows with one resource
     const bool reaches = B == ROWS || p.k * p.bs * 2 <= 0x7FFFFFFF;
     const double tiled = std::is_same_v<O, float> ? cost.best : std::min(cost.best, cost.fp8);
-    if (copied && reaches && few_cost(B, IS_PACKED, p) <= tiled_cost(tiled, IS_PACKED, p))
-      return launch_few<T, O, B, IS_PACKED>(p, s);
+    const bool few = g_kernel ? g_kernel == 16 : few_cost(B, IS_PACKED, p) <= tiled_cost(tiled, IS_PACKED, p);
+    if (copied && reaches && few) return launch_few<T, O, B, IS_PACKED>(p, s);
   }
   if constexpr (FORM == GRAD_WEIGHT) p.limit = cost.limit;
   if constexpr (FORM == FORWARD && IS_PACKED && !std::is_same_v<O, float>)
@@ -1139,6 +1153,15 @@ void run_product(int type, int out_type, const Product& p, hipStream_t s, uint64
 using namespace pxg;
 
 extern "C" {
+
+int pxg_grouped_matmul_set_kernel(int rows) {
+  return guard([&] {
+    if (rows != 0 && rows != 16 && rows != 64 && rows != 128 && rows != 256)
+      config_error("rows", (uint64_t)rows, "must be 0, 16, 64, 128 or 256");
+    g_kernel = rows;
+  });
+}
+uint32_t pxg_grouped_matmul_last_kernel(void) { return g_last_kernel; }
 
 int pxg_grouped_matmul_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride, const void* d_w,
                               uint64_t groups, uint64_t n, uint64_t w_stride, uint64_t w_group_stride,
@@ -1192,7 +1215,7 @@ uint64_t pxg_grouped_matmul_grad_weight_workspace(uint64_t rows, uint64_t n, uin
   p.groups = (int)groups;
   p.m = (int)n;
   p.n = (int)k;
-  const Cost cost = product_cost(GRAD_WEIGHT, p, false, UINT64_MAX);
+  const Cost cost = product_cost(GRAD_WEIGHT, p, false, UINT64_MAX, asked_tile(false));
   return 4 * group_slots_max(rows, groups, cost.limit) * n * k;
 }
 

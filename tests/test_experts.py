@@ -106,3 +106,10 @@ def test_matrices_of_a_result_may_not_overlap(lib):
         for groups, n, k, stride, apart in ((2, 8, 8, 8, 0), (2, 8, 8, 8, 56), (3, 8, 8, 8, 63), (3, 8, 8, 23, 8),
                                             (2, 8, 8, 16, 4), (2, 1, 8, 8, 7), (2, 8, 8, (1 << 63) + 8, 7)):
             _refused(lib, call(groups, n, k, stride, apart), b"dw_group_stride")
+
+
+def test_kernels_that_are_not_there_are_refused(lib):
+    for rows in (-1, 1, 32, 512):
+        _refused(lib, lib.pxg_grouped_matmul_set_kernel(rows), b"rows")
+    for rows in (16, 64, 128, 256, 0):
+        assert lib.pxg_grouped_matmul_set_kernel(rows) == 0

@@ -442,7 +442,8 @@ typedef enum pxg_activation { PXG_SILU = 0, PXG_GELU = 1 } pxg_activation;
  * in [-126, 127] with max |x| <= 448 * 2^e over the block's finite x; codes
  * are x * 2^-e rounded to e4m3 (nearest, ties to even; a non-finite x gives
  * NaN) and the scale byte is e + 127. A code's value times 2^e is exact in
- * f32 and bf16. Codes are rows of code_stride(cols) bytes (cols rounded up to
+ * f32 and bf16, but for 2^128, to which magnitudes from 1.9375 * 2^127 on
+ * round: that is infinity there, and an activation's gradient NaN. Codes are rows of code_stride(cols) bytes (cols rounded up to
  * 128, zero past cols), 16-byte aligned; scales are rows of
  * scale_stride(cols) bytes (blocks rounded up to 4, 127 past the blocks),
  * 4-byte aligned. */

@@ -10,7 +10,8 @@
 // The scale is a power of two so that x * 2^-e is exact (the only rounding is
 // to the code's three fraction bits; one as fine as the block's values allow
 // would save nothing, for e4m3's step follows each value's binade), so that a
-// decoded value is exact in bf16, and because gfx950's matrix cores multiply
+// decoded value is exact in bf16 (magnitudes from 1.9375 2^127 on round to 2^128,
+// which decodes as infinity), and because gfx950's matrix cores multiply
 // by scales of this form themselves.
 //
 // Layout: codes row-major, rows BLOCK8_BLOCK * ceil(cols / 128) bytes apart,
@@ -40,7 +41,7 @@ __device__ __forceinline__ uint32_t block8_scale_byte(float m) {
   const int s = (int)(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   return (uint32_t)(s < 1 ? 1 : s);
 }
-// 2^e and 2^-e from the byte (2^-127, for the never written byte 254, is subnormal).
+// 2^e and 2^-e from a byte that packing writes, 1 to 247.
 __device__ __forceinline__ float block8_scale(uint32_t byte) { return __builtin_bit_cast(float, byte << 23); }
 __device__ __forceinline__ float block8_inverse(uint32_t byte) {
   return __builtin_bit_cast(float, (254u - byte) << 23);

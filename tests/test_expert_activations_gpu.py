@@ -61,7 +61,11 @@ def test_slopes_of_every_kept_value(gpu, act, dtype):
     h = _all_values(torch, dt).reshape(-1, 1).contiguous()
     p = gpu.block8_pack(h)
     kept = gpu.block8_unpack(p, torch.float32).double()
+    # magnitudes that round to 2^128 are infinity when unpacked, and nothing else is
+    over = torch.isinf(kept)
+    assert torch.equal(over, h.double().abs() >= 1.9375 * 2.0 ** 127)
+    assert torch.equal(torch.sign(kept[over]), torch.sign(h[over].double()))
     _, slope, terms = _tails(torch, kept, act)
     got = gpu.activation_grad(torch.ones_like(h), p, act)
-    ok, worst = _within(torch, got, slope, terms)
+    ok, worst = _within(torch, got[~over], slope[~over], terms[~over])
     assert ok, worst

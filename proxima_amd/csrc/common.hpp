@@ -97,6 +97,15 @@ int guard(F&& f) {
   }
 }
 
+// A launch has less than 2^32 work-items along x: more wrap around silently.
+// Kernels that give a workgroup to each row are launched for at most this many
+// rows (of up to 512 threads), by_launches calling launch(first, count).
+constexpr size_t LAUNCH_ROWS = (size_t)1 << 22;
+template <class F>
+void by_launches(size_t rows, F&& launch) {
+  for (size_t a = 0; a < rows; a += LAUNCH_ROWS) launch(a, rows - a < LAUNCH_ROWS ? rows - a : LAUNCH_ROWS);
+}
+
 // Owning device allocation.
 template <class T>
 struct DevBuf {

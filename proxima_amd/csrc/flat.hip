@@ -991,7 +991,7 @@ void FlatIndex::insert(const uint64_t* in_ids, const float* vecs, uint64_t n, ui
   }
   maxnorm = newmax;
   // stage and scatter in chunks of <= 64 MiB of rows
-  const size_t rows_per = std::max<size_t>(1, (64u << 20) / ((size_t)ld * 4));
+  const size_t rows_per = std::min(LAUNCH_ROWS, std::max<size_t>(1, (64u << 20) / ((size_t)ld * 4)));
   DevBuf<float> st_rows(std::min<size_t>(rows_per, n) * ld);
   DevBuf<uint32_t> st_slots(std::min<size_t>(rows_per, n));
   DevBuf<float> st_bias(std::min<size_t>(rows_per, n));
@@ -1287,7 +1287,7 @@ void FlatIndex::insert_device(const uint64_t* in_ids, const float* d_vecs, uint6
   }
   if (by_id.size() + n > (size_t)UINT32_MAX - 1)
     capacity_error("slot allocator", UINT32_MAX, "capacity exceeded: slot allocator limit is 4294967295");
-  const size_t rows_per = std::max<size_t>(1, (256u << 20) / ((size_t)ld * 4));
+  const size_t rows_per = std::min(LAUNCH_ROWS, std::max<size_t>(1, (256u << 20) / ((size_t)ld * 4)));
   const size_t chunk = std::min<size_t>(rows_per, n);
   DevBuf<float> st_rows(chunk * ld);
   DevBuf<float> st_b(chunk), st_n(chunk);

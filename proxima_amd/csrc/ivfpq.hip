@@ -2236,8 +2236,10 @@ struct IvfPqIndex {
     DevBuf<uint32_t> d_sample(ns);
     PXG_HIP(hipMemcpyAsync(d_sample.p, sample.data(), ns * 4, hipMemcpyHostToDevice, stream));
     DevBuf<float> S(ns * dim);
-    hipLaunchKernelGGL(ivf_gather_rows, dim3((unsigned)ns), dim3(256), 0, stream, X.p, (int)ld, d_sample.p, (int)ns,
-                       (int)dim, S.p);
+    by_launches(ns, [&](size_t a, size_t m) {
+      hipLaunchKernelGGL(ivf_gather_rows, dim3((unsigned)m), dim3(256), 0, stream, X.p, (int)ld, d_sample.p + a, (int)m,
+                         (int)dim, S.p + a * dim);
+    });
     PXG_HIP(hipGetLastError());
     // coarse quantizer: kmeans with ChaCha8Rng::seed_from_u64(seed) (ivfpq.rs:770-777)
     ChaCha8 rng(cfg.seed);
@@ -2248,7 +2250,10 @@ struct IvfPqIndex {
     DevBuf<uint32_t> as(ns);
     nearest_device(S.p, (int)dim, nullptr, ns, (int)dim, coarse.p, (int)dim, kc.k, true, as.p, nullptr, stream);
     DevBuf<float> R(ns * dim);
-    hipLaunchKernelGGL(ivf_residuals, dim3((unsigned)ns), dim3(256), 0, stream, S.p, coarse.p, as.p, (int)dim, R.p);
+    by_launches(ns, [&](size_t a, size_t m) {
+      hipLaunchKernelGGL(ivf_residuals, dim3((unsigned)m), dim3(256), 0, stream, S.p + a * dim, coarse.p, as.p + a,
+                         (int)dim, R.p + a * dim);
+    });
     PXG_HIP(hipGetLastError());
     {
       // ProductQuantizer::train validates every residual (product.rs:221-223):
@@ -2328,19 +2333,21 @@ struct IvfPqIndex {
     st.alloc(n * ld);
     DevBuf<float> b(n), nn(n);
     DevBuf<unsigned long long> bad(1);
-    PXG_HIP(hipMemsetAsync(bad.p, 0xFF, 8, stream));
-    hipLaunchKernelGGL(flat_prep_queries, dim3((unsigned)n), dim3(64), 0, stream, d_vecs, (int)dim, (int)ld, metric,
-                       1, st.p, b.p, nn.p, bad.p);
-    PXG_HIP(hipGetLastError());
-    unsigned long long bv = 0;
-    PXG_HIP(hipMemcpyAsync(&bv, bad.p, 8, hipMemcpyDeviceToHost, stream));
-    PXG_HIP(hipStreamSynchronize(stream));
-    if (bv != ~0ull) {
-      const uint64_t row = bv >> 32, comp = (uint32_t)bv;
-      raise(PXG_ERR_NON_FINITE,
-            "vector component " + std::to_string(comp) + " is not finite (vector " + std::to_string(row) + ")", comp,
-            row, NAN);
-    }
+    by_launches(n, [&](size_t a, size_t m) {
+      PXG_HIP(hipMemsetAsync(bad.p, 0xFF, 8, stream));
+      hipLaunchKernelGGL(flat_prep_queries, dim3((unsigned)m), dim3(64), 0, stream, d_vecs + a * dim, (int)dim, (int)ld,
+                         metric, 1, st.p + a * ld, b.p + a, nn.p + a, bad.p);
+      PXG_HIP(hipGetLastError());
+      unsigned long long bv = 0;
+      PXG_HIP(hipMemcpyAsync(&bv, bad.p, 8, hipMemcpyDeviceToHost, stream));
+      PXG_HIP(hipStreamSynchronize(stream));
+      if (bv != ~0ull) {
+        const uint64_t row = a + (bv >> 32), comp = (uint32_t)bv;
+        raise(PXG_ERR_NON_FINITE,
+              "vector component " + std::to_string(comp) + " is not finite (vector " + std::to_string(row) + ")", comp,
+              row, NAN);
+      }
+    });
   }
 
   // Insert prepared rows staged on the device (ivfpq.rs:1129-1158).
@@ -2367,9 +2374,11 @@ struct IvfPqIndex {
     DevBuf<uint64_t> st_ids(n);
     PXG_HIP(hipMemcpyAsync(st_sl.p, sl.data(), n * 4, hipMemcpyHostToDevice, stream));
     PXG_HIP(hipMemcpyAsync(st_ids.p, in_ids, n * 8, hipMemcpyHostToDevice, stream));
-    hipLaunchKernelGGL(flat_scatter_rows, dim3((unsigned)n), dim3(256), 0, stream, st.p, st_sl.p, (const float*)nullptr,
-                       st_ids.p, (int)n, (int)ld, vectors_kept ? X.p : (float*)nullptr, (float*)nullptr, d_live.p,
-                       d_ids.p);
+    by_launches(n, [&](size_t a, size_t m) {
+      hipLaunchKernelGGL(flat_scatter_rows, dim3((unsigned)m), dim3(256), 0, stream, st.p + a * ld, st_sl.p + a,
+                         (const float*)nullptr, st_ids.p + a, (int)m, (int)ld, vectors_kept ? X.p : (float*)nullptr,
+                         (float*)nullptr, d_live.p, d_ids.p);
+    });
     PXG_HIP(hipGetLastError());
     PXG_HIP(hipStreamSynchronize(stream));
     for (uint64_t i = 0; i < n; ++i) {
@@ -2407,9 +2416,11 @@ struct IvfPqIndex {
     PXG_HIP(hipMemsetAsync(live1.p, 0, nc, stream));
     if (n) {
       PXG_HIP(hipMemcpyAsync(d_keep.p, keep.data(), n * 4, hipMemcpyHostToDevice, stream));
-      hipLaunchKernelGGL(ivf_compact_rows, dim3((unsigned)n), dim3(128), 0, stream, d_keep.p, (int)n, (int)ld,
-                         (int)M(), vectors_kept ? X.p : (const float*)nullptr, X1.p, codes.p, c1.p, d_list_of.p, l1.p,
-                         d_ids.p, i1.p, ranks.rank.p, r1.p, live1.p);
+      by_launches(n, [&](size_t a, size_t m) {
+        hipLaunchKernelGGL(ivf_compact_rows, dim3((unsigned)m), dim3(128), 0, stream, d_keep.p + a, (int)m, (int)ld,
+                           (int)M(), vectors_kept ? X.p : (const float*)nullptr, X1.p + a * ld, codes.p, c1.p + a * M(),
+                           d_list_of.p, l1.p + a, d_ids.p, i1.p + a, ranks.rank.p, r1.p + a, live1.p + a);
+      });
       PXG_HIP(hipMemcpyAsync(d_map.p, new_of_old.data(), hw * 4, hipMemcpyHostToDevice, stream));
       hipLaunchKernelGGL(ivf_remap_slots, dim3((ranks.len + 255) / 256), dim3(256), 0, stream, ranks.rank_slot.p,
                          ranks.len, d_map.p);

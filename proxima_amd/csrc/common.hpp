@@ -97,7 +97,21 @@ int guard(F&& f) {
   }
 }
 
-// A launch has less than 2^32 work-items along x: more wrap around silently.
+// A launch has less than 2^32 work-items along x: more wrap around silently, so
+// every launch of this library is checked on its way through HIP's macro.
+inline void check_launch(dim3 grid, dim3 block) {
+  if (((uint64_t)grid.x * block.x | (uint64_t)grid.y * block.y | (uint64_t)grid.z * block.z) >> 32)
+    capacity_error("launch", UINT32_MAX,
+                   "capacity exceeded: launch limit is 4294967295 work-items; pass fewer rows or queries in a call");
+}
+#undef hipLaunchKernelGGL
+#define hipLaunchKernelGGL(kernel, grid, block, lds, stream, ...)  \
+  do {                                                             \
+    const dim3 grid_ = (grid), block_ = (block);                   \
+    ::pxg::check_launch(grid_, block_);                            \
+    (kernel)<<<grid_, block_, (lds), (stream)>>>(__VA_ARGS__);     \
+  } while (0)
+
 // Kernels that give a workgroup to each row are launched for at most this many
 // rows (of up to 512 threads), by_launches calling launch(first, count).
 constexpr size_t LAUNCH_ROWS = (size_t)1 << 22;

@@ -1,5 +1,5 @@
 """Inserts of more rows than one launch may give a workgroup of 256 threads each
-(2^24): every row is stored and found."""
+(2^24): every row is stored and found; and calls that no launch holds."""
 import numpy as np
 import pytest
 
@@ -31,3 +31,20 @@ def test_more_rows_than_a_launch(gpu, kind):
     bad[13, 2] = float("nan")
     with pytest.raises(px.NonFinite):
         index.insert_device(np.arange(20, dtype=np.uint64) + 2 * ROWS, bad)
+
+
+def test_calls_that_a_launch_cannot_hold_are_refused(gpu):
+    # one workgroup of 64 threads for each vector: 2^26 vectors are 2^32 work-items, which would wrap around
+    px = gpu
+    q = px.ScalarQuantizer.train(px.VectorSpace(1, px.Metric.EUCLIDEAN), np.array([-1.0, 1.0], np.float32))
+    x = np.linspace(-1, 1, 2 ** 26 + 3, dtype=np.float32)
+    codes = np.full(x.size, 77, np.uint8)
+
+    def encode(n):
+        return px._lib.pxg_sq_encode(px._ptr(x), n, 1, 1, 0, px._ptr(q.min), px._ptr(q.inverse_scale), px._ptr(codes))
+
+    with pytest.raises(px.Capacity, match="fewer rows or queries"):
+        px._check(encode(x.size))
+    assert (codes == 77).all()
+    assert encode(2 ** 26 - 1) == 0
+    assert codes[0] == 0 and codes[2 ** 26 - 2] == 255 and (np.diff(codes[:2 ** 26 - 1].astype(int)) >= 0).all()

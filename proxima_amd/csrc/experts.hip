@@ -57,7 +57,7 @@ struct Product {
   bool c_vec;           // C's rows are 16-byte aligned
   int limit = 0;        // grad weight: longer groups are summed in parts (groups.hpp),
   float* workspace = nullptr;  // in slots of m x n
-  unsigned across = 0;  // workgroups to a row of the grid
+  unsigned first = 0;   // workgroups of the launches before this one
 };
 
 template <class T>
@@ -94,8 +94,8 @@ constexpr bool is_copied(int l) { return l == ROWS || l == COLS; }
 struct Fp8 {};  // packed operands multiplied as they are
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// A workgroup's place among all of its launch.
-__device__ __forceinline__ unsigned workgroup(const Product& p) { return blockIdx.y * p.across + blockIdx.x; }
+// A workgroup's place among all of a product's launches.
+__device__ __forceinline__ unsigned workgroup(const Product& p) { return p.first + blockIdx.x; }
 
 // A raw buffer resource over [p, p + bytes), from wave-uniform scalars;
 // accesses at offsets outside it read zeros.
@@ -203,7 +203,9 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
   // takes an eighth of the tiles, in order, so that tiles that share operands
   // meet in one L2; the longest come first, as what begins last ends last.
   const int tiles_n = (p.n + TN - 1) / TN;
-  const int die = workgroup(p) & 7, at = workgroup(p) >> 3;
+  // weight gradients fit one launch (their first place added costs 1 to 4%)
+  const unsigned place = FORM == GRAD_WEIGHT ? blockIdx.x : workgroup(p);
+  const int die = place & 7, at = place >> 3;
   int m0, n0, rows, cols, steps, group, tail;
   uint64_t a0, b0;  // first elements of the operands' tiles
   [[maybe_unused]] uint64_t sa0 = 0, sb0 = 0;  // and their rows, packed
@@ -894,14 +896,17 @@ void by_types(int type, int out_type, F f) {
   else g((__bf16)0.0f);
 }
 
-// A launch has less than 2^32 work-items along x (more wrap around silently):
-// what is over goes along y, in rows of a multiple of eight workgroups, so that
-// the dies still take them in turn.
-dim3 grid_of(uint64_t tiles, Product& p) {
-  constexpr uint64_t ACROSS = 1u << 22;  // of at most 512 threads
-  if (tiles > PRODUCT_SIZE_MAX) config_error("rows", tiles, "gives more tiles than a launch has workgroups");
-  p.across = (unsigned)std::min(tiles, ACROSS);
-  return dim3(p.across, (unsigned)((tiles + ACROSS - 1) / ACROSS));
+// Calls launch(workgroups) for a product's tiles, p.first being those before: a
+// launch has less than 2^32 work-items along x. Each launch begins with a
+// multiple of eight, so that the dies take tiles in turn.
+template <class F>
+void by_tiles(uint64_t tiles, Product& p, F launch) {
+  if (tiles > PRODUCT_SIZE_MAX) config_error("rows", tiles, "gives more tiles than there are places for");
+  by_launches(tiles, [&](uint64_t a, uint64_t m) {
+    p.first = (unsigned)a;
+    launch(dim3((unsigned)m));
+    PXG_HIP(hipGetLastError());
+  });
 }
 
 void check_groups(uint64_t groups, const int64_t* offsets) {
@@ -955,9 +960,16 @@ void launch_tiled(Product p, hipStream_t s) {
   if (FORM == GRAD_WEIGHT)
     tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * group_parts_max(p.rows, p.groups, p.limit);
   else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn / 8 + 2) * 8;  // both kinds' eighths
-  const dim3 grid = grid_of(tiles, p);
-  hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), grid, dim3(K::THREADS), 0, s, p);
-  PXG_HIP(hipGetLastError());
+  auto launch = [&](dim3 grid) {
+    hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT>), grid, dim3(K::THREADS), 0, s, p);
+  };
+  if (FORM == GRAD_WEIGHT) {
+    if (tiles > PRODUCT_SIZE_MAX) config_error("n", tiles, "gives more tiles than a launch has workgroups");
+    launch(dim3((unsigned)tiles));
+    PXG_HIP(hipGetLastError());
+  } else {
+    by_tiles(tiles, p, launch);
+  }
   g_last_kernel = K::TM | (K::FP8 ? PXG_KERNEL_8_BIT : 0) | (is_any(LA) ? PXG_KERNEL_UNALIGNED : 0) |
                   (p.limit ? PXG_KERNEL_PARTS : 0);
 }
@@ -971,9 +983,9 @@ template <class T, class O, int LB, bool IS_PACKED>
 void launch_few(Product p, hipStream_t s) {
   constexpr uint64_t TN = LB == ROWS ? 16 : 128;
   const uint64_t tiles = row_tiles_max(p.rows, p.groups, 16, p.offsets != nullptr) * ((p.n + TN - 1) / TN);
-  const dim3 grid = grid_of(tiles, p);
-  hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED>), grid, dim3(512), 0, s, p);
-  PXG_HIP(hipGetLastError());
+  by_tiles(tiles, p, [&](dim3 grid) {
+    hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED>), grid, dim3(512), 0, s, p);
+  });
   g_last_kernel = 16;
 }
 

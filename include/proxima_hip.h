@@ -477,8 +477,8 @@ int pxg_grouped_matmul_device(int type, const void* d_x, uint64_t rows, uint64_t
 /* Its gradients, grad being y's: dx = grad w_g, and dw_g = the sum over the
  * group's rows t of grad[t]^T x[t] (zeros for an empty group); the groups' dw
  * lie dw_group_stride apart and may not overlap. Long sums into
- * small matrices are faster with a workspace (16-byte aligned device memory,
- * not kept after the work is done): workspace() says how many bytes, 0 where
+ * small matrices, and groups much longer than the others, are faster with a
+ * workspace (16-byte aligned device memory, not kept after the work is done): workspace() says how many bytes, 0 where
  * none helps; with less, or NULL, sums are taken in fewer parts, or one. */
 uint64_t pxg_grouped_matmul_grad_weight_workspace(uint64_t rows, uint64_t n, uint64_t k, uint64_t groups);
 int pxg_grouped_matmul_grad_input_device(int type, const void* d_grad, uint64_t rows, uint64_t n, uint64_t grad_stride,

@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(Product p) {
     // for a subnormal code; zeros do not count), and adds the eights' sums and
     // the accumulator in f32. A product of normal codes whose exponents' sum is
     // within 7 of E loses nothing. As a whole the result is off by 1.5e-5 of itself for normal
-    // data, 2.7e-5 with columns' magnitudes spread as exp(0.7 normal), 7.9e-5
+    // data, 2.7e-5 with columns' magnitudes spread as exp(0.7 normal), 7.6e-5
     // with exp(2 normal) (8192 x 4096 x 4096). Rounding to f16 costs 2.08e-4,
     // to bf16 1.66e-3, so that an f16 result's error grows by 0.3, 0.8 and 6%
     // and a bf16 one's by 0.1% at most; packing has cost 2.6e-2 before. Of
@@ -1050,7 +1050,9 @@ Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0, in
       }
       const double step = t.least + t.more * std::min(1.0, (double)all / t.slots);
       const double summed = form == GRAD_WEIGHT ? (double)tiles * p.rows / all : p.k;
-      // one group's half tile of padding does not begin a round
+      // one group's half tile of padding does not begin a round, up to 7680
+      // columns; of more it does, and 128 x 128 tiles are taken where 256 x 256
+      // would be faster (2048 rows, 4096 -> 8192: 150 us, 108)
       const double rounds = std::ceil((double)all / t.slots - (p.groups == 1 ? 0.12 : 0.0));
       double us = std::max(1.0, rounds) * (t.fixed + std::ceil(summed / 64) * step);
       us = std::max(us, t.fixed + (limit ? (double)limit : longest) / 64 * step);

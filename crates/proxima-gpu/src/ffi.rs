@@ -233,6 +233,20 @@ extern "C" {
         grad_stride: u64, d_codes: *const c_void, d_scales: *const c_void, k: u64, d_offsets: *const i64,
         groups: u64, out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64,
         d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_linear_device(kind: c_int, d_x: *const c_void, rows: u64, k: u64, x_stride: u64,
+        d_w: *const c_void, groups: u64, n: u64, w_stride: u64, w_group_stride: u64, d_offsets: *const i64,
+        bias_type: c_int, d_bias: *const c_void, bias_stride: u64, activation: c_int, out_type: c_int,
+        d_residual: *const c_void, residual_stride: u64, d_h: *mut c_void, h_stride: u64, d_y: *mut c_void,
+        y_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_block8_linear_device(d_codes: *const c_void, d_scales: *const c_void, rows: u64, k: u64,
+        d_w_codes: *const c_void, d_w_scales: *const c_void, groups: u64, n: u64, d_offsets: *const i64,
+        bias_type: c_int, d_bias: *const c_void, bias_stride: u64, activation: c_int, out_type: c_int,
+        d_residual: *const c_void, residual_stride: u64, d_y: *mut c_void, y_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_linear_grad_workspace(rows: u64, n: u64, groups: u64) -> u64;
+    pub(crate) fn pxg_grouped_linear_grad_device(activation: c_int, kind: c_int, d_grad: *const c_void, rows: u64,
+        n: u64, grad_stride: u64, d_h: *const c_void, h_stride: u64, d_offsets: *const i64, groups: u64,
+        d_dh: *mut c_void, dh_stride: u64, bias_type: c_int, d_dbias: *mut c_void, dbias_stride: u64,
+        d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_grouped_matmul_set_kernel(rows: c_int) -> c_int;
     pub(crate) fn pxg_grouped_matmul_last_kernel() -> u32;
     pub(crate) fn pxg_activation_pack_device(activation: c_int, kind: c_int, d_h: *const c_void, rows: u64,

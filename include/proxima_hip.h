@@ -426,8 +426,9 @@ int pxg_uniform_generate_device(uint64_t count, uint32_t dim, float lo, float hi
 /* `type` is a pxg_type. Work is ordered on `stream` (a hipStream_t; NULL =   */
 /* the null stream) and the calls return without waiting for it; they         */
 /* allocate nothing and can be captured in a graph. Outputs may not overlap   */
-/* inputs. Sums are held in f32 and rounded once, to the output's type;       */
-/* pxg_block8_matmul_device says where its products are cut before.           */
+/* inputs, but where an entry says so. Sums are held in f32 and rounded once, */
+/* to the output's type; pxg_block8_matmul_device says where its products are */
+/* cut before.                                                                */
 /* Results are the same bit for bit from call to call.                        */
 /*                                                                            */
 /* Groups: `offsets` are groups + 1 values in device memory, and group g is   */
@@ -497,6 +498,37 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
                                                  const int64_t* d_offsets, uint64_t groups, int out_type, void* d_dw,
                                                  uint64_t dw_stride, uint64_t dw_group_stride, void* d_workspace,
                                                  uint64_t workspace_bytes, void* stream);
+
+/* A layer: h = x w_g^T + b_g and y = f(h) + r, summed in f32 and y rounded
+ * once, from h before its rounding. `activation` is a pxg_activation, or -1 for
+ * f(h) = h. d_bias (NULL: none) is groups rows of n, bias_stride apart, of
+ * bias_type: the operands' type (packed rows': bf16) or f32. d_residual (NULL:
+ * none) is r, rows x n of out_type, and may be y itself. d_h (NULL: not kept)
+ * takes h in out_type. Rows of no group: y = r (zeros without), h = 0. */
+int pxg_grouped_linear_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride, const void* d_w,
+                              uint64_t groups, uint64_t n, uint64_t w_stride, uint64_t w_group_stride,
+                              const int64_t* d_offsets, int bias_type, const void* d_bias, uint64_t bias_stride,
+                              int activation, int out_type, const void* d_residual, uint64_t residual_stride,
+                              void* d_h, uint64_t h_stride, void* d_y, uint64_t y_stride, void* stream);
+/* The same over packed rows, multiplied as pxg_block8_matmul_device does. */
+int pxg_block8_linear_device(const void* d_codes, const void* d_scales, uint64_t rows, uint64_t k,
+                             const void* d_w_codes, const void* d_w_scales, uint64_t groups, uint64_t n,
+                             const int64_t* d_offsets, int bias_type, const void* d_bias, uint64_t bias_stride,
+                             int activation, int out_type, const void* d_residual, uint64_t residual_stride,
+                             void* d_y, uint64_t y_stride, void* stream);
+/* A layer's backward pass up to the products: dh = grad * f'(h), rows x n of
+ * `type` (f32, f16 or bf16, as grad and h), zeros for rows of no group; and
+ * dbias_g = the sum of the group's dh, groups rows of n of bias_type (`type` or
+ * f32), taken before dh is rounded. dh may be grad or h itself; d_dbias may be
+ * NULL. With activation -1, dh is grad, which is not written again: d_h and d_dh
+ * are not looked at. dx and dw are then the products' gradients with dh, and r's
+ * gradient is grad. workspace() says how many bytes (16-byte aligned, not kept
+ * after the work is done) long groups' sums are faster with. */
+uint64_t pxg_grouped_linear_grad_workspace(uint64_t rows, uint64_t n, uint64_t groups);
+int pxg_grouped_linear_grad_device(int activation, int type, const void* d_grad, uint64_t rows, uint64_t n,
+                                   uint64_t grad_stride, const void* d_h, uint64_t h_stride, const int64_t* d_offsets,
+                                   uint64_t groups, void* d_dh, uint64_t dh_stride, int bias_type, void* d_dbias,
+                                   uint64_t dbias_stride, void* d_workspace, uint64_t workspace_bytes, void* stream);
 
 /* Which kernel the products of this thread take (for tests and tuning): 0 =
  * the one estimated fastest, 16 = that for few rows, 64, 128 or 256 = tiles of

@@ -175,6 +175,13 @@ SIGNATURES = {
     "pxg_grouped_matmul_grad_weight_block8_device": (_i32, [_vp, _u64, _u64, _u64, _vp, _vp, _u64, _vp, _u64, _i32,
                                                             _vp, _u64, _u64, _vp, _u64, _vp]),
     "pxg_grouped_matmul_grad_weight_workspace": (_u64, [_u64, _u64, _u64, _u64]),
+    "pxg_grouped_linear_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp, _i32, _vp,
+                                         _u64, _i32, _i32, _vp, _u64, _vp, _u64, _vp, _u64, _vp]),
+    "pxg_block8_linear_device": (_i32, [_vp, _vp, _u64, _u64, _vp, _vp, _u64, _u64, _vp, _i32, _vp, _u64, _i32, _i32,
+                                        _vp, _u64, _vp, _u64, _vp]),
+    "pxg_grouped_linear_grad_workspace": (_u64, [_u64, _u64, _u64]),
+    "pxg_grouped_linear_grad_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _u64, _vp, _u64,
+                                              _i32, _vp, _u64, _vp, _u64, _vp]),
     "pxg_grouped_matmul_set_kernel": (_i32, [_i32]),
     "pxg_grouped_matmul_last_kernel": (_u32, []),
     "pxg_activation_pack_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp]),

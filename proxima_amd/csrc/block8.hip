@@ -9,62 +9,17 @@
 #include <algorithm>
 #include <cmath>
 
+#include "activation.hpp"
 #include "block8.hpp"
 #include "common.hpp"
 #include "device.hpp"
 #include "products.hpp"
+#include "rows.hpp"
 
 namespace pxg {
 namespace {
 
 constexpr int ROW_THREADS = 256;
-
-template <class T>
-__device__ __forceinline__ float to_float(T x) {
-  return (float)x;
-}
-
-// 8 columns of a row from column c: one or two 16-byte loads where VEC (the
-// row 16-byte aligned) and all eight exist, else one by one, zero past cols.
-template <class T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ row, uint64_t c, uint64_t cols, float (&x)[8]) {
-  if (VEC && c + 8 <= cols) {
-    T v[8];
-    const uint4* p = reinterpret_cast<const uint4*>(row + c);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = p[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_float(v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = c + i < cols ? to_float(row[c + i]) : 0.0f;
-  }
-}
-
-// One rounding of the f32 value: kept apart from the product before it, which
-// the compiler may otherwise fuse into the conversion to f16 in some variants
-// of a kernel and not in others.
-template <class T>
-__device__ __forceinline__ T rounded(float x) {
-  if constexpr (std::is_same_v<T, _Float16>) asm("" : "+v"(x));
-  return (T)x;
-}
-
-template <class T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ row, uint64_t c, uint64_t cols, const float (&x)[8]) {
-  if (VEC && c + 8 <= cols) {
-    T v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = rounded<T>(x[i]);
-    uint4* p = reinterpret_cast<uint4*>(row + c);
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) p[i] = reinterpret_cast<uint4*>(v)[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < cols) row[c + i] = rounded<T>(x[i]);
-  }
-}
 
 // The codes of 8 columns and their block's scale byte; all 16 threads of a
 // block call it together. The maximum passes NaN over, and NaN times a scale
@@ -158,70 +113,6 @@ block8_unpack_rows(const uint8_t* __restrict__ codes, const uint8_t* __restrict_
   }
 }
 
-// f(h) and f'(h) of the activations:
-//   silu: h s, s = 1 / (1 + exp(-h));  s (1 + h (1 - s))
-//   gelu: h P, P = (1 + erf(h / sqrt 2)) / 2;  P + h exp(-h^2 / 2) / sqrt(2 pi)
-//
-// f32 takes the math library's functions. For 16-bit types these would cost
-// more than the memory (gelu's backward pass, 16384 x 4096 in bf16: 90 us with
-// them), so they take the hardware's exp2 and reciprocal, and for gelu one
-// polynomial: 1 - P(|h|) = exp(-h^2 / 2) t R(t), t = 1 / (1 + 0.28 |h|), with R
-// the polynomial of degree 8 of least largest relative error over all h
-// (1.7e-7). Evaluated in f32 the tail is off by 6e-7 of itself up to |h| = 3,
-// 2e-6 to 6 and 7.4e-6 at 13, from the rounding of h^2 in the exponent; half of
-// f16's last place is 2^-11, 4.9e-4. SiLU's exp is off by 5e-6 where it is
-// largest. The tail's exp is the slope's second term's too.
-template <class T>
-constexpr bool fast_activation = sizeof(T) == 2;
-
-__device__ __forceinline__ float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
-
-// 1 - P(|h|), and exp(-h^2 / 2).
-__device__ __forceinline__ float gelu_tail(float h, float& e) {
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.28f, fabsf(h), 1.0f));
-  float r = 0.0247248504f;
-  r = __builtin_fmaf(r, t, -0.0936122835f);
-  r = __builtin_fmaf(r, t, 0.0924588069f);
-  r = __builtin_fmaf(r, t, -0.00647497689f);
-  r = __builtin_fmaf(r, t, 0.0727872029f);
-  r = __builtin_fmaf(r, t, 0.0836275741f);
-  r = __builtin_fmaf(r, t, 0.103085108f);
-  r = __builtin_fmaf(r, t, 0.111699775f);
-  r = __builtin_fmaf(r, t, 0.111703858f);
-  e = __builtin_amdgcn_exp2f(h * h * -0.72134752f);
-  return e * (t * r);
-}
-
-template <class T, int ACT>
-__device__ __forceinline__ float act_value(float h) {
-  if constexpr (ACT == PXG_SILU) {
-    if constexpr (fast_activation<T>) return h * __builtin_amdgcn_rcpf(1.0f + fast_exp(-h));
-    return h / (1.0f + expf(-h));
-  }
-  if constexpr (fast_activation<T>) {
-    float e;
-    const float q = gelu_tail(h, e);
-    return h * (h < 0.0f ? q : 1.0f - q);
-  }
-  return h * (0.5f * (1.0f + erff(h * 0.70710678f)));
-}
-template <class T, int ACT>
-__device__ __forceinline__ float act_slope(float h) {
-  if constexpr (ACT == PXG_SILU) {
-    float s;
-    if constexpr (fast_activation<T>) s = __builtin_amdgcn_rcpf(1.0f + fast_exp(-h));
-    else s = 1.0f / (1.0f + expf(-h));
-    return s * (1.0f + h * (1.0f - s));
-  }
-  if constexpr (fast_activation<T>) {
-    float e;
-    const float q = gelu_tail(h, e);
-    return __builtin_fmaf(h * 0.39894228f, e, h < 0.0f ? q : 1.0f - q);
-  }
-  const float p = 0.5f * (1.0f + erff(h * 0.70710678f));
-  return p + h * (0.39894228f * expf(-0.5f * h * h));
-}
-
 template <class T, bool VEC, int ACT>
 __global__ void __launch_bounds__(ROW_THREADS)
 activation_pack_rows(const T* __restrict__ h, uint64_t hs, uint32_t rows, uint32_t cols, uint32_t wide,
@@ -278,26 +169,9 @@ void by_rows(uint64_t rows, uint64_t wide, F launch) {
   });
 }
 
-// Calls f with a value of the element type and whether 16-byte accesses are
-// aligned in every row.
-template <class F>
-void by_type(int type, bool vec, F f) {
-  auto g = [&](auto t) {
-    if (vec) f(t, std::true_type{});
-    else f(t, std::false_type{});
-  };
-  if (type == PXG_F32) g(float{});
-  else if (type == PXG_F16) g((_Float16)0);
-  else g((__bf16)0.0f);
-}
-
 void check_packed(uint64_t rows, uint64_t cols, const void* codes, const void* scales) {
   check_size("cols", cols);
   check_packed_rows("codes", codes, "scales", scales, rows);
-}
-
-void check_activation(int kind) {
-  if (kind != PXG_SILU && kind != PXG_GELU) config_error("activation", (uint64_t)kind, "must be SiLU or GELU");
 }
 
 }  // namespace

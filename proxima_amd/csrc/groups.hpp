@@ -105,6 +105,35 @@ __device__ __forceinline__ bool find_row_tile(const int64_t* __restrict__ offset
   return false;
 }
 
+// The tiles (of all, in order) of group g: its first and how many. A
+// wavefront's lanes all call it and get the same.
+__device__ __forceinline__ void find_group_tiles(const int64_t* __restrict__ offsets, int groups, int rows, int size,
+                                                 int g, int& first_tile, int& tiles_of) {
+  if (!offsets) {
+    first_tile = 0;
+    tiles_of = row_tiles_of<ALL_TILES>(rows, size);
+    return;
+  }
+  const int lane = threadIdx.x & (WAVE - 1);
+  int begin = 0, before = 0;
+  for (int s0 = 0;; s0 += WAVE) {  // group g is segment g + 1
+    const int s = s0 + lane;
+    int end = s <= groups ? clamp_offset(offsets[s], rows) : rows;
+    end = wave_max_scan(end > begin ? end : begin, lane);
+    int first = __shfl_up(end, 1, WAVE);
+    if (lane == 0) first = begin;
+    const int tiles = row_tiles_of<ALL_TILES>(end - first, size);
+    const int last = before + wave_sum_scan(tiles, lane);
+    if (g + 1 < s0 + WAVE) {
+      tiles_of = __builtin_amdgcn_readlane(tiles, g + 1 - s0);
+      first_tile = __builtin_amdgcn_readlane(last, g + 1 - s0) - tiles_of;
+      return;
+    }
+    begin = __builtin_amdgcn_readlane(end, WAVE - 1);
+    before = __builtin_amdgcn_readlane(last, WAVE - 1);
+  }
+}
+
 // How many whole and partial tiles there are.
 __device__ __forceinline__ void count_row_tiles(const int64_t* __restrict__ offsets, int groups, int rows, int size,
                                                 int& whole, int& partial) {

@@ -1,0 +1,73 @@
+// Rows of f32, f16 or bf16 read and written 8 columns a thread.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <type_traits>
+
+#include "../../include/proxima_hip.h"
+
+namespace pxg {
+
+template <class T>
+__device__ __forceinline__ float to_float(T x) {
+  return (float)x;
+}
+
+// 8 columns of a row from column c: one or two 16-byte loads where VEC (the
+// row 16-byte aligned) and all eight exist, else one by one, zero past cols.
+template <class T, bool VEC>
+__device__ __forceinline__ void load8(const T* __restrict__ row, uint64_t c, uint64_t cols, float (&x)[8]) {
+  if (VEC && c + 8 <= cols) {
+    T v[8];
+    const uint4* p = reinterpret_cast<const uint4*>(row + c);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(v)[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = c + i < cols ? to_float(row[c + i]) : 0.0f;
+  }
+}
+
+// One rounding of the f32 value: kept apart from the product before it, which
+// the compiler may otherwise fuse into the conversion to f16 in some variants
+// of a kernel and not in others.
+template <class T>
+__device__ __forceinline__ T rounded(float x) {
+  if constexpr (std::is_same_v<T, _Float16>) asm("" : "+v"(x));
+  return (T)x;
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void store8(T* __restrict__ row, uint64_t c, uint64_t cols, const float (&x)[8]) {
+  if (VEC && c + 8 <= cols) {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = rounded<T>(x[i]);
+    uint4* p = reinterpret_cast<uint4*>(row + c);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) p[i] = reinterpret_cast<uint4*>(v)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) row[c + i] = rounded<T>(x[i]);
+  }
+}
+
+// Calls f with a value of the element type and whether 16-byte accesses are
+// aligned in every row.
+template <class F>
+inline void by_type(int type, bool vec, F f) {
+  auto g = [&](auto t) {
+    if (vec) f(t, std::true_type{});
+    else f(t, std::false_type{});
+  };
+  if (type == PXG_F32) g(float{});
+  else if (type == PXG_F16) g((_Float16)0);
+  else g((__bf16)0.0f);
+}
+
+}  // namespace pxg

@@ -23,7 +23,8 @@ from ._capi import lib as _lib
 
 __all__ = [
     "Block8", "block8_pack", "block8_unpack", "block8_matmul", "grouped_matmul", "grouped_matmul_grad_input",
-    "grouped_matmul_grad_weight", "activation_pack", "activation_grad",
+    "grouped_matmul_grad_weight", "grouped_linear", "block8_linear", "grouped_linear_grad", "activation_pack",
+    "activation_grad",
 ]
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
@@ -198,6 +199,19 @@ def block8_unpack(packed, dtype=None, out=None):
     return out
 
 
+def _packed_weights(w, offsets, k):
+    """(codes, scales, groups, n, offsets' pointer) of packed [groups * n, k] matrices"""
+    wcodes, wscales, wrows, wk = _packed(w, "w")
+    if wk != k:
+        _mismatch(wk, k, "w's columns")
+    ptr, groups = _groups(offsets)
+    n, left = divmod(wrows, groups)
+    if left:
+        raise DimensionMismatch(f"dimension mismatch: w's {wrows} rows are not a multiple of {groups} groups", groups,
+                                wrows)
+    return wcodes, wscales, groups, n, ptr
+
+
 def block8_matmul(x, w, offsets=None, out_dtype=None, out=None):
     """y[t] = x[t] w_g^T for t in group g: x a Block8 of [rows, k], w a Block8 of
     [groups * n, k] (the groups' matrices one after the other), y [rows, n] of
@@ -210,14 +224,7 @@ def block8_matmul(x, w, offsets=None, out_dtype=None, out=None):
     the result as a whole, where rounding costs 2e-4 (f16) or 1.7e-3 (bf16); a
     sum that cancels may be off by more of itself."""
     codes, scales, rows, k = _packed(x, "x")
-    wcodes, wscales, wrows, wk = _packed(w, "w")
-    if wk != k:
-        _mismatch(wk, k, "w's columns")
-    ptr, groups = _groups(offsets)
-    n, left = divmod(wrows, groups)
-    if left:
-        raise DimensionMismatch(f"dimension mismatch: w's {wrows} rows are not a multiple of {groups} groups", groups,
-                                wrows)
+    wcodes, wscales, groups, n, ptr = _packed_weights(w, offsets, k)
     dtype = out_dtype or (out.dtype if out is not None else _torch.bfloat16)
     kind = _type(dtype, "out_dtype")
     out, stride = _out(out, (rows, n), dtype, codes)
@@ -305,6 +312,109 @@ def grouped_matmul_grad_weight(grad, x, offsets, out_dtype=None, out=None):
              _stride(grad), x.data_ptr(), k, _stride(x), ptr, groups, out_kind, out.data_ptr(), stride, out.stride(0),
              at, size)
     return out
+
+
+def _bias(bias, offsets, groups, n, dtype):
+    """(tensor, pointer, pxg_type, elements from group to group) of a bias of `dtype` or f32: [groups, n], or [n]
+    without offsets."""
+    if bias is None:
+        return None, None, 0, 0
+    if offsets is None and bias.dim() == 1:
+        bias = bias.unsqueeze(0)
+    shape = _matrix(bias, "bias")
+    if shape != (groups, n):
+        _mismatch(tuple(shape), (groups, n), "bias' shape")
+    if bias.dtype is not dtype and bias.dtype is not _torch.float32:
+        raise ValueError(f"bias must be {dtype} or float32, got {bias.dtype}")
+    return bias, bias.data_ptr(), _KINDS[bias.dtype], _stride(bias)
+
+
+def _residual(residual, shape, dtype):
+    """(pointer, elements from row to row)"""
+    if residual is None:
+        return None, 0
+    if _matrix(residual, "residual") != shape:
+        _mismatch(tuple(residual.shape), tuple(shape), "residual's shape")
+    if residual.dtype is not dtype:
+        raise ValueError(f"residual must be {dtype}, got {residual.dtype}")
+    return residual.data_ptr(), _stride(residual)
+
+
+def _optional(activation):
+    return -1 if activation is None else _activation(activation)
+
+
+def grouped_linear(x, w, offsets=None, bias=None, activation=None, residual=None, out_dtype=None, out=None, keep=False):
+    """y[t] = f(h[t]) + residual[t], h[t] = x[t] w[g]^T + bias[g] for t in group g: x and w as grouped_matmul takes
+    them, bias [groups, n] (or [n] without offsets) in x's type or f32, f "silu", "gelu" or None, residual [rows, n]
+    in y's type. `out` may be the residual itself. With keep, (y, h), h in y's type for grouped_linear_grad. y is
+    rounded once, from the unrounded h. Rows of no group: y is the residual, or zeros, and h zeros."""
+    rows, xk = _matrix(x, "x")
+    kind = _type(x.dtype, "x", False)
+    w, ptr, groups, n, k = _weights(w, offsets, x)
+    if xk != k:
+        _mismatch(xk, k, "x's columns")
+    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    out_kind, which = _type(dtype, "out_dtype"), _optional(activation)
+    bias, bias_ptr, bias_kind, bias_stride = _bias(bias, offsets, groups, n, x.dtype)
+    r, r_stride = _residual(residual, (rows, n), dtype)
+    out, stride = _out(out, (rows, n), dtype, x)
+    h = x.new_empty((rows, n), dtype=dtype) if keep else None
+    _run(_lib.pxg_grouped_linear_device, (x, w, offsets, bias, residual, out), kind, x.data_ptr(), rows, k, _stride(x),
+         w.data_ptr(), groups, n, _stride(w), w.stride(0), ptr, bias_kind, bias_ptr, bias_stride, which, out_kind, r,
+         r_stride, h.data_ptr() if keep else None, n, out.data_ptr(), stride)
+    return (out, h) if keep else out
+
+
+def block8_linear(x, w, offsets=None, bias=None, activation=None, residual=None, out_dtype=None, out=None):
+    """y[t] = f(x[t] w_g^T + bias[g]) + residual[t] for t in group g: x and w Block8, multiplied as block8_matmul
+    does, bias bf16 or f32, the rest as grouped_linear."""
+    codes, scales, rows, k = _packed(x, "x")
+    wcodes, wscales, groups, n, ptr = _packed_weights(w, offsets, k)
+    dtype = out_dtype or (out.dtype if out is not None else _torch.bfloat16)
+    out_kind, which = _type(dtype, "out_dtype"), _optional(activation)
+    bias, bias_ptr, bias_kind, bias_stride = _bias(bias, offsets, groups, n, _torch.bfloat16)
+    r, r_stride = _residual(residual, (rows, n), dtype)
+    out, stride = _out(out, (rows, n), dtype, codes)
+    _run(_lib.pxg_block8_linear_device, (codes, scales, wcodes, wscales, offsets, bias, residual, out),
+         codes.data_ptr(), scales.data_ptr(), rows, k, wcodes.data_ptr(), wscales.data_ptr(), groups, n, ptr,
+         bias_kind, bias_ptr, bias_stride, which, out_kind, r, r_stride, out.data_ptr(), stride)
+    return out
+
+
+def grouped_linear_grad(grad, h=None, activation=None, offsets=None, bias_dtype=None, out=None):
+    """(dh, dbias): grouped_linear's backward pass up to the products. dh = grad * f'(h), h as grouped_linear kept it
+    and of grad's type, zeros for rows of no group; dbias[g] is the sum of group g's dh before its rounding,
+    [groups, n] (or [n] without offsets) of bias_dtype (f32 by default, or grad's type). Without an activation dh is
+    grad itself. `out` may be grad or h itself. dx and dw are grouped_matmul_grad_input's and
+    grouped_matmul_grad_weight's of dh, and the residual's gradient is grad."""
+    rows, n = _matrix(grad, "grad")
+    kind = _type(grad.dtype, "grad")
+    ptr, groups = _groups(offsets)
+    which = _optional(activation)
+    if which < 0:
+        if h is not None or out is not None:
+            raise ValueError("h and out are for an activation")
+        dh, h_ptr, h_stride, stride = grad, None, 0, 0
+    else:
+        if h is None:
+            raise ValueError("h must be given with an activation")
+        if _matrix(h, "h") != (rows, n):
+            _mismatch(tuple(h.shape), (rows, n), "h's shape")
+        if h.dtype is not grad.dtype:
+            raise ValueError(f"h must be {grad.dtype}, got {h.dtype}")
+        h_ptr, h_stride = h.data_ptr(), _stride(h)
+        dh, stride = _out(out, (rows, n), grad.dtype, grad)
+    bias_dtype = bias_dtype or _torch.float32
+    if bias_dtype is not grad.dtype and bias_dtype is not _torch.float32:
+        raise ValueError(f"bias_dtype must be {grad.dtype} or float32, got {bias_dtype}")
+    dbias = grad.new_empty((groups, n) if offsets is not None else (n,), dtype=bias_dtype)
+    size = _lib.pxg_grouped_linear_grad_workspace(rows, n, groups)
+    space = grad.new_empty(size, dtype=_torch.uint8) if size else None
+    _run(_lib.pxg_grouped_linear_grad_device, (grad, h, offsets, dh), which, kind, grad.data_ptr(), rows, n,
+         _stride(grad), h_ptr, h_stride, ptr, groups, dh.data_ptr(), stride, _KINDS[bias_dtype], dbias.data_ptr(), n,
+         space.data_ptr() if size else None, size)
+    return dh, dbias
 
 
 def _activation(name):

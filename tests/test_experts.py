@@ -113,3 +113,57 @@ def test_kernels_that_are_not_there_are_refused(lib):
         _refused(lib, lib.pxg_grouped_matmul_set_kernel(rows), b"rows")
     for rows in (16, 64, 128, 256, 0):
         assert lib.pxg_grouped_matmul_set_kernel(rows) == 0
+
+
+def test_layers_refuse(lib):
+    p, odd = C.c_void_p(4096), C.c_void_p(4097)
+
+    def f(kind=2, x=p, rows=4, k=8, xs=8, w=p, groups=1, n=8, ws=8, offsets=None, bias_type=0, bias=p, bs=8, act=1,
+          out=2, r=p, rs=8, h=p, hs=8, y=p, ys=8):
+        return lib.pxg_grouped_linear_device(kind, x, rows, k, xs, w, groups, n, ws, 64, offsets, bias_type, bias, bs, act,
+                                             out, r, rs, h, hs, y, ys, None)
+
+    for more, parameter in (
+            (dict(kind=0), b"type"), (dict(out=1), b"out_type"), (dict(k=0), b"k"), (dict(n=0), b"n"),
+            (dict(groups=0), b"groups"), (dict(groups=2), b"groups"), (dict(xs=7), b"stride"),
+            (dict(xs=1 << 23), b"stride"), (dict(w=None), b"w"), (dict(y=None), b"y"), (dict(x=odd), b"x"),
+            (dict(bias_type=1), b"bias_type"), (dict(bias=C.c_void_p(4098)), b"bias"),
+            (dict(groups=2, offsets=p, bs=7), b"stride"), (dict(act=2), b"activation"), (dict(act=-2), b"activation"),
+            (dict(rs=7), b"stride"), (dict(r=odd), b"residual"), (dict(hs=7), b"stride"), (dict(h=odd), b"h"),
+            (dict(ys=7), b"stride"), (dict(rows=1 << 31), b"rows")):
+        _refused(lib, f(**more), parameter)
+    assert f(rows=0, x=None, y=None, r=None, h=None) == 0
+
+    def b(codes=p, scales=p, rows=4, k=8, wc=p, ws=p, groups=1, n=8, offsets=None, bias_type=0, bias=p, bs=8, act=1,
+          out=2, r=p, rs=8, y=p, ys=8):
+        return lib.pxg_block8_linear_device(codes, scales, rows, k, wc, ws, groups, n, offsets, bias_type, bias, bs, act,
+                                            out, r, rs, y, ys, None)
+
+    for more, parameter in (
+            (dict(out=3), b"type"), (dict(scales=None), b"scales"), (dict(wc=C.c_void_p(4104)), b"w_codes"),
+            (dict(bias_type=1), b"bias_type"), (dict(act=5), b"activation"), (dict(rs=4), b"stride"),
+            (dict(groups=3), b"groups"), (dict(y=odd), b"y"), (dict(k=0), b"k")):
+        _refused(lib, b(**more), parameter)
+    assert b(rows=0, codes=None, scales=None, y=None, r=None) == 0
+
+
+def test_layers_backward_pass_refuses(lib):
+    p, odd = C.c_void_p(4096), C.c_void_p(4097)
+
+    def f(act=1, kind=2, grad=p, rows=4, n=8, gs=8, h=p, hs=8, offsets=None, groups=1, dh=p, ds=8, bias_type=0, db=p,
+          dbs=8, space=None, size=0):
+        return lib.pxg_grouped_linear_grad_device(act, kind, grad, rows, n, gs, h, hs, offsets, groups, dh, ds, bias_type,
+                                                  db, dbs, space, size, None)
+
+    for more, parameter in (
+            (dict(kind=3), b"type"), (dict(act=2), b"activation"), (dict(n=0), b"n"), (dict(groups=4), b"groups"),
+            (dict(offsets=C.c_void_p(4100)), b"offsets"), (dict(grad=None), b"grad"), (dict(gs=7), b"stride"),
+            (dict(h=None), b"h"), (dict(hs=7), b"stride"), (dict(dh=None), b"dh"), (dict(dh=odd), b"dh"),
+            (dict(bias_type=1), b"bias_type"), (dict(db=C.c_void_p(4098)), b"dbias"),
+            (dict(offsets=p, groups=2, dbs=7), b"stride"), (dict(space=C.c_void_p(4104)), b"workspace"),
+            (dict(rows=1 << 31), b"rows")):
+        _refused(lib, f(**more), parameter)
+    assert f(act=-1, h=None, dh=None, db=None) == 0  # nothing to do
+    size = lib.pxg_grouped_linear_grad_workspace
+    assert size(100_000, 1024, 8) > 0 and size(100_000, 1024, 8) % (4 * 1024) == 0
+    assert size(8, 1024, 8) == 0 and size(0, 8, 1) == 0 and size(8, 0, 1) == 0 and size(8, 8, 0) == 0

@@ -22,6 +22,15 @@ pub(crate) struct PxgSq8 {
     _p: [u8; 0],
 }
 
+/// `pxg_expert_matrix`.
+#[repr(C)]
+pub(crate) struct PxgExpertMatrix {
+    pub(crate) data: *const c_void,
+    pub(crate) stride: u64,
+    pub(crate) group_stride: u64,
+    pub(crate) scales: *const c_void,
+}
+
 /// `pxg_index_stats` (index.rs:68-130).
 #[repr(C)]
 #[derive(Default)]
@@ -247,6 +256,14 @@ extern "C" {
         n: u64, grad_stride: u64, d_h: *const c_void, h_stride: u64, d_offsets: *const i64, groups: u64,
         d_dh: *mut c_void, dh_stride: u64, bias_type: c_int, d_dbias: *mut c_void, dbias_stride: u64,
         d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_expert_layer_workspace(rows: u64, picks: u64, experts: u64, hidden: u64, n: u64,
+        out_type: c_int) -> u64;
+    pub(crate) fn pxg_expert_layer_device(kind: c_int, d_x: *const c_void, rows: u64, k: u64, x_stride: u64,
+        d_experts: *const i64, picks: u64, experts_stride: u64, d_gates: *const f32, gates_stride: u64, experts: u64,
+        hidden: u64, n: u64, w1: *const PxgExpertMatrix, up: *const PxgExpertMatrix, w2: *const PxgExpertMatrix,
+        packed: c_int, activation: c_int, bias_type: c_int, d_bias1: *const c_void, bias1_stride: u64,
+        d_bias2: *const c_void, bias2_stride: u64, out_type: c_int, d_residual: *const c_void, residual_stride: u64,
+        d_y: *mut c_void, y_stride: u64, d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_grouped_matmul_set_kernel(rows: c_int) -> c_int;
     pub(crate) fn pxg_grouped_matmul_last_kernel() -> u32;
     pub(crate) fn pxg_activation_pack_device(activation: c_int, kind: c_int, d_h: *const c_void, rows: u64,

@@ -530,6 +530,36 @@ int pxg_grouped_linear_grad_device(int activation, int type, const void* d_grad,
                                    uint64_t groups, void* d_dh, uint64_t dh_stride, int bias_type, void* d_dbias,
                                    uint64_t dbias_stride, void* d_workspace, uint64_t workspace_bytes, void* stream);
 
+/* A whole expert layer for a few tokens:
+ *   y_t = r_t + sum over j of gate_tj (W2_e (f(W1_e x_t + b1_e) * up_e x_t) + b2_e),   e = experts_tj
+ * with matrices of `type` (f16 or bf16) or packed rows (`packed`; x is bf16),
+ * out_type that type or f32. x is rows x k; d_experts and d_gates are rows of
+ * `picks` (at most 16); an id outside [0, experts) is no expert, one that a token
+ * has twice counts with both gates. w1 and up (NULL: without its factor) are
+ * hidden x k of each expert, w2 n x hidden. `activation` is a pxg_activation or
+ * -1 for f(h) = h. The biases (NULL: none) are rows of bias_type (`type` or f32),
+ * d_residual (NULL: none) is r in out_type and may be y itself. Sums, and what is
+ * between the two products, are held in f32 (for a 16-bit result to 2^-17).
+ * Rows go in blocks of 64, for each of which the matrices of the experts in use
+ * are read once; rows, experts <= 65536. The workspace, of the size that
+ * workspace() says and 16-byte aligned, is not kept after the work is done. */
+typedef struct pxg_expert_matrix {
+  const void* data;       /* the first expert's first row; packed: its codes */
+  uint64_t stride;        /* elements from row to row, and from expert to expert; */
+  uint64_t group_stride;  /* packed rows lie one after the other and these are not looked at */
+  const void* scales;     /* packed rows' scales, or NULL */
+} pxg_expert_matrix;
+uint64_t pxg_expert_layer_workspace(uint64_t rows, uint64_t picks, uint64_t experts, uint64_t hidden, uint64_t n,
+                                    int out_type);
+int pxg_expert_layer_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride,
+                            const int64_t* d_experts, uint64_t picks, uint64_t experts_stride, const float* d_gates,
+                            uint64_t gates_stride, uint64_t experts, uint64_t hidden, uint64_t n,
+                            const pxg_expert_matrix* w1, const pxg_expert_matrix* up, const pxg_expert_matrix* w2,
+                            int packed, int activation, int bias_type, const void* d_bias1, uint64_t bias1_stride,
+                            const void* d_bias2, uint64_t bias2_stride, int out_type, const void* d_residual,
+                            uint64_t residual_stride, void* d_y, uint64_t y_stride, void* d_workspace,
+                            uint64_t workspace_bytes, void* stream);
+
 /* Which kernel the products of this thread take (for tests and tuning): 0 =
  * the one estimated fastest, 16 = that for few rows, 64, 128 or 256 = tiles of
  * as many rows and columns; where it cannot take a product's operands, the

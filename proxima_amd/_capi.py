@@ -55,6 +55,10 @@ class IvfPqConfigC(C.Structure):
     ]
 
 
+class ExpertMatrixC(C.Structure):
+    _fields_ = [("data", _vp), ("stride", _u64), ("group_stride", _u64), ("scales", _vp)]
+
+
 class TrainingReportC(C.Structure):
     _fields_ = [
         ("sampled", _u64),
@@ -182,6 +186,10 @@ SIGNATURES = {
     "pxg_grouped_linear_grad_workspace": (_u64, [_u64, _u64, _u64]),
     "pxg_grouped_linear_grad_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _u64, _vp, _u64,
                                               _i32, _vp, _u64, _vp, _u64, _vp]),
+    "pxg_expert_layer_workspace": (_u64, [_u64, _u64, _u64, _u64, _u64, _i32]),
+    "pxg_expert_layer_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64,
+                                       _P(ExpertMatrixC), _P(ExpertMatrixC), _P(ExpertMatrixC), _i32, _i32, _i32, _vp,
+                                       _u64, _vp, _u64, _i32, _vp, _u64, _vp, _u64, _vp, _u64, _vp]),
     "pxg_grouped_matmul_set_kernel": (_i32, [_i32]),
     "pxg_grouped_matmul_last_kernel": (_u32, []),
     "pxg_activation_pack_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp]),

@@ -71,8 +71,25 @@ __device__ __forceinline__ float act_slope(float h) {
   return p + h * (0.39894228f * expf(-0.5f * h * h));
 }
 
+// f(v) in place, evaluated as precisely as a result of type O shows.
+template <class O, int N>
+__device__ __forceinline__ void activate(float (&v)[N], int activation) {
+  if (activation == PXG_GELU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = act_value<O, PXG_GELU>(v[e]);
+  } else if (activation == PXG_SILU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = act_value<O, PXG_SILU>(v[e]);
+  }
+}
+
+constexpr int NO_ACTIVATION = -1;
+
 inline void check_activation(int kind) {
   if (kind != PXG_SILU && kind != PXG_GELU) config_error("activation", (uint64_t)kind, "must be SiLU or GELU");
+}
+inline void check_optional_activation(int kind) {
+  if (kind != NO_ACTIVATION) check_activation(kind);
 }
 
 }  // namespace pxg

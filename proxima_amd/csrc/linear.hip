@@ -22,7 +22,6 @@ namespace {
 // workspace; grad_bias_join adds a group's tiles in order. Without a workspace
 // a workgroup takes a whole group by its columns (tile 0: none).
 constexpr int GRAD_THREADS = 256, GRAD_BATCH = 4;  // rows that a thread has in flight
-constexpr int NO_ACTIVATION = -1;
 
 struct LinearGrad {
   const void *grad, *h;
@@ -168,9 +167,6 @@ void launch_grad(int activation, const LinearGrad& p, const GradPlan& g, hipStre
   }
 }
 
-void check_optional_activation(int activation) {
-  if (activation != NO_ACTIVATION) check_activation(activation);
-}
 // `name` must be a string literal.
 void check_bias(const char* name, int type, int bias_type, const void* bias, uint64_t groups, uint64_t n,
                 uint64_t stride) {

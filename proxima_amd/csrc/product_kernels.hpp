@@ -31,6 +31,7 @@
 #include "common.hpp"
 #include "device.hpp"
 #include "groups.hpp"
+#include "matrix_cores.hpp"
 #include "products.hpp"
 #include "rows.hpp"
 
@@ -41,11 +42,6 @@ inline thread_local int g_kernel = 0;
 inline thread_local uint32_t g_last_kernel = 0;
 
 namespace {
-
-typedef int i8v __attribute__((ext_vector_type(8)));
-typedef float f4v __attribute__((ext_vector_type(4)));
-typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
-typedef _Float16 hf8v __attribute__((ext_vector_type(8)));
 
 enum Form { FORWARD, GRAD_INPUT, GRAD_WEIGHT };
 
@@ -77,20 +73,12 @@ struct LinearProduct : Product {
   const void* bias = nullptr;  // bias_stride elements from group to group, f32 or the operands' type
   uint64_t bias_stride = 0;
   bool bias_f32 = false;
-  int activation = -1;             // a pxg_activation, or none
+  int activation = NO_ACTIVATION;  // or a pxg_activation
   const void* residual = nullptr;  // of the result's type, rows rs apart; may be the result itself
   uint64_t rs = 0;
   void* kept = nullptr;  // h in the result's type, rows hs apart
   uint64_t hs = 0;
 };
-
-template <class T>
-__device__ __forceinline__ f4v mfma16(uint4 a, uint4 b, f4v c) {
-  if constexpr (std::is_same_v<T, __bf16>)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8v, a), __builtin_bit_cast(bf8v, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8v, a), __builtin_bit_cast(hf8v, b), c, 0, 0, 0);
-}
 
 // ---------------------------------------------------------------------------
 // The tiled product: operands go to LDS by direct copies, 128 bytes of each
@@ -124,30 +112,8 @@ template <class T>
 using linear_bias = std::conditional_t<std::is_same_v<T, Fp8>, __bf16, T>;
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// f(v) in place, evaluated as precisely as a result of type O shows.
-template <class O, int N>
-__device__ __forceinline__ void activate(float (&v)[N], int activation) {
-  if (activation == PXG_GELU) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = act_value<O, PXG_GELU>(v[e]);
-  } else if (activation == PXG_SILU) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = act_value<O, PXG_SILU>(v[e]);
-  }
-}
-
 // A workgroup's place among all of a product's launches.
 __device__ __forceinline__ unsigned workgroup(const Product& p) { return p.first + blockIdx.x; }
-
-// A raw buffer resource over [p, p + bytes), from wave-uniform scalars;
-// accesses at offsets outside it read zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* p, uint64_t bytes) {
-  const uint64_t a = (uint64_t)(uintptr_t)p;
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a);
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32));
-  const int n = __builtin_amdgcn_readfirstlane((int)(uint32_t)(bytes < 0x7FFFFFFF ? bytes : 0x7FFFFFFF));
-  return __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)(((uint64_t)hi << 32) | lo), 0, n, 0x00020000);
-}
 
 // Copies of 16 (and 4) bytes a lane straight into LDS: lane i's land at
 // lds + 16 i (4 i), zeros for offsets outside the resource. Inline asm, so
@@ -176,21 +142,8 @@ __device__ __forceinline__ void wait_copies_but() {
 }
 __device__ __forceinline__ void wait_copies() { wait_copies_but<0>(); }
 
-constexpr uint32_t NOWHERE = 0xFFFFFF00u;  // an offset outside every resource
-
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
-}
-
-// 8 codes times their scale, in bf16.
-__device__ __forceinline__ uint4 decode_bf16(uint32_t x, uint32_t y, float s) {
-  typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
-  const bf2v a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, s, false);
-  const bf2v b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, s, true);
-  const bf2v c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, s, false);
-  const bf2v d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, s, true);
-  return make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
-                    __builtin_bit_cast(uint32_t, d));
 }
 
 // A barrier after the wavefront's LDS accesses; copies stay in flight.

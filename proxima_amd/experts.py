@@ -19,12 +19,12 @@ it is off.
 import sys
 
 from . import DimensionMismatch, _check
-from ._capi import lib as _lib
+from ._capi import ExpertMatrixC as _ExpertMatrix, lib as _lib
 
 __all__ = [
     "Block8", "block8_pack", "block8_unpack", "block8_matmul", "grouped_matmul", "grouped_matmul_grad_input",
-    "grouped_matmul_grad_weight", "grouped_linear", "block8_linear", "grouped_linear_grad", "activation_pack",
-    "activation_grad",
+    "grouped_matmul_grad_weight", "grouped_linear", "block8_linear", "grouped_linear_grad", "expert_layer",
+    "activation_pack", "activation_grad",
 ]
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
@@ -415,6 +415,90 @@ def grouped_linear_grad(grad, h=None, activation=None, offsets=None, bias_dtype=
          _stride(grad), h_ptr, h_stride, ptr, groups, dh.data_ptr(), stride, _KINDS[bias_dtype], dbias.data_ptr(), n,
          space.data_ptr() if size else None, size)
     return dh, dbias
+
+
+def _expert_matrix(w, name, experts, height, width, dtype, device_tensors):
+    """The C struct of [experts, height, width] matrices, or of a Block8 of [experts * height, width]."""
+    if dtype is None:
+        codes, scales, rows, cols = _packed(w, name)
+        if (rows, cols) != (experts * height, width):
+            _mismatch((rows, cols), (experts * height, width), f"{name}'s shape")
+        device_tensors += (codes, scales)
+        return _ExpertMatrix(codes.data_ptr(), 0, 0, scales.data_ptr())
+    if _matrix(w, name, 3) != (experts, height, width):
+        _mismatch(tuple(w.shape), (experts, height, width), f"{name}'s shape")
+    if w.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, got {w.dtype}")
+    device_tensors.append(w)
+    return _ExpertMatrix(w.data_ptr(), _stride(w), w.stride(0), None)
+
+
+def _routes(t, name, dtype, shape=None):
+    """Checks a router's [rows, picks] tensor; its shape."""
+    got = _matrix(t, name)
+    if t.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and got != shape:
+        _mismatch(tuple(got), tuple(shape), f"{name}'s shape")
+    return got
+
+
+def expert_layer(x, experts, w1, w2, gates, activation=None, up=None, bias1=None, bias2=None, residual=None,
+                 out_dtype=None, out=None):
+    """A whole expert layer for a few tokens, in the rows' own order:
+    y[t] = residual[t] + sum over j of gates[t, j] * (w2[e] (f(w1[e] x[t] + bias1[e]) * up[e] x[t]) + bias2[e]),
+    e = experts[t, j].
+
+    x [rows, k] f16 or bf16; experts [rows, picks] int64 and gates [rows, picks] f32, picks at most 16 (an id that is
+    no expert's is left out, one that a token has twice counts with both gates); w1 and up (optional) [experts, hidden,
+    k] and w2 [experts, n, hidden] of x's type, or each a Block8 of the experts' rows one after the other (x is then
+    bf16); biases [experts, .] of x's type or f32; residual and y [rows,
+    n] of x's type or f32. `out` may be the residual itself. Nothing between the two products is rounded to x's type.
+    The matrices of the experts in use are read once for each 64 rows: for batches use grouped_linear."""
+    rows, k = _matrix(x, "x")
+    kind = _type(x.dtype, "x", False)
+    _, picks = shape = _routes(experts, "experts", _torch.int64)
+    if shape[0] != rows:
+        _mismatch(shape[0], rows, "experts' rows")
+    _routes(gates, "gates", _torch.float32, shape)
+    tensors = [x, experts, gates]
+    packed = type(w1) is Block8
+    if packed:
+        if x.dtype is not _torch.bfloat16:
+            raise ValueError(f"x must be bfloat16 with packed matrices, got {x.dtype}")
+        _, _, rows2, hidden = _packed(w2, "w2")
+        number, left = divmod(w1.rows, hidden)
+        if left or not number:
+            raise DimensionMismatch(f"dimension mismatch: w1's {w1.rows} rows are not a multiple of w2's {hidden} columns",
+                                    hidden, w1.rows)
+        n, left = divmod(rows2, number)
+        if left or not n:
+            raise DimensionMismatch(f"dimension mismatch: w2's {rows2} rows are not a multiple of {number} experts",
+                                    number, rows2)
+    else:
+        number, hidden, _ = _matrix(w1, "w1", 3)
+        n = _matrix(w2, "w2", 3)[1]
+    of = None if packed else x.dtype
+    m1 = _expert_matrix(w1, "w1", number, hidden, k, of, tensors)
+    m2 = _expert_matrix(w2, "w2", number, n, hidden, of, tensors)
+    m3 = _expert_matrix(up, "up", number, hidden, k, of, tensors) if up is not None else None
+    which = _optional(activation)
+    if bias1 is not None and bias2 is not None and bias1.dtype is not bias2.dtype:
+        raise ValueError(f"biases must be of one type, got {bias1.dtype} and {bias2.dtype}")
+    bias1, b1, kind1, stride1 = _bias(bias1, experts, number, hidden, x.dtype)
+    bias2, b2, kind2, stride2 = _bias(bias2, experts, number, n, x.dtype)
+    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    out_kind = _type(dtype, "out_dtype")
+    r, r_stride = _residual(residual, (rows, n), dtype)
+    out, stride = _out(out, (rows, n), dtype, x)
+    size = _lib.pxg_expert_layer_workspace(rows, picks, number, hidden, n, out_kind)
+    space = x.new_empty(size, dtype=_torch.uint8) if size else None
+    tensors += (bias1, bias2, residual, out)
+    _run(_lib.pxg_expert_layer_device, tensors, kind, x.data_ptr(), rows, k, _stride(x), experts.data_ptr(), picks,
+         _stride(experts), gates.data_ptr(), _stride(gates), number, hidden, n, m1, m3, m2, packed, which,
+         kind1 if b1 else kind2, b1, stride1, b2, stride2, out_kind, r, r_stride, out.data_ptr(), stride,
+         space.data_ptr() if size else None, size)
+    return out
 
 
 def _activation(name):

@@ -264,6 +264,14 @@ extern "C" {
         packed: c_int, activation: c_int, bias_type: c_int, d_bias1: *const c_void, bias1_stride: u64,
         d_bias2: *const c_void, bias2_stride: u64, out_type: c_int, d_residual: *const c_void, residual_stride: u64,
         d_y: *mut c_void, y_stride: u64, d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_distill_workspace(kind: c_int, rows: u64, cols: u64, top: u64) -> u64;
+    pub(crate) fn pxg_distill_loss_device(kind: c_int, d_logits: *const c_void, rows: u64, cols: u64, logits_stride: u64,
+        d_ids: *const i64, ids_stride: u64, d_scores: *const f32, scores_stride: u64, d_counts: *const i32, top: u64,
+        temperature: f64, d_loss: *mut f32, d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_distill_loss_grad_device(kind: c_int, d_weight: *const f32, d_logits: *const c_void, rows: u64,
+        cols: u64, logits_stride: u64, d_ids: *const i64, ids_stride: u64, d_scores: *const f32, scores_stride: u64,
+        d_counts: *const i32, top: u64, temperature: f64, d_loss: *mut f32, d_dx: *mut c_void, dx_stride: u64,
+        d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_grouped_matmul_set_kernel(rows: c_int) -> c_int;
     pub(crate) fn pxg_grouped_matmul_last_kernel() -> u32;
     pub(crate) fn pxg_activation_pack_device(activation: c_int, kind: c_int, d_h: *const c_void, rows: u64,

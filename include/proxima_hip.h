@@ -560,6 +560,30 @@ int pxg_expert_layer_device(int type, const void* d_x, uint64_t rows, uint64_t k
                             uint64_t residual_stride, void* d_y, uint64_t y_stride, void* d_workspace,
                             uint64_t workspace_bytes, void* stream);
 
+/* The loss of a model trained to rank as a teacher does: p is the softmax of the
+ * teacher's scores over T, q that of the model's logits over T, and
+ *   loss = sum over entries of p_i (log p_i - log q_id(i))
+ *   dx_c = weight / T (q_c - sum of p_i with id(i) = c)
+ * for each of `rows` rows of `cols` logits (f32, f16 or bf16; dx in the same
+ * type, where it may overwrite the logits). The teacher's entries are as a search
+ * returns them: rows of `top` (at most 4096) ids and scores, of which the first
+ * count (clamped to [0, top]) are looked at; those with an id outside [0, cols) are
+ * left out. A row without entries, or whose scores are all -inf, has loss 0 and no
+ * gradient; entries of p = 0 add nothing; a logit of -inf has q = 0. `weight` is
+ * the loss' own gradient, one f32 a row. T lies between 1e-6 and 1e6. Sums are
+ * held in f32. The workspace is of the size that workspace() says (0: none),
+ * 16-byte aligned and not kept after the work is done. */
+uint64_t pxg_distill_workspace(int type, uint64_t rows, uint64_t cols, uint64_t top);
+int pxg_distill_loss_device(int type, const void* d_logits, uint64_t rows, uint64_t cols, uint64_t logits_stride,
+                            const int64_t* d_ids, uint64_t ids_stride, const float* d_scores, uint64_t scores_stride,
+                            const int32_t* d_counts, uint64_t top, double temperature, float* d_loss,
+                            void* d_workspace, uint64_t workspace_bytes, void* stream);
+int pxg_distill_loss_grad_device(int type, const float* d_weight, const void* d_logits, uint64_t rows, uint64_t cols,
+                                 uint64_t logits_stride, const int64_t* d_ids, uint64_t ids_stride,
+                                 const float* d_scores, uint64_t scores_stride, const int32_t* d_counts, uint64_t top,
+                                 double temperature, float* d_loss, void* d_dx, uint64_t dx_stride, void* d_workspace,
+                                 uint64_t workspace_bytes, void* stream);
+
 /* Which kernel the products of this thread take (for tests and tuning): 0 =
  * the one estimated fastest, 16 = that for few rows, 64, 128 or 256 = tiles of
  * as many rows and columns; where it cannot take a product's operands, the

@@ -190,6 +190,11 @@ SIGNATURES = {
     "pxg_expert_layer_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64,
                                        _P(ExpertMatrixC), _P(ExpertMatrixC), _P(ExpertMatrixC), _i32, _i32, _i32, _vp,
                                        _u64, _vp, _u64, _i32, _vp, _u64, _vp, _u64, _vp, _u64, _vp]),
+    "pxg_distill_workspace": (_u64, [_i32, _u64, _u64, _u64]),
+    "pxg_distill_loss_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _u64, _vp, _u64, C.c_double, _vp, _vp,
+                                       _u64, _vp]),
+    "pxg_distill_loss_grad_device": (_i32, [_i32, _vp, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _u64, _vp, _u64, C.c_double,
+                                            _vp, _vp, _u64, _vp, _u64, _vp]),
     "pxg_grouped_matmul_set_kernel": (_i32, [_i32]),
     "pxg_grouped_matmul_last_kernel": (_u32, []),
     "pxg_activation_pack_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp]),

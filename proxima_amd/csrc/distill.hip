@@ -1,0 +1,565 @@
+// The loss of a model that is trained to rank as a teacher does, whose best
+// results (ids, scores and how many, as a search returns them) are the target:
+//
+//   p = softmax(s / T) over the entries with an id in [0, cols),   q = softmax(x / T) over the row
+//   loss = sum over entries of p_i (log p_i - log q_id(i))
+//   dx_c = g / T (q_c - sum of p_i with id(i) = c)
+//
+// A row without entries (or whose scores are all -inf) has loss 0 and no
+// gradient; an entry of p = 0 adds nothing; a logit of -inf has q = 0, so that p
+// > 0 there costs infinity.
+//
+// Memory bounds it: x is read and dx written once, q never stored. Rows of up
+// to 128 KB stay in a workgroup's registers between the softmax' sums and dx
+// (two workgroups of 1024 threads fit a CU, so that one loads while the other
+// stores). Longer rows, and rows too few to fill the chip, are cut into parts:
+// one kernel finds each part's maximum and sum, a second joins them, and for dx
+// reads x again.
+#include <algorithm>
+#include <cmath>
+
+#include "common.hpp"
+#include "device.hpp"
+#include "products.hpp"
+#include "rows.hpp"
+
+namespace pxg {
+namespace {
+
+constexpr uint64_t TOP_MAX = 4096;
+constexpr int PART_THREADS = 256;
+
+struct Distill {
+  const void* x;
+  void* dx;
+  const int64_t* ids;
+  const float* scores;
+  const int32_t* counts;
+  const float* weight;
+  float* loss;
+  uint64_t xs, ds, is, ss;  // row strides
+  float2* sums;             // each part's maximum and sum of a row
+  float* picked;            // the entries' logits, rows of top
+  uint64_t rows, first;     // first: rows of the launches before this one
+  int cols, top, parts;
+  float c, c_low;  // log2 e / T, and what its rounding left
+  float t, t_low;  // 1 / T
+};
+
+template <class T>
+constexpr int EACH = 16 / sizeof(T);  // elements of a vector
+
+template <class T>
+__device__ __forceinline__ uint32_t negative_infinities() {
+  if constexpr (sizeof(T) == 4) return 0xFF800000u;
+  return std::is_same_v<T, _Float16> ? 0xFC00FC00u : 0xFF80FF80u;
+}
+
+// d / T * log2 e for one element of type T: exp2 of it to T's last place. In
+// f32 the product's rounding would show (|d| / T * 2^-24), so it is added.
+template <class T>
+__device__ __forceinline__ float exp_scaled(const Distill& p, float d) {
+  const float y = d * p.c;
+  const float e = __builtin_amdgcn_exp2f(y);
+  if constexpr (sizeof(T) == 4) {
+    const float r = __builtin_fmaf(d, p.c, -y) + d * p.c_low;
+    return y > -150.0f ? __builtin_fmaf(e * r, 0.69314718f, e) : e;  // -inf: 0 (and NaN stays)
+  }
+  return e;
+}
+// d / T
+__device__ __forceinline__ float scaled(const Distill& p, float d) {
+  const float y = d * p.t;
+  return fabsf(y) < __builtin_inff() ? y + (__builtin_fmaf(d, p.t, -y) + d * p.t_low) : y;
+}
+
+// The maximum m of some elements and the sum s of exp((x - m) / T); none: -inf, 0.
+struct Softmax {
+  float m, s;
+};
+__device__ __forceinline__ float or_zero(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+__device__ __forceinline__ Softmax joined(const Distill& p, Softmax a, Softmax b) {
+  const float m = fmaxf(a.m, b.m), z = or_zero(m);
+  return {m, a.s * exp_scaled<float>(p, a.m - z) + b.s * exp_scaled<float>(p, b.m - z)};
+}
+__device__ __forceinline__ Softmax wave_joined(const Distill& p, Softmax a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float s = a.s * exp_scaled<float>(p, a.m - or_zero(m));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+  return {m, s};
+}
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// The teacher's entries of a row, in LDS: top ids (-1: not valid), p, and logits.
+struct Teacher {
+  int* ids;
+  float *p, *logits;
+};
+__device__ __forceinline__ Teacher teacher_at(char* lds, int top) {
+  return {(int*)lds, (float*)lds + top, (float*)lds + 2 * top};
+}
+// By one wavefront: p and the sum over entries of p log p; `none` if nothing is left of it.
+template <class T>
+__device__ __forceinline__ float read_teacher(const Distill& p, uint64_t row, const T* x, const float* picked,
+                                              const Teacher& t, bool& none) {
+  const int lane = threadIdx.x & 63;
+  const int count = min(max(p.counts[row], 0), p.top);
+  float best = -__builtin_inff();
+  for (int i = lane; i < p.top; i += 64) {
+    const int64_t id = i < count ? p.ids[row * p.is + i] : -1;
+    const bool valid = (uint64_t)id < (uint64_t)p.cols;
+    const float s = valid ? p.scores[row * p.ss + i] : -__builtin_inff();
+    t.ids[i] = valid ? (int)id : -1;
+    t.logits[i] = !valid ? 0.0f : picked ? picked[i] : (float)x[id];
+    t.p[i] = s;
+    best = fmaxf(best, s);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+  float mass = 0.0f;
+  for (int i = lane; i < p.top; i += 64)
+    if (t.ids[i] >= 0) mass += exp_scaled<float>(p, t.p[i] - or_zero(best));
+  mass = wave_sum(mass);
+  none = mass == 0.0f;
+  const float inverse = 1.0f / mass, log_mass = logf(mass);
+  float sum = 0.0f;
+  for (int i = lane; i < p.top; i += 64) {
+    const float d = t.p[i] - or_zero(best);
+    const float v = t.ids[i] < 0 || none ? 0.0f : exp_scaled<float>(p, d) * inverse;
+    t.p[i] = v;
+    if (v != 0.0f) sum += v * (scaled(p, d) - log_mass);
+  }
+  return wave_sum(sum);
+}
+// By the same wavefront: - sum over entries of p log q.
+__device__ __forceinline__ float cross_entropy(const Distill& p, const Teacher& t, Softmax row) {
+  const float log_sum = row.s == 0.0f ? 0.0f : logf(row.s);  // 0: all logits are -inf, as d is
+  float sum = 0.0f;
+  for (int i = threadIdx.x & 63; i < p.top; i += 64)
+    if (t.p[i] != 0.0f) sum -= t.p[i] * (scaled(p, t.logits[i] - or_zero(row.m)) - log_sum);
+  return wave_sum(sum);
+}
+// The gradient at the entries' ids in [lo, hi), over what is stored for the
+// row: eight lanes to an entry add up p of its id.
+template <class T, int THREADS>
+__device__ __forceinline__ void store_entries(const Distill& p, const Teacher& t, Softmax row, float k, T* dx, int lo,
+                                              int hi) {
+  const float inverse = row.s == 0.0f ? 0.0f : 1.0f / row.s;
+  const int sub = threadIdx.x & 7;
+  for (int i0 = 0; i0 < p.top; i0 += THREADS / 8) {
+    const int i = i0 + threadIdx.x / 8, id = i < p.top ? t.ids[i] : -1;
+    float sum = 0.0f;
+    if (id >= lo && id < hi)
+      for (int j = sub; j < p.top; j += 8) sum += t.ids[j] == id ? t.p[j] : 0.0f;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (sub == 0 && id >= lo && id < hi) {
+      const float q = exp_scaled<T>(p, t.logits[i] - or_zero(row.m)) * inverse;
+      dx[id] = rounded<T>(k * (q - sum));
+    }
+  }
+}
+
+// Vector v of a row is its elements from v EACH - phase on, 16-byte aligned;
+// the first and the last may lie across its ends.
+template <class T>
+__device__ __forceinline__ int phase_of(const void* row) {
+  return (int)((uintptr_t)row % 16 / sizeof(T));
+}
+template <class T>
+__device__ __forceinline__ bool is_whole(int v, int phase, int cols) {
+  const int64_t at = (int64_t)v * EACH<T> - phase;
+  return at >= 0 && at + EACH<T> <= cols;
+}
+template <class T>
+__device__ __forceinline__ uint4 load_ends(const T* row, int v, int phase, int cols) {
+  T x[EACH<T>];
+  uint4 fill = make_uint4(negative_infinities<T>(), negative_infinities<T>(), negative_infinities<T>(),
+                          negative_infinities<T>());
+  __builtin_memcpy(x, &fill, 16);
+  const int64_t at = (int64_t)v * EACH<T> - phase;
+#pragma unroll
+  for (int e = 0; e < EACH<T>; ++e)
+    if (at + e >= 0 && at + e < cols) x[e] = row[at + e];
+  __builtin_memcpy(&fill, x, 16);
+  return fill;
+}
+template <class T>
+__device__ __forceinline__ void unpack(uint4 raw, float (&x)[EACH<T>]) {
+  T v[EACH<T>];
+  __builtin_memcpy(v, &raw, 16);
+#pragma unroll
+  for (int e = 0; e < EACH<T>; ++e) x[e] = (float)v[e];
+}
+template <class T>
+__device__ __forceinline__ void store_vector(T* row, int v, int phase, int cols, bool aligned, const float (&x)[EACH<T>]) {
+  T y[EACH<T>];
+#pragma unroll
+  for (int e = 0; e < EACH<T>; ++e) y[e] = rounded<T>(x[e]);
+  const int64_t at = (int64_t)v * EACH<T> - phase;
+  if (aligned && at >= 0 && at + EACH<T> <= cols) {
+    *reinterpret_cast<uint4*>(row + at) = *reinterpret_cast<const uint4*>(y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < EACH<T>; ++e)
+      if (at + e >= 0 && at + e < cols) row[at + e] = y[e];
+  }
+}
+// dx = f exp((x - m) / T) of a vector.
+template <class T>
+__device__ __forceinline__ void store_gradient(const Distill& p, uint4 raw, float m, float f, T* dx, int v, int phase,
+                                               bool aligned) {
+  float x[EACH<T>];
+  unpack<T>(raw, x);
+#pragma unroll
+  for (int e = 0; e < EACH<T>; ++e) x[e] = f == 0.0f ? 0.0f : exp_scaled<T>(p, x[e] - m) * f;
+  store_vector<T>(dx, v, phase, p.cols, aligned, x);
+}
+// Vectors that are unpacked in another pass are unpacked anew: their floats would not fit the registers.
+template <int N>
+__device__ __forceinline__ void keep_packed(uint4 (&raw)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
+}
+template <class T, int N>
+__device__ __forceinline__ Softmax softmax_of(const Distill& p, uint4 (&raw)[N], Softmax before = {-__builtin_inff(), 0.0f}) {
+  float m = before.m;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float x[EACH<T>];
+    unpack<T>(raw[i], x);
+#pragma unroll
+    for (int e = 0; e < EACH<T>; ++e) m = fmaxf(m, x[e]);
+  }
+  if constexpr (N > 4) keep_packed(raw);
+  const float z = or_zero(m);
+  float s = before.s * exp_scaled<float>(p, before.m - z);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float x[EACH<T>];
+    unpack<T>(raw[i], x);
+#pragma unroll
+    for (int e = 0; e < EACH<T>; ++e) s += exp_scaled<T>(p, x[e] - z);
+  }
+  return {m, s};
+}
+
+// A workgroup's row in registers: N vectors of a thread.
+template <class T, int THREADS, int N, bool GRAD>
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 4) distill_row(Distill p) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ Softmax waves[THREADS / 64];
+  __shared__ int no_teacher;
+  const uint64_t row = p.first + blockIdx.x;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T* x = (const T*)p.x + row * p.xs;
+  const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
+  uint4 raw[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int v = i * THREADS + threadIdx.x;
+    if (is_whole<T>(v, phase, p.cols)) raw[i] = *reinterpret_cast<const uint4*>(x + ((int64_t)v * EACH<T> - phase));
+  }
+  const Teacher t = teacher_at(lds, p.top);
+  float entropy = 0.0f;
+  bool none = false;
+  if (wave == 0) {
+    entropy = read_teacher<T>(p, row, x, nullptr, t, none);
+    if (lane == 0) no_teacher = none;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int v = i * THREADS + threadIdx.x;
+    if (!is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
+  }
+  Softmax mine = wave_joined(p, softmax_of<T>(p, raw));
+  if (lane == 0) waves[wave] = mine;
+  __syncthreads();
+  const Softmax all = wave_joined(p, lane < THREADS / 64 ? waves[lane] : Softmax{-__builtin_inff(), 0.0f});
+  none = no_teacher;
+  if (wave == 0) {
+    const float other = cross_entropy(p, t, all);
+    if (lane == 0) p.loss[row] = none ? 0.0f : entropy + other;
+  }
+  if constexpr (GRAD) {
+    T* dx = (T*)p.dx + row * p.ds;
+    const bool aligned = phase_of<T>(dx) == phase;
+    const float k = p.weight[row] * p.t, f = none || all.s == 0.0f ? 0.0f : k / all.s, m = or_zero(all.m);
+    keep_packed(raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int v = i * THREADS + threadIdx.x;
+      if (v < vectors) store_gradient<T>(p, raw[i], m, f, dx, v, phase, aligned);
+    }
+    if (none) return;
+    __syncthreads();  // what follows is stored over it
+    store_entries<T, THREADS>(p, t, all, k, dx, 0, p.cols);
+  }
+}
+
+// A part of a row: its maximum and sum. The first part gathers the entries' logits.
+template <class T>
+__global__ void __launch_bounds__(PART_THREADS) distill_part(Distill p) {
+  __shared__ Softmax waves[PART_THREADS / 64];
+  const uint64_t row = p.first + blockIdx.x / p.parts;
+  const int part = blockIdx.x % p.parts, lane = threadIdx.x & 63;
+  const T* x = (const T*)p.x + row * p.xs;
+  const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
+  const int lo = (int)((int64_t)vectors * part / p.parts), hi = (int)((int64_t)vectors * (part + 1) / p.parts);
+  if (part == 0) {
+    const int count = min(max(p.counts[row], 0), p.top);
+    for (int i = threadIdx.x; i < count; i += PART_THREADS) {
+      const int64_t id = p.ids[row * p.is + i];
+      if ((uint64_t)id < (uint64_t)p.cols) p.picked[row * p.top + i] = (float)x[id];
+    }
+  }
+  constexpr int AHEAD = 4;
+  const uint32_t fill = negative_infinities<T>();
+  Softmax mine{-__builtin_inff(), 0.0f};
+  for (int v0 = lo + (int)threadIdx.x; v0 < hi; v0 += PART_THREADS * AHEAD) {
+    uint4 raw[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int v = v0 + i * PART_THREADS;
+      raw[i] = make_uint4(fill, fill, fill, fill);
+      if (v < hi && is_whole<T>(v, phase, p.cols)) raw[i] = *reinterpret_cast<const uint4*>(x + ((int64_t)v * EACH<T> - phase));
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int v = v0 + i * PART_THREADS;
+      if (v < hi && !is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
+    }
+    mine = softmax_of<T>(p, raw, mine);
+  }
+  mine = wave_joined(p, mine);
+  if (lane == 0) waves[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    Softmax s = waves[0];
+#pragma unroll
+    for (int i = 1; i < PART_THREADS / 64; ++i) s = joined(p, s, waves[i]);
+    p.sums[row * p.parts + part] = make_float2(s.m, s.s);
+  }
+}
+
+// The parts joined: the row's loss, and the gradient's part. Without a gradient a workgroup to a row.
+template <class T, bool GRAD>
+__global__ void __launch_bounds__(PART_THREADS) distill_join(Distill p) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ int no_teacher;
+  const uint64_t row = p.first + (GRAD ? blockIdx.x / p.parts : blockIdx.x);
+  const int part = GRAD ? blockIdx.x % p.parts : 0, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (!GRAD && wave) return;  // one wavefront does it
+  const T* x = (const T*)p.x + row * p.xs;
+  Softmax all{-__builtin_inff(), 0.0f};
+  for (int i = lane; i < p.parts; i += 64) {
+    const float2 s = p.sums[row * p.parts + i];
+    all = joined(p, all, Softmax{s.x, s.y});
+  }
+  all = wave_joined(p, all);
+  const Teacher t = teacher_at(lds, p.top);
+  bool none = false;
+  if (wave == 0) {
+    const float entropy = read_teacher<T>(p, row, x, p.picked + row * p.top, t, none);
+    const float other = cross_entropy(p, t, all);
+    if (lane == 0) {
+      no_teacher = none;
+      if (part == 0) p.loss[row] = none ? 0.0f : entropy + other;
+    }
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    none = no_teacher;
+    T* dx = (T*)p.dx + row * p.ds;
+    const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
+    const int lo = (int)((int64_t)vectors * part / p.parts), hi = (int)((int64_t)vectors * (part + 1) / p.parts);
+    const bool aligned = phase_of<T>(dx) == phase;
+    const float k = p.weight[row] * p.t, f = none || all.s == 0.0f ? 0.0f : k / all.s, m = or_zero(all.m);
+    constexpr int AHEAD = 4;
+    for (int v0 = lo + (int)threadIdx.x; v0 < hi; v0 += PART_THREADS * AHEAD) {
+      uint4 raw[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int v = v0 + i * PART_THREADS;
+        if (v < hi && is_whole<T>(v, phase, p.cols)) raw[i] = *reinterpret_cast<const uint4*>(x + ((int64_t)v * EACH<T> - phase));
+      }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        const int v = v0 + i * PART_THREADS;
+        if (v >= hi) break;
+        if (!is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
+        store_gradient<T>(p, raw[i], m, f, dx, v, phase, aligned);
+      }
+    }
+    if (none) return;
+    __syncthreads();  // what follows is stored over it
+    const int64_t first = (int64_t)lo * EACH<T> - phase, last = (int64_t)hi * EACH<T> - phase;
+    store_entries<T, PART_THREADS>(p, t, all, k, dx, (int)std::max<int64_t>(first, 0), (int)std::min<int64_t>(last, p.cols));
+  }
+}
+
+// Which kernel takes a call: a row to a workgroup of `threads` with `each`
+// vectors a thread, or rows in `parts`.
+struct DistillPlan {
+  int threads, each, parts;
+  uint64_t bytes;
+};
+DistillPlan distill_plan(int type, uint64_t rows, uint64_t cols, uint64_t top) {
+  DistillPlan d{0, 0, 0, 0};
+  const uint64_t each = type == PXG_F32 ? 4 : 8, vectors = (cols + 2 * each - 2) / each;  // at any alignment
+  if (vectors <= 1024 || (vectors <= 8192 && rows >= 128)) {
+    d.threads = vectors <= 1024 ? 256 : 1024;
+    const uint64_t n = (vectors + d.threads - 1) / d.threads;
+    d.each = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
+    return d;
+  }
+  // about 2048 workgroups fill the chip; parts of less than 16 KB gain nothing
+  const uint64_t most = std::max<uint64_t>(1, std::min<uint64_t>(256, vectors / 1024));
+  d.parts = (int)std::min(most, (2048 + rows - 1) / rows);
+  d.bytes = rows * d.parts * sizeof(float2) + rows * top * 4;
+  return d;
+}
+
+template <class T, bool GRAD>
+void run_distill(Distill p, const DistillPlan& d, hipStream_t s) {
+  const unsigned lds = (unsigned)(p.top * 12);
+  auto row = [&](auto threads, auto each) {
+    constexpr int THREADS = decltype(threads)::value, N = decltype(each)::value;
+    constexpr uint64_t MOST = LAUNCH_ROWS / 2;  // of 1024 threads
+    for (uint64_t a = 0; a < p.rows; a += MOST) {
+      p.first = a;
+      hipLaunchKernelGGL((distill_row<T, THREADS, N, GRAD>), dim3((unsigned)std::min(MOST, p.rows - a)), dim3(THREADS), lds,
+                         s, p);
+      PXG_HIP(hipGetLastError());
+    }
+  };
+  using Small = std::integral_constant<int, 256>;
+  using Large = std::integral_constant<int, 1024>;
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  using Eight = std::integral_constant<int, 8>;
+  if (d.threads == 256) {
+    if (d.each == 1) row(Small{}, One{});
+    else if (d.each == 2) row(Small{}, Two{});
+    else row(Small{}, Four{});
+  } else if (d.threads) {
+    if (d.each <= 2) row(Large{}, Two{});
+    else if (d.each == 4) row(Large{}, Four{});
+    else row(Large{}, Eight{});
+  } else {
+    const uint64_t all = p.rows;
+    p.parts = d.parts;
+    for (uint64_t a = 0, most = LAUNCH_ROWS / d.parts; a < all; a += most) {
+      const unsigned m = (unsigned)std::min(most, all - a);
+      p.first = a;
+      hipLaunchKernelGGL(distill_part<T>, dim3(m * d.parts), dim3(PART_THREADS), 0, s, p);
+      PXG_HIP(hipGetLastError());
+      hipLaunchKernelGGL((distill_join<T, GRAD>), dim3(GRAD ? m * d.parts : m), dim3(GRAD ? PART_THREADS : 64), lds, s, p);
+      PXG_HIP(hipGetLastError());
+    }
+  }
+}
+
+void check_distill(int type, const void* d_x, uint64_t rows, uint64_t cols, uint64_t x_stride, const int64_t* d_ids,
+                   uint64_t ids_stride, const float* d_scores, uint64_t scores_stride, const int32_t* d_counts,
+                   uint64_t top, double temperature, const float* d_loss) {
+  check_type(type, true);
+  check_size("cols", cols);
+  if (top == 0 || top > TOP_MAX) config_error("top", top, "must be between 1 and 4096");
+  if (!(temperature >= 1e-6 && temperature <= 1e6))
+    config_error("temperature", 0, "must be between 1e-6 and 1e6");
+  check_rows(type, "logits", d_x, rows, cols, x_stride);
+  check_rows(PXG_F32, "ids", d_ids, rows, top, ids_stride);
+  check_aligned("ids", d_ids, 8);
+  check_rows(PXG_F32, "scores", d_scores, rows, top, scores_stride);
+  check_rows(PXG_F32, "counts", d_counts, rows, 1, 1);
+  check_rows(PXG_F32, "loss", d_loss, rows, 1, 1);
+}
+
+int distill(int type, const float* d_weight, const void* d_x, uint64_t rows, uint64_t cols, uint64_t x_stride,
+            const int64_t* d_ids, uint64_t ids_stride, const float* d_scores, uint64_t scores_stride,
+            const int32_t* d_counts, uint64_t top, double temperature, float* d_loss, bool grad, void* d_dx,
+            uint64_t dx_stride, void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  return guard([&] {
+    check_distill(type, d_x, rows, cols, x_stride, d_ids, ids_stride, d_scores, scores_stride, d_counts, top,
+                  temperature, d_loss);
+    if (grad) {
+      check_rows(PXG_F32, "weight", d_weight, rows, 1, 1);
+      check_rows(type, "dx", d_dx, rows, cols, dx_stride);
+    }
+    if (rows == 0) return;
+    const DistillPlan d = distill_plan(type, rows, cols, top);
+    check_aligned("workspace", d_workspace, 16);
+    if (d.bytes && (!d_workspace || workspace_bytes < d.bytes))
+      config_error("workspace_bytes", workspace_bytes, "must be what pxg_distill_workspace says");
+    Distill p{};
+    p.x = d_x;
+    p.dx = d_dx;
+    p.ids = d_ids;
+    p.scores = d_scores;
+    p.counts = d_counts;
+    p.weight = d_weight;
+    p.loss = d_loss;
+    p.xs = x_stride;
+    p.ds = dx_stride;
+    p.is = ids_stride;
+    p.ss = scores_stride;
+    p.sums = (float2*)d_workspace;
+    p.picked = (float*)((char*)d_workspace + rows * d.parts * sizeof(float2));
+    p.rows = rows;
+    p.cols = (int)cols;
+    p.top = (int)top;
+    const double c = 1.4426950408889634 / temperature, t = 1.0 / temperature;
+    p.c = (float)c;
+    p.c_low = (float)(c - p.c);
+    p.t = (float)t;
+    p.t_low = (float)(t - p.t);
+    auto run = [&](auto kind) {
+      using T = decltype(kind);
+      if (grad) run_distill<T, true>(p, d, (hipStream_t)stream);
+      else run_distill<T, false>(p, d, (hipStream_t)stream);
+    };
+    if (type == PXG_F32) run(float{});
+    else if (type == PXG_F16) run((_Float16)0);
+    else run((__bf16)0.0f);
+  });
+}
+
+}  // namespace
+}  // namespace pxg
+
+using namespace pxg;
+
+extern "C" {
+
+uint64_t pxg_distill_workspace(int type, uint64_t rows, uint64_t cols, uint64_t top) {
+  if (rows == 0 || rows > PRODUCT_SIZE_MAX || cols == 0 || cols > PRODUCT_SIZE_MAX || top == 0 || top > TOP_MAX) return 0;
+  return distill_plan(type, rows, cols, top).bytes;
+}
+
+int pxg_distill_loss_device(int type, const void* d_logits, uint64_t rows, uint64_t cols, uint64_t logits_stride,
+                            const int64_t* d_ids, uint64_t ids_stride, const float* d_scores, uint64_t scores_stride,
+                            const int32_t* d_counts, uint64_t top, double temperature, float* d_loss,
+                            void* d_workspace, uint64_t workspace_bytes, void* stream) {
+  return distill(type, nullptr, d_logits, rows, cols, logits_stride, d_ids, ids_stride, d_scores, scores_stride,
+                 d_counts, top, temperature, d_loss, false, nullptr, 0, d_workspace, workspace_bytes, stream);
+}
+
+int pxg_distill_loss_grad_device(int type, const float* d_weight, const void* d_logits, uint64_t rows, uint64_t cols,
+                                 uint64_t logits_stride, const int64_t* d_ids, uint64_t ids_stride,
+                                 const float* d_scores, uint64_t scores_stride, const int32_t* d_counts, uint64_t top,
+                                 double temperature, float* d_loss, void* d_dx, uint64_t dx_stride, void* d_workspace,
+                                 uint64_t workspace_bytes, void* stream) {
+  return distill(type, d_weight, d_logits, rows, cols, logits_stride, d_ids, ids_stride, d_scores, scores_stride,
+                 d_counts, top, temperature, d_loss, true, d_dx, dx_stride, d_workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

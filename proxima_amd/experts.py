@@ -24,7 +24,7 @@ from ._capi import ExpertMatrixC as _ExpertMatrix, lib as _lib
 __all__ = [
     "Block8", "block8_pack", "block8_unpack", "block8_matmul", "grouped_matmul", "grouped_matmul_grad_input",
     "grouped_matmul_grad_weight", "grouped_linear", "block8_linear", "grouped_linear_grad", "expert_layer",
-    "activation_pack", "activation_grad",
+    "activation_pack", "activation_grad", "distill_loss", "distill_loss_grad",
 ]
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
@@ -533,3 +533,58 @@ def activation_grad(grad, packed, activation, out=None):
     _run(_lib.pxg_activation_grad_device, (grad, codes, scales, out), which, kind, grad.data_ptr(), rows, cols,
          _stride(grad), codes.data_ptr(), scales.data_ptr(), out.data_ptr(), stride)
     return out
+
+
+def _vector(t, name, rows, dtype):
+    """Checks a contiguous GPU tensor of `rows` values."""
+    if not getattr(t, "is_cuda", False):
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.dim() != 1 or not t.is_contiguous() or t.dtype is not dtype:
+        raise ValueError(f"{name} must be a contiguous one-dimensional {dtype} tensor")
+    if t.shape[0] != rows:
+        _mismatch(t.shape[0], rows, f"{name}'s length")
+    return t.data_ptr()
+
+
+def _distill(weight, logits, ids, scores, counts, temperature, grad, out):
+    rows, cols = _matrix(logits, "logits")
+    kind = _type(logits.dtype, "logits")
+    _, top = shape = _routes(ids, "ids", _torch.int64)
+    if shape[0] != rows:
+        _mismatch(shape[0], rows, "ids' rows")
+    _routes(scores, "scores", _torch.float32, shape)
+    counts_ptr = _vector(counts, "counts", rows, _torch.int32)
+    tensors = [logits, ids, scores, counts]
+    loss = logits.new_empty((rows,), dtype=_torch.float32)
+    size = _lib.pxg_distill_workspace(kind, rows, cols, top)
+    space = logits.new_empty(size, dtype=_torch.uint8) if size else None
+    args = (logits.data_ptr(), rows, cols, _stride(logits), ids.data_ptr(), _stride(ids), scores.data_ptr(),
+            _stride(scores), counts_ptr, top, temperature, loss.data_ptr())
+    held = (space.data_ptr() if size else None, size)
+    if not grad:
+        _run(_lib.pxg_distill_loss_device, tensors, kind, *args, *held)
+        return loss
+    weight_ptr = _vector(weight, "weight", rows, _torch.float32)
+    out, stride = _out(out, (rows, cols), logits.dtype, logits)
+    tensors += (weight, out)
+    _run(_lib.pxg_distill_loss_grad_device, tensors, kind, weight_ptr, *args, out.data_ptr(), stride, *held)
+    return loss, out
+
+
+def distill_loss(logits, ids, scores, counts, temperature=1.0):
+    """The loss [rows] (f32) of a model that is to rank as a teacher does, as search_device gives the teacher's best:
+    sum over entries of p (log p - log q[id]), p the softmax of scores / temperature over a row's first counts[t]
+    entries, q that of its logits / temperature.
+
+    logits [rows, cols] f32, f16 or bf16; ids [rows, top] int64 and scores [rows, top] f32 (larger is nearer: of
+    distances their negatives), top at most 4096; counts [rows] int32. Entries whose id is outside [0, cols) are left
+    out. A row without entries, or whose scores are all -inf, has loss 0; an entry of p = 0 adds nothing; a logit of
+    -inf has q = 0, so that p > 0 there costs infinity. temperature is a number between 1e-6 and 1e6."""
+    return _distill(None, logits, ids, scores, counts, temperature, False, None)
+
+
+def distill_loss_grad(weight, logits, ids, scores, counts, temperature=1.0, out=None):
+    """(loss, dx): distill_loss and the logits' gradient, weight[t] / temperature (q - p), of the logits' type and
+    rounded once; weight [rows] f32 is the loss' own gradient (1 / rows for the mean). Rows without a teacher have zeros.
+    `out` may be the logits themselves."""
+    return _distill(weight, logits, ids, scores, counts, temperature, True, out)

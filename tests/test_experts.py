@@ -167,3 +167,73 @@ def test_layers_backward_pass_refuses(lib):
     size = lib.pxg_grouped_linear_grad_workspace
     assert size(100_000, 1024, 8) > 0 and size(100_000, 1024, 8) % (4 * 1024) == 0
     assert size(8, 1024, 8) == 0 and size(0, 8, 1) == 0 and size(8, 0, 1) == 0 and size(8, 8, 0) == 0
+
+
+def test_whole_layers_refuse(lib):
+    from proxima_amd._capi import ExpertMatrixC
+    p, odd = C.c_void_p(4096), C.c_void_p(4097)
+    m = ExpertMatrixC(4096, 8, 64, 4096)
+
+    def f(kind=2, x=p, rows=4, k=8, xs=8, ids=p, picks=2, is_=2, gates=p, gs=2, experts=3, hidden=8, n=8, w1=m, up=None,
+          w2=m, packed=0, act=1, bias_type=0, b1=p, b1s=8, b2=p, b2s=8, out=2, r=p, rs=8, y=p, ys=8, space=p,
+          size=1 << 30):
+        return lib.pxg_expert_layer_device(kind, x, rows, k, xs, ids, picks, is_, gates, gs, experts, hidden, n, w1, up, w2,
+                                           packed, act, bias_type, b1, b1s, b2, b2s, out, r, rs, y, ys, space, size, None)
+
+    for more, parameter in (
+            (dict(kind=0), b"type"), (dict(kind=1, packed=1, out=1), b"type"), (dict(out=1), b"out_type"),
+            (dict(rows=65537), b"rows"), (dict(picks=0), b"picks"), (dict(picks=17, is_=17, gs=17), b"picks"),
+            (dict(experts=0), b"experts"), (dict(experts=65537), b"experts"), (dict(k=0), b"k"),
+            (dict(k=(1 << 22) + 1), b"k"), (dict(hidden=0), b"hidden"), (dict(n=0), b"n"), (dict(act=2), b"activation"),
+            (dict(x=None), b"x"), (dict(xs=7), b"stride"), (dict(gates=None), b"gates"), (dict(gs=1), b"stride"),
+            (dict(ids=None), b"experts"), (dict(ids=C.c_void_p(4100)), b"experts"), (dict(w1=None), b"w1"),
+            (dict(w1=ExpertMatrixC(None, 8, 64, None)), b"w1"), (dict(w2=ExpertMatrixC(4097, 8, 64, None)), b"w2"),
+            (dict(up=ExpertMatrixC(4096, 7, 64, None)), b"stride"),
+            (dict(w2=ExpertMatrixC(4096, 8, 64, None), packed=1), b"w2"),
+            (dict(w1=ExpertMatrixC(4104, 8, 64, 4096), packed=1), b"w1"), (dict(bias_type=1), b"bias_type"),
+            (dict(b1=C.c_void_p(4098)), b"bias1"), (dict(b2s=7), b"stride"), (dict(r=odd), b"residual"),
+            (dict(rs=7), b"stride"), (dict(y=None), b"y"), (dict(space=None), b"workspace_bytes"),
+            (dict(size=64), b"workspace_bytes"), (dict(space=C.c_void_p(4104)), b"workspace")):
+        _refused(lib, f(**more), parameter)
+    assert f(rows=0, x=None, ids=None, gates=None, r=None, y=None, space=None, size=0) == 0
+    size = lib.pxg_expert_layer_workspace
+    assert size(8, 2, 16, 512, 512, 0) > size(8, 2, 16, 512, 512, 2) > 8 * 2 * 512 * 2 * 2
+    assert size(0, 2, 16, 512, 512, 0) == 0 and size(8, 17, 16, 512, 512, 0) == 0 and size(8, 2, 0, 512, 512, 0) == 0
+
+
+def test_distillation_refuses(lib):
+    p, odd = C.c_void_p(4096), C.c_void_p(4097)
+
+    def f(kind=0, weight=p, x=p, rows=4, cols=8, xs=8, ids=p, is_=2, scores=p, ss=2, counts=p, top=2, t=1.0, loss=p, dx=p,
+          ds=8, space=None, size=0):
+        return lib.pxg_distill_loss_grad_device(kind, weight, x, rows, cols, xs, ids, is_, scores, ss, counts, top, t, loss,
+                                                dx, ds, space, size, None)
+
+    for more, parameter in (
+            (dict(kind=3), b"type"), (dict(cols=0), b"cols"), (dict(top=0), b"top"), (dict(top=4097), b"top"),
+            (dict(t=0.0), b"temperature"), (dict(t=float("nan")), b"temperature"), (dict(t=1e7), b"temperature"),
+            (dict(x=None), b"logits"), (dict(xs=7), b"stride"), (dict(x=odd), b"logits"), (dict(ids=None), b"ids"),
+            (dict(ids=C.c_void_p(4100)), b"ids"), (dict(is_=1), b"stride"), (dict(scores=None), b"scores"),
+            (dict(counts=None), b"counts"), (dict(loss=None), b"loss"), (dict(weight=None), b"weight"),
+            (dict(dx=None), b"dx"), (dict(ds=7), b"stride"), (dict(rows=1 << 31), b"rows"),
+            (dict(cols=1 << 20, xs=1 << 20, ds=1 << 20), b"workspace_bytes"),
+            (dict(space=C.c_void_p(4104)), b"workspace")):
+        _refused(lib, f(**more), parameter)
+    assert f(rows=0, weight=None, x=None, ids=None, scores=None, counts=None, loss=None, dx=None) == 0
+    assert lib.pxg_distill_loss_device(0, None, 0, 8, 8, None, 2, None, 2, None, 2, 1.0, None, None, 0, None) == 0
+    _refused(lib, lib.pxg_distill_loss_device(0, None, 4, 8, 8, p, 2, p, 2, p, 2, 1.0, p, None, 0, None), b"logits")
+    size = lib.pxg_distill_workspace
+    assert size(0, 4, 1 << 20, 2) > 0 and size(0, 4, 8, 2) == 0 and size(0, 0, 8, 2) == 0 and size(0, 4, 8, 0) == 0
+
+
+def test_python_side_of_layers_and_losses_refuses_host_tensors():
+    import torch
+
+    import proxima_amd as px
+    x, w = torch.zeros(4, 8), torch.zeros(2, 8, 8)
+    ids, scores, counts = torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: px.grouped_linear(x, w), lambda: px.block8_linear(x, x), lambda: px.grouped_linear_grad(x),
+                 lambda: px.expert_layer(x, ids, w, w, scores), lambda: px.distill_loss(x, ids, scores, counts),
+                 lambda: px.distill_loss_grad(counts, x, ids, scores, counts)):
+        with pytest.raises(ValueError):
+            call()

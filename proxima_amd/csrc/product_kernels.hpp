@@ -693,8 +693,9 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
 
   // A lane holds columns 4 q to 4 q + 3 of row r16 of each tile. Through LDS,
   // 16 rows of the wavefront's columns at a time, so that what is stored
-  // together is whole rows of them and not 8 bytes of each of 16.
-  auto store = [&](auto type, void* result, uint64_t stride, bool whole) {
+  // together is whole rows of them and not 8 bytes of each of 16. finish(i)
+  // goes before row tile i.
+  auto store = [&](auto type, void* result, uint64_t stride, bool whole, auto finish) {
     using R = decltype(type);
     constexpr int EACH = 16 / sizeof(R), PER = NT * 16 / EACH;  // a lane's elements, lanes to a row
     constexpr int PITCH = NT * 16 * sizeof(R) + 16;             // 16 bytes more spread the rows over the banks
@@ -704,12 +705,13 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
     const int col = wn * NT * 16 + lane % PER * EACH;
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
+      finish(i);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         typedef R r4v __attribute__((ext_vector_type(4)));
         r4v v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (R)acc[i][j][e];
+        for (int e = 0; e < 4; ++e) v[e] = is_linear<P> ? rounded<R>(acc[i][j][e]) : (R)acc[i][j][e];
         *reinterpret_cast<r4v*>(mine + r16 * PITCH + (j * 16 + 4 * q) * sizeof(R)) = v;
       }
       if (whole) {
@@ -742,126 +744,70 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
       }
     }
   };
-  // The same with an epilogue, in f32 through LDS, so that the residual is read
-  // and all is stored by whole rows and rounded once. The residual of the next
-  // pieces is loaded while a piece is computed.
+  // The same with an epilogue, where the sums are: a lane has 4 columns of a row
+  // of each tile, whose residual it loads ahead. Then y, rounded, takes the way
+  // of a plain result (through LDS in f32 and by whole rows, residual and all:
+  // 8192 rows in 8 uneven groups, 1024 -> 4096, 99 us with a bias, for 88).
   [[maybe_unused]] auto store_linear = [&] {
     if constexpr (is_linear<P>) {
-      constexpr int W = NT * 16, PITCH = W * 4 + 16;
-      static_assert(WAVES * 16 * PITCH <= K::LDS);
-      char* mine = lds + wave * (16 * PITCH);
-      auto stage_tile = [&](int i) {
+      const int col = wn * NT * 16 + 4 * q;  // of tile j: 16 j on
+      if (p.bias && grouped) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          *reinterpret_cast<f4v*>(mine + r16 * PITCH + (j * 16 + 4 * q) * 4) = acc[i][j];
-      };
-      const bool biased = p.bias && grouped;
-      auto bias_at = [&](int c) {
-        const uint64_t at = group * p.bias_stride + n0 + c;
-        return !biased || c >= cols ? 0.0f
-               : p.bias_f32         ? ((const float*)p.bias)[at]
-                                    : (float)((const linear_bias<T>*)p.bias)[at];
-      };
-      O* c = (O*)p.c + (uint64_t)m0 * p.cs + n0;
-      const O* residual = (const O*)p.residual + (uint64_t)m0 * p.rs + n0;
-      O* kept = (O*)p.kept + (uint64_t)m0 * p.hs + n0;
-      const bool passes = p.residual != nullptr, keeps = p.kept != nullptr;
-      if (p.c_vec) {
-        constexpr int EACH = 16 / sizeof(O), PER = W / EACH, STEP = 64 / PER, TIMES = 16 / STEP;
-        constexpr int AHEAD = std::min(MT * TIMES, 8);  // pieces of the residual loaded ahead
-        const int col = wn * W + lane % PER * EACH;
-        float b[EACH];
+        for (int j = 0; j < NT; ++j) {
+          f4v b;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) b[e] = bias_at(col + e);
-        const bool all = col + EACH <= cols;
-        auto row_of = [&](int piece) { return (piece / TIMES * WM + wm) * 16 + lane / PER + piece % TIMES * STEP; };
-        struct Piece {
-          O v[EACH];
-        };
-        Piece r[AHEAD];
-        auto load = [&](int piece) {
-          Piece x{};
-          const int row = row_of(piece);
-          if (row < rows && col < cols) {
-            const O* from = residual + (uint64_t)row * p.rs + col;
-            if (all) {
-              *reinterpret_cast<uint4*>(x.v) = *reinterpret_cast<const uint4*>(from);
-            } else {
-#pragma unroll
-              for (int e = 0; e < EACH; ++e)
-                if (col + e < cols) x.v[e] = from[e];
-            }
+          for (int e = 0; e < 4; ++e) {
+            const int c = col + j * 16 + e;
+            const uint64_t at = group * p.bias_stride + n0 + c;
+            b[e] = c >= cols ? 0.0f : p.bias_f32 ? ((const float*)p.bias)[at] : (float)((const linear_bias<T>*)p.bias)[at];
           }
-          return x;
-        };
-        auto put = [&](O* to, const float (&v)[EACH]) {
-          O x[EACH];
 #pragma unroll
-          for (int e = 0; e < EACH; ++e) x[e] = rounded<O>(v[e]);
-          if (all) {
-            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(x);
-          } else {
-#pragma unroll
-            for (int e = 0; e < EACH; ++e)
-              if (col + e < cols) to[e] = x[e];
-          }
-        };
-        if (passes)
-#pragma unroll
-          for (int piece = 0; piece < AHEAD; ++piece) r[piece] = load(piece);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          stage_tile(i);
-#pragma unroll
-          for (int h = 0; h < TIMES; ++h) {
-            const int piece = i * TIMES + h, row = row_of(piece);
-            float v[EACH];
-#pragma unroll
-            for (int e = 0; e < EACH; e += 4)
-              *reinterpret_cast<f4v*>(v + e) = *reinterpret_cast<const f4v*>(
-                  mine + (lane / PER + h * STEP) * PITCH + (lane % PER * EACH + e) * 4);
-            Piece x{};
-            if (passes) {
-              x = r[piece % AHEAD];
-              if (piece + AHEAD < MT * TIMES) r[piece % AHEAD] = load(piece + AHEAD);
-            }
-            if (row >= rows || col >= cols) continue;
-#pragma unroll
-            for (int e = 0; e < EACH; ++e) v[e] += b[e];
-            if (keeps) put(kept + (uint64_t)row * p.hs + col, v);
-            activate<O>(v, p.activation);
-            if (passes)
-#pragma unroll
-              for (int e = 0; e < EACH; ++e) v[e] += (float)x.v[e];
-            put(c + (uint64_t)row * p.cs + col, v);
-          }
-        }
-      } else {
-        constexpr int TIMES = 16 * W / 64;  // an element a lane, of one row or two
-        const int col = wn * W + lane % W;
-        const float b = bias_at(col);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          stage_tile(i);
-          auto row_of = [&](int h) { return (i * WM + wm) * 16 + lane / W + h * (64 / W); };
-          O r[TIMES];
-          if (passes)
-#pragma unroll
-            for (int h = 0; h < TIMES; ++h)
-              r[h] = row_of(h) < rows && col < cols ? residual[(uint64_t)row_of(h) * p.rs + col] : (O)0.0f;
-#pragma unroll
-          for (int h = 0; h < TIMES; ++h) {
-            const int row = row_of(h);
-            float v[1] = {*reinterpret_cast<const float*>(mine + (lane / W + h * (64 / W)) * PITCH + lane % W * 4)};
-            if (row >= rows || col >= cols) continue;
-            v[0] += b;
-            if (keeps) kept[(uint64_t)row * p.hs + col] = rounded<O>(v[0]);
-            activate<O>(v, p.activation);
-            if (passes) v[0] += (float)r[h];
-            c[(uint64_t)row * p.cs + col] = rounded<O>(v[0]);
-          }
+          for (int i = 0; i < MT; ++i) acc[i][j] += b;
         }
       }
+      if (p.kept) store(O{}, p.kept, p.hs, p.c_vec, [](int) {});
+      struct Four {
+        O v[4];
+      };
+      constexpr int AHEAD = std::min(MT, sizeof(O) == 2 ? 4 : 2);  // row tiles whose residual is loaded ahead
+      [[maybe_unused]] Four r[AHEAD][NT];
+      auto load = [&](int i, Four (&x)[NT]) {
+        const int row = (i * WM + wm) * 16 + r16;
+        const O* from = (const O*)p.residual + (uint64_t)(m0 + row) * p.rs + n0;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int c = col + j * 16;
+          x[j] = Four{};
+          if (row >= rows) continue;
+          if (p.c_vec && c + 4 <= cols) {
+            x[j] = *reinterpret_cast<const Four*>(__builtin_assume_aligned(from + c, 4 * sizeof(O)));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < cols) x[j].v[e] = from[c + e];
+          }
+        }
+      };
+      const bool passes = p.residual != nullptr;
+      if (passes)
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) load(i, r[i]);
+      store(O{}, p.c, p.cs, p.c_vec, [&](int i) {
+        if (p.activation != NO_ACTIVATION)
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+            activate<O>(v, p.activation);
+            acc[i][j] = f4v{v[0], v[1], v[2], v[3]};
+          }
+        if (passes) {
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j][e] += (float)r[i % AHEAD][j].v[e];
+          if (i + AHEAD < MT) load(i + AHEAD, r[i % AHEAD]);
+        }
+      });
     }
   };
   lds_barrier();
@@ -871,14 +817,14 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
     float* part = p.workspace + (uint64_t)(slot < 0 ? 0 : slot) * p.m * p.n;
     const bool apart = slot >= 0;
     if constexpr (std::is_same_v<O, float>) {  // one piece of code for both
-      store(O{}, apart ? part : result, apart ? p.n : p.cs, apart ? p.n % 4 == 0 : p.c_vec);
+      store(O{}, apart ? part : result, apart ? p.n : p.cs, apart ? p.n % 4 == 0 : p.c_vec, [](int) {});
     } else if (apart) {
-      store(float{}, part, p.n, p.n % 4 == 0);
+      store(float{}, part, p.n, p.n % 4 == 0, [](int) {});
     } else {
-      store(O{}, result, p.cs, p.c_vec);
+      store(O{}, result, p.cs, p.c_vec, [](int) {});
     }
   } else {
-    store(O{}, result, p.cs, p.c_vec);
+    store(O{}, result, p.cs, p.c_vec, [](int) {});
   }
 #endif
 }
@@ -1139,6 +1085,26 @@ struct Tile {
 };
 constexpr Tile TILES[3] = {{256, 256, 6, 1.15, 0.45}, {128, 512, 4, 0.7, 0.35}, {64, 1024, 3, 0.42, 0.3}};
 constexpr Tile PACKED_TILES[3] = {{256, 256, 6, 0.6, 0.25}, {128, 512, 4, 0.95, 0.45}, {64, 1024, 3, 0.6, 0.4}};
+// What an epilogue adds to a tile of each size, in us: 128 and 64 share a CU with
+// others, whose products go on meanwhile. With GELU and h kept, 8192 rows in 8
+// uneven groups, 1024 -> 4096: 125 us with 256, 115 with 128 (88, 94 without).
+struct Epilogue {
+  double us[3] = {0, 0, 0};
+  void add(double a, double b, double c) {
+    us[0] += a;
+    us[1] += b;
+    us[2] += c;
+  }
+};
+inline Epilogue epilogue_cost(const Product&) { return {}; }
+inline Epilogue epilogue_cost(const LinearProduct& p) {
+  Epilogue e;
+  if (p.activation == PXG_GELU) e.add(9, 3.3, 1);
+  if (p.activation == PXG_SILU) e.add(3.2, 1.2, 0.4);
+  if (p.residual) e.add(6.8, 4.2, 1.8);
+  if (p.kept) e.add(3.1, 1.3, 0.8);
+  return e;
+}
 // Joining the parts of divided groups: a launch, and their bytes twice.
 constexpr double JOIN_US = 4, JOIN_BYTES_PER_US = 4e6;
 
@@ -1154,7 +1120,8 @@ struct Cost {
 //   1 of 4096, 768 x 768                           36 ->  21 (1536)
 //   8 uneven ones, 16384 rows in all, 512 x 512    39 ->  30 (1024)
 //   8 uneven, 8192 rows, 4096 x 1024               63 ->  87 (2048): the parts' traffic
-Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0, int tile_asked = 0) {
+Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0, int tile_asked = 0,
+                  const Epilogue& epilogue = {}) {
   Cost best;
   const double average = form == GRAD_WEIGHT ? (double)p.rows / p.groups : p.k;
   const double longest = form == GRAD_WEIGHT ? average * std::sqrt((double)p.groups) : p.k;
@@ -1181,7 +1148,7 @@ Cost product_cost(int form, const Product& p, bool packed, uint64_t room = 0, in
       // columns; of more it does, and 128 x 128 tiles are taken where 256 x 256
       // would be faster (2048 rows, 4096 -> 8192: 150 us, 108)
       const double rounds = std::ceil((double)all / t.slots - (p.groups == 1 ? 0.12 : 0.0));
-      double us = std::max(1.0, rounds) * (t.fixed + std::ceil(summed / 64) * step);
+      double us = std::max(1.0, rounds) * (t.fixed + epilogue.us[i] + std::ceil(summed / 64) * step);
       us = std::max(us, t.fixed + (limit ? (double)limit : longest) / 64 * step);
       if (limit) us += JOIN_US + 2.0 * bytes / JOIN_BYTES_PER_US;
       if (packed && i == 0) {
@@ -1246,7 +1213,8 @@ void launch_product(P p, uint64_t room, hipStream_t s) {
   const bool copied = (is_packed(LA) || copies(2, p.a, acols, p.as, 0)) &&
                       (is_packed(LB) || copies(2, p.b, bcols, p.bs, p.bg));
   constexpr bool PACKED_FORWARD = FORM == FORWARD && IS_PACKED;
-  const Cost cost = product_cost(FORM, p, PACKED_FORWARD, room, asked_tile(PACKED_FORWARD && std::is_same_v<O, float>));
+  const Cost cost = product_cost(FORM, p, PACKED_FORWARD, room, asked_tile(PACKED_FORWARD && std::is_same_v<O, float>),
+                                 epilogue_cost(p));
   if constexpr (FORM != GRAD_WEIGHT) {
     constexpr int B = FORM == GRAD_INPUT ? COLS : ROWS;
     // COLS spans a matrix' rows with one resource

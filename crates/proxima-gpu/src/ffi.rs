@@ -31,6 +31,115 @@ pub(crate) struct PxgExpertMatrix {
     pub(crate) scales: *const c_void,
 }
 
+/// `pxg_linear`.
+#[repr(C)]
+pub(crate) struct PxgLinear {
+    pub(crate) kind: i64,
+    pub(crate) out_type: i64,
+    pub(crate) bias_type: i64,
+    pub(crate) activation: i64,
+    pub(crate) rows: u64,
+    pub(crate) k: u64,
+    pub(crate) groups: u64,
+    pub(crate) n: u64,
+    pub(crate) x: *const c_void,
+    pub(crate) x_stride: u64,
+    pub(crate) w: *const c_void,
+    pub(crate) w_stride: u64,
+    pub(crate) w_group_stride: u64,
+    pub(crate) offsets: *const i64,
+    pub(crate) bias: *const c_void,
+    pub(crate) bias_stride: u64,
+    pub(crate) residual: *const c_void,
+    pub(crate) residual_stride: u64,
+    pub(crate) h: *mut c_void,
+    pub(crate) h_stride: u64,
+    pub(crate) y: *mut c_void,
+    pub(crate) y_stride: u64,
+    pub(crate) x_scales: *const c_void,
+    pub(crate) w_scales: *const c_void,
+}
+
+/// `pxg_linear_grad`.
+#[repr(C)]
+pub(crate) struct PxgLinearGrad {
+    pub(crate) kind: i64,
+    pub(crate) bias_type: i64,
+    pub(crate) activation: i64,
+    pub(crate) rows: u64,
+    pub(crate) n: u64,
+    pub(crate) groups: u64,
+    pub(crate) grad: *const c_void,
+    pub(crate) grad_stride: u64,
+    pub(crate) h: *const c_void,
+    pub(crate) h_stride: u64,
+    pub(crate) offsets: *const i64,
+    pub(crate) dh: *mut c_void,
+    pub(crate) dh_stride: u64,
+    pub(crate) dbias: *mut c_void,
+    pub(crate) dbias_stride: u64,
+    pub(crate) workspace: *mut c_void,
+    pub(crate) workspace_bytes: u64,
+}
+
+/// `pxg_expert_layer`.
+#[repr(C)]
+pub(crate) struct PxgExpertLayer {
+    pub(crate) kind: i64,
+    pub(crate) out_type: i64,
+    pub(crate) bias_type: i64,
+    pub(crate) activation: i64,
+    pub(crate) packed: i64,
+    pub(crate) rows: u64,
+    pub(crate) k: u64,
+    pub(crate) picks: u64,
+    pub(crate) experts: u64,
+    pub(crate) hidden: u64,
+    pub(crate) n: u64,
+    pub(crate) x: *const c_void,
+    pub(crate) x_stride: u64,
+    pub(crate) ids: *const i64,
+    pub(crate) ids_stride: u64,
+    pub(crate) gates: *const f32,
+    pub(crate) gates_stride: u64,
+    pub(crate) w1: PxgExpertMatrix,
+    pub(crate) up: PxgExpertMatrix,
+    pub(crate) w2: PxgExpertMatrix,
+    pub(crate) bias1: *const c_void,
+    pub(crate) bias1_stride: u64,
+    pub(crate) bias2: *const c_void,
+    pub(crate) bias2_stride: u64,
+    pub(crate) residual: *const c_void,
+    pub(crate) residual_stride: u64,
+    pub(crate) y: *mut c_void,
+    pub(crate) y_stride: u64,
+    pub(crate) workspace: *mut c_void,
+    pub(crate) workspace_bytes: u64,
+}
+
+/// `pxg_distill`.
+#[repr(C)]
+pub(crate) struct PxgDistill {
+    pub(crate) kind: i64,
+    pub(crate) rows: u64,
+    pub(crate) cols: u64,
+    pub(crate) top: u64,
+    pub(crate) logits: *const c_void,
+    pub(crate) logits_stride: u64,
+    pub(crate) ids: *const i64,
+    pub(crate) ids_stride: u64,
+    pub(crate) scores: *const f32,
+    pub(crate) scores_stride: u64,
+    pub(crate) counts: *const i32,
+    pub(crate) temperature: f64,
+    pub(crate) loss: *mut f32,
+    pub(crate) weight: *const f32,
+    pub(crate) dx: *mut c_void,
+    pub(crate) dx_stride: u64,
+    pub(crate) workspace: *mut c_void,
+    pub(crate) workspace_bytes: u64,
+}
+
 /// `pxg_index_stats` (index.rs:68-130).
 #[repr(C)]
 #[derive(Default)]
@@ -242,36 +351,16 @@ extern "C" {
         grad_stride: u64, d_codes: *const c_void, d_scales: *const c_void, k: u64, d_offsets: *const i64,
         groups: u64, out_type: c_int, d_dw: *mut c_void, dw_stride: u64, dw_group_stride: u64,
         d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
-    pub(crate) fn pxg_grouped_linear_device(kind: c_int, d_x: *const c_void, rows: u64, k: u64, x_stride: u64,
-        d_w: *const c_void, groups: u64, n: u64, w_stride: u64, w_group_stride: u64, d_offsets: *const i64,
-        bias_type: c_int, d_bias: *const c_void, bias_stride: u64, activation: c_int, out_type: c_int,
-        d_residual: *const c_void, residual_stride: u64, d_h: *mut c_void, h_stride: u64, d_y: *mut c_void,
-        y_stride: u64, stream: *mut c_void) -> c_int;
-    pub(crate) fn pxg_block8_linear_device(d_codes: *const c_void, d_scales: *const c_void, rows: u64, k: u64,
-        d_w_codes: *const c_void, d_w_scales: *const c_void, groups: u64, n: u64, d_offsets: *const i64,
-        bias_type: c_int, d_bias: *const c_void, bias_stride: u64, activation: c_int, out_type: c_int,
-        d_residual: *const c_void, residual_stride: u64, d_y: *mut c_void, y_stride: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_linear_device(layer: *const PxgLinear, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_block8_linear_device(layer: *const PxgLinear, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_grouped_linear_grad_workspace(rows: u64, n: u64, groups: u64) -> u64;
-    pub(crate) fn pxg_grouped_linear_grad_device(activation: c_int, kind: c_int, d_grad: *const c_void, rows: u64,
-        n: u64, grad_stride: u64, d_h: *const c_void, h_stride: u64, d_offsets: *const i64, groups: u64,
-        d_dh: *mut c_void, dh_stride: u64, bias_type: c_int, d_dbias: *mut c_void, dbias_stride: u64,
-        d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_grouped_linear_grad_device(layer: *const PxgLinearGrad, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_expert_layer_workspace(rows: u64, picks: u64, experts: u64, hidden: u64, n: u64,
         out_type: c_int) -> u64;
-    pub(crate) fn pxg_expert_layer_device(kind: c_int, d_x: *const c_void, rows: u64, k: u64, x_stride: u64,
-        d_experts: *const i64, picks: u64, experts_stride: u64, d_gates: *const f32, gates_stride: u64, experts: u64,
-        hidden: u64, n: u64, w1: *const PxgExpertMatrix, up: *const PxgExpertMatrix, w2: *const PxgExpertMatrix,
-        packed: c_int, activation: c_int, bias_type: c_int, d_bias1: *const c_void, bias1_stride: u64,
-        d_bias2: *const c_void, bias2_stride: u64, out_type: c_int, d_residual: *const c_void, residual_stride: u64,
-        d_y: *mut c_void, y_stride: u64, d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_expert_layer_device(layer: *const PxgExpertLayer, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_distill_workspace(kind: c_int, rows: u64, cols: u64, top: u64) -> u64;
-    pub(crate) fn pxg_distill_loss_device(kind: c_int, d_logits: *const c_void, rows: u64, cols: u64, logits_stride: u64,
-        d_ids: *const i64, ids_stride: u64, d_scores: *const f32, scores_stride: u64, d_counts: *const i32, top: u64,
-        temperature: f64, d_loss: *mut f32, d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
-    pub(crate) fn pxg_distill_loss_grad_device(kind: c_int, d_weight: *const f32, d_logits: *const c_void, rows: u64,
-        cols: u64, logits_stride: u64, d_ids: *const i64, ids_stride: u64, d_scores: *const f32, scores_stride: u64,
-        d_counts: *const i32, top: u64, temperature: f64, d_loss: *mut f32, d_dx: *mut c_void, dx_stride: u64,
-        d_workspace: *mut c_void, workspace_bytes: u64, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_distill_loss_device(distill: *const PxgDistill, stream: *mut c_void) -> c_int;
+    pub(crate) fn pxg_distill_loss_grad_device(distill: *const PxgDistill, stream: *mut c_void) -> c_int;
     pub(crate) fn pxg_grouped_matmul_set_kernel(rows: c_int) -> c_int;
     pub(crate) fn pxg_grouped_matmul_last_kernel() -> u32;
     pub(crate) fn pxg_activation_pack_device(activation: c_int, kind: c_int, d_h: *const c_void, rows: u64,

@@ -499,66 +499,108 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
                                                  uint64_t dw_stride, uint64_t dw_group_stride, void* d_workspace,
                                                  uint64_t workspace_bytes, void* stream);
 
+/* The calls from here on take their arguments as a struct, of fields of 8 bytes
+ * each; strides are in elements, and pointers that may be NULL are said to. */
+
 /* A layer: h = x w_g^T + b_g and y = f(h) + r, summed in f32 and y rounded
- * once, from h before its rounding. `activation` is a pxg_activation, or -1 for
- * f(h) = h. d_bias (NULL: none) is groups rows of n, bias_stride apart, of
- * bias_type: the operands' type (packed rows': bf16) or f32. d_residual (NULL:
- * none) is r, rows x n of out_type, and may be y itself. d_h (NULL: not kept)
- * takes h in out_type. Rows of no group: y = r (zeros without), h = 0. */
-int pxg_grouped_linear_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride, const void* d_w,
-                              uint64_t groups, uint64_t n, uint64_t w_stride, uint64_t w_group_stride,
-                              const int64_t* d_offsets, int bias_type, const void* d_bias, uint64_t bias_stride,
-                              int activation, int out_type, const void* d_residual, uint64_t residual_stride,
-                              void* d_h, uint64_t h_stride, void* d_y, uint64_t y_stride, void* stream);
-/* The same over packed rows, multiplied as pxg_block8_matmul_device does. */
-int pxg_block8_linear_device(const void* d_codes, const void* d_scales, uint64_t rows, uint64_t k,
-                             const void* d_w_codes, const void* d_w_scales, uint64_t groups, uint64_t n,
-                             const int64_t* d_offsets, int bias_type, const void* d_bias, uint64_t bias_stride,
-                             int activation, int out_type, const void* d_residual, uint64_t residual_stride,
-                             void* d_y, uint64_t y_stride, void* stream);
+ * once, from h before its rounding. x is rows x k, w_g n x k, of `type` (f16 or
+ * bf16), y of out_type (that or f32). `activation` is a pxg_activation, or -1 for
+ * f(h) = h. `bias` (or NULL) is groups rows of n of bias_type: the operands' type
+ * (packed rows': bf16) or f32. `residual` (or NULL) is r, rows x n of out_type, and
+ * may be y itself. `h` (or NULL) takes h in out_type. Rows of no group: y = r
+ * (zeros without), h = 0. block8: the same over packed rows, multiplied as
+ * pxg_block8_matmul_device does: x and w are codes with x_scales and w_scales,
+ * whose strides, `type` and h are not looked at, and out_type is any. */
+typedef struct pxg_linear {
+  int64_t type, out_type, bias_type, activation;
+  uint64_t rows, k, groups, n;
+  const void* x;
+  uint64_t x_stride;
+  const void* w;
+  uint64_t w_stride, w_group_stride;
+  const int64_t* offsets;
+  const void* bias;
+  uint64_t bias_stride;
+  const void* residual;
+  uint64_t residual_stride;
+  void* h;
+  uint64_t h_stride;
+  void* y;
+  uint64_t y_stride;
+  const void* x_scales;
+  const void* w_scales;
+} pxg_linear;
+int pxg_grouped_linear_device(const pxg_linear* layer, void* stream);
+int pxg_block8_linear_device(const pxg_linear* layer, void* stream);
+
 /* A layer's backward pass up to the products: dh = grad * f'(h), rows x n of
  * `type` (f32, f16 or bf16, as grad and h), zeros for rows of no group; and
  * dbias_g = the sum of the group's dh, groups rows of n of bias_type (`type` or
- * f32), taken before dh is rounded. dh may be grad or h itself; d_dbias may be
- * NULL. With activation -1, dh is grad, which is not written again: d_h and d_dh
+ * f32), taken before dh is rounded. dh may be grad or h itself; dbias may be
+ * NULL. With activation -1, dh is grad, which is not written again: h and dh
  * are not looked at. dx and dw are then the products' gradients with dh, and r's
  * gradient is grad. workspace() says how many bytes (16-byte aligned, not kept
  * after the work is done) long groups' sums are faster with. */
+typedef struct pxg_linear_grad {
+  int64_t type, bias_type, activation;
+  uint64_t rows, n, groups;
+  const void* grad;
+  uint64_t grad_stride;
+  const void* h;
+  uint64_t h_stride;
+  const int64_t* offsets;
+  void* dh;
+  uint64_t dh_stride;
+  void* dbias;
+  uint64_t dbias_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+} pxg_linear_grad;
 uint64_t pxg_grouped_linear_grad_workspace(uint64_t rows, uint64_t n, uint64_t groups);
-int pxg_grouped_linear_grad_device(int activation, int type, const void* d_grad, uint64_t rows, uint64_t n,
-                                   uint64_t grad_stride, const void* d_h, uint64_t h_stride, const int64_t* d_offsets,
-                                   uint64_t groups, void* d_dh, uint64_t dh_stride, int bias_type, void* d_dbias,
-                                   uint64_t dbias_stride, void* d_workspace, uint64_t workspace_bytes, void* stream);
+int pxg_grouped_linear_grad_device(const pxg_linear_grad* layer, void* stream);
 
 /* A whole expert layer for a few tokens:
- *   y_t = r_t + sum over j of gate_tj (W2_e (f(W1_e x_t + b1_e) * up_e x_t) + b2_e),   e = experts_tj
- * with matrices of `type` (f16 or bf16) or packed rows (`packed`; x is bf16),
- * out_type that type or f32. x is rows x k; d_experts and d_gates are rows of
- * `picks` (at most 16); an id outside [0, experts) is no expert, one that a token
- * has twice counts with both gates. w1 and up (NULL: without its factor) are
- * hidden x k of each expert, w2 n x hidden. `activation` is a pxg_activation or
- * -1 for f(h) = h. The biases (NULL: none) are rows of bias_type (`type` or f32),
- * d_residual (NULL: none) is r in out_type and may be y itself. Sums, and what is
- * between the two products, are held in f32 (for a 16-bit result to 2^-17).
- * Rows go in blocks of 64, for each of which the matrices of the experts in use
- * are read once; rows, experts <= 65536. The workspace, of the size that
- * workspace() says and 16-byte aligned, is not kept after the work is done. */
+ *   y_t = r_t + sum over j of gate_tj (W2_e (f(W1_e x_t + b1_e) * up_e x_t) + b2_e),   e = ids_tj
+ * with matrices of `type` (f16 or bf16) or packed rows (`packed` not 0; x is bf16),
+ * out_type that type or f32. x is rows x k; ids and gates are rows of `picks` (at
+ * most 16); an id outside [0, experts) is no expert, one that a token has twice
+ * counts with both gates. w1 and up (data NULL: without its factor) are hidden x k
+ * of each expert, w2 n x hidden. `activation` is a pxg_activation or -1 for f(h) =
+ * h. The biases (or NULL) are rows of bias_type (`type` or f32), `residual` (or
+ * NULL) is r in out_type and may be y itself. Sums, and what is between the two
+ * products, are held in f32 (for a 16-bit result to 2^-17). Rows go in blocks of
+ * 64, for each of which the matrices of the experts in use are read once; rows and
+ * experts <= 65536. The workspace, of the size that workspace() says and 16-byte
+ * aligned, is not kept after the work is done. */
 typedef struct pxg_expert_matrix {
-  const void* data;       /* the first expert's first row; packed: its codes */
-  uint64_t stride;        /* elements from row to row, and from expert to expert; */
-  uint64_t group_stride;  /* packed rows lie one after the other and these are not looked at */
-  const void* scales;     /* packed rows' scales, or NULL */
+  const void* data;                /* the first expert's first row; packed: its codes */
+  uint64_t stride, group_stride;   /* from row to row and from expert to expert; packed: not looked at */
+  const void* scales;              /* packed rows' scales */
 } pxg_expert_matrix;
+typedef struct pxg_expert_layer {
+  int64_t type, out_type, bias_type, activation, packed;
+  uint64_t rows, k, picks, experts, hidden, n;
+  const void* x;
+  uint64_t x_stride;
+  const int64_t* ids;
+  uint64_t ids_stride;
+  const float* gates;
+  uint64_t gates_stride;
+  pxg_expert_matrix w1, up, w2;
+  const void* bias1;
+  uint64_t bias1_stride;
+  const void* bias2;
+  uint64_t bias2_stride;
+  const void* residual;
+  uint64_t residual_stride;
+  void* y;
+  uint64_t y_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+} pxg_expert_layer;
 uint64_t pxg_expert_layer_workspace(uint64_t rows, uint64_t picks, uint64_t experts, uint64_t hidden, uint64_t n,
                                     int out_type);
-int pxg_expert_layer_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride,
-                            const int64_t* d_experts, uint64_t picks, uint64_t experts_stride, const float* d_gates,
-                            uint64_t gates_stride, uint64_t experts, uint64_t hidden, uint64_t n,
-                            const pxg_expert_matrix* w1, const pxg_expert_matrix* up, const pxg_expert_matrix* w2,
-                            int packed, int activation, int bias_type, const void* d_bias1, uint64_t bias1_stride,
-                            const void* d_bias2, uint64_t bias2_stride, int out_type, const void* d_residual,
-                            uint64_t residual_stride, void* d_y, uint64_t y_stride, void* d_workspace,
-                            uint64_t workspace_bytes, void* stream);
+int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream);
 
 /* The loss of a model trained to rank as a teacher does: p is the softmax of the
  * teacher's scores over T, q that of the model's logits over T, and
@@ -570,19 +612,30 @@ int pxg_expert_layer_device(int type, const void* d_x, uint64_t rows, uint64_t k
  * count (clamped to [0, top]) are looked at; those with an id outside [0, cols) are
  * left out. A row without entries, or whose scores are all -inf, has loss 0 and no
  * gradient; entries of p = 0 add nothing; a logit of -inf has q = 0. `weight` is
- * the loss' own gradient, one f32 a row. T lies between 1e-6 and 1e6. Sums are
+ * the loss' own gradient, one f32 a row; the loss alone looks at neither it nor dx. T lies between 1e-6 and 1e6. Sums are
  * held in f32. The workspace is of the size that workspace() says (0: none),
  * 16-byte aligned and not kept after the work is done. */
+typedef struct pxg_distill {
+  int64_t type;
+  uint64_t rows, cols, top;
+  const void* logits;
+  uint64_t logits_stride;
+  const int64_t* ids;
+  uint64_t ids_stride;
+  const float* scores;
+  uint64_t scores_stride;
+  const int32_t* counts;
+  double temperature;
+  float* loss;
+  const float* weight;
+  void* dx;
+  uint64_t dx_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+} pxg_distill;
 uint64_t pxg_distill_workspace(int type, uint64_t rows, uint64_t cols, uint64_t top);
-int pxg_distill_loss_device(int type, const void* d_logits, uint64_t rows, uint64_t cols, uint64_t logits_stride,
-                            const int64_t* d_ids, uint64_t ids_stride, const float* d_scores, uint64_t scores_stride,
-                            const int32_t* d_counts, uint64_t top, double temperature, float* d_loss,
-                            void* d_workspace, uint64_t workspace_bytes, void* stream);
-int pxg_distill_loss_grad_device(int type, const float* d_weight, const void* d_logits, uint64_t rows, uint64_t cols,
-                                 uint64_t logits_stride, const int64_t* d_ids, uint64_t ids_stride,
-                                 const float* d_scores, uint64_t scores_stride, const int32_t* d_counts, uint64_t top,
-                                 double temperature, float* d_loss, void* d_dx, uint64_t dx_stride, void* d_workspace,
-                                 uint64_t workspace_bytes, void* stream);
+int pxg_distill_loss_device(const pxg_distill* distill, void* stream);
+int pxg_distill_loss_grad_device(const pxg_distill* distill, void* stream);
 
 /* Which kernel the products of this thread take (for tests and tuning): 0 =
  * the one estimated fastest, 16 = that for few rows, 64, 128 or 256 = tiles of

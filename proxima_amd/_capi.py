@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libproxima_hip.so")
 
 _vp = C.c_void_p
 _u64 = C.c_uint64
+_i64 = C.c_int64
 _u32 = C.c_uint32
 _i32 = C.c_int
 _f32 = C.c_float
@@ -57,6 +58,46 @@ class IvfPqConfigC(C.Structure):
 
 class ExpertMatrixC(C.Structure):
     _fields_ = [("data", _vp), ("stride", _u64), ("group_stride", _u64), ("scales", _vp)]
+
+
+class LinearC(C.Structure):
+    _fields_ = [
+        ("type", _i64), ("out_type", _i64), ("bias_type", _i64), ("activation", _i64), ("rows", _u64),
+        ("k", _u64), ("groups", _u64), ("n", _u64), ("x", _vp), ("x_stride", _u64), ("w", _vp),
+        ("w_stride", _u64), ("w_group_stride", _u64), ("offsets", _vp), ("bias", _vp), ("bias_stride", _u64),
+        ("residual", _vp), ("residual_stride", _u64), ("h", _vp), ("h_stride", _u64), ("y", _vp),
+        ("y_stride", _u64), ("x_scales", _vp), ("w_scales", _vp),
+    ]
+
+
+class LinearGradC(C.Structure):
+    _fields_ = [
+        ("type", _i64), ("bias_type", _i64), ("activation", _i64), ("rows", _u64), ("n", _u64),
+        ("groups", _u64), ("grad", _vp), ("grad_stride", _u64), ("h", _vp), ("h_stride", _u64),
+        ("offsets", _vp), ("dh", _vp), ("dh_stride", _u64), ("dbias", _vp), ("dbias_stride", _u64),
+        ("workspace", _vp), ("workspace_bytes", _u64),
+    ]
+
+
+class ExpertLayerC(C.Structure):
+    _fields_ = [
+        ("type", _i64), ("out_type", _i64), ("bias_type", _i64), ("activation", _i64), ("packed", _i64),
+        ("rows", _u64), ("k", _u64), ("picks", _u64), ("experts", _u64), ("hidden", _u64), ("n", _u64),
+        ("x", _vp), ("x_stride", _u64), ("ids", _vp), ("ids_stride", _u64), ("gates", _vp),
+        ("gates_stride", _u64), ("w1", ExpertMatrixC), ("up", ExpertMatrixC), ("w2", ExpertMatrixC),
+        ("bias1", _vp), ("bias1_stride", _u64), ("bias2", _vp), ("bias2_stride", _u64), ("residual", _vp),
+        ("residual_stride", _u64), ("y", _vp), ("y_stride", _u64), ("workspace", _vp),
+        ("workspace_bytes", _u64),
+    ]
+
+
+class DistillC(C.Structure):
+    _fields_ = [
+        ("type", _i64), ("rows", _u64), ("cols", _u64), ("top", _u64), ("logits", _vp), ("logits_stride", _u64),
+        ("ids", _vp), ("ids_stride", _u64), ("scores", _vp), ("scores_stride", _u64), ("counts", _vp),
+        ("temperature", _f64), ("loss", _vp), ("weight", _vp), ("dx", _vp), ("dx_stride", _u64),
+        ("workspace", _vp), ("workspace_bytes", _u64),
+    ]
 
 
 class TrainingReportC(C.Structure):
@@ -179,22 +220,16 @@ SIGNATURES = {
     "pxg_grouped_matmul_grad_weight_block8_device": (_i32, [_vp, _u64, _u64, _u64, _vp, _vp, _u64, _vp, _u64, _i32,
                                                             _vp, _u64, _u64, _vp, _u64, _vp]),
     "pxg_grouped_matmul_grad_weight_workspace": (_u64, [_u64, _u64, _u64, _u64]),
-    "pxg_grouped_linear_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _u64, _u64, _vp, _i32, _vp,
-                                         _u64, _i32, _i32, _vp, _u64, _vp, _u64, _vp, _u64, _vp]),
-    "pxg_block8_linear_device": (_i32, [_vp, _vp, _u64, _u64, _vp, _vp, _u64, _u64, _vp, _i32, _vp, _u64, _i32, _i32,
-                                        _vp, _u64, _vp, _u64, _vp]),
+    # structs by address, or as bytes laid out alike
+    "pxg_grouped_linear_device": (_i32, [_vp, _vp]),
+    "pxg_block8_linear_device": (_i32, [_vp, _vp]),
     "pxg_grouped_linear_grad_workspace": (_u64, [_u64, _u64, _u64]),
-    "pxg_grouped_linear_grad_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _u64, _vp, _u64,
-                                              _i32, _vp, _u64, _vp, _u64, _vp]),
+    "pxg_grouped_linear_grad_device": (_i32, [_vp, _vp]),
     "pxg_expert_layer_workspace": (_u64, [_u64, _u64, _u64, _u64, _u64, _i32]),
-    "pxg_expert_layer_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _u64, _vp, _u64, _u64, _u64, _u64,
-                                       _P(ExpertMatrixC), _P(ExpertMatrixC), _P(ExpertMatrixC), _i32, _i32, _i32, _vp,
-                                       _u64, _vp, _u64, _i32, _vp, _u64, _vp, _u64, _vp, _u64, _vp]),
+    "pxg_expert_layer_device": (_i32, [_vp, _vp]),
     "pxg_distill_workspace": (_u64, [_i32, _u64, _u64, _u64]),
-    "pxg_distill_loss_device": (_i32, [_i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _u64, _vp, _u64, C.c_double, _vp, _vp,
-                                       _u64, _vp]),
-    "pxg_distill_loss_grad_device": (_i32, [_i32, _vp, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _u64, _vp, _u64, C.c_double,
-                                            _vp, _vp, _u64, _vp, _u64, _vp]),
+    "pxg_distill_loss_device": (_i32, [_vp, _vp]),
+    "pxg_distill_loss_grad_device": (_i32, [_vp, _vp]),
     "pxg_grouped_matmul_set_kernel": (_i32, [_i32]),
     "pxg_grouped_matmul_last_kernel": (_u32, []),
     "pxg_activation_pack_device": (_i32, [_i32, _i32, _vp, _u64, _u64, _u64, _vp, _u64, _vp, _vp, _vp]),

@@ -85,10 +85,10 @@ __device__ __forceinline__ void activate(float (&v)[N], int activation) {
 
 constexpr int NO_ACTIVATION = -1;
 
-inline void check_activation(int kind) {
+inline void check_activation(int64_t kind) {
   if (kind != PXG_SILU && kind != PXG_GELU) config_error("activation", (uint64_t)kind, "must be SiLU or GELU");
 }
-inline void check_optional_activation(int kind) {
+inline void check_optional_activation(int64_t kind) {
   if (kind != NO_ACTIVATION) check_activation(kind);
 }
 

@@ -468,56 +468,45 @@ void run_distill(Distill p, const DistillPlan& d, hipStream_t s) {
   }
 }
 
-void check_distill(int type, const void* d_x, uint64_t rows, uint64_t cols, uint64_t x_stride, const int64_t* d_ids,
-                   uint64_t ids_stride, const float* d_scores, uint64_t scores_stride, const int32_t* d_counts,
-                   uint64_t top, double temperature, const float* d_loss) {
-  check_type(type, true);
-  check_size("cols", cols);
-  if (top == 0 || top > TOP_MAX) config_error("top", top, "must be between 1 and 4096");
-  if (!(temperature >= 1e-6 && temperature <= 1e6))
-    config_error("temperature", 0, "must be between 1e-6 and 1e6");
-  check_rows(type, "logits", d_x, rows, cols, x_stride);
-  check_rows(PXG_F32, "ids", d_ids, rows, top, ids_stride);
-  check_aligned("ids", d_ids, 8);
-  check_rows(PXG_F32, "scores", d_scores, rows, top, scores_stride);
-  check_rows(PXG_F32, "counts", d_counts, rows, 1, 1);
-  check_rows(PXG_F32, "loss", d_loss, rows, 1, 1);
-}
-
-int distill(int type, const float* d_weight, const void* d_x, uint64_t rows, uint64_t cols, uint64_t x_stride,
-            const int64_t* d_ids, uint64_t ids_stride, const float* d_scores, uint64_t scores_stride,
-            const int32_t* d_counts, uint64_t top, double temperature, float* d_loss, bool grad, void* d_dx,
-            uint64_t dx_stride, void* d_workspace, uint64_t workspace_bytes, void* stream) {
+int distill(const pxg_distill& a, bool grad, void* stream) {
   return guard([&] {
-    check_distill(type, d_x, rows, cols, x_stride, d_ids, ids_stride, d_scores, scores_stride, d_counts, top,
-                  temperature, d_loss);
+    check_type(a.type, true);
+    check_size("cols", a.cols);
+    if (a.top == 0 || a.top > TOP_MAX) config_error("top", a.top, "must be between 1 and 4096");
+    if (!(a.temperature >= 1e-6 && a.temperature <= 1e6)) config_error("temperature", 0, "must be between 1e-6 and 1e6");
+    check_rows(a.type, "logits", a.logits, a.rows, a.cols, a.logits_stride);
+    check_rows(PXG_F32, "ids", a.ids, a.rows, a.top, a.ids_stride);
+    check_aligned("ids", a.ids, 8);
+    check_rows(PXG_F32, "scores", a.scores, a.rows, a.top, a.scores_stride);
+    check_rows(PXG_F32, "counts", a.counts, a.rows, 1, 1);
+    check_rows(PXG_F32, "loss", a.loss, a.rows, 1, 1);
     if (grad) {
-      check_rows(PXG_F32, "weight", d_weight, rows, 1, 1);
-      check_rows(type, "dx", d_dx, rows, cols, dx_stride);
+      check_rows(PXG_F32, "weight", a.weight, a.rows, 1, 1);
+      check_rows(a.type, "dx", a.dx, a.rows, a.cols, a.dx_stride);
     }
-    if (rows == 0) return;
-    const DistillPlan d = distill_plan(type, rows, cols, top);
-    check_aligned("workspace", d_workspace, 16);
-    if (d.bytes && (!d_workspace || workspace_bytes < d.bytes))
-      config_error("workspace_bytes", workspace_bytes, "must be what pxg_distill_workspace says");
+    if (a.rows == 0) return;
+    const DistillPlan d = distill_plan(a.type, a.rows, a.cols, a.top);
+    check_aligned("workspace", a.workspace, 16);
+    if (d.bytes && (!a.workspace || a.workspace_bytes < d.bytes))
+      config_error("workspace_bytes", a.workspace_bytes, "must be what pxg_distill_workspace says");
     Distill p{};
-    p.x = d_x;
-    p.dx = d_dx;
-    p.ids = d_ids;
-    p.scores = d_scores;
-    p.counts = d_counts;
-    p.weight = d_weight;
-    p.loss = d_loss;
-    p.xs = x_stride;
-    p.ds = dx_stride;
-    p.is = ids_stride;
-    p.ss = scores_stride;
-    p.sums = (float2*)d_workspace;
-    p.picked = (float*)((char*)d_workspace + rows * d.parts * sizeof(float2));
-    p.rows = rows;
-    p.cols = (int)cols;
-    p.top = (int)top;
-    const double c = 1.4426950408889634 / temperature, t = 1.0 / temperature;
+    p.x = a.logits;
+    p.dx = a.dx;
+    p.ids = a.ids;
+    p.scores = a.scores;
+    p.counts = a.counts;
+    p.weight = a.weight;
+    p.loss = a.loss;
+    p.xs = a.logits_stride;
+    p.ds = a.dx_stride;
+    p.is = a.ids_stride;
+    p.ss = a.scores_stride;
+    p.sums = (float2*)a.workspace;
+    p.picked = (float*)((char*)a.workspace + a.rows * d.parts * sizeof(float2));
+    p.rows = a.rows;
+    p.cols = (int)a.cols;
+    p.top = (int)a.top;
+    const double c = 1.4426950408889634 / a.temperature, t = 1.0 / a.temperature;
     p.c = (float)c;
     p.c_low = (float)(c - p.c);
     p.t = (float)t;
@@ -527,8 +516,8 @@ int distill(int type, const float* d_weight, const void* d_x, uint64_t rows, uin
       if (grad) run_distill<T, true>(p, d, (hipStream_t)stream);
       else run_distill<T, false>(p, d, (hipStream_t)stream);
     };
-    if (type == PXG_F32) run(float{});
-    else if (type == PXG_F16) run((_Float16)0);
+    if (a.type == PXG_F32) run(float{});
+    else if (a.type == PXG_F16) run((_Float16)0);
     else run((__bf16)0.0f);
   });
 }
@@ -545,21 +534,7 @@ uint64_t pxg_distill_workspace(int type, uint64_t rows, uint64_t cols, uint64_t 
   return distill_plan(type, rows, cols, top).bytes;
 }
 
-int pxg_distill_loss_device(int type, const void* d_logits, uint64_t rows, uint64_t cols, uint64_t logits_stride,
-                            const int64_t* d_ids, uint64_t ids_stride, const float* d_scores, uint64_t scores_stride,
-                            const int32_t* d_counts, uint64_t top, double temperature, float* d_loss,
-                            void* d_workspace, uint64_t workspace_bytes, void* stream) {
-  return distill(type, nullptr, d_logits, rows, cols, logits_stride, d_ids, ids_stride, d_scores, scores_stride,
-                 d_counts, top, temperature, d_loss, false, nullptr, 0, d_workspace, workspace_bytes, stream);
-}
-
-int pxg_distill_loss_grad_device(int type, const float* d_weight, const void* d_logits, uint64_t rows, uint64_t cols,
-                                 uint64_t logits_stride, const int64_t* d_ids, uint64_t ids_stride,
-                                 const float* d_scores, uint64_t scores_stride, const int32_t* d_counts, uint64_t top,
-                                 double temperature, float* d_loss, void* d_dx, uint64_t dx_stride, void* d_workspace,
-                                 uint64_t workspace_bytes, void* stream) {
-  return distill(type, d_weight, d_logits, rows, cols, logits_stride, d_ids, ids_stride, d_scores, scores_stride,
-                 d_counts, top, temperature, d_loss, true, d_dx, dx_stride, d_workspace, workspace_bytes, stream);
-}
+int pxg_distill_loss_device(const pxg_distill* a, void* stream) { return distill(*a, false, stream); }
+int pxg_distill_loss_grad_device(const pxg_distill* a, void* stream) { return distill(*a, true, stream); }
 
 }  // extern "C"

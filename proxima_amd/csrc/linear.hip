@@ -168,29 +168,27 @@ void launch_grad(int activation, const LinearGrad& p, const GradPlan& g, hipStre
 }
 
 // `name` must be a string literal.
-void check_bias(const char* name, int type, int bias_type, const void* bias, uint64_t groups, uint64_t n,
+void check_bias(const char* name, int type, int64_t bias_type, const void* bias, uint64_t groups, uint64_t n,
                 uint64_t stride) {
   if (!bias) return;
   if (bias_type != type && bias_type != PXG_F32)
     config_error("bias_type", (uint64_t)bias_type, "must be the operands' type or f32");
   check_rows(bias_type, name, bias, groups, n, stride);
 }
-// The epilogue's part of a product whose result is of out_type.
-void set_epilogue(LinearProduct& p, int type, int out_type, uint64_t rows, uint64_t n, uint64_t groups, int bias_type,
-                  const void* d_bias, uint64_t bias_stride, int activation, const void* d_residual,
-                  uint64_t residual_stride, void* d_h, uint64_t h_stride) {
-  check_bias("bias", type, bias_type, d_bias, groups, n, bias_stride);
-  check_optional_activation(activation);
-  if (d_residual) check_rows(out_type, "residual", d_residual, rows, n, residual_stride);
-  if (d_h) check_rows(out_type, "h", d_h, rows, n, h_stride);
-  p.bias = d_bias;
-  p.bias_stride = bias_stride;
-  p.bias_f32 = bias_type == PXG_F32;
-  p.activation = activation;
-  p.residual = d_residual;
-  p.rs = residual_stride;
-  p.kept = d_h;
-  p.hs = h_stride;
+// The epilogue's part of a product of operands of `type`.
+void set_epilogue(LinearProduct& p, const pxg_linear& a, int type, void* h) {
+  check_bias("bias", type, a.bias_type, a.bias, a.groups, a.n, a.bias_stride);
+  check_optional_activation(a.activation);
+  if (a.residual) check_rows(a.out_type, "residual", a.residual, a.rows, a.n, a.residual_stride);
+  if (h) check_rows(a.out_type, "h", h, a.rows, a.n, a.h_stride);
+  p.bias = a.bias;
+  p.bias_stride = a.bias_stride;
+  p.bias_f32 = a.bias_type == PXG_F32;
+  p.activation = (int)a.activation;
+  p.residual = a.residual;
+  p.rs = a.residual_stride;
+  p.kept = h;
+  p.hs = a.h_stride;
 }
 
 }  // namespace
@@ -200,54 +198,45 @@ using namespace pxg;
 
 extern "C" {
 
-int pxg_grouped_linear_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride, const void* d_w,
-                              uint64_t groups, uint64_t n, uint64_t w_stride, uint64_t w_group_stride,
-                              const int64_t* d_offsets, int bias_type, const void* d_bias, uint64_t bias_stride,
-                              int activation, int out_type, const void* d_residual, uint64_t residual_stride,
-                              void* d_h, uint64_t h_stride, void* d_y, uint64_t y_stride, void* stream) {
+int pxg_grouped_linear_device(const pxg_linear* layer, void* stream) {
   return guard([&] {
-    check_type(type, false);
-    check_out_type(type, out_type);
-    check_size("k", k);
-    check_size("n", n);
-    check_groups(groups, d_offsets);
-    check_rows(type, "x", d_x, rows, k, x_stride);
-    check_rows(type, "w", d_w, n, k, w_stride);
-    check_rows(out_type, "y", d_y, rows, n, y_stride);
-    x_stride = check_stride(rows, k, x_stride);
-    w_stride = check_stride(n, k, w_stride);
-    LinearProduct p{{d_x, d_w, d_y, d_offsets, x_stride, w_stride, y_stride, w_group_stride, 0, nullptr, nullptr, 0,
-                     (int)rows, (int)groups, (int)rows, (int)n, (int)k, false}};
-    set_epilogue(p, type, out_type, rows, n, groups, bias_type, d_bias, bias_stride, activation, d_residual,
-                 residual_stride, d_h, h_stride);
-    if (rows == 0) return;
-    run_product<FORWARD>(type, out_type, p, (hipStream_t)stream);
+    const pxg_linear& a = *layer;
+    check_type(a.type, false);
+    check_out_type(a.type, a.out_type);
+    check_size("k", a.k);
+    check_size("n", a.n);
+    check_groups(a.groups, a.offsets);
+    check_rows(a.type, "x", a.x, a.rows, a.k, a.x_stride);
+    check_rows(a.type, "w", a.w, a.n, a.k, a.w_stride);
+    check_rows(a.out_type, "y", a.y, a.rows, a.n, a.y_stride);
+    LinearProduct p{{a.x, a.w, a.y, a.offsets, check_stride(a.rows, a.k, a.x_stride), check_stride(a.n, a.k, a.w_stride),
+                     a.y_stride, a.w_group_stride, 0, nullptr, nullptr, 0, (int)a.rows, (int)a.groups, (int)a.rows,
+                     (int)a.n, (int)a.k, false}};
+    set_epilogue(p, a, a.type, a.h);
+    if (a.rows == 0) return;
+    run_product<FORWARD>(a.type, a.out_type, p, (hipStream_t)stream);
   });
 }
 
-int pxg_block8_linear_device(const void* d_codes, const void* d_scales, uint64_t rows, uint64_t k,
-                             const void* d_w_codes, const void* d_w_scales, uint64_t groups, uint64_t n,
-                             const int64_t* d_offsets, int bias_type, const void* d_bias, uint64_t bias_stride,
-                             int activation, int out_type, const void* d_residual, uint64_t residual_stride,
-                             void* d_y, uint64_t y_stride, void* stream) {
+int pxg_block8_linear_device(const pxg_linear* layer, void* stream) {
   return guard([&] {
-    check_type(out_type, true);
-    check_size("k", k);
-    check_size("n", n);
-    check_groups(groups, d_offsets);
-    check_packed_rows("codes", d_codes, "scales", d_scales, rows);
-    check_packed_rows("w_codes", d_w_codes, "w_scales", d_w_scales, n);
-    check_rows(out_type, "y", d_y, rows, n, y_stride);
-    const uint64_t wide = check_stride(2, k, block8_code_stride(k));
-    LinearProduct p{{d_codes, d_w_codes, d_y, d_offsets, wide, wide, y_stride, n * wide, 0, (const uint8_t*)d_scales,
-                     (const uint8_t*)d_w_scales, block8_scale_stride(k), (int)rows, (int)groups, (int)rows, (int)n,
-                     (int)wide, false}};
-    set_epilogue(p, PXG_BF16, out_type, rows, n, groups, bias_type, d_bias, bias_stride, activation, d_residual,
-                 residual_stride, nullptr, 0);
-    if (rows == 0) return;
+    const pxg_linear& a = *layer;
+    check_type(a.out_type, true);
+    check_size("k", a.k);
+    check_size("n", a.n);
+    check_groups(a.groups, a.offsets);
+    check_packed_rows("x", a.x, "x_scales", a.x_scales, a.rows);
+    check_packed_rows("w", a.w, "w_scales", a.w_scales, a.n);
+    check_rows(a.out_type, "y", a.y, a.rows, a.n, a.y_stride);
+    const uint64_t wide = check_stride(2, a.k, block8_code_stride(a.k));
+    LinearProduct p{{a.x, a.w, a.y, a.offsets, wide, wide, a.y_stride, a.n * wide, 0, (const uint8_t*)a.x_scales,
+                     (const uint8_t*)a.w_scales, block8_scale_stride(a.k), (int)a.rows, (int)a.groups, (int)a.rows,
+                     (int)a.n, (int)wide, false}};
+    set_epilogue(p, a, PXG_BF16, nullptr);
+    if (a.rows == 0) return;
     const hipStream_t s = (hipStream_t)stream;
-    if (out_type == PXG_F32) launch_product<FORWARD, __bf16, float, true>(p, 0, s);
-    else if (out_type == PXG_F16) launch_product<FORWARD, __bf16, _Float16, true>(p, 0, s);
+    if (a.out_type == PXG_F32) launch_product<FORWARD, __bf16, float, true>(p, 0, s);
+    else if (a.out_type == PXG_F16) launch_product<FORWARD, __bf16, _Float16, true>(p, 0, s);
     else launch_product<FORWARD, __bf16, __bf16, true>(p, 0, s);
   });
 }
@@ -258,36 +247,34 @@ uint64_t pxg_grouped_linear_grad_workspace(uint64_t rows, uint64_t n, uint64_t g
   return grad_plan(rows, n, groups, true).bytes;
 }
 
-int pxg_grouped_linear_grad_device(int activation, int type, const void* d_grad, uint64_t rows, uint64_t n,
-                                   uint64_t grad_stride, const void* d_h, uint64_t h_stride, const int64_t* d_offsets,
-                                   uint64_t groups, void* d_dh, uint64_t dh_stride, int bias_type, void* d_dbias,
-                                   uint64_t dbias_stride, void* d_workspace, uint64_t workspace_bytes, void* stream) {
+int pxg_grouped_linear_grad_device(const pxg_linear_grad* layer, void* stream) {
   return guard([&] {
-    check_type(type, true);
-    check_optional_activation(activation);
-    check_size("n", n);
-    check_groups(groups, d_offsets);
-    check_rows(type, "grad", d_grad, rows, n, grad_stride);
-    const bool slope = activation != NO_ACTIVATION;
+    const pxg_linear_grad& a = *layer;
+    check_type(a.type, true);
+    check_optional_activation(a.activation);
+    check_size("n", a.n);
+    check_groups(a.groups, a.offsets);
+    check_rows(a.type, "grad", a.grad, a.rows, a.n, a.grad_stride);
+    const bool slope = a.activation != NO_ACTIVATION;
     if (slope) {
-      check_rows(type, "h", d_h, rows, n, h_stride);
-      check_rows(type, "dh", d_dh, rows, n, dh_stride);
+      check_rows(a.type, "h", a.h, a.rows, a.n, a.h_stride);
+      check_rows(a.type, "dh", a.dh, a.rows, a.n, a.dh_stride);
     }
-    check_bias("dbias", type, bias_type, d_dbias, groups, n, dbias_stride);
-    check_aligned("workspace", d_workspace, 16);
-    if (!slope && !d_dbias) return;
-    LinearGrad p{d_grad, d_h, d_dh, d_dbias, d_offsets, grad_stride, h_stride, dh_stride, dbias_stride,
-                 (float*)d_workspace, (int)rows, (int)n, (int)groups, 0, 0};
-    GradPlan g = grad_plan(rows, n, groups, d_offsets != nullptr);
-    if (!d_dbias || (d_workspace && workspace_bytes >= g.bytes)) p.tile = g.tile;
+    check_bias("dbias", a.type, a.bias_type, a.dbias, a.groups, a.n, a.dbias_stride);
+    check_aligned("workspace", a.workspace, 16);
+    if (!slope && !a.dbias) return;
+    LinearGrad p{a.grad, a.h, a.dh, a.dbias, a.offsets, a.grad_stride, a.h_stride, a.dh_stride, a.dbias_stride,
+                 (float*)a.workspace, (int)a.rows, (int)a.n, (int)a.groups, 0, 0};
+    const GradPlan g = grad_plan(a.rows, a.n, a.groups, a.offsets != nullptr);
+    if (!a.dbias || (a.workspace && a.workspace_bytes >= g.bytes)) p.tile = g.tile;
     p.x = (int)g.x;
-    const bool vec = rows_aligned(type, d_grad, grad_stride) &&
-                     (!slope || (rows_aligned(type, d_h, h_stride) && rows_aligned(type, d_dh, dh_stride)));
-    by_type(type, vec, [&](auto t, auto v) {
+    const bool vec = rows_aligned(a.type, a.grad, a.grad_stride) &&
+                     (!slope || (rows_aligned(a.type, a.h, a.h_stride) && rows_aligned(a.type, a.dh, a.dh_stride)));
+    by_type(a.type, vec, [&](auto t, auto v) {
       using T = decltype(t);
       constexpr bool V = decltype(v)::value;
-      if (bias_type == PXG_F32) launch_grad<T, float, V>(activation, p, g, (hipStream_t)stream);
-      else launch_grad<T, T, V>(activation, p, g, (hipStream_t)stream);
+      if (a.bias_type == PXG_F32) launch_grad<T, float, V>(a.activation, p, g, (hipStream_t)stream);
+      else launch_grad<T, T, V>(a.activation, p, g, (hipStream_t)stream);
     });
   });
 }

@@ -991,7 +991,7 @@ void check_groups(uint64_t groups, const int64_t* offsets) {
   if (!offsets && groups != 1) config_error("groups", groups, "must be 1 without offsets");
   check_aligned("offsets", offsets, 8);
 }
-void check_out_type(int type, int out_type) {
+void check_out_type(int64_t type, int64_t out_type) {
   if (out_type != type && out_type != PXG_F32)
     config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
 }

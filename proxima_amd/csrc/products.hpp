@@ -11,7 +11,7 @@ constexpr uint64_t PRODUCT_SIZE_MAX = (1ull << 31) - 1024;
 
 inline uint64_t type_bytes(int type) { return type == PXG_F32 ? 4 : 2; }
 
-inline void check_type(int type, bool f32) {
+inline void check_type(int64_t type, bool f32) {
   if (type != PXG_F16 && type != PXG_BF16 && !(f32 && type == PXG_F32))
     config_error("type", (uint64_t)type, f32 ? "must be f32, f16 or bf16" : "must be f16 or bf16");
 }

@@ -592,93 +592,88 @@ uint64_t pxg_expert_layer_workspace(uint64_t rows, uint64_t picks, uint64_t expe
   return workspace_bytes_of(tokens_plan(rows, picks, experts, hidden, n, out_type == PXG_F32));
 }
 
-int pxg_expert_layer_device(int type, const void* d_x, uint64_t rows, uint64_t k, uint64_t x_stride,
-                            const int64_t* d_experts, uint64_t picks, uint64_t experts_stride, const float* d_gates,
-                            uint64_t gates_stride, uint64_t experts, uint64_t hidden, uint64_t n,
-                            const pxg_expert_matrix* w1, const pxg_expert_matrix* up, const pxg_expert_matrix* w2,
-                            int packed, int activation, int bias_type, const void* d_bias1, uint64_t bias1_stride,
-                            const void* d_bias2, uint64_t bias2_stride, int out_type, const void* d_residual,
-                            uint64_t residual_stride, void* d_y, uint64_t y_stride, void* d_workspace,
-                            uint64_t workspace_bytes, void* stream) {
+int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream) {
   return guard([&] {
-    check_type(type, false);
-    if (packed && type != PXG_BF16) config_error("type", (uint64_t)type, "must be bf16 with packed matrices");
-    if (out_type != type && out_type != PXG_F32)
-      config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
-    check_tokens(rows, picks, experts);
-    check_width("k", k);
-    check_width("hidden", hidden);
-    check_size("n", n);
-    check_optional_activation(activation);
-    check_rows(type, "x", d_x, rows, k, x_stride);
-    check_rows(PXG_F32, "gates", d_gates, rows, picks, gates_stride);
-    check_rows(PXG_F32, "experts", d_experts, rows, picks, experts_stride);
-    check_aligned("experts", d_experts, 8);
-    x_stride = check_stride(rows, k, x_stride);
-    auto matrix = [&](const char* name, const pxg_expert_matrix* m, uint64_t height, uint64_t width) {
-      if (!m || !m->data) config_error(name, 0, "must not be null");
+    const pxg_expert_layer& a = *layer;
+    const bool packed = a.packed != 0;
+    check_type(a.type, false);
+    if (packed && a.type != PXG_BF16) config_error("type", (uint64_t)a.type, "must be bf16 with packed matrices");
+    if (a.out_type != a.type && a.out_type != PXG_F32)
+      config_error("out_type", (uint64_t)a.out_type, "must be the operands' type or f32");
+    check_tokens(a.rows, a.picks, a.experts);
+    check_width("k", a.k);
+    check_width("hidden", a.hidden);
+    check_size("n", a.n);
+    check_optional_activation(a.activation);
+    check_rows(a.type, "x", a.x, a.rows, a.k, a.x_stride);
+    check_rows(PXG_F32, "gates", a.gates, a.rows, a.picks, a.gates_stride);
+    check_rows(PXG_F32, "ids", a.ids, a.rows, a.picks, a.ids_stride);
+    check_aligned("ids", a.ids, 8);
+    auto matrix = [&](const char* name, const pxg_expert_matrix& m, uint64_t height, uint64_t width) {
+      if (!m.data) config_error(name, 0, "must not be null");
       if (packed) {
-        check_packed_rows(name, m->data, name, m->scales, height);
+        check_packed_rows(name, m.data, name, m.scales, height);
         const uint64_t wide = check_stride(2, width, block8_code_stride(width));
-        return ExpertMatrix{m->data, wide, height * wide, (const uint8_t*)m->scales, block8_scale_stride(width)};
+        return ExpertMatrix{m.data, wide, height * wide, (const uint8_t*)m.scales, block8_scale_stride(width)};
       }
-      check_rows(type, name, m->data, height, width, m->stride);
-      return ExpertMatrix{m->data, check_stride(height, width, m->stride), m->group_stride, nullptr, 0};
+      check_rows(a.type, name, m.data, height, width, m.stride);
+      return ExpertMatrix{m.data, check_stride(height, width, m.stride), m.group_stride, nullptr, 0};
     };
     TokenLayer p{};
-    p.w1 = matrix("w1", w1, hidden, k);
-    if (up) p.up = matrix("up", up, hidden, k);
-    p.w2 = matrix("w2", w2, n, hidden);
-    if (d_bias1 || d_bias2) {
-      if (bias_type != type && bias_type != PXG_F32)
-        config_error("bias_type", (uint64_t)bias_type, "must be the operands' type or f32");
-      if (d_bias1) check_rows(bias_type, "bias1", d_bias1, experts, hidden, bias1_stride);
-      if (d_bias2) check_rows(bias_type, "bias2", d_bias2, experts, n, bias2_stride);
+    p.w1 = matrix("w1", a.w1, a.hidden, a.k);
+    if (a.up.data) p.up = matrix("up", a.up, a.hidden, a.k);
+    p.w2 = matrix("w2", a.w2, a.n, a.hidden);
+    if (a.bias1 || a.bias2) {
+      if (a.bias_type != a.type && a.bias_type != PXG_F32)
+        config_error("bias_type", (uint64_t)a.bias_type, "must be the operands' type or f32");
+      if (a.bias1) check_rows(a.bias_type, "bias1", a.bias1, a.experts, a.hidden, a.bias1_stride);
+      if (a.bias2) check_rows(a.bias_type, "bias2", a.bias2, a.experts, a.n, a.bias2_stride);
     }
-    if (d_residual) check_rows(out_type, "residual", d_residual, rows, n, residual_stride);
-    check_rows(out_type, "y", d_y, rows, n, y_stride);
-    if (rows == 0) return;
-    const TokensPlan t = tokens_plan(rows, picks, experts, hidden, n, out_type == PXG_F32);
-    check_aligned("workspace", d_workspace, 16);
-    if (!d_workspace || workspace_bytes < workspace_bytes_of(t))
-      config_error("workspace_bytes", workspace_bytes, "must be what pxg_expert_layer_workspace says");
-    p.x = d_x;
-    p.xs = x_stride;
-    p.ids = d_experts;
-    p.gates = d_gates;
-    p.is = experts_stride;
-    p.gs = gates_stride;
-    p.bias1 = d_bias1;
-    p.bias2 = d_bias2;
-    p.b1s = bias1_stride;
-    p.b2s = bias2_stride;
-    p.residual = d_residual;
-    p.rs = residual_stride;
-    p.y = d_y;
-    p.ys = y_stride;
-    p.planes = (char*)d_workspace;
+    if (a.residual) check_rows(a.out_type, "residual", a.residual, a.rows, a.n, a.residual_stride);
+    check_rows(a.out_type, "y", a.y, a.rows, a.n, a.y_stride);
+    p.xs = check_stride(a.rows, a.k, a.x_stride);
+    if (a.rows == 0) return;
+    const TokensPlan t = tokens_plan(a.rows, a.picks, a.experts, a.hidden, a.n, a.out_type == PXG_F32);
+    check_aligned("workspace", a.workspace, 16);
+    if (!a.workspace || a.workspace_bytes < workspace_bytes_of(t))
+      config_error("workspace_bytes", a.workspace_bytes, "must be what pxg_expert_layer_workspace says");
+    p.x = a.x;
+    p.ids = a.ids;
+    p.gates = a.gates;
+    p.is = a.ids_stride;
+    p.gs = a.gates_stride;
+    p.bias1 = a.bias1;
+    p.bias2 = a.bias2;
+    p.b1s = a.bias1_stride;
+    p.b2s = a.bias2_stride;
+    p.residual = a.residual;
+    p.rs = a.residual_stride;
+    p.y = a.y;
+    p.ys = a.y_stride;
+    p.planes = (char*)a.workspace;
     p.entries = (Entry*)(p.planes + t.planes_bytes);
     p.partial = (float*)(p.planes + t.planes_bytes + t.entries_bytes);
-    p.rows = (int)rows;
-    p.k = (int)k;
-    p.hidden = (int)hidden;
+    p.rows = (int)a.rows;
+    p.k = (int)a.k;
+    p.hidden = (int)a.hidden;
     p.wide = (int)t.wide;
-    p.n = (int)n;
-    p.picks = (int)picks;
-    p.experts = (int)experts;
+    p.n = (int)a.n;
+    p.picks = (int)a.picks;
+    p.experts = (int)a.experts;
     p.entries_max = (int)t.entries_max;
     p.slices = t.slices;
-    p.activation = activation;
-    p.bias_f32 = bias_type == PXG_F32;
+    p.activation = (int)a.activation;
+    p.bias_f32 = a.bias_type == PXG_F32;
     const hipStream_t s = (hipStream_t)stream;
+    const bool f32_out = a.out_type == PXG_F32;
     if (packed) {
-      if (out_type == PXG_F32) run_tokens<__bf16, true, float>(p, t, s);
+      if (f32_out) run_tokens<__bf16, true, float>(p, t, s);
       else run_tokens<__bf16, true, __bf16>(p, t, s);
-    } else if (type == PXG_F16) {
-      if (out_type == PXG_F32) run_tokens<_Float16, false, float>(p, t, s);
+    } else if (a.type == PXG_F16) {
+      if (f32_out) run_tokens<_Float16, false, float>(p, t, s);
       else run_tokens<_Float16, false, _Float16>(p, t, s);
     } else {
-      if (out_type == PXG_F32) run_tokens<__bf16, false, float>(p, t, s);
+      if (f32_out) run_tokens<__bf16, false, float>(p, t, s);
       else run_tokens<__bf16, false, __bf16>(p, t, s);
     }
   });

@@ -17,9 +17,11 @@ gradient is lost unseen; inside torch.no_grad() and a torch.autograd.Function
 it is off.
 """
 import sys
+from functools import lru_cache as _lru_cache
+from struct import Struct as _Struct
 
 from . import DimensionMismatch, _check
-from ._capi import ExpertMatrixC as _ExpertMatrix, lib as _lib
+from ._capi import lib as _lib
 
 __all__ = [
     "Block8", "block8_pack", "block8_unpack", "block8_matmul", "grouped_matmul", "grouped_matmul_grad_input",
@@ -146,6 +148,10 @@ def _stride(t):
     return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
 
 
+_NO_HISTORY = ("an operand requires grad, but no history is recorded here: call the gradients' own functions, under "
+               "torch.no_grad() or from a torch.autograd.Function")
+
+
 def _run(fn, tensors, *args):
     """fn(*args, stream) on torch's current stream of the device that all tensors share."""
     device = tensors[0].get_device()
@@ -154,8 +160,7 @@ def _run(fn, tensors, *args):
             if t.get_device() != device:
                 raise ValueError("operands must be on one device")
             if t.requires_grad and _torch.is_grad_enabled():
-                raise ValueError("an operand requires grad, but no history is recorded here: call the gradients' own "
-                                 "functions, under torch.no_grad() or from a torch.autograd.Function")
+                raise ValueError(_NO_HISTORY)
     if _current_device() == device:
         status = fn(*args, _current_stream(device))
     else:
@@ -314,30 +319,81 @@ def grouped_matmul_grad_weight(grad, x, offsets, out_dtype=None, out=None):
     return out
 
 
-def _bias(bias, offsets, groups, n, dtype):
-    """(tensor, pointer, pxg_type, elements from group to group) of a bias of `dtype` or f32: [groups, n], or [n]
-    without offsets."""
+# The C structs' arguments, 8 bytes each: packing them as bytes takes a third of the time of 20 converted one by one.
+_LINEAR, _LINEAR_GRAD, _EXPERT_LAYER, _DISTILL = map(_Struct, ("4q20Q", "3q14Q", "5q34Q", "q10Qd6Q"))
+
+
+def _rows(t, name, dims=2):
+    """Checks a GPU tensor of contiguous rows; (shape, elements from row to row)."""
+    if not getattr(t, "is_cuda", False):
+        raise ValueError(f"{name} must be a GPU tensor")
+    shape, strides = t.shape, t.stride()
+    if len(strides) != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, got {len(strides)}")
+    if strides[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name} must have contiguous rows")
+    return shape, strides[-2] if shape[-2] > 1 else shape[-1]
+
+
+def _call(fn, tensors, args):
+    """fn(struct, stream) on torch's current stream of the device that all tensors share."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("operands must be on one device")
+        if t.requires_grad and _torch.is_grad_enabled():
+            raise ValueError(_NO_HISTORY)
+    if _current_device() == device:
+        status = fn(args, _current_stream(device))
+    else:
+        with _torch.cuda.device(device):
+            status = fn(args, _current_stream(device))
+    if status:
+        _check(status)
+
+
+def _bias(bias, name, rows, n, dtype, tensors):
+    """(pointer, pxg_type, elements from row to row) of a bias [rows, n] of `dtype` or f32, [n] where rows is None."""
     if bias is None:
-        return None, None, 0, 0
-    if offsets is None and bias.dim() == 1:
-        bias = bias.unsqueeze(0)
-    shape = _matrix(bias, "bias")
-    if shape != (groups, n):
-        _mismatch(tuple(shape), (groups, n), "bias' shape")
-    if bias.dtype is not dtype and bias.dtype is not _torch.float32:
-        raise ValueError(f"bias must be {dtype} or float32, got {bias.dtype}")
-    return bias, bias.data_ptr(), _KINDS[bias.dtype], _stride(bias)
+        return 0, 0, 0
+    if rows is None:
+        rows = 1
+        if bias.dim() == 1:
+            bias = bias.unsqueeze(0)
+    shape, stride = _rows(bias, name)
+    if shape != (rows, n):
+        _mismatch(tuple(shape), (rows, n), f"{name}'s shape")
+    kind = bias.dtype
+    if kind is not dtype and kind is not _torch.float32:
+        raise ValueError(f"{name} must be {dtype} or float32, got {kind}")
+    tensors.append(bias)
+    return bias.data_ptr(), _KINDS[kind], stride
 
 
-def _residual(residual, shape, dtype):
+def _residual(residual, shape, dtype, tensors):
     """(pointer, elements from row to row)"""
     if residual is None:
-        return None, 0
-    if _matrix(residual, "residual") != shape:
-        _mismatch(tuple(residual.shape), tuple(shape), "residual's shape")
+        return 0, 0
+    got, stride = _rows(residual, "residual")
+    if got != shape:
+        _mismatch(tuple(got), shape, "residual's shape")
     if residual.dtype is not dtype:
         raise ValueError(f"residual must be {dtype}, got {residual.dtype}")
-    return residual.data_ptr(), _stride(residual)
+    tensors.append(residual)
+    return residual.data_ptr(), stride
+
+
+def _result(out, shape, dtype, like, tensors):
+    """(tensor, elements from row to row)"""
+    if out is None:
+        return like.new_empty(shape, dtype=dtype), shape[-1]
+    got, stride = _rows(out, "out", len(shape))
+    if got != shape:
+        _mismatch(tuple(got), shape, "out's shape")
+    if out.dtype is not dtype:
+        raise ValueError(f"out must be {dtype}, got {out.dtype}")
+    tensors.append(out)
+    return out, stride
 
 
 def _optional(activation):
@@ -349,20 +405,23 @@ def grouped_linear(x, w, offsets=None, bias=None, activation=None, residual=None
     them, bias [groups, n] (or [n] without offsets) in x's type or f32, f "silu", "gelu" or None, residual [rows, n]
     in y's type. `out` may be the residual itself. With keep, (y, h), h in y's type for grouped_linear_grad. y is
     rounded once, from the unrounded h. Rows of no group: y is the residual, or zeros, and h zeros."""
-    rows, xk = _matrix(x, "x")
-    kind = _type(x.dtype, "x", False)
+    (rows, xk), x_stride = _rows(x, "x")
+    xtype = x.dtype
+    kind = _type(xtype, "x", False)
     w, ptr, groups, n, k = _weights(w, offsets, x)
     if xk != k:
         _mismatch(xk, k, "x's columns")
-    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    tensors = [x, w] if offsets is None else [x, w, offsets]
+    dtype = out_dtype or (out.dtype if out is not None else xtype)
     out_kind, which = _type(dtype, "out_dtype"), _optional(activation)
-    bias, bias_ptr, bias_kind, bias_stride = _bias(bias, offsets, groups, n, x.dtype)
-    r, r_stride = _residual(residual, (rows, n), dtype)
-    out, stride = _out(out, (rows, n), dtype, x)
+    bias_ptr, bias_kind, bias_stride = _bias(bias, "bias", None if offsets is None else groups, n, xtype, tensors)
+    r, r_stride = _residual(residual, (rows, n), dtype, tensors)
+    out, stride = _result(out, (rows, n), dtype, x, tensors)
     h = x.new_empty((rows, n), dtype=dtype) if keep else None
-    _run(_lib.pxg_grouped_linear_device, (x, w, offsets, bias, residual, out), kind, x.data_ptr(), rows, k, _stride(x),
-         w.data_ptr(), groups, n, _stride(w), w.stride(0), ptr, bias_kind, bias_ptr, bias_stride, which, out_kind, r,
-         r_stride, h.data_ptr() if keep else None, n, out.data_ptr(), stride)
+    _call(_lib.pxg_grouped_linear_device, tensors,
+          _LINEAR.pack(kind, out_kind, bias_kind, which, rows, k, groups, n, x.data_ptr(), x_stride, w.data_ptr(),
+                       _stride(w), w.stride(0), ptr or 0, bias_ptr, bias_stride, r, r_stride,
+                       h.data_ptr() if keep else 0, n, out.data_ptr(), stride, 0, 0))
     return (out, h) if keep else out
 
 
@@ -371,15 +430,22 @@ def block8_linear(x, w, offsets=None, bias=None, activation=None, residual=None,
     does, bias bf16 or f32, the rest as grouped_linear."""
     codes, scales, rows, k = _packed(x, "x")
     wcodes, wscales, groups, n, ptr = _packed_weights(w, offsets, k)
+    tensors = [codes, scales, wcodes, wscales]
+    if offsets is not None:
+        tensors.append(offsets)
     dtype = out_dtype or (out.dtype if out is not None else _torch.bfloat16)
     out_kind, which = _type(dtype, "out_dtype"), _optional(activation)
-    bias, bias_ptr, bias_kind, bias_stride = _bias(bias, offsets, groups, n, _torch.bfloat16)
-    r, r_stride = _residual(residual, (rows, n), dtype)
-    out, stride = _out(out, (rows, n), dtype, codes)
-    _run(_lib.pxg_block8_linear_device, (codes, scales, wcodes, wscales, offsets, bias, residual, out),
-         codes.data_ptr(), scales.data_ptr(), rows, k, wcodes.data_ptr(), wscales.data_ptr(), groups, n, ptr,
-         bias_kind, bias_ptr, bias_stride, which, out_kind, r, r_stride, out.data_ptr(), stride)
+    bias_ptr, bias_kind, bias_stride = _bias(bias, "bias", None if offsets is None else groups, n, _torch.bfloat16, tensors)
+    r, r_stride = _residual(residual, (rows, n), dtype, tensors)
+    out, stride = _result(out, (rows, n), dtype, codes, tensors)
+    _call(_lib.pxg_block8_linear_device, tensors,
+          _LINEAR.pack(0, out_kind, bias_kind, which, rows, k, groups, n, codes.data_ptr(), 0, wcodes.data_ptr(), 0, 0,
+                       ptr or 0, bias_ptr, bias_stride, r, r_stride, 0, 0, out.data_ptr(), stride, scales.data_ptr(),
+                       wscales.data_ptr()))
     return out
+
+
+_grad_space = _lru_cache(1024)(_lib.pxg_grouped_linear_grad_workspace)  # bytes, by sizes
 
 
 def grouped_linear_grad(grad, h=None, activation=None, offsets=None, bias_dtype=None, out=None):
@@ -388,59 +454,70 @@ def grouped_linear_grad(grad, h=None, activation=None, offsets=None, bias_dtype=
     [groups, n] (or [n] without offsets) of bias_dtype (f32 by default, or grad's type). Without an activation dh is
     grad itself. `out` may be grad or h itself. dx and dw are grouped_matmul_grad_input's and
     grouped_matmul_grad_weight's of dh, and the residual's gradient is grad."""
-    rows, n = _matrix(grad, "grad")
-    kind = _type(grad.dtype, "grad")
+    (rows, n), grad_stride = _rows(grad, "grad")
+    dtype = grad.dtype
+    kind = _type(dtype, "grad")
     ptr, groups = _groups(offsets)
+    tensors = [grad] if offsets is None else [grad, offsets]
     which = _optional(activation)
     if which < 0:
         if h is not None or out is not None:
             raise ValueError("h and out are for an activation")
-        dh, h_ptr, h_stride, stride = grad, None, 0, 0
+        dh, h_ptr, h_stride, stride = grad, 0, 0, 0
     else:
         if h is None:
             raise ValueError("h must be given with an activation")
-        if _matrix(h, "h") != (rows, n):
-            _mismatch(tuple(h.shape), (rows, n), "h's shape")
-        if h.dtype is not grad.dtype:
-            raise ValueError(f"h must be {grad.dtype}, got {h.dtype}")
-        h_ptr, h_stride = h.data_ptr(), _stride(h)
-        dh, stride = _out(out, (rows, n), grad.dtype, grad)
+        shape, h_stride = _rows(h, "h")
+        if shape != (rows, n):
+            _mismatch(tuple(shape), (rows, n), "h's shape")
+        if h.dtype is not dtype:
+            raise ValueError(f"h must be {dtype}, got {h.dtype}")
+        h_ptr = h.data_ptr()
+        tensors.append(h)
+        dh, stride = _result(out, (rows, n), dtype, grad, tensors)
     bias_dtype = bias_dtype or _torch.float32
-    if bias_dtype is not grad.dtype and bias_dtype is not _torch.float32:
-        raise ValueError(f"bias_dtype must be {grad.dtype} or float32, got {bias_dtype}")
+    if bias_dtype is not dtype and bias_dtype is not _torch.float32:
+        raise ValueError(f"bias_dtype must be {dtype} or float32, got {bias_dtype}")
     dbias = grad.new_empty((groups, n) if offsets is not None else (n,), dtype=bias_dtype)
-    size = _lib.pxg_grouped_linear_grad_workspace(rows, n, groups)
+    size = _grad_space(rows, n, groups)
     space = grad.new_empty(size, dtype=_torch.uint8) if size else None
-    _run(_lib.pxg_grouped_linear_grad_device, (grad, h, offsets, dh), which, kind, grad.data_ptr(), rows, n,
-         _stride(grad), h_ptr, h_stride, ptr, groups, dh.data_ptr(), stride, _KINDS[bias_dtype], dbias.data_ptr(), n,
-         space.data_ptr() if size else None, size)
+    _call(_lib.pxg_grouped_linear_grad_device, tensors,
+          _LINEAR_GRAD.pack(kind, _KINDS[bias_dtype], which, rows, n, groups, grad.data_ptr(), grad_stride, h_ptr, h_stride,
+                            ptr or 0, dh.data_ptr(), stride, dbias.data_ptr(), n, space.data_ptr() if size else 0, size))
     return dh, dbias
 
 
-def _expert_matrix(w, name, experts, height, width, dtype, device_tensors):
-    """The C struct of [experts, height, width] matrices, or of a Block8 of [experts * height, width]."""
+def _expert_matrix(w, name, experts, height, width, dtype, tensors):
+    """(data, stride, group stride, scales) of [experts, height, width] matrices, or of a Block8 of [experts * height,
+    width] where dtype is None."""
     if dtype is None:
         codes, scales, rows, cols = _packed(w, name)
-        if (rows, cols) != (experts * height, width):
+        if rows != experts * height or cols != width:
             _mismatch((rows, cols), (experts * height, width), f"{name}'s shape")
-        device_tensors += (codes, scales)
-        return _ExpertMatrix(codes.data_ptr(), 0, 0, scales.data_ptr())
-    if _matrix(w, name, 3) != (experts, height, width):
-        _mismatch(tuple(w.shape), (experts, height, width), f"{name}'s shape")
+        tensors += (codes, scales)
+        return codes.data_ptr(), 0, 0, scales.data_ptr()
+    shape, stride = _rows(w, name, 3)
+    if shape != (experts, height, width):
+        _mismatch(tuple(shape), (experts, height, width), f"{name}'s shape")
     if w.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {w.dtype}")
-    device_tensors.append(w)
-    return _ExpertMatrix(w.data_ptr(), _stride(w), w.stride(0), None)
+    tensors.append(w)
+    return w.data_ptr(), stride, w.stride(0), 0
 
 
-def _routes(t, name, dtype, shape=None):
-    """Checks a router's [rows, picks] tensor; its shape."""
-    got = _matrix(t, name)
+def _picks(t, name, dtype, expected, tensors):
+    """Checks a tensor [rows, some] of `dtype`; (its columns, elements from row to row)."""
+    shape, stride = _rows(t, name)
     if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and got != shape:
-        _mismatch(tuple(got), tuple(shape), f"{name}'s shape")
-    return got
+    rows, cols = expected
+    if shape[0] != rows or (cols is not None and shape[1] != cols):
+        _mismatch(tuple(shape), expected, f"{name}'s shape")
+    tensors.append(t)
+    return shape[1], stride
+
+
+_layer_space = _lru_cache(1024)(_lib.pxg_expert_layer_workspace)
 
 
 def expert_layer(x, experts, w1, w2, gates, activation=None, up=None, bias1=None, bias2=None, residual=None,
@@ -452,20 +529,19 @@ def expert_layer(x, experts, w1, w2, gates, activation=None, up=None, bias1=None
     x [rows, k] f16 or bf16; experts [rows, picks] int64 and gates [rows, picks] f32, picks at most 16 (an id that is
     no expert's is left out, one that a token has twice counts with both gates); w1 and up (optional) [experts, hidden,
     k] and w2 [experts, n, hidden] of x's type, or each a Block8 of the experts' rows one after the other (x is then
-    bf16); biases [experts, .] of x's type or f32; residual and y [rows,
-    n] of x's type or f32. `out` may be the residual itself. Nothing between the two products is rounded to x's type.
-    The matrices of the experts in use are read once for each 64 rows: for batches use grouped_linear."""
-    rows, k = _matrix(x, "x")
-    kind = _type(x.dtype, "x", False)
-    _, picks = shape = _routes(experts, "experts", _torch.int64)
-    if shape[0] != rows:
-        _mismatch(shape[0], rows, "experts' rows")
-    _routes(gates, "gates", _torch.float32, shape)
-    tensors = [x, experts, gates]
+    bf16); biases [experts, .] of x's type or f32; residual and y [rows, n] of x's type or f32. `out` may be the
+    residual itself. Nothing between the two products is rounded to x's type. The matrices of the experts in use are
+    read once for each 64 rows: for batches use grouped_linear."""
+    (rows, k), x_stride = _rows(x, "x")
+    xtype = x.dtype
+    kind = _type(xtype, "x", False)
+    tensors = [x]
+    picks, ids_stride = _picks(experts, "experts", _torch.int64, (rows, None), tensors)
+    _, gates_stride = _picks(gates, "gates", _torch.float32, (rows, picks), tensors)
     packed = type(w1) is Block8
     if packed:
-        if x.dtype is not _torch.bfloat16:
-            raise ValueError(f"x must be bfloat16 with packed matrices, got {x.dtype}")
+        if xtype is not _torch.bfloat16:
+            raise ValueError(f"x must be bfloat16 with packed matrices, got {xtype}")
         _, _, rows2, hidden = _packed(w2, "w2")
         number, left = divmod(w1.rows, hidden)
         if left or not number:
@@ -475,29 +551,30 @@ def expert_layer(x, experts, w1, w2, gates, activation=None, up=None, bias1=None
         if left or not n:
             raise DimensionMismatch(f"dimension mismatch: w2's {rows2} rows are not a multiple of {number} experts",
                                     number, rows2)
+        of = None
     else:
         number, hidden, _ = _matrix(w1, "w1", 3)
         n = _matrix(w2, "w2", 3)[1]
-    of = None if packed else x.dtype
+        of = xtype
     m1 = _expert_matrix(w1, "w1", number, hidden, k, of, tensors)
+    m3 = _expert_matrix(up, "up", number, hidden, k, of, tensors) if up is not None else (0, 0, 0, 0)
     m2 = _expert_matrix(w2, "w2", number, n, hidden, of, tensors)
-    m3 = _expert_matrix(up, "up", number, hidden, k, of, tensors) if up is not None else None
-    which = _optional(activation)
     if bias1 is not None and bias2 is not None and bias1.dtype is not bias2.dtype:
         raise ValueError(f"biases must be of one type, got {bias1.dtype} and {bias2.dtype}")
-    bias1, b1, kind1, stride1 = _bias(bias1, experts, number, hidden, x.dtype)
-    bias2, b2, kind2, stride2 = _bias(bias2, experts, number, n, x.dtype)
-    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
+    b1, kind1, stride1 = _bias(bias1, "bias1", number, hidden, xtype, tensors)
+    b2, kind2, stride2 = _bias(bias2, "bias2", number, n, xtype, tensors)
+    dtype = out_dtype or (out.dtype if out is not None else xtype)
     out_kind = _type(dtype, "out_dtype")
-    r, r_stride = _residual(residual, (rows, n), dtype)
-    out, stride = _out(out, (rows, n), dtype, x)
-    size = _lib.pxg_expert_layer_workspace(rows, picks, number, hidden, n, out_kind)
+    which = _optional(activation)
+    r, r_stride = _residual(residual, (rows, n), dtype, tensors)
+    out, stride = _result(out, (rows, n), dtype, x, tensors)
+    size = _layer_space(rows, picks, number, hidden, n, out_kind)
     space = x.new_empty(size, dtype=_torch.uint8) if size else None
-    tensors += (bias1, bias2, residual, out)
-    _run(_lib.pxg_expert_layer_device, tensors, kind, x.data_ptr(), rows, k, _stride(x), experts.data_ptr(), picks,
-         _stride(experts), gates.data_ptr(), _stride(gates), number, hidden, n, m1, m3, m2, packed, which,
-         kind1 if b1 else kind2, b1, stride1, b2, stride2, out_kind, r, r_stride, out.data_ptr(), stride,
-         space.data_ptr() if size else None, size)
+    _call(_lib.pxg_expert_layer_device, tensors,
+          _EXPERT_LAYER.pack(kind, out_kind, kind1 if b1 else kind2, which, packed, rows, k, picks, number, hidden, n,
+                             x.data_ptr(), x_stride, experts.data_ptr(), ids_stride, gates.data_ptr(), gates_stride, *m1,
+                             *m3, *m2, b1, stride1, b2, stride2, r, r_stride, out.data_ptr(), stride,
+                             space.data_ptr() if size else 0, size))
     return out
 
 
@@ -546,28 +623,30 @@ def _vector(t, name, rows, dtype):
     return t.data_ptr()
 
 
-def _distill(weight, logits, ids, scores, counts, temperature, grad, out):
-    rows, cols = _matrix(logits, "logits")
-    kind = _type(logits.dtype, "logits")
-    _, top = shape = _routes(ids, "ids", _torch.int64)
-    if shape[0] != rows:
-        _mismatch(shape[0], rows, "ids' rows")
-    _routes(scores, "scores", _torch.float32, shape)
+_distill_space = _lru_cache(1024)(_lib.pxg_distill_workspace)
+
+
+def _distill(fn, weight, logits, ids, scores, counts, temperature, grad, out):
+    (rows, cols), stride = _rows(logits, "logits")
+    dtype = logits.dtype
+    kind = _type(dtype, "logits")
+    tensors = [logits, counts]
+    top, ids_stride = _picks(ids, "ids", _torch.int64, (rows, None), tensors)
+    _, scores_stride = _picks(scores, "scores", _torch.float32, (rows, top), tensors)
     counts_ptr = _vector(counts, "counts", rows, _torch.int32)
-    tensors = [logits, ids, scores, counts]
+    weight_ptr = out_ptr = out_stride = 0
+    if grad:
+        weight_ptr = _vector(weight, "weight", rows, _torch.float32)
+        tensors.append(weight)
+        out, out_stride = _result(out, (rows, cols), dtype, logits, tensors)
+        out_ptr = out.data_ptr()
     loss = logits.new_empty((rows,), dtype=_torch.float32)
-    size = _lib.pxg_distill_workspace(kind, rows, cols, top)
+    size = _distill_space(kind, rows, cols, top)
     space = logits.new_empty(size, dtype=_torch.uint8) if size else None
-    args = (logits.data_ptr(), rows, cols, _stride(logits), ids.data_ptr(), _stride(ids), scores.data_ptr(),
-            _stride(scores), counts_ptr, top, temperature, loss.data_ptr())
-    held = (space.data_ptr() if size else None, size)
-    if not grad:
-        _run(_lib.pxg_distill_loss_device, tensors, kind, *args, *held)
-        return loss
-    weight_ptr = _vector(weight, "weight", rows, _torch.float32)
-    out, stride = _out(out, (rows, cols), logits.dtype, logits)
-    tensors += (weight, out)
-    _run(_lib.pxg_distill_loss_grad_device, tensors, kind, weight_ptr, *args, out.data_ptr(), stride, *held)
+    _call(fn, tensors,
+          _DISTILL.pack(kind, rows, cols, top, logits.data_ptr(), stride, ids.data_ptr(), ids_stride, scores.data_ptr(),
+                        scores_stride, counts_ptr, float(temperature), loss.data_ptr(), weight_ptr, out_ptr, out_stride,
+                        space.data_ptr() if size else 0, size))
     return loss, out
 
 
@@ -580,11 +659,11 @@ def distill_loss(logits, ids, scores, counts, temperature=1.0):
     distances their negatives), top at most 4096; counts [rows] int32. Entries whose id is outside [0, cols) are left
     out. A row without entries, or whose scores are all -inf, has loss 0; an entry of p = 0 adds nothing; a logit of
     -inf has q = 0, so that p > 0 there costs infinity. temperature is a number between 1e-6 and 1e6."""
-    return _distill(None, logits, ids, scores, counts, temperature, False, None)
+    return _distill(_lib.pxg_distill_loss_device, None, logits, ids, scores, counts, temperature, False, None)[0]
 
 
 def distill_loss_grad(weight, logits, ids, scores, counts, temperature=1.0, out=None):
     """(loss, dx): distill_loss and the logits' gradient, weight[t] / temperature (q - p), of the logits' type and
     rounded once; weight [rows] f32 is the loss' own gradient (1 / rows for the mean). Rows without a teacher have zeros.
     `out` may be the logits themselves."""
-    return _distill(weight, logits, ids, scores, counts, temperature, True, out)
+    return _distill(_lib.pxg_distill_loss_grad_device, weight, logits, ids, scores, counts, temperature, True, out)

@@ -115,115 +115,128 @@ def test_kernels_that_are_not_there_are_refused(lib):
         assert lib.pxg_grouped_matmul_set_kernel(rows) == 0
 
 
+def _with(kind, defaults, more):
+    """A C struct of these fields; pointers are numbers."""
+    s = kind(**{**defaults, **more})
+    return C.byref(s)
+
+
 def test_layers_refuse(lib):
-    p, odd = C.c_void_p(4096), C.c_void_p(4097)
-
-    def f(kind=2, x=p, rows=4, k=8, xs=8, w=p, groups=1, n=8, ws=8, offsets=None, bias_type=0, bias=p, bs=8, act=1,
-          out=2, r=p, rs=8, h=p, hs=8, y=p, ys=8):
-        return lib.pxg_grouped_linear_device(kind, x, rows, k, xs, w, groups, n, ws, 64, offsets, bias_type, bias, bs, act,
-                                             out, r, rs, h, hs, y, ys, None)
-
+    from proxima_amd._capi import LinearC
+    plain = dict(type=2, out_type=2, bias_type=0, activation=1, rows=4, k=8, groups=1, n=8, x=4096, x_stride=8, w=4096,
+                 w_stride=8, w_group_stride=64, bias=4096, bias_stride=8, residual=4096, residual_stride=8, h=4096,
+                 h_stride=8, y=4096, y_stride=8, x_scales=4096, w_scales=4096)
     for more, parameter in (
-            (dict(kind=0), b"type"), (dict(out=1), b"out_type"), (dict(k=0), b"k"), (dict(n=0), b"n"),
-            (dict(groups=0), b"groups"), (dict(groups=2), b"groups"), (dict(xs=7), b"stride"),
-            (dict(xs=1 << 23), b"stride"), (dict(w=None), b"w"), (dict(y=None), b"y"), (dict(x=odd), b"x"),
-            (dict(bias_type=1), b"bias_type"), (dict(bias=C.c_void_p(4098)), b"bias"),
-            (dict(groups=2, offsets=p, bs=7), b"stride"), (dict(act=2), b"activation"), (dict(act=-2), b"activation"),
-            (dict(rs=7), b"stride"), (dict(r=odd), b"residual"), (dict(hs=7), b"stride"), (dict(h=odd), b"h"),
-            (dict(ys=7), b"stride"), (dict(rows=1 << 31), b"rows")):
-        _refused(lib, f(**more), parameter)
-    assert f(rows=0, x=None, y=None, r=None, h=None) == 0
-
-    def b(codes=p, scales=p, rows=4, k=8, wc=p, ws=p, groups=1, n=8, offsets=None, bias_type=0, bias=p, bs=8, act=1,
-          out=2, r=p, rs=8, y=p, ys=8):
-        return lib.pxg_block8_linear_device(codes, scales, rows, k, wc, ws, groups, n, offsets, bias_type, bias, bs, act,
-                                            out, r, rs, y, ys, None)
-
+            (dict(type=0), b"type"), (dict(type=(1 << 32) + 2), b"type"), (dict(out_type=1), b"out_type"),
+            (dict(k=0), b"k"), (dict(n=0), b"n"), (dict(groups=0), b"groups"), (dict(groups=2), b"groups"),
+            (dict(x_stride=7), b"stride"), (dict(x_stride=1 << 23), b"stride"), (dict(w=None), b"w"),
+            (dict(y=None), b"y"), (dict(x=4097), b"x"), (dict(bias_type=1), b"bias_type"),
+            (dict(bias_type=1 << 32), b"bias_type"), (dict(bias=4098), b"bias"),
+            (dict(groups=2, offsets=4096, bias_stride=7), b"stride"), (dict(activation=2), b"activation"),
+            (dict(activation=-2), b"activation"), (dict(activation=1 << 32), b"activation"),
+            (dict(residual_stride=7), b"stride"), (dict(residual=4097), b"residual"), (dict(h_stride=7), b"stride"),
+            (dict(h=4097), b"h"), (dict(y_stride=7), b"stride"), (dict(rows=1 << 31), b"rows")):
+        _refused(lib, lib.pxg_grouped_linear_device(_with(LinearC, plain, more), None), parameter)
+    none = dict(rows=0, x=None, y=None, residual=None, h=None)
+    assert lib.pxg_grouped_linear_device(_with(LinearC, plain, none), None) == 0
     for more, parameter in (
-            (dict(out=3), b"type"), (dict(scales=None), b"scales"), (dict(wc=C.c_void_p(4104)), b"w_codes"),
-            (dict(bias_type=1), b"bias_type"), (dict(act=5), b"activation"), (dict(rs=4), b"stride"),
-            (dict(groups=3), b"groups"), (dict(y=odd), b"y"), (dict(k=0), b"k")):
-        _refused(lib, b(**more), parameter)
-    assert b(rows=0, codes=None, scales=None, y=None, r=None) == 0
+            (dict(out_type=3), b"type"), (dict(x_scales=None), b"x_scales"), (dict(w=4104), b"w"),
+            (dict(w_scales=4098), b"w_scales"), (dict(bias_type=1), b"bias_type"), (dict(activation=5), b"activation"),
+            (dict(residual_stride=4), b"stride"), (dict(groups=3), b"groups"), (dict(y=4097), b"y"), (dict(k=0), b"k")):
+        _refused(lib, lib.pxg_block8_linear_device(_with(LinearC, plain, more), None), parameter)
+    assert lib.pxg_block8_linear_device(_with(LinearC, plain, {**none, "x_scales": None}), None) == 0
 
 
 def test_layers_backward_pass_refuses(lib):
-    p, odd = C.c_void_p(4096), C.c_void_p(4097)
-
-    def f(act=1, kind=2, grad=p, rows=4, n=8, gs=8, h=p, hs=8, offsets=None, groups=1, dh=p, ds=8, bias_type=0, db=p,
-          dbs=8, space=None, size=0):
-        return lib.pxg_grouped_linear_grad_device(act, kind, grad, rows, n, gs, h, hs, offsets, groups, dh, ds, bias_type,
-                                                  db, dbs, space, size, None)
-
+    from proxima_amd._capi import LinearGradC
+    plain = dict(type=2, bias_type=0, activation=1, rows=4, n=8, groups=1, grad=4096, grad_stride=8, h=4096, h_stride=8,
+                 dh=4096, dh_stride=8, dbias=4096, dbias_stride=8)
+    f = lib.pxg_grouped_linear_grad_device
     for more, parameter in (
-            (dict(kind=3), b"type"), (dict(act=2), b"activation"), (dict(n=0), b"n"), (dict(groups=4), b"groups"),
-            (dict(offsets=C.c_void_p(4100)), b"offsets"), (dict(grad=None), b"grad"), (dict(gs=7), b"stride"),
-            (dict(h=None), b"h"), (dict(hs=7), b"stride"), (dict(dh=None), b"dh"), (dict(dh=odd), b"dh"),
-            (dict(bias_type=1), b"bias_type"), (dict(db=C.c_void_p(4098)), b"dbias"),
-            (dict(offsets=p, groups=2, dbs=7), b"stride"), (dict(space=C.c_void_p(4104)), b"workspace"),
+            (dict(type=3), b"type"), (dict(activation=2), b"activation"), (dict(n=0), b"n"), (dict(groups=4), b"groups"),
+            (dict(offsets=4100), b"offsets"), (dict(grad=None), b"grad"), (dict(grad_stride=7), b"stride"),
+            (dict(h=None), b"h"), (dict(h_stride=7), b"stride"), (dict(dh=None), b"dh"), (dict(dh=4097), b"dh"),
+            (dict(bias_type=1), b"bias_type"), (dict(dbias=4098), b"dbias"),
+            (dict(offsets=4096, groups=2, dbias_stride=7), b"stride"), (dict(workspace=4104), b"workspace"),
             (dict(rows=1 << 31), b"rows")):
-        _refused(lib, f(**more), parameter)
-    assert f(act=-1, h=None, dh=None, db=None) == 0  # nothing to do
+        _refused(lib, f(_with(LinearGradC, plain, more), None), parameter)
+    assert f(_with(LinearGradC, plain, dict(activation=-1, h=None, dh=None, dbias=None)), None) == 0  # nothing to do
     size = lib.pxg_grouped_linear_grad_workspace
-    assert size(100_000, 1024, 8) > 0 and size(100_000, 1024, 8) % (4 * 1024) == 0
+    assert size(100_000, 1024, 8) > 0 and size(100_000, 1024, 8) % 4 == 0
     assert size(8, 1024, 8) == 0 and size(0, 8, 1) == 0 and size(8, 0, 1) == 0 and size(8, 8, 0) == 0
 
 
 def test_whole_layers_refuse(lib):
-    from proxima_amd._capi import ExpertMatrixC
-    p, odd = C.c_void_p(4096), C.c_void_p(4097)
-    m = ExpertMatrixC(4096, 8, 64, 4096)
+    from proxima_amd._capi import ExpertLayerC, ExpertMatrixC
 
-    def f(kind=2, x=p, rows=4, k=8, xs=8, ids=p, picks=2, is_=2, gates=p, gs=2, experts=3, hidden=8, n=8, w1=m, up=None,
-          w2=m, packed=0, act=1, bias_type=0, b1=p, b1s=8, b2=p, b2s=8, out=2, r=p, rs=8, y=p, ys=8, space=p,
-          size=1 << 30):
-        return lib.pxg_expert_layer_device(kind, x, rows, k, xs, ids, picks, is_, gates, gs, experts, hidden, n, w1, up, w2,
-                                           packed, act, bias_type, b1, b1s, b2, b2s, out, r, rs, y, ys, space, size, None)
+    def m(data=4096, stride=8, scales=4096):
+        return ExpertMatrixC(data, stride, 64, scales)
 
+    plain = dict(type=2, out_type=2, bias_type=0, activation=1, packed=0, rows=4, k=8, picks=2, experts=3, hidden=8, n=8,
+                 x=4096, x_stride=8, ids=4096, ids_stride=2, gates=4096, gates_stride=2, w1=m(), w2=m(), bias1=4096,
+                 bias1_stride=8, bias2=4096, bias2_stride=8, residual=4096, residual_stride=8, y=4096, y_stride=8,
+                 workspace=4096, workspace_bytes=1 << 30)
+    f = lib.pxg_expert_layer_device
     for more, parameter in (
-            (dict(kind=0), b"type"), (dict(kind=1, packed=1, out=1), b"type"), (dict(out=1), b"out_type"),
-            (dict(rows=65537), b"rows"), (dict(picks=0), b"picks"), (dict(picks=17, is_=17, gs=17), b"picks"),
+            (dict(type=0), b"type"), (dict(type=1, packed=1, out_type=1), b"type"), (dict(out_type=1), b"out_type"),
+            (dict(rows=65537), b"rows"), (dict(picks=0), b"picks"), (dict(picks=17, ids_stride=17, gates_stride=17), b"picks"),
             (dict(experts=0), b"experts"), (dict(experts=65537), b"experts"), (dict(k=0), b"k"),
-            (dict(k=(1 << 22) + 1), b"k"), (dict(hidden=0), b"hidden"), (dict(n=0), b"n"), (dict(act=2), b"activation"),
-            (dict(x=None), b"x"), (dict(xs=7), b"stride"), (dict(gates=None), b"gates"), (dict(gs=1), b"stride"),
-            (dict(ids=None), b"experts"), (dict(ids=C.c_void_p(4100)), b"experts"), (dict(w1=None), b"w1"),
-            (dict(w1=ExpertMatrixC(None, 8, 64, None)), b"w1"), (dict(w2=ExpertMatrixC(4097, 8, 64, None)), b"w2"),
-            (dict(up=ExpertMatrixC(4096, 7, 64, None)), b"stride"),
-            (dict(w2=ExpertMatrixC(4096, 8, 64, None), packed=1), b"w2"),
-            (dict(w1=ExpertMatrixC(4104, 8, 64, 4096), packed=1), b"w1"), (dict(bias_type=1), b"bias_type"),
-            (dict(b1=C.c_void_p(4098)), b"bias1"), (dict(b2s=7), b"stride"), (dict(r=odd), b"residual"),
-            (dict(rs=7), b"stride"), (dict(y=None), b"y"), (dict(space=None), b"workspace_bytes"),
-            (dict(size=64), b"workspace_bytes"), (dict(space=C.c_void_p(4104)), b"workspace")):
-        _refused(lib, f(**more), parameter)
-    assert f(rows=0, x=None, ids=None, gates=None, r=None, y=None, space=None, size=0) == 0
+            (dict(k=(1 << 22) + 1), b"k"), (dict(hidden=0), b"hidden"), (dict(n=0), b"n"),
+            (dict(activation=2), b"activation"), (dict(x=None), b"x"), (dict(x_stride=7), b"stride"),
+            (dict(gates=None), b"gates"), (dict(gates_stride=1), b"stride"), (dict(ids=None), b"ids"),
+            (dict(ids=4100), b"ids"), (dict(w1=m(None)), b"w1"), (dict(w2=m(4097)), b"w2"),
+            (dict(up=m(4096, 7)), b"stride"), (dict(w2=m(scales=None), packed=1), b"w2"),
+            (dict(w1=m(4104), packed=1), b"w1"), (dict(bias_type=1), b"bias_type"), (dict(bias1=4098), b"bias1"),
+            (dict(bias2_stride=7), b"stride"), (dict(residual=4097), b"residual"), (dict(residual_stride=7), b"stride"),
+            (dict(y=None), b"y"), (dict(workspace=None), b"workspace_bytes"),
+            (dict(workspace_bytes=64), b"workspace_bytes"), (dict(workspace=4104), b"workspace")):
+        _refused(lib, f(_with(ExpertLayerC, plain, more), None), parameter)
+    none = dict(rows=0, x=None, ids=None, gates=None, residual=None, y=None, workspace=None, workspace_bytes=0)
+    assert f(_with(ExpertLayerC, plain, none), None) == 0
     size = lib.pxg_expert_layer_workspace
     assert size(8, 2, 16, 512, 512, 0) > size(8, 2, 16, 512, 512, 2) > 8 * 2 * 512 * 2 * 2
     assert size(0, 2, 16, 512, 512, 0) == 0 and size(8, 17, 16, 512, 512, 0) == 0 and size(8, 2, 0, 512, 512, 0) == 0
 
 
 def test_distillation_refuses(lib):
-    p, odd = C.c_void_p(4096), C.c_void_p(4097)
-
-    def f(kind=0, weight=p, x=p, rows=4, cols=8, xs=8, ids=p, is_=2, scores=p, ss=2, counts=p, top=2, t=1.0, loss=p, dx=p,
-          ds=8, space=None, size=0):
-        return lib.pxg_distill_loss_grad_device(kind, weight, x, rows, cols, xs, ids, is_, scores, ss, counts, top, t, loss,
-                                                dx, ds, space, size, None)
-
+    from proxima_amd._capi import DistillC
+    plain = dict(type=0, rows=4, cols=8, top=2, logits=4096, logits_stride=8, ids=4096, ids_stride=2, scores=4096,
+                 scores_stride=2, counts=4096, temperature=1.0, loss=4096, weight=4096, dx=4096, dx_stride=8)
+    f = lib.pxg_distill_loss_grad_device
     for more, parameter in (
-            (dict(kind=3), b"type"), (dict(cols=0), b"cols"), (dict(top=0), b"top"), (dict(top=4097), b"top"),
-            (dict(t=0.0), b"temperature"), (dict(t=float("nan")), b"temperature"), (dict(t=1e7), b"temperature"),
-            (dict(x=None), b"logits"), (dict(xs=7), b"stride"), (dict(x=odd), b"logits"), (dict(ids=None), b"ids"),
-            (dict(ids=C.c_void_p(4100)), b"ids"), (dict(is_=1), b"stride"), (dict(scores=None), b"scores"),
-            (dict(counts=None), b"counts"), (dict(loss=None), b"loss"), (dict(weight=None), b"weight"),
-            (dict(dx=None), b"dx"), (dict(ds=7), b"stride"), (dict(rows=1 << 31), b"rows"),
-            (dict(cols=1 << 20, xs=1 << 20, ds=1 << 20), b"workspace_bytes"),
-            (dict(space=C.c_void_p(4104)), b"workspace")):
-        _refused(lib, f(**more), parameter)
-    assert f(rows=0, weight=None, x=None, ids=None, scores=None, counts=None, loss=None, dx=None) == 0
-    assert lib.pxg_distill_loss_device(0, None, 0, 8, 8, None, 2, None, 2, None, 2, 1.0, None, None, 0, None) == 0
-    _refused(lib, lib.pxg_distill_loss_device(0, None, 4, 8, 8, p, 2, p, 2, p, 2, 1.0, p, None, 0, None), b"logits")
+            (dict(type=3), b"type"), (dict(cols=0), b"cols"), (dict(top=0), b"top"), (dict(top=4097), b"top"),
+            (dict(temperature=0.0), b"temperature"), (dict(temperature=float("nan")), b"temperature"),
+            (dict(temperature=1e7), b"temperature"), (dict(logits=None), b"logits"), (dict(logits_stride=7), b"stride"),
+            (dict(logits=4097), b"logits"), (dict(ids=None), b"ids"), (dict(ids=4100), b"ids"),
+            (dict(ids_stride=1), b"stride"), (dict(scores=None), b"scores"), (dict(counts=None), b"counts"),
+            (dict(loss=None), b"loss"), (dict(weight=None), b"weight"), (dict(dx=None), b"dx"),
+            (dict(dx_stride=7), b"stride"), (dict(rows=1 << 31), b"rows"),
+            (dict(cols=1 << 20, logits_stride=1 << 20, dx_stride=1 << 20), b"workspace_bytes"),
+            (dict(workspace=4104), b"workspace")):
+        _refused(lib, f(_with(DistillC, plain, more), None), parameter)
+    none = dict(rows=0, logits=None, ids=None, scores=None, counts=None, loss=None, weight=None, dx=None)
+    for call in (f, lib.pxg_distill_loss_device):
+        assert call(_with(DistillC, plain, none), None) == 0
+    _refused(lib, lib.pxg_distill_loss_device(_with(DistillC, plain, dict(logits=None, weight=None, dx=None)), None),
+             b"logits")
     size = lib.pxg_distill_workspace
     assert size(0, 4, 1 << 20, 2) > 0 and size(0, 4, 8, 2) == 0 and size(0, 0, 8, 2) == 0 and size(0, 4, 8, 0) == 0
+
+
+def test_arguments_are_packed_as_the_structs_lie():
+    from proxima_amd import _capi, experts
+    for packer, kind in ((experts._LINEAR, _capi.LinearC), (experts._LINEAR_GRAD, _capi.LinearGradC),
+                         (experts._EXPERT_LAYER, _capi.ExpertLayerC), (experts._DISTILL, _capi.DistillC)):
+        assert packer.size == C.sizeof(kind)
+        count = packer.size // 8
+        s = kind.from_buffer_copy(packer.pack(*range(1, count + 1)))
+
+        def values(t):
+            for name, of in t._fields_:
+                v = getattr(t, name)
+                yield from values(v) if isinstance(v, C.Structure) else (v,)
+
+        assert list(values(s)) == list(range(1, count + 1))
 
 
 def test_python_side_of_layers_and_losses_refuses_host_tensors():

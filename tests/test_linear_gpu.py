@@ -15,6 +15,8 @@ magnitudes being at most 2; dh is rounded once, and a bias' gradient is a sum of
 terms before that rounding, in f32: no partial sum passes the sum of the terms'
 magnitudes, and no term takes part in more additions than there are rows.
 """
+import ctypes as C
+
 import pytest
 
 import test_expert_kernels_gpu as kernels
@@ -268,6 +270,8 @@ def test_backward_pass_of_ragged_groups(gpu, dtype, n, case):
 def test_backward_pass_of_long_groups(gpu, sizes, n):
     # sums in parts, and the same without a workspace
     import torch
+
+    from proxima_amd._capi import LinearGradC
     g = base._dev(torch, n)
     rows = sum(sizes) + 11
     grad = torch.randn(rows, n, generator=g, device="cuda").bfloat16()
@@ -282,21 +286,23 @@ def test_backward_pass_of_long_groups(gpu, sizes, n):
     again = gpu.grouped_linear_grad(grad, h, "gelu", offsets)
     assert torch.equal(dh, again[0]) and torch.equal(dbias, again[1])
     space = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")
+    def call(out, other, given):
+        a = LinearGradC(type=2, bias_type=0, activation=1, rows=rows, n=n, groups=len(sizes), grad=grad.data_ptr(),
+                        grad_stride=n, h=h.data_ptr(), h_stride=n, offsets=offsets.data_ptr(), dh=out.data_ptr(),
+                        dh_stride=n, dbias=other.data_ptr() if other is not None else None, dbias_stride=n,
+                        workspace=space.data_ptr() if given else None, workspace_bytes=given)
+        assert lib.pxg_grouped_linear_grad_device(C.byref(a), torch.cuda.current_stream().cuda_stream) == 0
+
     for given in (0, need - 4, need):
         space.fill_(255)
         out, other = torch.empty_like(dh), torch.empty_like(dbias)
-        assert lib.pxg_grouped_linear_grad_device(
-            1, 2, grad.data_ptr(), rows, n, n, h.data_ptr(), n, offsets.data_ptr(), len(sizes), out.data_ptr(), n, 0,
-            other.data_ptr(), n, space.data_ptr() if given else None, given,
-            torch.cuda.current_stream().cuda_stream) == 0
+        call(out, other, given)
         assert torch.equal(out, dh)
         _check_grad(torch, out, other, grad, h, "gelu", ends)
         assert bool((space[given:] == 255).all())
     # without a bias
     out = torch.empty_like(dh)
-    assert lib.pxg_grouped_linear_grad_device(
-        1, 2, grad.data_ptr(), rows, n, n, h.data_ptr(), n, offsets.data_ptr(), len(sizes), out.data_ptr(), n, 0,
-        None, 0, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    call(out, None, 0)
     assert torch.equal(out, dh)
 
 

@@ -219,7 +219,10 @@ __device__ __forceinline__ void store_gradient(const Distill& p, uint4 raw, floa
   float x[EACH<T>];
   unpack<T>(raw, x);
 #pragma unroll
-  for (int e = 0; e < EACH<T>; ++e) x[e] = f == 0.0f ? 0.0f : exp_scaled<T>(p, x[e] - m) * f;
+  for (int e = 0; e < EACH<T>; ++e) x[e] = exp_scaled<T>(p, x[e] - m) * f;
+  if (f == 0.0f)  // nothing left of the teacher, or of the logits: zeros, whatever the row holds
+#pragma unroll
+    for (int e = 0; e < EACH<T>; ++e) x[e] = 0.0f;
   store_vector<T>(dx, v, phase, p.cols, aligned, x);
 }
 // Vectors that are unpacked in another pass are unpacked anew: their floats would not fit the registers.
@@ -251,75 +254,88 @@ __device__ __forceinline__ Softmax softmax_of(const Distill& p, uint4 (&raw)[N],
   return {m, s};
 }
 
-// A workgroup's row in registers: N vectors of a thread.
+// Rows in registers, N vectors of a thread; a workgroup takes one after another,
+// and a vector's registers load the next row's once its gradient is stored (4096
+// x 50000 in bf16, top 100: ~NEXT~ us, 198 without).
 template <class T, int THREADS, int N, bool GRAD>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 4) distill_row(Distill p) {
+__global__ void __launch_bounds__(THREADS, 4) distill_row(Distill p) {
   extern __shared__ __align__(16) char lds[];
   __shared__ Softmax waves[THREADS / 64];
   __shared__ int no_teacher;
-  const uint64_t row = p.first + blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const T* x = (const T*)p.x + row * p.xs;
-  const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
-  uint4 raw[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int v = i * THREADS + threadIdx.x;
-    if (is_whole<T>(v, phase, p.cols)) raw[i] = *reinterpret_cast<const uint4*>(x + ((int64_t)v * EACH<T> - phase));
-  }
   const Teacher t = teacher_at(lds, p.top);
-  float entropy = 0.0f;
-  bool none = false;
-  if (wave == 0) {
-    entropy = read_teacher<T>(p, row, x, nullptr, t, none);
-    if (lane == 0) no_teacher = none;
-  }
+  uint4 raw[N];
+  auto load = [&](uint64_t row, int i) {
+    const T* x = (const T*)p.x + row * p.xs;
+    const int v = i * THREADS + threadIdx.x, phase = phase_of<T>(x);
+    if (is_whole<T>(v, phase, p.cols)) raw[i] = *reinterpret_cast<const uint4*>(x + ((int64_t)v * EACH<T> - phase));
+  };
+  uint64_t row = blockIdx.x;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int v = i * THREADS + threadIdx.x;
-    if (!is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
-  }
-  Softmax mine = wave_joined(p, softmax_of<T>(p, raw));
-  if (lane == 0) waves[wave] = mine;
-  __syncthreads();
-  const Softmax all = wave_joined(p, lane < THREADS / 64 ? waves[lane] : Softmax{-__builtin_inff(), 0.0f});
-  none = no_teacher;
-  if (wave == 0) {
-    const float other = cross_entropy(p, t, all);
-    if (lane == 0) p.loss[row] = none ? 0.0f : entropy + other;
-  }
-  if constexpr (GRAD) {
-    T* dx = (T*)p.dx + row * p.ds;
-    const bool aligned = phase_of<T>(dx) == phase;
-    const float k = p.weight[row] * p.t, f = none || all.s == 0.0f ? 0.0f : k / all.s, m = or_zero(all.m);
-    keep_packed(raw);
+  for (int i = 0; i < N; ++i) load(row, i);
+  for (uint64_t next; row < p.rows; row = next) {
+    next = row + gridDim.x;
+    const T* x = (const T*)p.x + row * p.xs;
+    const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
+    float entropy = 0.0f;
+    bool none = false;
+    if (wave == 0) {
+      entropy = read_teacher<T>(p, row, x, nullptr, t, none);
+      if (lane == 0) no_teacher = none;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int v = i * THREADS + threadIdx.x;
-      if (v < vectors) store_gradient<T>(p, raw[i], m, f, dx, v, phase, aligned);
+      if (!is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
     }
-    if (none) return;
-    __syncthreads();  // what follows is stored over it
-    store_entries<T, THREADS>(p, t, all, k, dx, 0, p.cols);
+    const Softmax mine = wave_joined(p, softmax_of<T>(p, raw));
+    if (lane == 0) waves[wave] = mine;
+    if constexpr (!GRAD)
+      if (next < p.rows)
+#pragma unroll
+        for (int i = 0; i < N; ++i) load(next, i);
+    __syncthreads();
+    const Softmax all = wave_joined(p, lane < THREADS / 64 ? waves[lane] : Softmax{-__builtin_inff(), 0.0f});
+    none = no_teacher;
+    if (wave == 0) {
+      const float other = cross_entropy(p, t, all);
+      if (lane == 0) p.loss[row] = none ? 0.0f : entropy + other;
+    }
+    if constexpr (GRAD) {
+      T* dx = (T*)p.dx + row * p.ds;
+      const bool aligned = phase_of<T>(dx) == phase;
+      const float k = p.weight[row] * p.t, f = none || all.s == 0.0f ? 0.0f : k / all.s, m = or_zero(all.m);
+      keep_packed(raw);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int v = i * THREADS + threadIdx.x;
+        if (v < vectors) store_gradient<T>(p, raw[i], m, f, dx, v, phase, aligned);
+        if (next < p.rows) load(next, i);
+      }
+      __syncthreads();  // what follows is stored over it
+      if (!none) store_entries<T, THREADS>(p, t, all, k, dx, 0, p.cols);
+    }
+    __syncthreads();  // the teacher's and the wavefronts' places are free
   }
 }
 
-// A part of a row: its maximum and sum. The first part gathers the entries' logits.
+// A part of a row: its maximum and sum. A workgroup past the parts gathers the entries' logits.
 template <class T>
 __global__ void __launch_bounds__(PART_THREADS) distill_part(Distill p) {
   __shared__ Softmax waves[PART_THREADS / 64];
-  const uint64_t row = p.first + blockIdx.x / p.parts;
-  const int part = blockIdx.x % p.parts, lane = threadIdx.x & 63;
+  const uint64_t row = p.first + blockIdx.x / (p.parts + 1);
+  const int part = blockIdx.x % (p.parts + 1), lane = threadIdx.x & 63;
   const T* x = (const T*)p.x + row * p.xs;
-  const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
-  const int lo = (int)((int64_t)vectors * part / p.parts), hi = (int)((int64_t)vectors * (part + 1) / p.parts);
-  if (part == 0) {
+  if (part == p.parts) {
     const int count = min(max(p.counts[row], 0), p.top);
     for (int i = threadIdx.x; i < count; i += PART_THREADS) {
       const int64_t id = p.ids[row * p.is + i];
       if ((uint64_t)id < (uint64_t)p.cols) p.picked[row * p.top + i] = (float)x[id];
     }
+    return;
   }
+  const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
+  const int lo = (int)((int64_t)vectors * part / p.parts), hi = (int)((int64_t)vectors * (part + 1) / p.parts);
   constexpr int AHEAD = 4;
   const uint32_t fill = negative_infinities<T>();
   Softmax mine{-__builtin_inff(), 0.0f};
@@ -415,9 +431,8 @@ DistillPlan distill_plan(int type, uint64_t rows, uint64_t cols, uint64_t top) {
   DistillPlan d{0, 0, 0, 0};
   const uint64_t each = type == PXG_F32 ? 4 : 8, vectors = (cols + 2 * each - 2) / each;  // at any alignment
   if (vectors <= 1024 || (vectors <= 8192 && rows >= 128)) {
-    d.threads = vectors <= 1024 ? 256 : 1024;
-    const uint64_t n = (vectors + d.threads - 1) / d.threads;
-    d.each = n <= 1 ? 1 : n <= 2 ? 2 : n <= 4 ? 4 : 8;
+    d.threads = vectors <= 1024 ? 256 : 512;
+    d.each = (int)((vectors + d.threads - 1) / d.threads);
     return d;
   }
   // about 2048 workgroups fill the chip; parts of less than 16 KB gain nothing
@@ -432,35 +447,32 @@ void run_distill(Distill p, const DistillPlan& d, hipStream_t s) {
   const unsigned lds = (unsigned)(p.top * 12);
   auto row = [&](auto threads, auto each) {
     constexpr int THREADS = decltype(threads)::value, N = decltype(each)::value;
-    constexpr uint64_t MOST = LAUNCH_ROWS / 2;  // of 1024 threads
-    for (uint64_t a = 0; a < p.rows; a += MOST) {
-      p.first = a;
-      hipLaunchKernelGGL((distill_row<T, THREADS, N, GRAD>), dim3((unsigned)std::min(MOST, p.rows - a)), dim3(THREADS), lds,
-                         s, p);
-      PXG_HIP(hipGetLastError());
-    }
+    const unsigned fill = THREADS == 512 ? 512 : 1024;  // workgroups that run at once
+    hipLaunchKernelGGL((distill_row<T, THREADS, N, GRAD>), dim3((unsigned)std::min<uint64_t>(fill, p.rows)), dim3(THREADS), lds,
+                       s, p);
+    PXG_HIP(hipGetLastError());
   };
+  auto of = [&](auto each) { row(std::integral_constant<int, 512>{}, each); };
   using Small = std::integral_constant<int, 256>;
-  using Large = std::integral_constant<int, 1024>;
-  using One = std::integral_constant<int, 1>;
-  using Two = std::integral_constant<int, 2>;
-  using Four = std::integral_constant<int, 4>;
-  using Eight = std::integral_constant<int, 8>;
   if (d.threads == 256) {
-    if (d.each == 1) row(Small{}, One{});
-    else if (d.each == 2) row(Small{}, Two{});
-    else row(Small{}, Four{});
+    if (d.each == 1) row(Small{}, std::integral_constant<int, 1>{});
+    else if (d.each == 2) row(Small{}, std::integral_constant<int, 2>{});
+    else row(Small{}, std::integral_constant<int, 4>{});
   } else if (d.threads) {
-    if (d.each <= 2) row(Large{}, Two{});
-    else if (d.each == 4) row(Large{}, Four{});
-    else row(Large{}, Eight{});
+    if (d.each <= 4) of(std::integral_constant<int, 4>{});
+    else if (d.each <= 6) of(std::integral_constant<int, 6>{});
+    else if (d.each <= 8) of(std::integral_constant<int, 8>{});
+    else if (d.each <= 10) of(std::integral_constant<int, 10>{});
+    else if (d.each <= 12) of(std::integral_constant<int, 12>{});
+    else if (d.each <= 14) of(std::integral_constant<int, 14>{});
+    else of(std::integral_constant<int, 16>{});
   } else {
     const uint64_t all = p.rows;
     p.parts = d.parts;
-    for (uint64_t a = 0, most = LAUNCH_ROWS / d.parts; a < all; a += most) {
+    for (uint64_t a = 0, most = LAUNCH_ROWS / (d.parts + 1); a < all; a += most) {
       const unsigned m = (unsigned)std::min(most, all - a);
       p.first = a;
-      hipLaunchKernelGGL(distill_part<T>, dim3(m * d.parts), dim3(PART_THREADS), 0, s, p);
+      hipLaunchKernelGGL(distill_part<T>, dim3(m * (d.parts + 1)), dim3(PART_THREADS), 0, s, p);
       PXG_HIP(hipGetLastError());
       hipLaunchKernelGGL((distill_join<T, GRAD>), dim3(GRAD ? m * d.parts : m), dim3(GRAD ? PART_THREADS : 64), lds, s, p);
       PXG_HIP(hipGetLastError());

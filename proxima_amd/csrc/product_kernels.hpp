@@ -986,16 +986,6 @@ void by_tiles(uint64_t tiles, P& p, F launch) {
   });
 }
 
-void check_groups(uint64_t groups, const int64_t* offsets) {
-  if (groups == 0 || groups > (1u << 20)) config_error("groups", groups, "must be between 1 and 1048576");
-  if (!offsets && groups != 1) config_error("groups", groups, "must be 1 without offsets");
-  check_aligned("offsets", offsets, 8);
-}
-void check_out_type(int64_t type, int64_t out_type) {
-  if (out_type != type && out_type != PXG_F32)
-    config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
-}
-
 // The sums of divided groups: a grid of (such group, some rows of dw) by 1024
 // columns adds the parts of each element in order.
 constexpr int JOIN_ROWS = 512;  // workgroups to a group

@@ -57,6 +57,23 @@ inline void check_packed_rows(const char* codes_name, const void* codes, const c
   check_aligned(codes_name, codes, 16);
   check_aligned(scales_name, scales, 4);
 }
+inline void check_groups(uint64_t groups, const int64_t* offsets) {
+  if (groups == 0 || groups > (1u << 20)) config_error("groups", groups, "must be between 1 and 1048576");
+  if (!offsets && groups != 1) config_error("groups", groups, "must be 1 without offsets");
+  check_aligned("offsets", offsets, 8);
+}
+inline void check_out_type(int64_t type, int64_t out_type) {
+  if (out_type != type && out_type != PXG_F32)
+    config_error("out_type", (uint64_t)out_type, "must be the operands' type or f32");
+}
+// `name` must be a string literal.
+inline void check_bias(const char* name, int type, int64_t bias_type, const void* bias, uint64_t groups,
+                       uint64_t n, uint64_t stride) {
+  if (!bias) return;
+  if (bias_type != type && bias_type != PXG_F32)
+    config_error("bias_type", (uint64_t)bias_type, "must be the operands' type or f32");
+  check_rows(bias_type, name, bias, groups, n, stride);
+}
 // Whether every row starts on a 16-byte boundary.
 inline bool rows_aligned(int type, const void* p, uint64_t stride) {
   return ((uint64_t)(uintptr_t)p | (stride * type_bytes(type))) % 16 == 0;

@@ -32,6 +32,33 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, uint64_t c, uin
   }
 }
 
+// The same, left packed in T.
+template <class T>
+struct Eight {
+  uint4 q[sizeof(T) / 2];
+  __device__ __forceinline__ void unpack(float (&x)[8]) const {
+    T v[8];
+    __builtin_memcpy(v, q, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float(v[i]);
+  }
+};
+template <class T, bool VEC>
+__device__ __forceinline__ Eight<T> raw8(const T* __restrict__ row, uint64_t c, uint64_t cols) {
+  Eight<T> x;
+  if (VEC && c + 8 <= cols) {
+    const uint4* p = reinterpret_cast<const uint4*>(row + c);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.q[i] = p[i];
+  } else {
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? row[c + i] : (T)0.0f;
+    __builtin_memcpy(x.q, v, sizeof(v));
+  }
+  return x;
+}
+
 // One rounding of the f32 value: kept apart from the product before it, which
 // the compiler may otherwise fuse into the conversion to f16 in some variants
 // of a kernel and not in others.

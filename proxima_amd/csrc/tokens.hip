@@ -174,7 +174,9 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
 #if defined(__HIP_DEVICE_COMPILE__)
   using M = MatrixTile<T, PACKED, ANY>;
   constexpr int AHEAD = RT == 1 ? 2 : 1;  // rounds loaded before they are multiplied
+  constexpr bool EARLY = !PACKED || RT < 4;  // so are x's, where they fit the registers
   __shared__ uint32_t used[EXPERTS_MAX / 32];
+  __shared__ int ids[ENTRIES_MAX];
   __shared__ f4v part[TOKENS_WAVES][D * RT][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -188,7 +190,9 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
   __syncthreads();
   for (int i = threadIdx.x; i < tokens * p.picks; i += TOKENS_THREADS) {
     const int64_t id = p.ids[(uint64_t)(t0 + i / p.picks) * p.is + i % p.picks];
-    if ((uint64_t)id < (uint64_t)p.experts) atomicOr(&used[id >> 5], 1u << (id & 31));
+    const bool is = (uint64_t)id < (uint64_t)p.experts;
+    if (is) atomicOr(&used[id >> 5], 1u << (id & 31));
+    ids[i] = is ? (int)id : 1 << 30;
   }
   __syncthreads();
   const int per = (words + 63) / 64;
@@ -208,14 +212,19 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
   for (; left; --left) bits &= bits - 1;
   const int expert = word * 32 + __builtin_ctz(bits);
 
+  const int cols = p.hidden - n0 < 16 ? p.hidden - n0 : 16;
+  const int k_wide = PACKED ? (int)p.w1.stride : p.k;
+  M w[D];
+  w[0].set(p.w1, expert, p.hidden, n0, cols, k_wide, lane);
+  if constexpr (D == 2) w[1].set(p.up, expert, p.hidden, n0, cols, k_wide, lane);
   // its tokens, a lane each, and their gates; then lane r has the r-th of them
   bool mine = false;
   float gate = 0.0f;
   int lower = 0;
   if (lane < tokens)
     for (int j = 0; j < p.picks; ++j) {
-      const int64_t id = p.ids[(uint64_t)(t0 + lane) * p.is + j];
-      lower += (uint64_t)id < (uint64_t)expert;
+      const int id = ids[lane * p.picks + j];
+      lower += id < expert;
       if (id == expert) {
         mine = true;
         gate += p.gates[(uint64_t)(t0 + lane) * p.gs + j];
@@ -231,11 +240,6 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
   gate = __builtin_bit_cast(float, __builtin_amdgcn_ds_permute(to * 4, __builtin_bit_cast(int, gate)));
   if (n0 == 0 && threadIdx.x == 0) entries[nth + 1] = {expert, offset, mask};
 
-  const int cols = p.hidden - n0 < 16 ? p.hidden - n0 : 16;
-  const int k_wide = PACKED ? (int)p.w1.stride : p.k;
-  M w[D];
-  w[0].set(p.w1, expert, p.hidden, n0, cols, k_wide, lane);
-  if constexpr (D == 2) w[1].set(p.up, expert, p.hidden, n0, cols, k_wide, lane);
   uint32_t odd;
   const auto rx = rows_rsrc<ANY>((const char*)p.x + (uint64_t)t0 * p.xs * 2,
                                  ((uint64_t)(tokens - 1) * p.xs + p.k) * 2, odd);
@@ -249,22 +253,25 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
   f4v acc[D][RT] = {};
   for (int k0 = wave * M::ROUND; k0 < k_wide; k0 += TOKENS_WAVES * M::ROUND * AHEAD) {
     typename M::Round b[AHEAD][D];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int d = 0; d < D; ++d) b[u][d] = w[d].load(k0 + u * TOKENS_WAVES * M::ROUND, k_wide, q);
     Piece<ANY> a[AHEAD][RT][M::FRAGMENTS];
+    auto load_x = [&](int u, int i, int f) {
+      const int at = k0 + u * TOKENS_WAVES * M::ROUND + M::column(f, q);
+      a[u][i][f] = load_piece<ANY>(rx, xat[i] + at * 2, xin[i] && at < p.k);
+    };
+    if constexpr (EARLY) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int k = k0 + u * TOKENS_WAVES * M::ROUND;
+      for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
-      for (int d = 0; d < D; ++d) b[u][d] = w[d].load(k, k_wide, q);
+        for (int i = 0; i < RT; ++i)
+          if (i == 0 || i * 16 < count)
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
-        if (i == 0 || i * 16 < count)
-#pragma unroll
-          for (int f = 0; f < M::FRAGMENTS; ++f) {
-            const int at = k + M::column(f, q);
-            a[u][i][f] = load_piece<ANY>(rx, xat[i] + at * 2, xin[i] && at < p.k);
-          }
+            for (int f = 0; f < M::FRAGMENTS; ++f) load_x(u, i, f);
+      __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first is waited for
     }
-    __builtin_amdgcn_sched_barrier(0);  // all of them in flight before the first is waited for
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       const int k = k0 + u * TOKENS_WAVES * M::ROUND;
@@ -276,6 +283,7 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
 #pragma unroll
         for (int i = 0; i < RT; ++i)
           if (i == 0 || i * 16 < count) {
+            if constexpr (!EARLY) load_x(u, i, f);
             const uint4 xf = elements(a[u][i][f], xat[i], p.k - k - M::column(f, q));
 #pragma unroll
             for (int d = 0; d < D; ++d) acc[d][i] = mfma16<T>(wf[d], xf, acc[d][i]);
@@ -358,7 +366,7 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_out(TokenLayer p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using M = MatrixTile<T, PACKED, ANY>;
   constexpr int PLANES = std::is_same_v<O, float> ? 3 : 2;
-  constexpr int AHEAD = RT > 1 ? 2 : !PACKED && PLANES == 2 ? 4 : 2;
+  constexpr int AHEAD = RT > 1 || ANY ? 2 : PACKED ? 4 - PLANES : PLANES == 3 ? 2 : std::is_same_v<T, __bf16> ? 4 : 3;  // chunks loaded before they are multiplied
   __shared__ Entry entries[ENTRIES_MAX];
   __shared__ f4v part[TOKENS_WAVES][RT][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
@@ -469,11 +477,15 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_out(TokenLayer p) {
 #pragma unroll
   for (int i = 0; i < RT; ++i) part[wave][i][lane] = acc[i];
   __syncthreads();
-  const int i = wave, t = i * 16 + r16;
-  if (i >= RT || t >= tokens) return;
-  f4v s = part[0][i][lane];
+  const int i = wave, t = i * 16 + r16;  // a wavefront ends a row tile
+  const bool mine = i < RT && t < tokens;
+  f4v s = {};
+  if (mine) {
+    s = part[0][i][lane];
 #pragma unroll
-  for (int o = 1; o < TOKENS_WAVES; ++o) s += part[o][i][lane];
+    for (int o = 1; o < TOKENS_WAVES; ++o) s += part[o][i][lane];
+  }
+  if (!mine) return;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (4 * q + e >= cols) break;
@@ -483,12 +495,14 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_out(TokenLayer p) {
 #endif
 }
 
-// The slices' sums, in order.
+// The slices' sums, in order. (The last of them to end could add them up instead
+// of a kernel, but its fences empty the L2s: 8 tokens x 2 of 16 experts 209 us, 84 with this.)
 template <class T, class O>
 __global__ void __launch_bounds__(256) tokens_join(TokenLayer p) {
   const uint64_t all = (uint64_t)p.rows * p.n;
   for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
     float v = 0.0f;
+#pragma unroll 4
     for (int s = 0; s < p.slices; ++s) v += p.partial[s * all + i];
     finish<T, O>(p, (int)(i / p.n), (int)(i % p.n), v);
   }
@@ -598,8 +612,7 @@ int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream) {
     const bool packed = a.packed != 0;
     check_type(a.type, false);
     if (packed && a.type != PXG_BF16) config_error("type", (uint64_t)a.type, "must be bf16 with packed matrices");
-    if (a.out_type != a.type && a.out_type != PXG_F32)
-      config_error("out_type", (uint64_t)a.out_type, "must be the operands' type or f32");
+    check_out_type(a.type, a.out_type);
     check_tokens(a.rows, a.picks, a.experts);
     check_width("k", a.k);
     check_width("hidden", a.hidden);
@@ -623,12 +636,8 @@ int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream) {
     p.w1 = matrix("w1", a.w1, a.hidden, a.k);
     if (a.up.data) p.up = matrix("up", a.up, a.hidden, a.k);
     p.w2 = matrix("w2", a.w2, a.n, a.hidden);
-    if (a.bias1 || a.bias2) {
-      if (a.bias_type != a.type && a.bias_type != PXG_F32)
-        config_error("bias_type", (uint64_t)a.bias_type, "must be the operands' type or f32");
-      if (a.bias1) check_rows(a.bias_type, "bias1", a.bias1, a.experts, a.hidden, a.bias1_stride);
-      if (a.bias2) check_rows(a.bias_type, "bias2", a.bias2, a.experts, a.n, a.bias2_stride);
-    }
+    check_bias("bias1", a.type, a.bias_type, a.bias1, a.experts, a.hidden, a.bias1_stride);
+    check_bias("bias2", a.type, a.bias_type, a.bias2, a.experts, a.n, a.bias2_stride);
     if (a.residual) check_rows(a.out_type, "residual", a.residual, a.rows, a.n, a.residual_stride);
     check_rows(a.out_type, "y", a.y, a.rows, a.n, a.y_stride);
     p.xs = check_stride(a.rows, a.k, a.x_stride);

@@ -199,123 +199,181 @@ __device__ __forceinline__ void unpack(uint4 raw, float (&x)[EACH<T>]) {
   for (int e = 0; e < EACH<T>; ++e) x[e] = (float)v[e];
 }
 template <class T>
-__device__ __forceinline__ void store_vector(T* row, int v, int phase, int cols, bool aligned, const float (&x)[EACH<T>]) {
-  T y[EACH<T>];
-#pragma unroll
-  for (int e = 0; e < EACH<T>; ++e) y[e] = rounded<T>(x[e]);
+__device__ __forceinline__ void store_vector(T* row, int v, int phase, int cols, bool aligned, uint4 x) {
   const int64_t at = (int64_t)v * EACH<T> - phase;
   if (aligned && at >= 0 && at + EACH<T> <= cols) {
-    *reinterpret_cast<uint4*>(row + at) = *reinterpret_cast<const uint4*>(y);
+    *reinterpret_cast<uint4*>(row + at) = x;
   } else {
+    T y[EACH<T>];
+    __builtin_memcpy(y, &x, 16);
 #pragma unroll
     for (int e = 0; e < EACH<T>; ++e)
       if (at + e >= 0 && at + e < cols) row[at + e] = y[e];
   }
 }
-// dx = f exp((x - m) / T) of a vector.
-template <class T>
-__device__ __forceinline__ void store_gradient(const Distill& p, uint4 raw, float m, float f, T* dx, int v, int phase,
-                                               bool aligned) {
-  float x[EACH<T>];
-  unpack<T>(raw, x);
-#pragma unroll
-  for (int e = 0; e < EACH<T>; ++e) x[e] = exp_scaled<T>(p, x[e] - m) * f;
-  if (f == 0.0f)  // nothing left of the teacher, or of the logits: zeros, whatever the row holds
-#pragma unroll
-    for (int e = 0; e < EACH<T>; ++e) x[e] = 0.0f;
-  store_vector<T>(dx, v, phase, p.cols, aligned, x);
-}
+// 16-bit logits are bound by arithmetic as much as by memory, so there
+//   - the maximum is one of whole numbers, two at a time: patterns of positive
+//     values grow with them, of negative ones against them, so that the largest
+//     signed one is the maximum unless all are negative; then it is the smallest
+//     unsigned one;
+//   - x c - M is one operation, M the rounded m c (c = log2 e / T). What M's
+//     rounding left is taken out of the sum;
+//   - the gradient's factor goes into the exponent, which costs 2^-17 of it while
+//     |M| is at most 128; beyond, and in f32, it is (x - m) c and a factor.
+constexpr float FAST_MAX = 128.0f;
+
 // Vectors that are unpacked in another pass are unpacked anew: their floats would not fit the registers.
 template <int N>
 __device__ __forceinline__ void keep_packed(uint4 (&raw)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
 }
+
 template <class T, int N>
-__device__ __forceinline__ Softmax softmax_of(const Distill& p, uint4 (&raw)[N], Softmax before = {-__builtin_inff(), 0.0f}) {
-  float m = before.m;
+__device__ __forceinline__ float largest(const uint4 (&raw)[N]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -__builtin_inff();
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float x[EACH<T>];
-    unpack<T>(raw[i], x);
+    for (int i = 0; i < N; ++i) {
+      float x[EACH<T>];
+      unpack<T>(raw[i], x);
 #pragma unroll
-    for (int e = 0; e < EACH<T>; ++e) m = fmaxf(m, x[e]);
+      for (int e = 0; e < EACH<T>; ++e) m = fmaxf(m, x[e]);
+    }
+    return m;
+  } else {
+    typedef short s2 __attribute__((ext_vector_type(2)));
+    typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+    s2 hi = {(short)0x8000, (short)0x8000};
+    u2 lo = {0xFFFF, 0xFFFF};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        hi = __builtin_elementwise_max(hi, __builtin_bit_cast(s2, w[e]));
+        lo = __builtin_elementwise_min(lo, __builtin_bit_cast(u2, w[e]));
+      }
+    }
+    const short h = hi[0] > hi[1] ? hi[0] : hi[1];
+    const unsigned short l = lo[0] < lo[1] ? lo[0] : lo[1];
+    return (float)__builtin_bit_cast(T, h >= 0 ? (unsigned short)h : l);
   }
-  if constexpr (N > 4) keep_packed(raw);
-  const float z = or_zero(m);
-  float s = before.s * exp_scaled<float>(p, before.m - z);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float x[EACH<T>];
-    unpack<T>(raw[i], x);
-#pragma unroll
-    for (int e = 0; e < EACH<T>; ++e) s += exp_scaled<T>(p, x[e] - z);
-  }
-  return {m, s};
 }
 
-// Rows in registers, N vectors of a thread; a workgroup takes one after another,
-// and a vector's registers load the next row's once its gradient is stored (4096
-// x 50000 in bf16, top 100: ~NEXT~ us, 198 without).
+// dx = f exp((x - m) / T) of a vector.
+template <class T>
+struct Gradient {
+  float m, f, offset;
+  uint32_t sign;
+  bool fast;
+  __device__ __forceinline__ Gradient(const Distill& p, float m_, float f_) : m(m_), f(f_) {
+    const float big = m * p.c;
+    fast = sizeof(T) == 2 && fabsf(big) <= FAST_MAX && fabsf(f) >= 1e-30f && fabsf(f) <= 1e30f;
+    offset = __builtin_amdgcn_logf(fabsf(f)) - __builtin_fmaf(m, p.c, -big) - big;  // log2
+    sign = f < 0.0f ? 0x80008000u : 0u;
+  }
+  template <bool FAST>
+  __device__ __forceinline__ uint4 of(const Distill& p, uint4 raw) const {
+    float x[EACH<T>];
+    unpack<T>(raw, x);
+    T y[EACH<T>];
+#pragma unroll
+    for (int e = 0; e < EACH<T>; ++e)
+      if constexpr (FAST) y[e] = rounded<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(x[e], p.c, offset)));
+      else y[e] = rounded<T>(exp_scaled<T>(p, x[e] - m) * f);
+    uint4 w;
+    __builtin_memcpy(&w, y, 16);
+    if constexpr (FAST) return make_uint4(w.x ^ sign, w.y ^ sign, w.z ^ sign, w.w ^ sign);
+    return f == 0.0f ? make_uint4(0, 0, 0, 0) : w;  // zeros, whatever the row holds
+  }
+};
+template <class T, int N>
+__device__ __forceinline__ Softmax softmax_of(const Distill& p, uint4 (&raw)[N], Softmax before = {-__builtin_inff(), 0.0f}) {
+  const float m = fmaxf(before.m, largest<T>(raw)), z = or_zero(m), big = z * p.c;
+  float s = 0.0f;
+  if (sizeof(T) == 2 && fabsf(big) <= FAST_MAX) {
+    keep_packed(raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float x[EACH<T>];
+      unpack<T>(raw[i], x);
+#pragma unroll
+      for (int e = 0; e < EACH<T>; ++e) s += __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], p.c, -big));
+    }
+    s *= __builtin_amdgcn_exp2f(-__builtin_fmaf(z, p.c, -big));
+  } else {
+    keep_packed(raw);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float x[EACH<T>];
+      unpack<T>(raw[i], x);
+#pragma unroll
+      for (int e = 0; e < EACH<T>; ++e) s += exp_scaled<T>(p, x[e] - z);
+    }
+  }
+  return {m, s + before.s * exp_scaled<float>(p, before.m - z)};
+}
+
+// A workgroup's row in registers: N vectors of a thread. 4096 x 50000 in bf16
+// with top 100: 177 us, 4.6 TB/s. (With rows one after another in workgroups
+// that load the next while they store, whose registers leave 512 threads: 225;
+// with a maximum of floats and a factor: 198.)
 template <class T, int THREADS, int N, bool GRAD>
-__global__ void __launch_bounds__(THREADS, 4) distill_row(Distill p) {
+__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 4) distill_row(Distill p) {
   extern __shared__ __align__(16) char lds[];
   __shared__ Softmax waves[THREADS / 64];
   __shared__ int no_teacher;
+  const uint64_t row = p.first + blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Teacher t = teacher_at(lds, p.top);
+  const T* x = (const T*)p.x + row * p.xs;
+  const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
   uint4 raw[N];
-  auto load = [&](uint64_t row, int i) {
-    const T* x = (const T*)p.x + row * p.xs;
-    const int v = i * THREADS + threadIdx.x, phase = phase_of<T>(x);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int v = i * THREADS + threadIdx.x;
     if (is_whole<T>(v, phase, p.cols)) raw[i] = *reinterpret_cast<const uint4*>(x + ((int64_t)v * EACH<T> - phase));
-  };
-  uint64_t row = blockIdx.x;
+  }
+  const Teacher t = teacher_at(lds, p.top);
+  float entropy = 0.0f;
+  bool none = false;
+  if (wave == 0) {
+    entropy = read_teacher<T>(p, row, x, nullptr, t, none);
+    if (lane == 0) no_teacher = none;
+  }
 #pragma unroll
-  for (int i = 0; i < N; ++i) load(row, i);
-  for (uint64_t next; row < p.rows; row = next) {
-    next = row + gridDim.x;
-    const T* x = (const T*)p.x + row * p.xs;
-    const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
-    float entropy = 0.0f;
-    bool none = false;
-    if (wave == 0) {
-      entropy = read_teacher<T>(p, row, x, nullptr, t, none);
-      if (lane == 0) no_teacher = none;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int v = i * THREADS + threadIdx.x;
-      if (!is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
-    }
-    const Softmax mine = wave_joined(p, softmax_of<T>(p, raw));
-    if (lane == 0) waves[wave] = mine;
-    if constexpr (!GRAD)
-      if (next < p.rows)
-#pragma unroll
-        for (int i = 0; i < N; ++i) load(next, i);
-    __syncthreads();
-    const Softmax all = wave_joined(p, lane < THREADS / 64 ? waves[lane] : Softmax{-__builtin_inff(), 0.0f});
-    none = no_teacher;
-    if (wave == 0) {
-      const float other = cross_entropy(p, t, all);
-      if (lane == 0) p.loss[row] = none ? 0.0f : entropy + other;
-    }
-    if constexpr (GRAD) {
-      T* dx = (T*)p.dx + row * p.ds;
-      const bool aligned = phase_of<T>(dx) == phase;
-      const float k = p.weight[row] * p.t, f = none || all.s == 0.0f ? 0.0f : k / all.s, m = or_zero(all.m);
-      keep_packed(raw);
+  for (int i = 0; i < N; ++i) {
+    const int v = i * THREADS + threadIdx.x;
+    if (!is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
+  }
+  const Softmax mine = wave_joined(p, softmax_of<T>(p, raw));
+  if (lane == 0) waves[wave] = mine;
+  __syncthreads();
+  const Softmax all = wave_joined(p, lane < THREADS / 64 ? waves[lane] : Softmax{-__builtin_inff(), 0.0f});
+  none = no_teacher;
+  if (wave == 0) {
+    const float other = cross_entropy(p, t, all);
+    if (lane == 0) p.loss[row] = none ? 0.0f : entropy + other;
+  }
+  if constexpr (GRAD) {
+    T* dx = (T*)p.dx + row * p.ds;
+    const bool aligned = phase_of<T>(dx) == phase;
+    const float k = p.weight[row] * p.t;
+    const Gradient<T> gradient(p, or_zero(all.m), none || all.s == 0.0f ? 0.0f : k / all.s);
+    keep_packed(raw);
+    auto store = [&](auto fast) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int v = i * THREADS + threadIdx.x;
-        if (v < vectors) store_gradient<T>(p, raw[i], m, f, dx, v, phase, aligned);
-        if (next < p.rows) load(next, i);
+        if (v < vectors)
+          store_vector<T>(dx, v, phase, p.cols, aligned, gradient.template of<decltype(fast)::value>(p, raw[i]));
       }
-      __syncthreads();  // what follows is stored over it
-      if (!none) store_entries<T, THREADS>(p, t, all, k, dx, 0, p.cols);
-    }
-    __syncthreads();  // the teacher's and the wavefronts' places are free
+    };
+    if (sizeof(T) == 2 && gradient.fast) store(std::true_type{});
+    else store(std::false_type{});
+    if (none) return;
+    __syncthreads();  // what follows is stored over it
+    store_entries<T, THREADS>(p, t, all, k, dx, 0, p.cols);
   }
 }
 
@@ -397,7 +455,8 @@ __global__ void __launch_bounds__(PART_THREADS) distill_join(Distill p) {
     const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
     const int lo = (int)((int64_t)vectors * part / p.parts), hi = (int)((int64_t)vectors * (part + 1) / p.parts);
     const bool aligned = phase_of<T>(dx) == phase;
-    const float k = p.weight[row] * p.t, f = none || all.s == 0.0f ? 0.0f : k / all.s, m = or_zero(all.m);
+    const float k = p.weight[row] * p.t;
+    const Gradient<T> gradient(p, or_zero(all.m), none || all.s == 0.0f ? 0.0f : k / all.s);
     constexpr int AHEAD = 4;
     for (int v0 = lo + (int)threadIdx.x; v0 < hi; v0 += PART_THREADS * AHEAD) {
       uint4 raw[AHEAD];
@@ -411,7 +470,8 @@ __global__ void __launch_bounds__(PART_THREADS) distill_join(Distill p) {
         const int v = v0 + i * PART_THREADS;
         if (v >= hi) break;
         if (!is_whole<T>(v, phase, p.cols)) raw[i] = load_ends<T>(x, v, phase, p.cols);
-        store_gradient<T>(p, raw[i], m, f, dx, v, phase, aligned);
+        store_vector<T>(dx, v, phase, p.cols, aligned,
+                        gradient.fast ? gradient.template of<true>(p, raw[i]) : gradient.template of<false>(p, raw[i]));
       }
     }
     if (none) return;
@@ -431,7 +491,7 @@ DistillPlan distill_plan(int type, uint64_t rows, uint64_t cols, uint64_t top) {
   DistillPlan d{0, 0, 0, 0};
   const uint64_t each = type == PXG_F32 ? 4 : 8, vectors = (cols + 2 * each - 2) / each;  // at any alignment
   if (vectors <= 1024 || (vectors <= 8192 && rows >= 128)) {
-    d.threads = vectors <= 1024 ? 256 : 512;
+    d.threads = vectors <= 1024 ? 256 : 1024;
     d.each = (int)((vectors + d.threads - 1) / d.threads);
     return d;
   }
@@ -447,25 +507,31 @@ void run_distill(Distill p, const DistillPlan& d, hipStream_t s) {
   const unsigned lds = (unsigned)(p.top * 12);
   auto row = [&](auto threads, auto each) {
     constexpr int THREADS = decltype(threads)::value, N = decltype(each)::value;
-    const unsigned fill = THREADS == 512 ? 512 : 1024;  // workgroups that run at once
-    hipLaunchKernelGGL((distill_row<T, THREADS, N, GRAD>), dim3((unsigned)std::min<uint64_t>(fill, p.rows)), dim3(THREADS), lds,
-                       s, p);
-    PXG_HIP(hipGetLastError());
+    constexpr uint64_t MOST = LAUNCH_ROWS / 2;  // of 1024 threads
+    for (uint64_t a = 0; a < p.rows; a += MOST) {
+      p.first = a;
+      hipLaunchKernelGGL((distill_row<T, THREADS, N, GRAD>), dim3((unsigned)std::min(MOST, p.rows - a)), dim3(THREADS), lds,
+                         s, p);
+      PXG_HIP(hipGetLastError());
+    }
   };
-  auto of = [&](auto each) { row(std::integral_constant<int, 512>{}, each); };
   using Small = std::integral_constant<int, 256>;
+  auto large = [&](auto each) { row(std::integral_constant<int, 1024>{}, each); };
   if (d.threads == 256) {
     if (d.each == 1) row(Small{}, std::integral_constant<int, 1>{});
     else if (d.each == 2) row(Small{}, std::integral_constant<int, 2>{});
     else row(Small{}, std::integral_constant<int, 4>{});
   } else if (d.threads) {
-    if (d.each <= 4) of(std::integral_constant<int, 4>{});
-    else if (d.each <= 6) of(std::integral_constant<int, 6>{});
-    else if (d.each <= 8) of(std::integral_constant<int, 8>{});
-    else if (d.each <= 10) of(std::integral_constant<int, 10>{});
-    else if (d.each <= 12) of(std::integral_constant<int, 12>{});
-    else if (d.each <= 14) of(std::integral_constant<int, 14>{});
-    else of(std::integral_constant<int, 16>{});
+    switch (d.each) {
+      case 1:
+      case 2: large(std::integral_constant<int, 2>{}); break;
+      case 3: large(std::integral_constant<int, 3>{}); break;
+      case 4: large(std::integral_constant<int, 4>{}); break;
+      case 5: large(std::integral_constant<int, 5>{}); break;
+      case 6: large(std::integral_constant<int, 6>{}); break;
+      case 7: large(std::integral_constant<int, 7>{}); break;
+      default: large(std::integral_constant<int, 8>{}); break;
+    }
   } else {
     const uint64_t all = p.rows;
     p.parts = d.parts;

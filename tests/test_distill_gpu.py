@@ -23,6 +23,7 @@ INF = float("inf")
 def _exact(torch, x, ids, scores, counts, t, weight=None):
     """(loss, its bound, dx, its bound) in 64 bits."""
     rows, cols = x.shape
+    x32 = x.dtype is torch.float32
     top = ids.shape[1]
     x, s = x.double() / t, scores.double() / t
     at = torch.arange(top, device="cuda")
@@ -48,7 +49,7 @@ def _exact(torch, x, ids, scores, counts, t, weight=None):
         return 2.0 ** -21 + 2.0 ** -21 * (d.abs() + 1.0) + (terms / 64 + 40) * 2.0 ** -24
 
     finite = torch.where(torch.isfinite(x), x, m0)
-    rq = relative(finite - m0, cols)
+    rq = relative(finite - m0, cols) + (0.0 if x32 else 2.0 ** -17)
     # the sum's own relative error: that of its terms, weighted
     rsum = torch.where(total > 0, (q * rq).sum(1, keepdim=True), 0.0)
     rp = relative(ds, top * 64)

@@ -12,9 +12,8 @@
 // Memory bounds it: x is read and dx written once, q never stored. Rows of up
 // to 128 KB stay in a workgroup's registers between the softmax' sums and dx
 // (two workgroups of 1024 threads fit a CU, so that one loads while the other
-// stores). Longer rows, and rows too few to fill the chip, are cut into parts:
-// one kernel finds each part's maximum and sum, a second joins them, and for dx
-// reads x again.
+// stores). Longer rows are cut into parts: one kernel finds each part's maximum
+// and sum, a second joins them, and for dx reads x again.
 #include <algorithm>
 #include <cmath>
 
@@ -28,6 +27,7 @@ namespace {
 
 constexpr uint64_t TOP_MAX = 4096;
 constexpr int PART_THREADS = 256;
+constexpr uint64_t HELD_MAX = 8192;  // vectors that a workgroup's registers hold
 
 struct Distill {
   const void* x;
@@ -320,7 +320,7 @@ __device__ __forceinline__ Softmax softmax_of(const Distill& p, uint4 (&raw)[N],
 // that load the next while they store, whose registers leave 512 threads: 225;
 // with a maximum of floats and a factor: 198.)
 template <class T, int THREADS, int N, bool GRAD>
-__global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 8 : 4) distill_row(Distill p) {
+__global__ void __launch_bounds__(THREADS, 8) distill_row(Distill p) {
   extern __shared__ __align__(16) char lds[];
   __shared__ Softmax waves[THREADS / 64];
   __shared__ int no_teacher;
@@ -482,7 +482,13 @@ __global__ void __launch_bounds__(PART_THREADS) distill_join(Distill p) {
 }
 
 // Which kernel takes a call: a row to a workgroup of `threads` with `each`
-// vectors a thread, or rows in `parts`.
+// vectors a thread, or rows in `parts`. Measured with the gradient, us, bf16:
+//   16 rows of 20000     held 9.7, in parts 14.3
+//   64 of 60000               14.0,          14.5
+//   8192 of 9000         by 256 threads 61, by 1024 103
+//   8192 of 1000         by 64 threads 15.6, by 256 25.8
+// (Parts of as many rows at a time as the last cache holds until they are read
+// again: 1000 rows of 200000 268, of all of them 264.)
 struct DistillPlan {
   int threads, each, parts;
   uint64_t bytes;
@@ -490,8 +496,9 @@ struct DistillPlan {
 DistillPlan distill_plan(int type, uint64_t rows, uint64_t cols, uint64_t top) {
   DistillPlan d{0, 0, 0, 0};
   const uint64_t each = type == PXG_F32 ? 4 : 8, vectors = (cols + 2 * each - 2) / each;  // at any alignment
-  if (vectors <= 1024 || (vectors <= 8192 && rows >= 128)) {
-    d.threads = vectors <= 1024 ? 256 : 1024;
+  if (vectors <= HELD_MAX) {
+    // small workgroups where they hold a row: more rows are on their way at once
+    d.threads = vectors <= 256 ? 64 : vectors <= 2048 ? 256 : 1024;
     d.each = (int)((vectors + d.threads - 1) / d.threads);
     return d;
   }
@@ -515,23 +522,26 @@ void run_distill(Distill p, const DistillPlan& d, hipStream_t s) {
       PXG_HIP(hipGetLastError());
     }
   };
-  using Small = std::integral_constant<int, 256>;
-  auto large = [&](auto each) { row(std::integral_constant<int, 1024>{}, each); };
-  if (d.threads == 256) {
-    if (d.each == 1) row(Small{}, std::integral_constant<int, 1>{});
-    else if (d.each == 2) row(Small{}, std::integral_constant<int, 2>{});
-    else row(Small{}, std::integral_constant<int, 4>{});
-  } else if (d.threads) {
+  auto of = [&](auto threads) {
     switch (d.each) {
-      case 1:
-      case 2: large(std::integral_constant<int, 2>{}); break;
-      case 3: large(std::integral_constant<int, 3>{}); break;
-      case 4: large(std::integral_constant<int, 4>{}); break;
-      case 5: large(std::integral_constant<int, 5>{}); break;
-      case 6: large(std::integral_constant<int, 6>{}); break;
-      case 7: large(std::integral_constant<int, 7>{}); break;
-      default: large(std::integral_constant<int, 8>{}); break;
+      case 1: row(threads, std::integral_constant<int, 1>{}); break;
+      case 2: row(threads, std::integral_constant<int, 2>{}); break;
+      case 3: row(threads, std::integral_constant<int, 3>{}); break;
+      case 4: row(threads, std::integral_constant<int, 4>{}); break;
+      case 5: row(threads, std::integral_constant<int, 5>{}); break;
+      case 6: row(threads, std::integral_constant<int, 6>{}); break;
+      case 7: row(threads, std::integral_constant<int, 7>{}); break;
+      default: row(threads, std::integral_constant<int, 8>{}); break;
     }
+  };
+  if (d.threads == 64) {
+    if (d.each == 1) row(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    else if (d.each == 2) row(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    else row(std::integral_constant<int, 64>{}, std::integral_constant<int, 4>{});
+  } else if (d.threads == 256) {
+    of(std::integral_constant<int, 256>{});
+  } else if (d.threads) {
+    of(std::integral_constant<int, 1024>{});
   } else {
     const uint64_t all = p.rows;
     p.parts = d.parts;

@@ -171,7 +171,7 @@ __device__ __forceinline__ void eighth(int n, int die, int& first, int& size) {
 
 // WM x WN wavefronts, each with MT x NT tiles of 16 x 16. T is the type
 // multiplied: bf16, f16 or Fp8.
-template <class T, int WM, int WN, int MT, int NT>
+template <class T, int WM, int WN, int MT, int NT, int DEPTH = 2>
 struct Tiled {
   static constexpr int THREADS = 64 * WM * WN, WAVES = WM * WN;
   static constexpr int TM = 16 * WM * MT, TN = 16 * WN * NT;
@@ -180,14 +180,14 @@ struct Tiled {
   static constexpr int STEP = 128 / BYTES;        // summed elements a stage holds
   static constexpr int A_BYTES = TM * 128, B_BYTES = TN * 128, STAGE = A_BYTES + B_BYTES;
   static constexpr int SCALES = FP8 ? (TM + TN) * 4 : 0;  // four blocks' scale bytes of each row
-  // a large tile's stages, or three of half its rows
-  static constexpr int LDS = std::max(2 * (STAGE + SCALES), THREADS == 512 && !FP8 ? 3 * (STAGE - A_BYTES / 2) : 0);
+  // the stages, or of a large tile three of half its rows
+  static constexpr int LDS = std::max(DEPTH * (STAGE + SCALES), THREADS == 512 && !FP8 ? 3 * (STAGE - A_BYTES / 2) : 0);
 };
 
-template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT, class P>
+template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT, int DEPTH, class P>
 __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  using K = Tiled<T, WM, WN, MT, NT>;
+  using K = Tiled<T, WM, WN, MT, NT, DEPTH>;
   constexpr int TM = K::TM, TN = K::TN, WAVES = K::WAVES;
   __shared__ __align__(1024) char lds[K::LDS];
   const int lane = threadIdx.x & 63;
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
     // rows, 2048 -> 2048: forward 51 us, 59 with two; without a loop for half the
     // rows 62. Uneven groups gain nothing: 16384 rows in 16, 160 us of either).
     constexpr bool DEEP = FORM != GRAD_WEIGHT && is_copied(LB) && K::THREADS == 512 && 2 * LIVE <= MT;
-    constexpr int STAGES = DEEP ? 3 : 2, AW = DEEP ? TM / 2 : TM, STAGE = AW * 128 + K::B_BYTES;
+    constexpr int STAGES = DEEP ? 3 : DEPTH, AW = DEEP ? TM / 2 : TM, STAGE = AW * 128 + K::B_BYTES;
     constexpr int COPIES = (AW + TN) / 8 / WAVES;  // of a wavefront in a step
     static_assert(STAGES * STAGE <= K::LDS);
     using WideA = std::integral_constant<int, AW>;
@@ -1015,7 +1015,7 @@ __global__ void __launch_bounds__(256) join_parts(Product p) {
   }
 }
 
-template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT, class P>
+template <class T, class O, int FORM, int LA, int LB, int WM, int WN, int MT, int NT, int DEPTH = 2, class P>
 void launch_tiled(P p, hipStream_t s) {
   using K = Tiled<T, WM, WN, MT, NT>;
   const uint64_t tn = (p.n + K::TN - 1) / K::TN;
@@ -1024,7 +1024,7 @@ void launch_tiled(P p, hipStream_t s) {
     tiles = (((p.m + K::TM - 1) / K::TM * tn + 7) / 8) * 8 * group_parts_max(p.rows, p.groups, p.limit);
   else tiles = (row_tiles_max(p.rows, p.groups, K::TM, p.offsets != nullptr) * tn / 8 + 2) * 8;  // both kinds' eighths
   auto launch = [&](dim3 grid) {
-    hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT, P>), grid, dim3(K::THREADS), 0, s, p);
+    hipLaunchKernelGGL((product_tiled<T, O, FORM, LA, LB, WM, WN, MT, NT, DEPTH, P>), grid, dim3(K::THREADS), 0, s, p);
   };
   if (FORM == GRAD_WEIGHT) {
     if (tiles > PRODUCT_SIZE_MAX) config_error("n", tiles, "gives more tiles than a launch has workgroups");
@@ -1185,6 +1185,11 @@ double tiled_cost(double cost, bool packed, const Product& p) {
   return std::max(cost, (double)std::min(p.rows, p.groups) * p.n * p.k * (packed ? 1 : 2) / 5.9e6);
 }
 
+// The 64 x 64 tiles that a product may have.
+uint64_t small_tiles(const Product& p) {
+  return row_tiles_max(p.rows, p.groups, 64, p.offsets != nullptr) * (((uint64_t)p.n + 63) / 64);
+}
+
 // The tile asked for on this thread, 0 if any; packed rows into f32 have no 256.
 int asked_tile(bool packed_into_f32) {
   return g_kernel == 16 || (packed_into_f32 && g_kernel == 256) ? 0 : g_kernel;
@@ -1221,6 +1226,12 @@ void launch_product(P p, uint64_t room, hipStream_t s) {
       if constexpr (LA != PACKED_ROWS) launch_tiled<T, O, FORM, LA, LB, 2, 4, 8, 4>(p, s);
     } else if (cost.tile >= 128) {
       launch_tiled<T, O, FORM, LA, LB, 2, 2, 4, 4>(p, s);
+    } else if (is_copied(LA) && is_copied(LB) && FORM != GRAD_WEIGHT && p.k > 512 && small_tiles(p) <= 512) {
+      // four stages hide more of the copies' latency, and their LDS is free where a
+      // CU has two workgroups at most (us with four and two: 333 rows, 1000 -> 1500
+      // 9.5, 12.0; 500 in 8 groups, 768 -> 768 7.9, 9.9; 200, 512 -> 512 5.3, 5.1)
+      if constexpr (is_copied(LA) && is_copied(LB) && FORM != GRAD_WEIGHT)
+        launch_tiled<T, O, FORM, LA, LB, 2, 2, 2, 2, 4>(p, s);
     } else {
       launch_tiled<T, O, FORM, LA, LB, 2, 2, 2, 2>(p, s);
     }

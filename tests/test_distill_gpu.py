@@ -342,3 +342,65 @@ def test_distillation_refuses(gpu):
     ]:
         with pytest.raises(error):
             call()
+
+
+def test_an_encoder_is_trained_by_an_index_and_served_token_by_token(gpu):
+    """The operators as they are used together: a layer of experts with a residual makes embeddings, an index' answers
+    are the target, the loss' gradient goes back through both products, and the trained matrices serve single tokens.
+    All gradients against autograd in 64 bits."""
+    import torch
+    g = base._dev(torch, 11)
+    dim, hidden, experts, docs, sizes, t = 64, 128, 4, 500, [40, 0, 21, 67], 0.5
+    rows = sum(sizes)
+    corpus = torch.nn.functional.normalize(torch.randn(docs, dim, generator=g, device="cuda"), dim=1)
+    index = gpu.FlatIndex(gpu.VectorSpace(dim, gpu.Metric.INNER_PRODUCT), docs)
+    index.insert_device(range(docs), corpus)
+    x = torch.randn(rows, dim, generator=g, device="cuda").half()
+    w1 = (torch.randn(experts, hidden, dim, generator=g, device="cuda") / dim ** 0.5).half()
+    w2 = (torch.randn(experts, dim, hidden, generator=g, device="cuda") / hidden ** 0.5).half()
+    b1, b2 = (torch.randn(experts, n, generator=g, device="cuda") * 0.1 for n in (hidden, dim))
+    offsets = base._offsets(torch, sizes)
+    teacher = torch.nn.functional.normalize(x.float() + torch.randn(rows, dim, generator=g, device="cuda"), dim=1)
+    ids = torch.zeros(rows, 10, dtype=torch.int64, device="cuda")
+    dist = torch.zeros(rows, 10, device="cuda")
+    count = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    index.search_device(teacher.contiguous(), 10, ids, dist, count)
+    keys = corpus.half()
+
+    a, h = gpu.grouped_linear(x, w1, offsets, bias=b1, activation="gelu", keep=True)
+    y = gpu.grouped_linear(a, w2, offsets, bias=b2, residual=x)
+    logits = gpu.grouped_linear(y, keys, out_dtype=torch.float32)
+    weight = torch.full((rows,), 1.0 / rows, device="cuda")
+    loss, dlogits = gpu.distill_loss_grad(weight, logits, ids, -dist, count, temperature=t)
+    scale = 1024.0  # f16 gradients of a mean
+    dy = gpu.grouped_matmul_grad_input((dlogits * scale).half(), keys)
+    dw2 = gpu.grouped_matmul_grad_weight(dy, a, offsets, out_dtype=torch.float32) / scale
+    _, db2 = gpu.grouped_linear_grad(dy, offsets=offsets)
+    dh, db1 = gpu.grouped_linear_grad(gpu.grouped_matmul_grad_input(dy, w2, offsets), h, "gelu", offsets)
+    dw1 = gpu.grouped_matmul_grad_weight(dh, x, offsets, out_dtype=torch.float32) / scale
+    db1, db2 = db1 / scale, db2 / scale
+
+    leaves = [v.double().cpu().requires_grad_() for v in (w1, b1, w2, b2)]
+    v1, c1, v2, c2 = leaves
+    out, ends = [], offsets.tolist()
+    for e, (lo, hi) in enumerate(zip(ends[:-1], ends[1:])):
+        z = x[lo:hi].double().cpu()
+        k = z @ v1[e].t() + c1[e]
+        out.append(k * torch.special.ndtr(k) @ v2[e].t() + c2[e] + z)
+    logq = torch.log_softmax(torch.cat(out) @ keys.double().cpu().t() / t, 1)
+    logp = torch.log_softmax(-dist.double().cpu() / t, 1)
+    want = (logp.exp() * (logp - logq.gather(1, ids.cpu()))).sum(1)
+    want.mean().backward()
+    # a, h, y, the logits' gradient, dy, da, dh: seven roundings of 2^-11 of normal values on any path
+    assert float((loss.double().cpu() - want.detach()).norm() / want.detach().norm()) < 7 * 2.0 ** -11
+    for got, leaf in zip((dw1, db1, dw2, db2), leaves):
+        assert float((got.double().cpu() - leaf.grad).norm() / leaf.grad.norm()) < 7 * 2.0 ** -11
+
+    # a few of the rows, each with its expert, as single tokens
+    expert = torch.repeat_interleave(torch.arange(experts, device="cuda"), torch.tensor(sizes, device="cuda"))
+    some = torch.randperm(rows, generator=g, device="cuda")[:9]
+    ones = torch.ones(9, 1, device="cuda")
+    served = gpu.expert_layer(x[some], expert[some, None], w1, w2, ones, activation="gelu", bias1=b1, bias2=b2,
+                              residual=x[some])
+    # the batch rounds a to f16 between the products (2^-11), and both their results
+    assert float((served.double() - y[some].double()).norm() / y[some].double().norm()) < 3 * 2.0 ** -11

@@ -97,6 +97,9 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// weight / T
+__device__ __forceinline__ float factor(const Distill& p, uint64_t row) { return scaled(p, p.weight[row]); }
+
 // The teacher's entries of a row, in LDS: top ids (-1: not valid), p, and logits.
 struct Teacher {
   int* ids;
@@ -128,11 +131,11 @@ __device__ __forceinline__ float read_teacher(const Distill& p, uint64_t row, co
     if (t.ids[i] >= 0) mass += exp_scaled<float>(p, t.p[i] - or_zero(best));
   mass = wave_sum(mass);
   none = mass == 0.0f;
-  const float inverse = 1.0f / mass, log_mass = logf(mass);
+  const float log_mass = logf(mass);
   float sum = 0.0f;
   for (int i = lane; i < p.top; i += 64) {
     const float d = t.p[i] - or_zero(best);
-    const float v = t.ids[i] < 0 || none ? 0.0f : exp_scaled<float>(p, d) * inverse;
+    const float v = t.ids[i] < 0 || none ? 0.0f : exp_scaled<float>(p, d) / mass;
     t.p[i] = v;
     if (v != 0.0f) sum += v * (scaled(p, d) - log_mass);
   }
@@ -151,7 +154,6 @@ __device__ __forceinline__ float cross_entropy(const Distill& p, const Teacher& 
 template <class T, int THREADS>
 __device__ __forceinline__ void store_entries(const Distill& p, const Teacher& t, Softmax row, float k, T* dx, int lo,
                                               int hi) {
-  const float inverse = row.s == 0.0f ? 0.0f : 1.0f / row.s;
   const int sub = threadIdx.x & 7;
   for (int i0 = 0; i0 < p.top; i0 += THREADS / 8) {
     const int i = i0 + threadIdx.x / 8, id = i < p.top ? t.ids[i] : -1;
@@ -161,7 +163,7 @@ __device__ __forceinline__ void store_entries(const Distill& p, const Teacher& t
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     if (sub == 0 && id >= lo && id < hi) {
-      const float q = exp_scaled<T>(p, t.logits[i] - or_zero(row.m)) * inverse;
+      const float q = row.s == 0.0f ? 0.0f : exp_scaled<float>(p, t.logits[i] - or_zero(row.m)) / row.s;
       dx[id] = rounded<T>(k * (q - sum));
     }
   }
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(THREADS, 8) distill_row(Distill p) {
   if constexpr (GRAD) {
     T* dx = (T*)p.dx + row * p.ds;
     const bool aligned = phase_of<T>(dx) == phase;
-    const float k = p.weight[row] * p.t;
+    const float k = factor(p, row);
     const Gradient<T> gradient(p, or_zero(all.m), none || all.s == 0.0f ? 0.0f : k / all.s);
     keep_packed(raw);
     auto store = [&](auto fast) {
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(PART_THREADS) distill_join(Distill p) {
     const int phase = phase_of<T>(x), vectors = (int)(((int64_t)p.cols + phase + EACH<T> - 1) / EACH<T>);
     const int lo = (int)((int64_t)vectors * part / p.parts), hi = (int)((int64_t)vectors * (part + 1) / p.parts);
     const bool aligned = phase_of<T>(dx) == phase;
-    const float k = p.weight[row] * p.t;
+    const float k = factor(p, row);
     const Gradient<T> gradient(p, or_zero(all.m), none || all.s == 0.0f ? 0.0f : k / all.s);
     constexpr int AHEAD = 4;
     for (int v0 = lo + (int)threadIdx.x; v0 < hi; v0 += PART_THREADS * AHEAD) {

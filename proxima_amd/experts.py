@@ -323,11 +323,23 @@ def grouped_matmul_grad_weight(grad, x, offsets, out_dtype=None, out=None):
 _LINEAR, _LINEAR_GRAD, _EXPERT_LAYER, _DISTILL = map(_Struct, ("4q20Q", "3q14Q", "5q34Q", "q10Qd6Q"))
 
 
-def _rows(t, name, dims=2):
-    """Checks a GPU tensor of contiguous rows; (shape, elements from row to row)."""
+def _device(t, name):
+    """The index of the GPU that a call's first operand is on, and so all others."""
     if not getattr(t, "is_cuda", False):
         raise ValueError(f"{name} must be a GPU tensor")
-    shape, strides = t.shape, t.stride()
+    return t.get_device()
+
+
+def _rows(t, name, device, dims=2):
+    """Checks a tensor of contiguous rows on that GPU; (shape, elements from row to row)."""
+    try:
+        on, shape, strides = t.get_device(), t.shape, t.stride()
+    except AttributeError:
+        on = -1
+    if on != device:
+        raise ValueError(f"{name} must be a GPU tensor" if on < 0 else "operands must be on one device")
+    if t.requires_grad and _torch.is_grad_enabled():
+        raise ValueError(_NO_HISTORY)
     if len(strides) != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got {len(strides)}")
     if strides[-1] != 1 and shape[-1] > 1:
@@ -335,14 +347,14 @@ def _rows(t, name, dims=2):
     return shape, strides[-2] if shape[-2] > 1 else shape[-1]
 
 
-def _call(fn, tensors, args):
-    """fn(struct, stream) on torch's current stream of the device that all tensors share."""
-    device = tensors[0].get_device()
+def _here(device, *tensors):
     for t in tensors:
-        if t.get_device() != device:
+        if t is not None and t.get_device() != device:
             raise ValueError("operands must be on one device")
-        if t.requires_grad and _torch.is_grad_enabled():
-            raise ValueError(_NO_HISTORY)
+
+
+def _call(fn, device, args):
+    """fn(struct, stream) on torch's current stream of a device."""
     if _current_device() == device:
         status = fn(args, _current_stream(device))
     else:
@@ -352,7 +364,7 @@ def _call(fn, tensors, args):
         _check(status)
 
 
-def _bias(bias, name, rows, n, dtype, tensors):
+def _bias(bias, name, rows, n, dtype, device):
     """(pointer, pxg_type, elements from row to row) of a bias [rows, n] of `dtype` or f32, [n] where rows is None."""
     if bias is None:
         return 0, 0, 0
@@ -360,39 +372,36 @@ def _bias(bias, name, rows, n, dtype, tensors):
         rows = 1
         if bias.dim() == 1:
             bias = bias.unsqueeze(0)
-    shape, stride = _rows(bias, name)
+    shape, stride = _rows(bias, name, device)
     if shape != (rows, n):
         _mismatch(tuple(shape), (rows, n), f"{name}'s shape")
     kind = bias.dtype
     if kind is not dtype and kind is not _torch.float32:
         raise ValueError(f"{name} must be {dtype} or float32, got {kind}")
-    tensors.append(bias)
     return bias.data_ptr(), _KINDS[kind], stride
 
 
-def _residual(residual, shape, dtype, tensors):
+def _residual(residual, shape, dtype, device):
     """(pointer, elements from row to row)"""
     if residual is None:
         return 0, 0
-    got, stride = _rows(residual, "residual")
+    got, stride = _rows(residual, "residual", device)
     if got != shape:
         _mismatch(tuple(got), shape, "residual's shape")
     if residual.dtype is not dtype:
         raise ValueError(f"residual must be {dtype}, got {residual.dtype}")
-    tensors.append(residual)
     return residual.data_ptr(), stride
 
 
-def _result(out, shape, dtype, like, tensors):
+def _result(out, shape, dtype, like, device):
     """(tensor, elements from row to row)"""
     if out is None:
         return like.new_empty(shape, dtype=dtype), shape[-1]
-    got, stride = _rows(out, "out", len(shape))
+    got, stride = _rows(out, "out", device, len(shape))
     if got != shape:
         _mismatch(tuple(got), shape, "out's shape")
     if out.dtype is not dtype:
         raise ValueError(f"out must be {dtype}, got {out.dtype}")
-    tensors.append(out)
     return out, stride
 
 
@@ -405,22 +414,24 @@ def grouped_linear(x, w, offsets=None, bias=None, activation=None, residual=None
     them, bias [groups, n] (or [n] without offsets) in x's type or f32, f "silu", "gelu" or None, residual [rows, n]
     in y's type. `out` may be the residual itself. With keep, (y, h), h in y's type for grouped_linear_grad. y is
     rounded once, from the unrounded h. Rows of no group: y is the residual, or zeros, and h zeros."""
-    (rows, xk), x_stride = _rows(x, "x")
+    device = _device(x, "x")
+    (rows, xk), x_stride = _rows(x, "x", device)
     xtype = x.dtype
     kind = _type(xtype, "x", False)
     w, ptr, groups, n, k = _weights(w, offsets, x)
+    _, w_stride = _rows(w, "w", device, 3)
     if xk != k:
         _mismatch(xk, k, "x's columns")
-    tensors = [x, w] if offsets is None else [x, w, offsets]
+    _here(device, offsets)
     dtype = out_dtype or (out.dtype if out is not None else xtype)
     out_kind, which = _type(dtype, "out_dtype"), _optional(activation)
-    bias_ptr, bias_kind, bias_stride = _bias(bias, "bias", None if offsets is None else groups, n, xtype, tensors)
-    r, r_stride = _residual(residual, (rows, n), dtype, tensors)
-    out, stride = _result(out, (rows, n), dtype, x, tensors)
+    bias_ptr, bias_kind, bias_stride = _bias(bias, "bias", None if offsets is None else groups, n, xtype, device)
+    r, r_stride = _residual(residual, (rows, n), dtype, device)
+    out, stride = _result(out, (rows, n), dtype, x, device)
     h = x.new_empty((rows, n), dtype=dtype) if keep else None
-    _call(_lib.pxg_grouped_linear_device, tensors,
+    _call(_lib.pxg_grouped_linear_device, device,
           _LINEAR.pack(kind, out_kind, bias_kind, which, rows, k, groups, n, x.data_ptr(), x_stride, w.data_ptr(),
-                       _stride(w), w.stride(0), ptr or 0, bias_ptr, bias_stride, r, r_stride,
+                       w_stride, w.stride(0), ptr or 0, bias_ptr, bias_stride, r, r_stride,
                        h.data_ptr() if keep else 0, n, out.data_ptr(), stride, 0, 0))
     return (out, h) if keep else out
 
@@ -430,15 +441,14 @@ def block8_linear(x, w, offsets=None, bias=None, activation=None, residual=None,
     does, bias bf16 or f32, the rest as grouped_linear."""
     codes, scales, rows, k = _packed(x, "x")
     wcodes, wscales, groups, n, ptr = _packed_weights(w, offsets, k)
-    tensors = [codes, scales, wcodes, wscales]
-    if offsets is not None:
-        tensors.append(offsets)
+    device = codes.get_device()
+    _here(device, scales, wcodes, wscales, offsets)
     dtype = out_dtype or (out.dtype if out is not None else _torch.bfloat16)
     out_kind, which = _type(dtype, "out_dtype"), _optional(activation)
-    bias_ptr, bias_kind, bias_stride = _bias(bias, "bias", None if offsets is None else groups, n, _torch.bfloat16, tensors)
-    r, r_stride = _residual(residual, (rows, n), dtype, tensors)
-    out, stride = _result(out, (rows, n), dtype, codes, tensors)
-    _call(_lib.pxg_block8_linear_device, tensors,
+    bias_ptr, bias_kind, bias_stride = _bias(bias, "bias", None if offsets is None else groups, n, _torch.bfloat16, device)
+    r, r_stride = _residual(residual, (rows, n), dtype, device)
+    out, stride = _result(out, (rows, n), dtype, codes, device)
+    _call(_lib.pxg_block8_linear_device, device,
           _LINEAR.pack(0, out_kind, bias_kind, which, rows, k, groups, n, codes.data_ptr(), 0, wcodes.data_ptr(), 0, 0,
                        ptr or 0, bias_ptr, bias_stride, r, r_stride, 0, 0, out.data_ptr(), stride, scales.data_ptr(),
                        wscales.data_ptr()))
@@ -454,11 +464,12 @@ def grouped_linear_grad(grad, h=None, activation=None, offsets=None, bias_dtype=
     [groups, n] (or [n] without offsets) of bias_dtype (f32 by default, or grad's type). Without an activation dh is
     grad itself. `out` may be grad or h itself. dx and dw are grouped_matmul_grad_input's and
     grouped_matmul_grad_weight's of dh, and the residual's gradient is grad."""
-    (rows, n), grad_stride = _rows(grad, "grad")
+    device = _device(grad, "grad")
+    (rows, n), grad_stride = _rows(grad, "grad", device)
     dtype = grad.dtype
     kind = _type(dtype, "grad")
     ptr, groups = _groups(offsets)
-    tensors = [grad] if offsets is None else [grad, offsets]
+    _here(device, offsets)
     which = _optional(activation)
     if which < 0:
         if h is not None or out is not None:
@@ -467,53 +478,50 @@ def grouped_linear_grad(grad, h=None, activation=None, offsets=None, bias_dtype=
     else:
         if h is None:
             raise ValueError("h must be given with an activation")
-        shape, h_stride = _rows(h, "h")
+        shape, h_stride = _rows(h, "h", device)
         if shape != (rows, n):
             _mismatch(tuple(shape), (rows, n), "h's shape")
         if h.dtype is not dtype:
             raise ValueError(f"h must be {dtype}, got {h.dtype}")
         h_ptr = h.data_ptr()
-        tensors.append(h)
-        dh, stride = _result(out, (rows, n), dtype, grad, tensors)
+        dh, stride = _result(out, (rows, n), dtype, grad, device)
     bias_dtype = bias_dtype or _torch.float32
     if bias_dtype is not dtype and bias_dtype is not _torch.float32:
         raise ValueError(f"bias_dtype must be {dtype} or float32, got {bias_dtype}")
     dbias = grad.new_empty((groups, n) if offsets is not None else (n,), dtype=bias_dtype)
     size = _grad_space(rows, n, groups)
     space = grad.new_empty(size, dtype=_torch.uint8) if size else None
-    _call(_lib.pxg_grouped_linear_grad_device, tensors,
+    _call(_lib.pxg_grouped_linear_grad_device, device,
           _LINEAR_GRAD.pack(kind, _KINDS[bias_dtype], which, rows, n, groups, grad.data_ptr(), grad_stride, h_ptr, h_stride,
                             ptr or 0, dh.data_ptr(), stride, dbias.data_ptr(), n, space.data_ptr() if size else 0, size))
     return dh, dbias
 
 
-def _expert_matrix(w, name, experts, height, width, dtype, tensors):
+def _expert_matrix(w, name, experts, height, width, dtype, device):
     """(data, stride, group stride, scales) of [experts, height, width] matrices, or of a Block8 of [experts * height,
     width] where dtype is None."""
     if dtype is None:
         codes, scales, rows, cols = _packed(w, name)
         if rows != experts * height or cols != width:
             _mismatch((rows, cols), (experts * height, width), f"{name}'s shape")
-        tensors += (codes, scales)
+        _here(device, codes, scales)
         return codes.data_ptr(), 0, 0, scales.data_ptr()
-    shape, stride = _rows(w, name, 3)
+    shape, stride = _rows(w, name, device, 3)
     if shape != (experts, height, width):
         _mismatch(tuple(shape), (experts, height, width), f"{name}'s shape")
     if w.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {w.dtype}")
-    tensors.append(w)
     return w.data_ptr(), stride, w.stride(0), 0
 
 
-def _picks(t, name, dtype, expected, tensors):
+def _picks(t, name, dtype, expected, device):
     """Checks a tensor [rows, some] of `dtype`; (its columns, elements from row to row)."""
-    shape, stride = _rows(t, name)
+    shape, stride = _rows(t, name, device)
     if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     rows, cols = expected
     if shape[0] != rows or (cols is not None and shape[1] != cols):
         _mismatch(tuple(shape), expected, f"{name}'s shape")
-    tensors.append(t)
     return shape[1], stride
 
 
@@ -532,12 +540,12 @@ def expert_layer(x, experts, w1, w2, gates, activation=None, up=None, bias1=None
     bf16); biases [experts, .] of x's type or f32; residual and y [rows, n] of x's type or f32. `out` may be the
     residual itself. Nothing between the two products is rounded to x's type. The matrices of the experts in use are
     read once for each 64 rows: for batches use grouped_linear."""
-    (rows, k), x_stride = _rows(x, "x")
+    device = _device(x, "x")
+    (rows, k), x_stride = _rows(x, "x", device)
     xtype = x.dtype
     kind = _type(xtype, "x", False)
-    tensors = [x]
-    picks, ids_stride = _picks(experts, "experts", _torch.int64, (rows, None), tensors)
-    _, gates_stride = _picks(gates, "gates", _torch.float32, (rows, picks), tensors)
+    picks, ids_stride = _picks(experts, "experts", _torch.int64, (rows, None), device)
+    _, gates_stride = _picks(gates, "gates", _torch.float32, (rows, picks), device)
     packed = type(w1) is Block8
     if packed:
         if xtype is not _torch.bfloat16:
@@ -556,21 +564,21 @@ def expert_layer(x, experts, w1, w2, gates, activation=None, up=None, bias1=None
         number, hidden, _ = _matrix(w1, "w1", 3)
         n = _matrix(w2, "w2", 3)[1]
         of = xtype
-    m1 = _expert_matrix(w1, "w1", number, hidden, k, of, tensors)
-    m3 = _expert_matrix(up, "up", number, hidden, k, of, tensors) if up is not None else (0, 0, 0, 0)
-    m2 = _expert_matrix(w2, "w2", number, n, hidden, of, tensors)
+    m1 = _expert_matrix(w1, "w1", number, hidden, k, of, device)
+    m3 = _expert_matrix(up, "up", number, hidden, k, of, device) if up is not None else (0, 0, 0, 0)
+    m2 = _expert_matrix(w2, "w2", number, n, hidden, of, device)
     if bias1 is not None and bias2 is not None and bias1.dtype is not bias2.dtype:
         raise ValueError(f"biases must be of one type, got {bias1.dtype} and {bias2.dtype}")
-    b1, kind1, stride1 = _bias(bias1, "bias1", number, hidden, xtype, tensors)
-    b2, kind2, stride2 = _bias(bias2, "bias2", number, n, xtype, tensors)
+    b1, kind1, stride1 = _bias(bias1, "bias1", number, hidden, xtype, device)
+    b2, kind2, stride2 = _bias(bias2, "bias2", number, n, xtype, device)
     dtype = out_dtype or (out.dtype if out is not None else xtype)
     out_kind = _type(dtype, "out_dtype")
     which = _optional(activation)
-    r, r_stride = _residual(residual, (rows, n), dtype, tensors)
-    out, stride = _result(out, (rows, n), dtype, x, tensors)
+    r, r_stride = _residual(residual, (rows, n), dtype, device)
+    out, stride = _result(out, (rows, n), dtype, x, device)
     size = _layer_space(rows, picks, number, hidden, n, out_kind)
     space = x.new_empty(size, dtype=_torch.uint8) if size else None
-    _call(_lib.pxg_expert_layer_device, tensors,
+    _call(_lib.pxg_expert_layer_device, device,
           _EXPERT_LAYER.pack(kind, out_kind, kind1 if b1 else kind2, which, packed, rows, k, picks, number, hidden, n,
                              x.data_ptr(), x_stride, experts.data_ptr(), ids_stride, gates.data_ptr(), gates_stride, *m1,
                              *m3, *m2, b1, stride1, b2, stride2, r, r_stride, out.data_ptr(), stride,
@@ -612,10 +620,12 @@ def activation_grad(grad, packed, activation, out=None):
     return out
 
 
-def _vector(t, name, rows, dtype):
-    """Checks a contiguous GPU tensor of `rows` values."""
-    if not getattr(t, "is_cuda", False):
-        raise ValueError(f"{name} must be a GPU tensor")
+def _vector(t, name, rows, dtype, device):
+    """Checks a contiguous tensor of `rows` values on a GPU."""
+    if _device(t, name) != device:
+        raise ValueError("operands must be on one device")
+    if t.requires_grad and _torch.is_grad_enabled():
+        raise ValueError(_NO_HISTORY)
     if t.dim() != 1 or not t.is_contiguous() or t.dtype is not dtype:
         raise ValueError(f"{name} must be a contiguous one-dimensional {dtype} tensor")
     if t.shape[0] != rows:
@@ -627,23 +637,22 @@ _distill_space = _lru_cache(1024)(_lib.pxg_distill_workspace)
 
 
 def _distill(fn, weight, logits, ids, scores, counts, temperature, grad, out):
-    (rows, cols), stride = _rows(logits, "logits")
+    device = _device(logits, "logits")
+    (rows, cols), stride = _rows(logits, "logits", device)
     dtype = logits.dtype
     kind = _type(dtype, "logits")
-    tensors = [logits, counts]
-    top, ids_stride = _picks(ids, "ids", _torch.int64, (rows, None), tensors)
-    _, scores_stride = _picks(scores, "scores", _torch.float32, (rows, top), tensors)
-    counts_ptr = _vector(counts, "counts", rows, _torch.int32)
+    top, ids_stride = _picks(ids, "ids", _torch.int64, (rows, None), device)
+    _, scores_stride = _picks(scores, "scores", _torch.float32, (rows, top), device)
+    counts_ptr = _vector(counts, "counts", rows, _torch.int32, device)
     weight_ptr = out_ptr = out_stride = 0
     if grad:
-        weight_ptr = _vector(weight, "weight", rows, _torch.float32)
-        tensors.append(weight)
-        out, out_stride = _result(out, (rows, cols), dtype, logits, tensors)
+        weight_ptr = _vector(weight, "weight", rows, _torch.float32, device)
+        out, out_stride = _result(out, (rows, cols), dtype, logits, device)
         out_ptr = out.data_ptr()
     loss = logits.new_empty((rows,), dtype=_torch.float32)
     size = _distill_space(kind, rows, cols, top)
     space = logits.new_empty(size, dtype=_torch.uint8) if size else None
-    _call(fn, tensors,
+    _call(fn, device,
           _DISTILL.pack(kind, rows, cols, top, logits.data_ptr(), stride, ids.data_ptr(), ids_stride, scores.data_ptr(),
                         scores_stride, counts_ptr, float(temperature), loss.data_ptr(), weight_ptr, out_ptr, out_stride,
                         space.data_ptr() if size else 0, size))

@@ -200,11 +200,12 @@ __device__ __forceinline__ void unpack(uint4 raw, float (&x)[EACH<T>]) {
 #pragma unroll
   for (int e = 0; e < EACH<T>; ++e) x[e] = (float)v[e];
 }
-template <class T>
+template <class T, bool ONCE = false>
 __device__ __forceinline__ void store_vector(T* row, int v, int phase, int cols, bool aligned, uint4 x) {
   const int64_t at = (int64_t)v * EACH<T> - phase;
   if (aligned && at >= 0 && at + EACH<T> <= cols) {
-    *reinterpret_cast<uint4*>(row + at) = x;
+    if constexpr (ONCE) store_once(row + at, x);
+    else *reinterpret_cast<uint4*>(row + at) = x;
   } else {
     T y[EACH<T>];
     __builtin_memcpy(y, &x, 16);
@@ -318,14 +319,16 @@ __device__ __forceinline__ Softmax softmax_of(const Distill& p, uint4 (&raw)[N],
 }
 
 // A workgroup's row in registers: N vectors of a thread. 4096 x 50000 in bf16
-// with top 100: 177 us, 4.6 TB/s. (With rows one after another in workgroups
+// with top 100: 180 us, 4.5 TB/s. (With rows one after another in workgroups
 // that load the next while they store, whose registers leave 512 threads: 225;
-// with a maximum of floats and a factor: 198.)
+// with a maximum of floats and a factor: 198, for 188 past no caches.)
 template <class T, int THREADS, int N, bool GRAD>
 __global__ void __launch_bounds__(THREADS, 8) distill_row(Distill p) {
   extern __shared__ __align__(16) char lds[];
   __shared__ Softmax waves[THREADS / 64];
   __shared__ int no_teacher;
+  // long rows are many bytes: past the caches (188 us without, 207 with loads alone)
+  constexpr bool ONCE = THREADS == 1024;
   const uint64_t row = p.first + blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T* x = (const T*)p.x + row * p.xs;
@@ -334,7 +337,10 @@ __global__ void __launch_bounds__(THREADS, 8) distill_row(Distill p) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int v = i * THREADS + threadIdx.x;
-    if (is_whole<T>(v, phase, p.cols)) raw[i] = *reinterpret_cast<const uint4*>(x + ((int64_t)v * EACH<T> - phase));
+    if (is_whole<T>(v, phase, p.cols)) {
+      const T* from = x + ((int64_t)v * EACH<T> - phase);
+      raw[i] = ONCE ? load_once(from) : *reinterpret_cast<const uint4*>(from);
+    }
   }
   const Teacher t = teacher_at(lds, p.top);
   float entropy = 0.0f;
@@ -368,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, 8) distill_row(Distill p) {
       for (int i = 0; i < N; ++i) {
         const int v = i * THREADS + threadIdx.x;
         if (v < vectors)
-          store_vector<T>(dx, v, phase, p.cols, aligned, gradient.template of<decltype(fast)::value>(p, raw[i]));
+          store_vector<T, ONCE>(dx, v, phase, p.cols, aligned, gradient.template of<decltype(fast)::value>(p, raw[i]));
       }
     };
     if (sizeof(T) == 2 && gradient.fast) store(std::true_type{});
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(PART_THREADS) distill_join(Distill p) {
 //   16 rows of 20000     held 9.7, in parts 14.3
 //   64 of 60000               14.0,          14.5
 //   8192 of 9000         by 256 threads 61, by 1024 103
-//   8192 of 1000         by 64 threads 15.6, by 256 25.8
+//   8192 of 1000         by 64 threads 15.6, by 256 25.8; 64 rows (f32) 7.3, 5.9
 // (Parts of as many rows at a time as the last cache holds until they are read
 // again: 1000 rows of 200000 268, of all of them 264.)
 struct DistillPlan {
@@ -499,8 +505,8 @@ DistillPlan distill_plan(int type, uint64_t rows, uint64_t cols, uint64_t top) {
   DistillPlan d{0, 0, 0, 0};
   const uint64_t each = type == PXG_F32 ? 4 : 8, vectors = (cols + 2 * each - 2) / each;  // at any alignment
   if (vectors <= HELD_MAX) {
-    // small workgroups where they hold a row: more rows are on their way at once
-    d.threads = vectors <= 256 ? 64 : vectors <= 2048 ? 256 : 1024;
+    // small workgroups where rows are many: more of them are on their way at once
+    d.threads = vectors <= 256 && rows > 1024 ? 64 : vectors <= 1024 || (vectors <= 2048 && rows > 512) ? 256 : 1024;
     d.each = (int)((vectors + d.threads - 1) / d.threads);
     return d;
   }

@@ -14,7 +14,9 @@
 namespace pxg {
 namespace {
 
-// The backward pass reads dy and h and writes dh once, and memory bounds it.
+// The backward pass reads dy and h and writes dh once, and memory bounds it: 16384
+// x 4096 in bf16, GELU 77 us, 5.2 TB/s, and 5 us for the bias (88 with dy and h
+// in the caches).
 // Rows go in tiles of one group; a workgroup takes a tile by 8 p.x columns, a
 // thread every 256 / p.x-th row of 8 columns, whose sums it keeps.
 // The workgroup's sums are joined in LDS and go to the tile's row of the
@@ -143,6 +145,8 @@ GradPlan grad_plan(uint64_t rows, uint64_t n, uint64_t groups, bool ragged) {
   while (g.x < 32 && g.x * 8 < n) g.x *= 2;
   const uint64_t strips = (n + g.x * 8 - 1) / (g.x * 8), high = GRAD_THREADS / g.x;
   g.strips = (unsigned)std::min<uint64_t>(strips, 1024);
+  // a few rounds of a group's rows cost less than a second kernel (35 rows x 3375: 11.4 us, 14.8)
+  if (rows <= 4 * high * GRAD_BATCH) return g;
   const uint64_t least = high * 2;
   uint64_t tile = std::max((rows * g.strips + 2047) / 2048, (rows >> 21) + 1);
   tile = (tile + least - 1) / least * least;

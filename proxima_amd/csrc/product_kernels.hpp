@@ -78,6 +78,10 @@ struct LinearProduct : Product {
   uint64_t rs = 0;
   void* kept = nullptr;  // h in the result's type, rows hs apart
   uint64_t hs = 0;
+  // y and h go past the caches, which keep the operands (with h kept 138 us, 127:
+  // 8192 rows in 8 groups, 1024 -> 4096; what reads results as large finds them
+  // in no L2 either way)
+  bool once = false;
 };
 
 // ---------------------------------------------------------------------------
@@ -722,7 +726,10 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
           if (row >= rows) continue;
           R* to = c + (uint64_t)row * stride + col;
           if (col + EACH <= cols) {
-            *reinterpret_cast<uint4*>(to) = v;
+            bool once = false;
+            if constexpr (is_linear<P>) once = p.once;
+            if (once) store_once(to, v);
+            else *reinterpret_cast<uint4*>(to) = v;
           } else {
             R x[EACH];
             *reinterpret_cast<uint4*>(x) = v;
@@ -1195,10 +1202,13 @@ int asked_tile(bool packed_into_f32) {
   return g_kernel == 16 || (packed_into_f32 && g_kernel == 256) ? 0 : g_kernel;
 }
 
+constexpr uint64_t ONCE_BYTES = 16 << 20;  // half of the L2s
+
 // `room`: bytes of p.workspace.
 template <int FORM, class T, class O, bool IS_PACKED, class P>
 void launch_product(P p, uint64_t room, hipStream_t s) {
   p.c_vec = ((uint64_t)(uintptr_t)p.c | p.cs * sizeof(O) | p.cg * sizeof(O)) % 16 == 0;
+  if constexpr (is_linear<P>) p.once = (uint64_t)p.rows * p.n * sizeof(O) * (p.kept ? 2 : 1) >= ONCE_BYTES;
   if constexpr (is_linear<P>)  // and the residual's and the kept rows
     p.c_vec = p.c_vec && ((uint64_t)(uintptr_t)p.residual | (p.residual ? p.rs * sizeof(O) : 0) |
                           (uint64_t)(uintptr_t)p.kept | (p.kept ? p.hs * sizeof(O) : 0)) % 16 == 0;

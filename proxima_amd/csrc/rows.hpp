@@ -32,7 +32,16 @@ __device__ __forceinline__ void load8(const T* __restrict__ row, uint64_t c, uin
   }
 }
 
-// The same, left packed in T.
+// 16 bytes that are read or written once: the caches keep others.
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u4v*)p));
+}
+__device__ __forceinline__ void store_once(void* p, uint4 x) {
+  __builtin_nontemporal_store(__builtin_bit_cast(u4v, x), (u4v*)p);
+}
+
+// The same, left packed in T and read once.
 template <class T>
 struct Eight {
   uint4 q[sizeof(T) / 2];
@@ -49,7 +58,7 @@ __device__ __forceinline__ Eight<T> raw8(const T* __restrict__ row, uint64_t c, 
   if (VEC && c + 8 <= cols) {
     const uint4* p = reinterpret_cast<const uint4*>(row + c);
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.q[i] = p[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.q[i] = load_once(p + i);
   } else {
     T v[8];
 #pragma unroll

@@ -34,6 +34,7 @@ namespace {
 constexpr int BLOCK_TOKENS = 64, PICKS_MAX = 16;
 [[maybe_unused]] constexpr int ENTRIES_MAX = BLOCK_TOKENS * PICKS_MAX;  // experts in use of a block
 constexpr uint64_t EXPERTS_MAX = 1u << 16, TOKENS_MAX = 1u << 16;
+constexpr uint64_t SLICE_BYTES = 32 << 10;
 constexpr int TOKENS_WAVES = 8, TOKENS_THREADS = 64 * TOKENS_WAVES;
 
 struct ExpertMatrix {  // of every expert; strides in elements (packed: bytes of codes)
@@ -515,7 +516,8 @@ struct TokensPlan {
 };
 uint64_t pieces_of(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-TokensPlan tokens_plan(uint64_t rows, uint64_t picks, uint64_t experts, uint64_t hidden, uint64_t n, bool f32_out) {
+TokensPlan tokens_plan(uint64_t rows, uint64_t picks, uint64_t experts, uint64_t hidden, uint64_t n, bool f32_out,
+                       bool packed) {
   TokensPlan t;
   t.blocks = (rows + BLOCK_TOKENS - 1) / BLOCK_TOKENS;
   const uint64_t pairs = std::min<uint64_t>(rows, BLOCK_TOKENS) * picks;
@@ -523,8 +525,11 @@ TokensPlan tokens_plan(uint64_t rows, uint64_t picks, uint64_t experts, uint64_t
   t.wide = (hidden + 127) / 128 * 128;
   t.planes_bytes = pieces_of(rows * picks * (f32_out ? 3 : 2) * t.wide * 2);
   t.entries_bytes = pieces_of(t.blocks * (t.entries_max + 1) * sizeof(Entry));
-  const uint64_t tiles = (n + 15) / 16 * t.blocks, chunks = t.entries_max * ((hidden + 63) / 64);
-  t.slices = (int)std::max<uint64_t>(1, std::min({(uint64_t)512 / tiles, chunks / (2 * TOKENS_WAVES), (uint64_t)32}));
+  // As many slices as fill the chip, of at least 32 KB each: two chunks for each
+  // wavefront of a workgroup (of at least 96 KB: 18 tokens, 512 -> 3904 -> 387, 3
+  // gated experts 33 us for 25; 53 tokens, 2672 -> 1193 -> 1344, 2 experts 40 for 33).
+  const uint64_t tiles = (n + 15) / 16 * t.blocks, bytes = t.entries_max * 16 * hidden * (packed ? 1 : 2);
+  t.slices = (int)std::max<uint64_t>(1, std::min({(uint64_t)512 / tiles, bytes / SLICE_BYTES, (uint64_t)32}));
   t.partial_bytes = t.slices > 1 ? pieces_of(4 * t.slices * rows * n) : 0;
   return t;
 }
@@ -603,7 +608,8 @@ uint64_t pxg_expert_layer_workspace(uint64_t rows, uint64_t picks, uint64_t expe
   if (rows == 0 || rows > TOKENS_MAX || picks == 0 || picks > PICKS_MAX || experts == 0 || experts > EXPERTS_MAX ||
       hidden == 0 || hidden > (1u << 22) || n == 0 || n > PRODUCT_SIZE_MAX)
     return 0;
-  return workspace_bytes_of(tokens_plan(rows, picks, experts, hidden, n, out_type == PXG_F32));
+  // enough for packed matrices as for others, whose slices are more
+  return workspace_bytes_of(tokens_plan(rows, picks, experts, hidden, n, out_type == PXG_F32, false));
 }
 
 int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream) {
@@ -642,7 +648,7 @@ int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream) {
     check_rows(a.out_type, "y", a.y, a.rows, a.n, a.y_stride);
     p.xs = check_stride(a.rows, a.k, a.x_stride);
     if (a.rows == 0) return;
-    const TokensPlan t = tokens_plan(a.rows, a.picks, a.experts, a.hidden, a.n, a.out_type == PXG_F32);
+    const TokensPlan t = tokens_plan(a.rows, a.picks, a.experts, a.hidden, a.n, a.out_type == PXG_F32, packed);
     check_aligned("workspace", a.workspace, 16);
     if (!a.workspace || a.workspace_bytes < workspace_bytes_of(t))
       config_error("workspace_bytes", a.workspace_bytes, "must be what pxg_expert_layer_workspace says");

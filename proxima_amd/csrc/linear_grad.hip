@@ -145,8 +145,9 @@ GradPlan grad_plan(uint64_t rows, uint64_t n, uint64_t groups, bool ragged) {
   while (g.x < 32 && g.x * 8 < n) g.x *= 2;
   const uint64_t strips = (n + g.x * 8 - 1) / (g.x * 8), high = GRAD_THREADS / g.x;
   g.strips = (unsigned)std::min<uint64_t>(strips, 1024);
-  // a few rounds of a group's rows cost less than a second kernel (35 rows x 3375: 11.4 us, 14.8)
-  if (rows <= 4 * high * GRAD_BATCH) return g;
+  // one round of a group's rows costs less than a second kernel (35 rows x 3375, GELU, bf16: 11.4 us, 14.8;
+  // of four, 120 rows x 1710 in f32 would take 38)
+  if (rows <= high * GRAD_BATCH) return g;
   const uint64_t least = high * 2;
   uint64_t tile = std::max((rows * g.strips + 2047) / 2048, (rows >> 21) + 1);
   tile = (tile + least - 1) / least * least;

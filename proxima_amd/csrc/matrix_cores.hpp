@@ -8,6 +8,7 @@
 
 namespace pxg {
 
+typedef uint32_t u4w __attribute__((ext_vector_type(4)));
 typedef int i8v __attribute__((ext_vector_type(8)));
 typedef float f4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
@@ -43,6 +44,45 @@ __device__ __forceinline__ uint4 decode_bf16(uint32_t x, uint32_t y, float s) {
   const bf2v d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(y, s, true);
   return make_uint4(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, c),
                     __builtin_bit_cast(uint32_t, d));
+}
+
+// 8 16-bit elements of a row that a resource covers, from byte `at` of it on.
+// ANY: rows begin at any multiple of two bytes; the words that hold them are
+// read and shifted.
+template <bool ANY>
+struct Piece {
+  uint4 v;
+  [[maybe_unused]] uint32_t last;
+};
+template <bool ANY>
+__device__ __forceinline__ Piece<ANY> load_piece(__amdgpu_buffer_rsrc_t rs, uint32_t at, bool in) {
+  Piece<ANY> x;
+  x.v = __builtin_bit_cast(uint4, (u4w)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)(in ? at & ~3u : NOWHERE), 0, 0));
+  if constexpr (ANY) x.last = __builtin_amdgcn_raw_buffer_load_b32(rs, (int)(in ? (at & ~3u) + 16 : NOWHERE), 0, 0);
+  return x;
+}
+// The elements, zeros from the `valid`-th on (without ANY all of them or none are).
+template <bool ANY>
+__device__ __forceinline__ uint4 elements(const Piece<ANY>& x, uint32_t at, int valid) {
+  if constexpr (!ANY) {
+    return x.v;
+  } else {
+    const uint32_t w[5] = {x.v.x, x.v.y, x.v.z, x.v.w, x.last}, shift = (at & 2) * 8;
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t both = __builtin_amdgcn_alignbit(w[e + 1], w[e], shift);
+      v[e] = valid > 2 * e + 1 ? both : valid > 2 * e ? both & 0xFFFF : 0;
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+}
+// A resource over rows of 16-bit elements whose last ends `bytes` from p on, and
+// what an offset of it begins at.
+template <bool ANY>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const char* p, uint64_t bytes, uint32_t& odd) {
+  odd = ANY ? (uint32_t)(uintptr_t)p & 2 : 0;
+  return tile_rsrc(p - odd, ANY ? (bytes + odd + 3) & ~3ull : bytes);
 }
 #endif
 

@@ -846,7 +846,8 @@ __global__ void __launch_bounds__(64 * WM * WN) product_tiled(P p) {
 // two rounds of loads in registers are faster than eight with one workgroup
 // (16 groups of one row, 2048 -> 2048: 29 us, 41; one row, 4096 -> 4096: 8.8, 8.9).
 // ---------------------------------------------------------------------------
-template <class T, class O, int LB, bool IS_PACKED, class P>
+// ANY (ROWS, not packed): rows of A and of the matrix begin at any multiple of two bytes.
+template <class T, class O, int LB, bool IS_PACKED, bool ANY, class P>
 __global__ void __launch_bounds__(512, 4) product_few(P p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   constexpr int WAVES = 8, N16 = LB == ROWS ? 1 : 8;     // tiles of 16 columns of C
@@ -863,26 +864,27 @@ __global__ void __launch_bounds__(512, 4) product_few(P p) {
   const int rows = t.end - t.row < 16 ? t.end - t.row : 16, cols = p.n - n0 < TN ? p.n - n0 : TN;
   const int k_end = t.group < 0 ? 0 : p.k, group = t.group < 0 ? 0 : t.group;
   constexpr int BYTES = IS_PACKED ? 1 : 2;
-  const auto ra = tile_rsrc((const char*)p.a + (uint64_t)t.row * p.as * BYTES,
-                            ((uint64_t)(rows - 1) * p.as + p.k) * BYTES);
-  const uint32_t oa = r16 < rows ? (uint32_t)(r16 * p.as * BYTES) + q * 16 : NOWHERE;  // this lane's row of A
+  uint32_t odd = 0;
+  const auto ra = rows_rsrc<ANY>((const char*)p.a + (uint64_t)t.row * p.as * BYTES,
+                                 ((uint64_t)(rows - 1) * p.as + p.k) * BYTES, odd);
+  const uint32_t oa = r16 < rows ? odd + (uint32_t)(r16 * p.as * BYTES) + q * 16 : NOWHERE;  // this lane's row of A
   f4v acc[N16] = {};
-  typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-  auto load = [&](__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
-    return __builtin_bit_cast(uint4, (u4v)__builtin_amdgcn_raw_buffer_load_b128(rs, (int)offset, 0, 0));
+  [[maybe_unused]] auto load = [&](__amdgpu_buffer_rsrc_t rs, uint32_t offset) {
+    return load_piece<false>(rs, offset, offset != NOWHERE).v;
   };
   if constexpr (LB == ROWS) {
     const uint64_t row = (uint64_t)group * p.n + n0;  // packed: of the codes
-    const auto rb = tile_rsrc(IS_PACKED ? (const char*)p.b + row * p.bs : (const char*)p.b + (group * p.bg + n0 * p.bs) * 2,
-                              ((uint64_t)(cols - 1) * p.bs + p.k) * BYTES);
-    const uint32_t ob = r16 < cols ? (uint32_t)(r16 * p.bs * BYTES) + q * 16 : NOWHERE;
+    const auto rb = rows_rsrc<ANY>(IS_PACKED ? (const char*)p.b + row * p.bs
+                                             : (const char*)p.b + (group * p.bg + n0 * p.bs) * 2,
+                                   ((uint64_t)(cols - 1) * p.bs + p.k) * BYTES, odd);
+    const uint32_t ob = r16 < cols ? odd + (uint32_t)(r16 * p.bs * BYTES) + q * 16 : NOWHERE;
     [[maybe_unused]] __amdgpu_buffer_rsrc_t rsa, rsb;
     if constexpr (IS_PACKED) {
       rsa = tile_rsrc(p.a_scales + (uint64_t)t.row * p.ss, (uint64_t)rows * p.ss);
       rsb = tile_rsrc(p.b_scales + row * p.ss, (uint64_t)cols * p.ss);
     }
     for (int k0 = wave * ROUND; k0 < k_end; k0 += WAVES * ROUND * AHEAD) {
-      uint4 b[AHEAD][PIECES], a[AHEAD][PIECES];
+      Piece<ANY> b[AHEAD][PIECES], a[AHEAD][PIECES];
       [[maybe_unused]] uint32_t xb[AHEAD], xa[AHEAD];
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
@@ -891,8 +893,8 @@ __global__ void __launch_bounds__(512, 4) product_few(P p) {
         for (int h = 0; h < PIECES; ++h) {
           // past the rows' end: zeros
           const bool in = (k * BYTES + h * 64 + q * 16) < k_end * BYTES;
-          b[u][h] = load(rb, in && ob != NOWHERE ? ob + k * BYTES + h * 64 : NOWHERE);
-          a[u][h] = load(ra, in && oa != NOWHERE ? oa + k * BYTES + h * 64 : NOWHERE);
+          b[u][h] = load_piece<ANY>(rb, ob + k * BYTES + h * 64, in && ob != NOWHERE);
+          a[u][h] = load_piece<ANY>(ra, oa + k * BYTES + h * 64, in && oa != NOWHERE);
         }
         if constexpr (IS_PACKED) {
           const bool in = k < k_end;
@@ -907,12 +909,13 @@ __global__ void __launch_bounds__(512, 4) product_few(P p) {
         for (int h = 0; h < PIECES; ++h) {
           if constexpr (IS_PACKED) {
             // 16 codes a lane: 8 for each of two instructions, of A as of B
-            const uint4 x = a[u][h], y = b[u][h];
+            const uint4 x = a[u][h].v, y = b[u][h].v;
             const float sa = block8_scale(xa[u]), sb = block8_scale(xb[u]);
             acc[0] = mfma16<T>(decode_bf16(y.x, y.y, sb), decode_bf16(x.x, x.y, sa), acc[0]);
             acc[0] = mfma16<T>(decode_bf16(y.z, y.w, sb), decode_bf16(x.z, x.w, sa), acc[0]);
           } else {
-            acc[0] = mfma16<T>(b[u][h], a[u][h], acc[0]);
+            const int left = k_end - (k0 + u * WAVES * ROUND + h * 32 + q * 8);
+            acc[0] = mfma16<T>(elements(b[u][h], ob, left), elements(a[u][h], oa, left), acc[0]);
           }
         }
     }
@@ -1049,14 +1052,14 @@ bool copies(int bytes, const void* d, uint64_t cols, uint64_t stride, uint64_t g
   return ((uint64_t)(uintptr_t)d | cols * bytes | stride * bytes | group_stride * bytes) % 16 == 0;
 }
 
-template <class T, class O, int LB, bool IS_PACKED, class P>
+template <class T, class O, int LB, bool IS_PACKED, bool ANY = false, class P>
 void launch_few(P p, hipStream_t s) {
   constexpr uint64_t TN = LB == ROWS ? 16 : 128;
   const uint64_t tiles = row_tiles_max(p.rows, p.groups, 16, p.offsets != nullptr) * ((p.n + TN - 1) / TN);
   by_tiles(tiles, p, [&](dim3 grid) {
-    hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED, P>), grid, dim3(512), 0, s, p);
+    hipLaunchKernelGGL((product_few<T, O, LB, IS_PACKED, ANY, P>), grid, dim3(512), 0, s, p);
   });
-  g_last_kernel = 16;
+  g_last_kernel = 16 | (ANY ? PXG_KERNEL_UNALIGNED : 0);
 }
 
 // Which tiles a product takes: the cheapest by what was measured, in us. A
@@ -1227,6 +1230,10 @@ void launch_product(P p, uint64_t room, hipStream_t s) {
     const double tiled = std::is_same_v<O, float> ? cost.best : std::min(cost.best, cost.fp8);
     const bool few = g_kernel ? g_kernel == 16 : few_cost(B, IS_PACKED, p) <= tiled_cost(tiled, IS_PACKED, p);
     if (copied && reaches && few) return launch_few<T, O, B, IS_PACKED>(p, s);
+    // rows that are not whole 16-byte pieces: their tiles take half as long again as estimated (us by this kernel and
+    // by tiles: 1 row, 4100 -> 4097 14, 55; 100 rows, 1001 -> 1501 10, 17; 64 in 8 groups, 2001 -> 513 12, 26)
+    if constexpr (FORM == FORWARD && !IS_PACKED && is_linear<P>)
+      if (!copied && (g_kernel ? g_kernel == 16 : few_cost(B, false, p) <= 1.5 * tiled)) return launch_few<T, O, B, false, true>(p, s);
   }
   if constexpr (FORM == GRAD_WEIGHT) p.limit = cost.limit;
   if constexpr (FORM == FORWARD && IS_PACKED && !std::is_same_v<O, float>)

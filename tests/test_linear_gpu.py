@@ -105,7 +105,7 @@ def test_layers_of_ragged_groups(gpu, take, kernel, n, k, case):
     assert torch.equal(got, again)
     if x.shape[0] and kernel:
         last = kernels._last(gpu)
-        assert last == kernel if k % 8 == 0 else last & kernels.UNALIGNED
+        assert last == kernel if k % 8 == 0 else last == (kernel if kernel == 16 else min(kernel, 128)) | kernels.UNALIGNED
 
 
 @pytest.mark.parametrize("kernel", [0, 16, 64, 128, 256])
@@ -135,7 +135,7 @@ def test_packed_layers_of_ragged_groups(gpu, take, kernel, n, k, case):
 
 def test_a_layer_without_anything_is_the_product(gpu):
     import torch
-    for sizes, n, k in (([5, 0, 70], 64, 136), ([700, 900], 512, 384), ([31], 77, 45)):
+    for sizes, n, k in (([5, 0, 70], 64, 136), ([700, 900], 512, 384), ([31], 77, 48)):
         x, w, _, offsets = base._make(torch, sizes, n, k, torch.bfloat16, 3, 1, 2)
         for out in (torch.bfloat16, torch.float32):
             assert torch.equal(gpu.grouped_linear(x, w, offsets, out_dtype=out),

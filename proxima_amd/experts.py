@@ -2,14 +2,17 @@
 
 The products of a layer whose rows are routed in ragged groups, each group with
 a matrix of its own, their gradients, the same product over rows packed in 8
-bits, and activations whose input is kept packed for their backward pass. No
-reference counterpart: these are the layers whose outputs an index stores.
+bits, and activations whose input is kept packed for their backward pass;
+layers with their bias, activation and residual, and their backward pass; whole
+layers for a few tokens; and the loss of an encoder that learns to rank as an
+index' answers do. No reference counterpart: these are the layers whose outputs
+an index stores.
 
 All functions take torch tensors on the GPU, run on torch's current stream and
 return without waiting; outputs are new tensors unless `out` is given. Rows may
 be strided; a row's columns are contiguous. `offsets` is an int64 tensor of
 groups + 1 values: group g is the rows offsets[g] to offsets[g + 1], and rows
-of no group get zeros.
+of no group get zeros (a layer's: its residual).
 
 None of them records history for autograd: the gradients are functions of their
 own. An operand that requires grad is refused while grad mode is on, so that no

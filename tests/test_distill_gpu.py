@@ -404,3 +404,26 @@ def test_an_encoder_is_trained_by_an_index_and_served_token_by_token(gpu):
                               residual=x[some])
     # the batch rounds a to f16 between the products (2^-11), and both their results
     assert float((served.double() - y[some].double()).norm() / y[some].double().norm()) < 3 * 2.0 ** -11
+
+
+def test_two_streams_and_two_graphs_at_once(gpu):
+    import torch
+    cases = [_make(torch, rows, cols, 8, torch.bfloat16, 1.0, cols) for rows, cols in ((70, 3000), (5, 90000))]
+    wants = [gpu.distill_loss_grad(w, x, i, s, c) for x, i, s, c, w in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    graphs, held = [], []
+    torch.cuda.synchronize()
+    for (x, i, s, c, w), stream in zip(cases, streams):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            held.append(gpu.distill_loss_grad(w, x, i, s, c))
+        graphs.append(graph)
+    for _ in range(6):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [gpu.distill_loss_grad(w, x, i, s, c) for x, i, s, c, w in cases]
+        torch.cuda.synchronize()
+        for got in (held, eager):
+            for a, b in zip(got, wants):
+                assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])

@@ -497,3 +497,22 @@ def test_layers_refuse(gpu):
     ]:
         with pytest.raises(error):
             call()
+
+
+@pytest.mark.parametrize("dtype,n,k", [("bfloat16", 2048, 192), ("float16", 2056, 200), ("bfloat16", 2049, 128)])
+def test_large_results_are_written_past_the_caches(gpu, dtype, n, k):
+    # y and h of 16 MB and more, of whole and of odd rows, which the next calls read
+    import torch
+    dtype = getattr(torch, dtype)
+    sizes = [2600, 90, 0, 1900, 128]
+    x, w, _, offsets = base._make(torch, sizes, n, k, dtype, 33, 4, 3)
+    ends = offsets.tolist()
+    bias, residual = _extras(torch, x, w, 5, dtype, dtype, 2)
+    h, size = base._per_row(torch, x, w, ends, True)
+    y, kept = gpu.grouped_linear(x, w, offsets, bias=bias, activation="gelu", residual=residual, keep=True)
+    _check_layer(torch, y, kept, h, size, k, bias, ends, "gelu", residual)
+    dh, dbias = gpu.grouped_linear_grad(y, kept, "silu", offsets)
+    _check_grad(torch, dh, dbias, y, kept, "silu", ends)
+    held = residual.clone()
+    gpu.grouped_linear(x, w, offsets, bias=bias, activation="gelu", residual=held, out=held)
+    assert torch.equal(held, y)

@@ -343,3 +343,27 @@ def test_tokens_refuse(gpu):
     ]:
         with pytest.raises(error):
             call()
+
+
+def test_two_streams_at_once_and_a_residual_in_place_of_a_sliced_sum(gpu):
+    import torch
+    a, b = (_make(torch, rows, 2, 16, 256, 2048, 256, torch.bfloat16, 40 + rows) for rows in (9, 40))
+    runs = []
+    for x, ids, gates, w1, up, w2, b1, b2, r in (a, b):
+        def run(out, x=x, ids=ids, gates=gates, w1=w1, up=up, w2=w2, b1=b1, b2=b2, r=r):
+            out.copy_(r)
+            return gpu.expert_layer(x, ids, w1, w2, gates, activation="gelu", up=up, bias1=b1, bias2=b2, residual=out, out=out)
+        want = gpu.expert_layer(x, ids, w1, w2, gates, activation="gelu", up=up, bias1=b1, bias2=b2,
+                                residual=r.bfloat16())
+        _check(torch, want, _layer64(torch, x, ids, w1, w2, gates, "gelu", up, b1, b2, r.bfloat16(), torch.bfloat16))
+        runs.append((run, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        held = []
+        for _ in range(6):
+            for run, want, stream in runs:
+                with torch.cuda.stream(stream):
+                    held.append((run(torch.empty_like(want)), want))
+        torch.cuda.synchronize()
+        for got, want in held:
+            assert torch.equal(got, want)

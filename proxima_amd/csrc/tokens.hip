@@ -84,18 +84,20 @@ struct MatrixTile {
   uint32_t at, scale_at;  // this lane's row
   bool in;
 
+  // TILE rows from row0 on; with fewer than 16 of them lanes share rows, and take other columns by load's k
+  template <int TILE>
   __device__ __forceinline__ void set(const ExpertMatrix& m, int expert, int height, int row0, int rows, int cols,
                                       int lane) {
-    const int r16 = lane & 15, q = lane >> 4;
+    const int row = (lane & 15) % TILE, q = lane >> 4;
     uint32_t odd = 0;
     constexpr int BYTES = PACKED ? 1 : 2;
     const char* p = (const char*)m.p + (expert * m.group + row0 * m.stride) * BYTES;
     rs = rows_rsrc<ANY && !PACKED>(p, ((uint64_t)(rows - 1) * m.stride + cols) * BYTES, odd);
-    in = r16 < rows;
-    at = odd + (uint32_t)(r16 * m.stride * BYTES) + q * 16;
+    in = row < rows;
+    at = odd + (uint32_t)(row * m.stride * BYTES) + q * 16;
     if constexpr (PACKED) {
       scales = tile_rsrc(m.scales + ((uint64_t)expert * height + row0) * m.scale_stride, rows * m.scale_stride);
-      scale_at = r16 * (uint32_t)m.scale_stride;
+      scale_at = row * (uint32_t)m.scale_stride;
     }
   }
   // `cols` is the matrix' width: packed, a multiple of 128
@@ -175,8 +177,8 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
   const int cols = p.hidden - n0 < 16 ? p.hidden - n0 : 16;
   const int k_wide = PACKED ? (int)p.w1.stride : p.k;
   M w[D];
-  w[0].set(p.w1, expert, p.hidden, n0, cols, k_wide, lane);
-  if constexpr (D == 2) w[1].set(p.up, expert, p.hidden, n0, cols, k_wide, lane);
+  w[0].template set<16>(p.w1, expert, p.hidden, n0, cols, k_wide, lane);
+  if constexpr (D == 2) w[1].template set<16>(p.up, expert, p.hidden, n0, cols, k_wide, lane);
   // its tokens, a lane each, and their gates; then lane r has the r-th of them
   bool mine = false;
   float gate = 0.0f;
@@ -321,36 +323,41 @@ __device__ __forceinline__ void finish(const TokenLayer& p, int token, int col, 
   ((O*)p.y)[(uint64_t)token * p.ys + col] = rounded<O>(v);
 }
 
-template <class T, bool PACKED, bool ANY, int RT, class O>
-__global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_out(TokenLayer p) {
+// PARTS (1 or 2): the matrix instruction's 16 rows are 16 / PARTS of a matrix by PARTS neighbouring pieces of the sum,
+// its 16 columns as many tokens by the same pieces; of the products, those of a piece with itself count. RT: row tiles
+// of 16 / PARTS tokens.
+template <class T, bool PACKED, bool ANY, int RT, class O, int PARTS, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 4) tokens_out(TokenLayer p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   using M = MatrixTile<T, PACKED, ANY>;
   constexpr int PLANES = std::is_same_v<O, float> ? 3 : 2;
   constexpr int AHEAD = RT > 1 || ANY ? 2 : PACKED ? 4 - PLANES : PLANES == 3 ? 2 : std::is_same_v<T, __bf16> ? 4 : 3;  // chunks loaded before they are multiplied
+  constexpr int TILE = 16 / PARTS, THREADS = 64 * WAVES;
   __shared__ Entry entries[ENTRIES_MAX];
-  __shared__ f4v part[TOKENS_WAVES][RT][64];
+  __shared__ f4v part[WAVES][RT][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = (p.n + 15) / 16, n0 = (int)blockIdx.x % tiles * 16, slice = (int)blockIdx.x / tiles;
+  const int tiles = (p.n + TILE - 1) / TILE, n0 = (int)blockIdx.x % tiles * TILE, slice = (int)blockIdx.x / tiles;
   const int t0 = blockIdx.y * BLOCK_TOKENS, tokens = p.rows - t0 < BLOCK_TOKENS ? p.rows - t0 : BLOCK_TOKENS;
   const Entry* from = p.entries + (uint64_t)blockIdx.y * (p.entries_max + 1);
   const int all = __builtin_amdgcn_readfirstlane(from[0].expert);
-  for (int i = threadIdx.x; i < all; i += TOKENS_THREADS) entries[i] = from[i + 1];
+  for (int i = threadIdx.x; i < all; i += THREADS) entries[i] = from[i + 1];
   __syncthreads();
 
-  const int cols = p.n - n0 < 16 ? p.n - n0 : 16, wide = PACKED ? p.wide : p.hidden;
-  const int chunks = (wide + M::ROUND - 1) / M::ROUND;  // of an expert's hidden columns
+  const int cols = p.n - n0 < TILE ? p.n - n0 : TILE, wide = PACKED ? p.wide : p.hidden;
+  const int chunks = (wide + PARTS * M::ROUND - 1) / (PARTS * M::ROUND);  // of an expert's hidden columns
+  const int mine_of = r16 % TILE, piece = r16 / TILE * M::ROUND;  // this lane's token of a row tile, and its columns
   const int64_t total = (int64_t)all * chunks;
   const int begin = (int)(total * slice / p.slices), end = (int)(total * (slice + 1) / p.slices);
   uint64_t below[RT];  // tokens before this lane's of row tile i
 #pragma unroll
-  for (int i = 0; i < RT; ++i) below[i] = (1ull << (i * 16 + r16)) - 1;
+  for (int i = 0; i < RT; ++i) below[i] = (1ull << (i * TILE + mine_of)) - 1;
   f4v acc[RT] = {};
   // a row tile's fragments of a: zeros in the rows of tokens that did not pick the expert
   auto load_a = [&](const Entry& e, int i, int k, uint4 (&a)[PLANES][M::FRAGMENTS]) {
     const uint64_t row_bytes = (uint64_t)PLANES * p.wide * 2;
     const auto ra = tile_rsrc(p.planes + ((uint64_t)t0 * p.picks + e.offset) * row_bytes, __popcll(e.tokens) * row_bytes);
-    const bool in = e.tokens >> (i * 16 + r16) & 1;
+    const bool in = e.tokens >> (i * TILE + mine_of) & 1;
     const uint32_t at = __popcll(e.tokens & below[i]) * (uint32_t)row_bytes;
 #pragma unroll
     for (int plane = 0; plane < PLANES; ++plane)
@@ -393,8 +400,8 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_out(TokenLayer p) {
   // chunk `c`: of the nth expert, from column `chunk` rounds on
   int c = begin + wave, nth = c / chunks, chunk = c % chunks;
   auto next = [&] {
-    c += TOKENS_WAVES;
-    chunk += TOKENS_WAVES;
+    c += WAVES;
+    chunk += WAVES;
     while (chunk >= chunks) {
       chunk -= chunks;
       ++nth;
@@ -410,8 +417,8 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_out(TokenLayer p) {
     for (int u = 0; u < AHEAD; ++u) {
       e[u] = entry_at(c < end ? nth : 0);
       if (c >= end) e[u].tokens = 0;
-      k[u] = c < end ? chunk * M::ROUND : wide;  // past the end: zeros
-      w[u].set(p.w2, e[u].expert, p.n, n0, cols, wide, lane);
+      k[u] = (c < end ? chunk * (PARTS * M::ROUND) : wide) + piece;  // past the end: zeros
+      w[u].template set<TILE>(p.w2, e[u].expert, p.n, n0, cols, wide, lane);
       b[u] = w[u].load(k[u], wide, q);
       if constexpr (RT == 1) load_a(e[u], 0, k[u], a[u]);
       next();
@@ -424,28 +431,26 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_out(TokenLayer p) {
       for (int f = 0; f < M::FRAGMENTS; ++f) wf[f] = w[u].fragment(b[u], f, k[u], wide, q);
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
-        if (RT > 1 && !(e[u].tokens >> (i * 16) & 0xFFFF)) continue;
+        if (RT > 1 && !(e[u].tokens >> (i * TILE) & ((1 << TILE) - 1))) continue;
         if constexpr (RT > 1) load_a(e[u], i, k[u], a[u]);
         f4v sum = {};
 #pragma unroll
         for (int f = 0; f < M::FRAGMENTS; ++f) multiply(wf[f], a[u], f, sum);
         // zeros times an infinity of another token's expert stay out
-        if (e[u].tokens >> (i * 16 + r16) & 1) acc[i] += sum;
+        if (e[u].tokens >> (i * TILE + mine_of) & 1) acc[i] += sum;
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < RT; ++i) part[wave][i][lane] = acc[i];
   __syncthreads();
-  const int i = wave, t = i * 16 + r16;  // a wavefront ends a row tile
-  const bool mine = i < RT && t < tokens;
+  const int i = wave, t = i * TILE + r16;  // a wavefront ends a row tile
+  if (i >= RT || r16 >= TILE || q >= 4 / PARTS || t >= tokens) return;
   f4v s = {};
-  if (mine) {
-    s = part[0][i][lane];
+#pragma unroll 4
+  for (int o = 0; o < WAVES; ++o)
 #pragma unroll
-    for (int o = 1; o < TOKENS_WAVES; ++o) s += part[o][i][lane];
-  }
-  if (!mine) return;
+    for (int h = 0; h < PARTS; ++h) s += part[o][i][lane + h * (64 / PARTS + TILE)];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     if (4 * q + e >= cols) break;
@@ -471,7 +476,7 @@ __global__ void __launch_bounds__(256) tokens_join(TokenLayer p) {
 // --- host ------------------------------------------------------------------------------
 struct TokensPlan {
   uint64_t blocks, entries_max, wide, planes_bytes, entries_bytes, partial_bytes;
-  int slices;
+  int slices, parts, waves;
 };
 uint64_t pieces_of(uint64_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -484,11 +489,18 @@ TokensPlan tokens_plan(uint64_t rows, uint64_t picks, uint64_t experts, uint64_t
   t.wide = (hidden + 127) / 128 * 128;
   t.planes_bytes = pieces_of(rows * picks * (f32_out ? 3 : 2) * t.wide * 2);
   t.entries_bytes = pieces_of(t.blocks * (t.entries_max + 1) * sizeof(Entry));
-  // As many slices as fill the chip, of at least 32 KB each: two chunks for each
-  // wavefront of a workgroup (of at least 96 KB: 18 tokens, 512 -> 3904 -> 387, 3
-  // gated experts 33 us for 25; 53 tokens, 2672 -> 1193 -> 1344, 2 experts 40 for 33).
+  // The second kernel wants 256 workgroups, one with 16 wavefronts on each CU. Where 16
+  // rows of a matrix each make fewer, 8 do it for up to 8 tokens (8 x 2 of 16 gated
+  // experts, 2048 -> 4096 -> 2048: 38 us, 34 and 5 with slices and two kernels; 32 x 4 of
+  // 64 packed ones, 2048 -> 1024 -> 2048: 38, for 26 and 5). Else the sum is cut into
+  // slices that a third kernel joins: as many as fill the chip, of at least 32 KB
+  // each, two chunks for each wavefront of a workgroup (of at least 96 KB: 18 tokens,
+  // 512 -> 3904 -> 387, 3 gated experts 33 us for 25; 53 tokens, 2672 -> 1193 -> 1344, 2
+  // experts 40 for 33).
   const uint64_t tiles = (n + 15) / 16 * t.blocks, bytes = t.entries_max * 16 * hidden * (packed ? 1 : 2);
-  t.slices = (int)std::max<uint64_t>(1, std::min({(uint64_t)512 / tiles, bytes / SLICE_BYTES, (uint64_t)32}));
+  t.parts = tiles < 256 && tiles >= 128 && rows <= 8 ? 2 : 1;
+  t.waves = tiles * t.parts >= 256 ? 16 : TOKENS_WAVES;
+  t.slices = t.waves == 16 ? 1 : (int)std::max<uint64_t>(1, std::min({(uint64_t)512 / tiles, bytes / SLICE_BYTES, (uint64_t)32}));
   t.partial_bytes = t.slices > 1 ? pieces_of(4 * t.slices * rows * n) : 0;
   return t;
 }
@@ -502,10 +514,11 @@ void run_tokens(TokenLayer p, const TokensPlan& t, hipStream_t s) {
                        grid, dim3(TOKENS_THREADS), 0, s, p);
     PXG_HIP(hipGetLastError());
   };
-  auto out = [&](auto any, auto rt) {
-    const dim3 grid((unsigned)((uint64_t)p.slices * ((p.n + 15) / 16)), (unsigned)t.blocks);
-    hipLaunchKernelGGL((tokens_out<T, PACKED, decltype(any)::value, decltype(rt)::value, O>), grid, dim3(TOKENS_THREADS), 0,
-                       s, p);
+  auto out_of = [&](auto any, auto rt, auto parts, auto waves) {
+    constexpr int PARTS = decltype(parts)::value, WAVES = decltype(waves)::value;
+    const dim3 grid((unsigned)((uint64_t)p.slices * ((p.n + 16 / PARTS - 1) / (16 / PARTS))), (unsigned)t.blocks);
+    hipLaunchKernelGGL((tokens_out<T, PACKED, decltype(any)::value, decltype(rt)::value, O, PARTS, WAVES>), grid,
+                       dim3(64 * WAVES), 0, s, p);
     PXG_HIP(hipGetLastError());
   };
   auto aligned = [](const void* d, uint64_t cols, uint64_t stride, uint64_t group) {
@@ -519,6 +532,17 @@ void run_tokens(TokenLayer p, const TokensPlan& t, hipStream_t s) {
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
   using Four = std::integral_constant<int, 4>;
+  auto out = [&](auto any, auto rt) {
+    using Few = std::integral_constant<int, TOKENS_WAVES>;
+    using Many = std::integral_constant<int, 16>;
+    if (t.parts == 2) {
+      out_of(any, One{}, Two{}, Many{});
+    } else if (t.waves == 16) {
+      out_of(any, rt, One{}, Many{});
+    } else {
+      out_of(any, rt, One{}, Few{});
+    }
+  };
   auto by_rows = [&](auto f) {
     if (p.rows <= 16) f(One{});
     else if (p.rows <= 32) f(Two{});

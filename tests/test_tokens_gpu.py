@@ -367,3 +367,29 @@ def test_two_streams_at_once_and_a_residual_in_place_of_a_sliced_sum(gpu):
         torch.cuda.synchronize()
         for got, want in held:
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("rows", [1, 7, 8, 9, 16, 21, 32, 33, 70])
+@pytest.mark.parametrize("n", [2040, 2048, 2500, 4096, 4101])
+def test_every_shape_of_the_second_product(gpu, rows, n):
+    # 8 or 16 rows of a matrix to a workgroup, 8 or 16 wavefronts, with slices or not
+    import torch
+    for i, dtype in enumerate((torch.bfloat16, torch.float16)):
+        hidden = (200, 331)[(rows + i) % 2]
+        x, ids, gates, w1, up, w2, b1, b2, r = _make(torch, rows, 3, 7, 72, hidden, n, dtype, rows + n)
+        w2[6] = float("inf")  # another token's
+        ids[ids == 6] = -1
+        ids[-1] = 6
+        out = (dtype, torch.float32)[(rows + n + i) % 2]
+        got = gpu.expert_layer(x, ids, w1, w2, gates, activation="gelu", bias2=b2, residual=r.to(out), out_dtype=out)
+        fine = w2.clone()
+        fine[6] = 0.0
+        y, off = _layer64(torch, x, ids, w1, fine, gates, "gelu", None, None, b2, r.to(out), out)
+        _check(torch, got[:-1], (y[:-1], off[:-1]))
+        assert not bool(torch.isfinite(got[-1]).any())
+        if i == 0:
+            p1, p2 = gpu.block8_pack(w1.reshape(-1, 72)), gpu.block8_pack(fine.reshape(-1, hidden))
+            v1 = gpu.block8_unpack(p1, torch.float32).view(w1.shape)
+            v2 = gpu.block8_unpack(p2, torch.float32).view(w2.shape)
+            got = gpu.expert_layer(x, ids, p1, p2, gates, activation="silu", out_dtype=out)
+            _check(torch, got, _layer64(torch, x, ids, v1, v2, gates, "silu", None, None, None, None, out))

@@ -564,8 +564,9 @@ void run_distill(Distill p, const DistillPlan& d, hipStream_t s) {
   }
 }
 
-int distill(const pxg_distill& a, bool grad, void* stream) {
+int distill(const pxg_distill* arguments, bool grad, void* stream) {
   return guard([&] {
+    const pxg_distill& a = check_arguments(arguments);
     check_type(a.type, true);
     check_size("cols", a.cols);
     if (a.top == 0 || a.top > TOP_MAX) config_error("top", a.top, "must be between 1 and 4096");
@@ -630,7 +631,7 @@ uint64_t pxg_distill_workspace(int type, uint64_t rows, uint64_t cols, uint64_t 
   return distill_plan(type, rows, cols, top).bytes;
 }
 
-int pxg_distill_loss_device(const pxg_distill* a, void* stream) { return distill(*a, false, stream); }
-int pxg_distill_loss_grad_device(const pxg_distill* a, void* stream) { return distill(*a, true, stream); }
+int pxg_distill_loss_device(const pxg_distill* a, void* stream) { return distill(a, false, stream); }
+int pxg_distill_loss_grad_device(const pxg_distill* a, void* stream) { return distill(a, true, stream); }
 
 }  // extern "C"

@@ -35,7 +35,7 @@ extern "C" {
 
 int pxg_grouped_linear_device(const pxg_linear* layer, void* stream) {
   return guard([&] {
-    const pxg_linear& a = *layer;
+    const pxg_linear& a = check_arguments(layer);
     check_type(a.type, false);
     check_out_type(a.type, a.out_type);
     check_size("k", a.k);
@@ -55,7 +55,7 @@ int pxg_grouped_linear_device(const pxg_linear* layer, void* stream) {
 
 int pxg_block8_linear_device(const pxg_linear* layer, void* stream) {
   return guard([&] {
-    const pxg_linear& a = *layer;
+    const pxg_linear& a = check_arguments(layer);
     check_type(a.out_type, true);
     check_size("k", a.k);
     check_size("n", a.n);

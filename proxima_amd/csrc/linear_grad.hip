@@ -189,7 +189,7 @@ uint64_t pxg_grouped_linear_grad_workspace(uint64_t rows, uint64_t n, uint64_t g
 
 int pxg_grouped_linear_grad_device(const pxg_linear_grad* layer, void* stream) {
   return guard([&] {
-    const pxg_linear_grad& a = *layer;
+    const pxg_linear_grad& a = check_arguments(layer);
     check_type(a.type, true);
     check_optional_activation(a.activation);
     check_size("n", a.n);

@@ -15,6 +15,12 @@ inline void check_type(int64_t type, bool f32) {
   if (type != PXG_F16 && type != PXG_BF16 && !(f32 && type == PXG_F32))
     config_error("type", (uint64_t)type, f32 ? "must be f32, f16 or bf16" : "must be f16 or bf16");
 }
+// The struct that an entry takes its arguments from.
+template <class A>
+const A& check_arguments(const A* a) {
+  if (!a) config_error("arguments", 0, "must not be null");
+  return *a;
+}
 // `name` must be a string literal.
 inline void check_size(const char* name, uint64_t size) {
   if (size == 0 || size > PRODUCT_SIZE_MAX) config_error(name, size, "must be between 1 and 2147482624");

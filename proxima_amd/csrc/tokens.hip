@@ -597,7 +597,7 @@ uint64_t pxg_expert_layer_workspace(uint64_t rows, uint64_t picks, uint64_t expe
 
 int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream) {
   return guard([&] {
-    const pxg_expert_layer& a = *layer;
+    const pxg_expert_layer& a = check_arguments(layer);
     const bool packed = a.packed != 0;
     check_type(a.type, false);
     if (packed && a.type != PXG_BF16) config_error("type", (uint64_t)a.type, "must be bf16 with packed matrices");

@@ -223,6 +223,12 @@ def test_distillation_refuses(lib):
     assert size(0, 4, 1 << 20, 2) > 0 and size(0, 4, 8, 2) == 0 and size(0, 0, 8, 2) == 0 and size(0, 4, 8, 0) == 0
 
 
+def test_no_struct_is_refused(lib):
+    for f in (lib.pxg_grouped_linear_device, lib.pxg_block8_linear_device, lib.pxg_grouped_linear_grad_device,
+              lib.pxg_expert_layer_device, lib.pxg_distill_loss_device, lib.pxg_distill_loss_grad_device):
+        _refused(lib, f(None, None), b"arguments")
+
+
 def test_arguments_are_packed_as_the_structs_lie():
     from proxima_amd import _capi, experts
     for packer, kind in ((experts._LINEAR, _capi.LinearC), (experts._LINEAR_GRAD, _capi.LinearGradC),

@@ -10,7 +10,8 @@ maps the query to where the documents are:
 - training sorts a batch by cell and runs the cells' ragged groups in one
   product each way; what the backward pass needs of the layers' inputs is kept
   in 8 bits (activation_pack, block8_pack);
-- serving packs the trained matrices once and multiplies in 8 bits.
+- serving packs the trained matrices once: batches are multiplied in 8 bits, a
+  few queries at a time take the layer whole (expert_layer).
 
     python examples/expert_adapters.py
 """
@@ -53,15 +54,19 @@ class Router:
         self.index = px.FlatIndex(px.VectorSpace(points.shape[1], px.Metric.EUCLIDEAN), cells)
         self.index.insert_device(range(cells), self.centroids)
 
-    def __call__(self, x):
-        """(order, offsets): the rows of x sorted by cell, and where each cell's begin."""
-        n, cells = x.shape[0], self.centroids.shape[0]
+    def cells(self, x):
+        """The cell of each row of x, [rows, 1]."""
+        n = x.shape[0]
         ids = torch.zeros(n, 1, dtype=torch.int64, device="cuda")
         dist = torch.zeros(n, 1, device="cuda")
         count = torch.zeros(n, dtype=torch.int32, device="cuda")
         self.index.search_device(x, 1, ids, dist, count)
-        cell, order = torch.sort(ids[:, 0], stable=True)
-        return order, torch.searchsorted(cell, torch.arange(cells + 1, device="cuda"))
+        return ids
+
+    def __call__(self, x):
+        """(order, offsets): the rows of x sorted by cell, and where each cell's begin."""
+        cell, order = torch.sort(self.cells(x)[:, 0], stable=True)
+        return order, torch.searchsorted(cell, torch.arange(self.centroids.shape[0] + 1, device="cuda"))
 
 
 class Adapters:
@@ -117,6 +122,14 @@ def serve(router, matrices, x):
     return out
 
 
+def serve_few(router, matrices, x):
+    """The same for a few queries: the layer whole, from their cells, without sorting or packing them."""
+    w1, w2 = matrices
+    gates = torch.ones(x.shape[0], 1, device="cuda")
+    return px.expert_layer(x.bfloat16(), router.cells(x), w1, w2, gates, activation="gelu", residual=x,
+                           out_dtype=torch.float32)
+
+
 def recall(index, queries, target, k=10):
     """The share of queries whose document is among the k nearest."""
     n = queries.shape[0]
@@ -141,8 +154,11 @@ def main(docs=50_000, train=32_768, test=1000, dim=128, hidden=256, cells=8, ste
         loss = adapters.train_step(x[order], d[target[rows[order]]], offsets, 3e-3 * (1 - step / steps))
         if step % 50 == 0:
             print(f"step {step}: mean squared error {loss:.4f}", flush=True)
-    after = recall(index, serve(router, adapters.packed(), q[train:].contiguous()), target[train:])
-    print(f"recall@10 without adapters {before:.3f}, with adapters served in 8 bits {after:.3f}")
+    matrices = adapters.packed()
+    after = recall(index, serve(router, matrices, q[train:].contiguous()), target[train:])
+    few = torch.cat([serve_few(router, matrices, q[i:i + 4].contiguous()) for i in range(train, train + 64, 4)])
+    print(f"recall@10 without adapters {before:.3f}, with adapters served in 8 bits {after:.3f}, "
+          f"of 64 queries served by fours {recall(index, few, target[train:train + 64]):.3f}")
     return before, after
 
 

@@ -612,9 +612,10 @@ int pxg_expert_layer_device(const pxg_expert_layer* layer, void* stream);
  * count (clamped to [0, top]) are looked at; those with an id outside [0, cols) are
  * left out. A row without entries, or whose scores are all -inf, has loss 0 and no
  * gradient; entries of p = 0 add nothing; a logit of -inf has q = 0. `weight` is
- * the loss' own gradient, one f32 a row; the loss alone looks at neither it nor dx. T lies between 1e-6 and 1e6. Sums are
- * held in f32. The workspace is of the size that workspace() says (0: none),
- * 16-byte aligned and not kept after the work is done. */
+ * the loss' own gradient, one f32 a row; the loss alone looks at neither it nor
+ * dx. T lies between 1e-6 and 1e6. Sums are held in f32. The workspace is of the
+ * size that workspace() says (0: none), 16-byte aligned and not kept after the
+ * work is done. */
 typedef struct pxg_distill {
   int64_t type;
   uint64_t rows, cols, top;

@@ -393,3 +393,27 @@ def test_every_shape_of_the_second_product(gpu, rows, n):
             v2 = gpu.block8_unpack(p2, torch.float32).view(w2.shape)
             got = gpu.expert_layer(x, ids, p1, p2, gates, activation="silu", out_dtype=out)
             _check(torch, got, _layer64(torch, x, ids, v1, v2, gates, "silu", None, None, None, None, out))
+
+
+def test_the_example_serves_a_few_queries_as_a_batch(gpu):
+    import importlib.util
+    import os
+
+    import torch
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "expert_adapters.py")
+    spec = importlib.util.spec_from_file_location("expert_adapters", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    g = base._dev(torch, 3)
+    x = torch.randn(300, 128, generator=g, device="cuda")
+    router = example.Router(x, 8, 2)
+    w1 = torch.randn(8, 256, 128, generator=g, device="cuda") / 128 ** 0.5
+    w2 = torch.randn(8, 128, 256, generator=g, device="cuda") / 256 ** 0.5
+    packed = tuple(gpu.block8_pack(w.reshape(-1, w.shape[2])) for w in (w1, w2))
+    few = torch.cat([example.serve_few(router, packed, x[i:i + 7].contiguous()) for i in range(0, 300, 7)])
+    v1, v2 = (gpu.block8_unpack(p, torch.float32).view(w.shape) for p, w in zip(packed, (w1, w2)))
+    ids, ones = router.cells(x), torch.ones(300, 1, device="cuda")
+    _check(torch, few, _layer64(torch, x.bfloat16(), ids, v1, v2, ones, "gelu", None, None, None, x, torch.float32))
+    # the batch packs its rows in 8 bits twice: half a step of 2^-3 each
+    batch = example.serve(router, packed, x)
+    assert float((few - batch).norm() / (batch - x).norm()) < 2 * 2.0 ** -4

@@ -417,3 +417,28 @@ def test_the_example_serves_a_few_queries_as_a_batch(gpu):
     # the batch packs its rows in 8 bits twice: half a step of 2^-3 each
     batch = example.serve(router, packed, x)
     assert float((few - batch).norm() / (batch - x).norm()) < 2 * 2.0 ** -4
+
+
+def test_rows_that_begin_between_words(gpu):
+    # every operand at an odd element of its storage, by itself and together; what lies around them is not a number
+    import torch
+
+    def shifted(t, by):
+        hold = torch.full((t.numel() + 2 * by + 8,), 0 if t.dtype is torch.int64 else float("nan"), dtype=t.dtype, device="cuda")
+        v = hold[by:by + t.numel()].view(t.shape)
+        return v.copy_(t)
+
+    for rows, k, hidden, n in ((5, 64, 72, 40), (20, 65, 33, 2049), (3, 1001, 130, 7), (40, 128, 127, 4096)):
+        x, ids, gates, w1, up, w2, b1, b2, r = _make(torch, rows, 2, 4, k, hidden, n, torch.float16, rows)
+        for which in range(5):
+            on = [shifted(t, 1) if which in (i, 4) else t for i, t in enumerate((x, w1, w2, up))]
+            rr = shifted(r.half(), 3)
+            got = gpu.expert_layer(on[0], ids, on[1], on[2], gates, activation="gelu", up=on[3], bias1=shifted(b1, 1),
+                                   bias2=shifted(b2, 1), residual=rr, out=shifted(torch.zeros_like(rr), 1))
+            _check(torch, got, _layer64(torch, x, ids, w1, w2, gates, "gelu", up, b1, b2, rr, torch.float16))
+            h = gpu.grouped_linear(on[0], on[1][1], bias=shifted(b1[1].contiguous(), 1), activation="silu")
+            want = x.double() @ w1[1].double().t().contiguous() + b1[1].double()
+            size = x.double().abs() @ w1[1].double().abs().t().contiguous() + b1[1].double().abs()
+            want, err = _act64(torch, want, "silu"), 1.13 * 1.25 * (k + 1) * 2.0 ** -24 * size + 2.0 ** -16 * size
+            bound = err + 2.0 ** -11 * (want.abs() + err) + 2.0 ** -25
+            assert bool(((h.double() - want).abs() <= bound).all())

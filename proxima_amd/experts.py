@@ -70,21 +70,21 @@ class Block8:
         return f"Block8({self.rows} x {self.cols})"
 
 
-# torch is the caller's: this package does not import it by itself. Filled on the first call with a tensor.
+# torch is the caller's: this package does not import it by itself. Filled by what looks at a call's first operand
+# (_matrix, _device, _packed, and Block8's constructor), _torch last: another thread takes it as the sign that all is.
 _KINDS = {}  # torch dtype -> pxg_type
 _torch = _current_device = _current_stream = None
 
 
 def _setup():
     global _torch, _current_device, _current_stream
-    _torch = sys.modules["torch"]
-    _current_device, _current_stream = _torch._C._cuda_getDevice, _torch._C._cuda_getCurrentRawStream
-    _KINDS.update({_torch.float32: 0, _torch.float16: 1, _torch.bfloat16: 2})
+    torch = sys.modules["torch"]
+    _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    _KINDS.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    _torch = torch
 
 
 def _type(dtype, name, f32=True):
-    if _torch is None:
-        _setup()
     kind = _KINDS.get(dtype)
     if kind is None or (kind == 0 and not f32):
         raise ValueError(f"{name} must be {'float32, ' if f32 else ''}float16 or bfloat16, got {dtype}")
@@ -95,6 +95,8 @@ def _matrix(t, name, dims=2):
     """Checks a GPU tensor of contiguous rows; its shape."""
     if not getattr(t, "is_cuda", False):
         raise ValueError(f"{name} must be a GPU tensor")
+    if _torch is None:
+        _setup()
     shape = t.shape
     if len(shape) != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got {len(shape)}")
@@ -117,6 +119,8 @@ def _packed(p, name):
     """(codes, scales, rows, cols) of a Block8."""
     if type(p) is not Block8:
         raise ValueError(f"{name} must be a Block8")
+    if _torch is None:
+        _setup()
     codes = p._codes
     return codes, p._scales, codes.shape[0], p._cols
 
@@ -125,8 +129,6 @@ def _groups(offsets):
     """(pointer or None, number of groups)"""
     if offsets is None:
         return None, 1
-    if _torch is None:
-        _setup()
     if not offsets.is_cuda or offsets.dtype is not _torch.int64 or offsets.dim() != 1 or not offsets.is_contiguous():
         raise ValueError("offsets must be a contiguous one-dimensional int64 GPU tensor")
     n = offsets.shape[0]
@@ -330,6 +332,8 @@ def _device(t, name):
     """The index of the GPU that a call's first operand is on, and so all others."""
     if not getattr(t, "is_cuda", False):
         raise ValueError(f"{name} must be a GPU tensor")
+    if _torch is None:
+        _setup()
     return t.get_device()
 
 

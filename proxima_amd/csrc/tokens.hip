@@ -66,6 +66,7 @@ struct TokenLayer {
   Entry* entries;    // entries_max + 1 of a block, the first's expert their number
   float* partial;    // tokens_out's sums by slice, row and column
   int rows, k, hidden, wide, n, picks, experts, entries_max, slices;
+  unsigned first = 0;  // tokens_out's workgroups (along x) of the launches before this one
   int activation;
   bool bias_f32;
 };
@@ -142,9 +143,10 @@ __global__ void __launch_bounds__(TOKENS_THREADS, 4) tokens_hidden(TokenLayer p)
   __shared__ f4v part[TOKENS_WAVES][D * RT][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = (p.hidden + 15) / 16, nth = (int)blockIdx.x / tiles, n0 = (int)blockIdx.x % tiles * 16;
-  const int t0 = blockIdx.y * BLOCK_TOKENS, tokens = p.rows - t0 < BLOCK_TOKENS ? p.rows - t0 : BLOCK_TOKENS;
-  Entry* entries = p.entries + (uint64_t)blockIdx.y * (p.entries_max + 1);
+  // along x the tiles of a matrix, then the experts in use, then the blocks of tokens
+  const int n0 = (int)blockIdx.x * 16, nth = (int)blockIdx.y;
+  const int t0 = blockIdx.z * BLOCK_TOKENS, tokens = p.rows - t0 < BLOCK_TOKENS ? p.rows - t0 : BLOCK_TOKENS;
+  Entry* entries = p.entries + (uint64_t)blockIdx.z * (p.entries_max + 1);
 
   // the nth expert in use
   const int words = (p.experts + 31) / 32;
@@ -337,7 +339,8 @@ __global__ void __launch_bounds__(64 * WAVES, 4) tokens_out(TokenLayer p) {
   __shared__ f4v part[WAVES][RT][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, q = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tiles = (p.n + TILE - 1) / TILE, n0 = (int)blockIdx.x % tiles * TILE, slice = (int)blockIdx.x / tiles;
+  const int tiles = (p.n + TILE - 1) / TILE, place = (int)(p.first + blockIdx.x);
+  const int n0 = place % tiles * TILE, slice = place / tiles;
   const int t0 = blockIdx.y * BLOCK_TOKENS, tokens = p.rows - t0 < BLOCK_TOKENS ? p.rows - t0 : BLOCK_TOKENS;
   const Entry* from = p.entries + (uint64_t)blockIdx.y * (p.entries_max + 1);
   const int all = __builtin_amdgcn_readfirstlane(from[0].expert);
@@ -509,17 +512,21 @@ template <class T, bool PACKED, class O>
 void run_tokens(TokenLayer p, const TokensPlan& t, hipStream_t s) {
   constexpr int PLANES = std::is_same_v<O, float> ? 3 : 2;
   auto hidden = [&](auto any, auto gated, auto rt) {
-    const dim3 grid((unsigned)(t.entries_max * ((p.hidden + 15) / 16)), (unsigned)t.blocks);
+    const dim3 grid((unsigned)((p.hidden + 15) / 16), (unsigned)t.entries_max, (unsigned)t.blocks);
     hipLaunchKernelGGL((tokens_hidden<T, PACKED, decltype(any)::value, decltype(gated)::value, decltype(rt)::value, PLANES>),
                        grid, dim3(TOKENS_THREADS), 0, s, p);
     PXG_HIP(hipGetLastError());
   };
   auto out_of = [&](auto any, auto rt, auto parts, auto waves) {
     constexpr int PARTS = decltype(parts)::value, WAVES = decltype(waves)::value;
-    const dim3 grid((unsigned)((uint64_t)p.slices * ((p.n + 16 / PARTS - 1) / (16 / PARTS))), (unsigned)t.blocks);
-    hipLaunchKernelGGL((tokens_out<T, PACKED, decltype(any)::value, decltype(rt)::value, O, PARTS, WAVES>), grid,
-                       dim3(64 * WAVES), 0, s, p);
-    PXG_HIP(hipGetLastError());
+    constexpr uint64_t MOST = LAUNCH_ROWS / 2;  // of 1024 threads
+    const uint64_t all = (uint64_t)p.slices * (((uint64_t)p.n + 16 / PARTS - 1) / (16 / PARTS));
+    for (uint64_t a = 0; a < all; a += MOST) {
+      p.first = (unsigned)a;
+      hipLaunchKernelGGL((tokens_out<T, PACKED, decltype(any)::value, decltype(rt)::value, O, PARTS, WAVES>),
+                         dim3((unsigned)std::min(MOST, all - a), (unsigned)t.blocks), dim3(64 * WAVES), 0, s, p);
+      PXG_HIP(hipGetLastError());
+    }
   };
   auto aligned = [](const void* d, uint64_t cols, uint64_t stride, uint64_t group) {
     return ((uint64_t)(uintptr_t)d | cols * 2 | stride * 2 | group * 2) % 16 == 0;

@@ -18,7 +18,7 @@
 // Sums are held in f32. a is kept as planes of bf16 whose sum it is: two for
 // 16-bit results (2^-17 of it is lost), three (all of f32's 24 bits) for f32.
 // Matrices in f16 are taken apart into two bf16 for the second product, which
-// is exact, so that a's range is f32's.
+// is exact but for 2^-40 (rest() says why), so that a's range is f32's.
 #include "activation.hpp"
 #include "block8.hpp"
 #include "common.hpp"
@@ -128,7 +128,11 @@ struct MatrixTile {
 // v cut after bf16's bits, toward zero, so that v - cut(v) is exact.
 __device__ __forceinline__ float cut(float v) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u); }
 __device__ __forceinline__ uint32_t high_half(float v) { return __builtin_bit_cast(uint32_t, v) >> 16; }
-__device__ __forceinline__ float rest(float v, float c) { return fabsf(v) < __builtin_inff() ? v - c : 0.0f; }
+// What is left of v; of what 16 bits hold exactly 2^-40 of it rather than nothing, as zero times an infinity of the other
+// factor is not a number. (f16 matrices, 8 x 2 of 16 gated experts: 84.9 us, 84.3 without.)
+__device__ __forceinline__ float rest(float v, float c) {
+  return fabsf(v) < __builtin_inff() ? __builtin_fmaf(c, 0x1p-40f, v - c) : v;
+}
 #endif
 
 // D: one matrix, or two (gated). RT: row tiles of 16 tokens that a block may need.

@@ -507,8 +507,9 @@ int pxg_grouped_matmul_grad_weight_block8_device(const void* d_grad, uint64_t ro
  * bf16), y of out_type (that or f32). `activation` is a pxg_activation, or -1 for
  * f(h) = h. `bias` (or NULL) is groups rows of n of bias_type: the operands' type
  * (packed rows': bf16) or f32. `residual` (or NULL) is r, rows x n of out_type, and
- * may be y itself. `h` (or NULL) takes h in out_type. Rows of no group: y = r
- * (zeros without), h = 0. block8: the same over packed rows, multiplied as
+ * may be y itself. `h` (or NULL) takes h in out_type. y and h share no memory with
+ * x, which is read while they are written (also where x is r). Rows of no group: y
+ * = r (zeros without), h = 0. block8: the same over packed rows, multiplied as
  * pxg_block8_matmul_device does: x and w are codes with x_scales and w_scales,
  * whose strides, `type` and h are not looked at, and out_type is any. */
 typedef struct pxg_linear {

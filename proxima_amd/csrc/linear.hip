@@ -48,6 +48,11 @@ int pxg_grouped_linear_device(const pxg_linear* layer, void* stream) {
                      a.y_stride, a.w_group_stride, 0, nullptr, nullptr, 0, (int)a.rows, (int)a.groups, (int)a.rows,
                      (int)a.n, (int)a.k, false}};
     set_epilogue(p, a, a.type, a.h);
+    check_rows_apart("y", a.y, a.n * type_bytes((int)a.out_type), a.y_stride * type_bytes((int)a.out_type), a.x, a.k * 2,
+                     a.x_stride * 2, a.rows);
+    if (a.h)
+      check_rows_apart("h", a.h, a.n * type_bytes((int)a.out_type), a.h_stride * type_bytes((int)a.out_type), a.x,
+                       a.k * 2, a.x_stride * 2, a.rows);
     if (a.rows == 0) return;
     run_product<FORWARD>(a.type, a.out_type, p, (hipStream_t)stream);
   });

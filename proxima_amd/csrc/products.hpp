@@ -43,6 +43,20 @@ inline void check_rows(int type, const char* name, const void* p, uint64_t rows,
   if (rows && (uint64_t)(uintptr_t)p % type_bytes(type))
     config_error(name, (uint64_t)(uintptr_t)p, "must be aligned to its type");
 }
+// A result's rows and an operand's, `bytes` each and a pitch apart, share no byte: they are apart or, at one pitch,
+// between one another. Workgroups read rows of the operand while others write the result.
+inline void check_rows_apart(const char* name, const void* result, uint64_t bytes, uint64_t pitch, const void* operand,
+                             uint64_t operand_bytes, uint64_t operand_pitch, uint64_t rows) {
+  using u128 = unsigned __int128;
+  if (rows == 0) return;
+  const u128 r = (uintptr_t)result, o = (uintptr_t)operand;
+  if (r + (u128)(rows - 1) * pitch + bytes <= o || o + (u128)(rows - 1) * operand_pitch + operand_bytes <= r) return;
+  if (rows > 1 && pitch == operand_pitch) {
+    const u128 at = ((u128)rows * pitch + r - o) % pitch;  // the result's place in the operand's rows; |r - o| < rows * pitch
+    if (at >= operand_bytes && at + bytes <= pitch) return;
+  }
+  config_error(name, (uint64_t)(uintptr_t)result, "must not share memory with x");
+}
 // The groups' matrices of a result, each of n rows of `cols`: one after the
 // other or, row by row, between one another. Overlapping ones would be written
 // by several groups at once.

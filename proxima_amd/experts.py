@@ -419,8 +419,9 @@ def _optional(activation):
 def grouped_linear(x, w, offsets=None, bias=None, activation=None, residual=None, out_dtype=None, out=None, keep=False):
     """y[t] = f(h[t]) + residual[t], h[t] = x[t] w[g]^T + bias[g] for t in group g: x and w as grouped_matmul takes
     them, bias [groups, n] (or [n] without offsets) in x's type or f32, f "silu", "gelu" or None, residual [rows, n]
-    in y's type. `out` may be the residual itself. With keep, (y, h), h in y's type for grouped_linear_grad. y is
-    rounded once, from the unrounded h. Rows of no group: y is the residual, or zeros, and h zeros."""
+    in y's type. `out` may be the residual itself, unless that is x: it shares no memory with x. With keep, (y, h), h in
+    y's type for grouped_linear_grad. y is rounded once, from the unrounded h. Rows of no group: y is the residual, or
+    zeros, and h zeros."""
     device = _device(x, "x")
     (rows, xk), x_stride = _rows(x, "x", device)
     xtype = x.dtype
@@ -545,7 +546,7 @@ def expert_layer(x, experts, w1, w2, gates, activation=None, up=None, bias1=None
     no expert's is left out, one that a token has twice counts with both gates); w1 and up (optional) [experts, hidden,
     k] and w2 [experts, n, hidden] of x's type, or each a Block8 of the experts' rows one after the other (x is then
     bf16); biases [experts, .] of x's type or f32; residual and y [rows, n] of x's type or f32. `out` may be the
-    residual itself. Nothing between the two products is rounded to x's type. The matrices of the experts in use are
+    residual itself, also where that is x. Nothing between the two products is rounded to x's type. The matrices of the experts in use are
     read once for each 64 rows: for batches use grouped_linear."""
     device = _device(x, "x")
     (rows, k), x_stride = _rows(x, "x", device)

@@ -12,8 +12,23 @@
 // Memory bounds it: x is read and dx written once, q never stored. Rows of up
 // to 128 KB stay in a workgroup's registers between the softmax' sums and dx
 // (two workgroups of 1024 threads fit a CU, so that one loads while the other
-// stores). Longer rows are cut into parts: one kernel finds each part's maximum
-// and sum, a second joins them, and for dx reads x again.
+// stores). That leaves a thread 64 registers, and 7 or 8 vectors of 16 bytes do
+// not fit beside the rest: of 7 the compiler puts 2 to 8 registers in scratch
+// memory (12 to 36 bytes a thread), of 8 up to 26 (in bf16 with the gradient and
+// 1024 threads 15, 64 bytes, beside 128 of the row). Longer rows are cut into
+// parts: one kernel finds each part's maximum and sum, a second joins them, and
+// for dx reads x again.
+//
+// The gradient adds up p of each entry's id by a search of all entries, for ids
+// may come twice: top^2 steps a row, which few entries hide behind the row's
+// bytes and many do not. us with top 10, 50, 200 and 1000: 8192 x 1000 in bf16 17,
+// 23, 82 and 3080 (the loss alone 17 with 200, 76 with 1000; torch's steps are
+// faster from some 500 on); with 10, 100, 1000 and 4096: 4096 x 50000 162, 178, 920
+// and 10600.
+//
+// f32 logits take the hardware's exp2 (off by its last place) with the product's
+// rounding added, and their sums are f32: against 64 bits the loss is off by 1.5e-7 to
+// 1.8e-7 of itself (64 x 1000), where torch's steps in f32 are by 1.4e-7.
 #include <algorithm>
 #include <cmath>
 
@@ -221,7 +236,8 @@ __device__ __forceinline__ void store_vector(T* row, int v, int phase, int cols,
 //     unsigned one;
 //   - x c - M is one operation, M the rounded m c (c = log2 e / T). What M's
 //     rounding left is taken out of the sum;
-//   - the gradient's factor goes into the exponent, which costs 2^-17 of it while
+//   - the gradient's factor goes into the exponent, which costs 2^-17 of an
+//     exponential while the factor is within 2^32 of 1, and 2^-16 at most, while
 //     |M| is at most 128; beyond, and in f32, it is (x - m) c and a factor.
 constexpr float FAST_MAX = 128.0f;
 

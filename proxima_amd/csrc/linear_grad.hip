@@ -133,7 +133,11 @@ __global__ void __launch_bounds__(GRAD_THREADS) grad_bias_join(LinearGrad p) {
 }
 
 // The tile's rows, 0 where each group has a workgroup of its own. About 2048
-// workgroups fill the chip; each then joins few sums for the rows it reads.
+// workgroups fill the chip; each then joins few sums for the rows it reads. The
+// choice goes by the average group, and a group of many that is much longer, or
+// rows of none, are then one workgroup's by its columns: 16384 x 4096 in bf16, GELU,
+// 71 to 83 us in 64 to 256 equal groups; with half the rows in one group 100 of 64,
+// 710 of 128 or 256; with half of them behind the last group 69, and 530 to 540.
 struct GradPlan {
   unsigned x;  // threads to a row
   unsigned strips;

@@ -78,9 +78,9 @@ struct LinearProduct : Product {
   uint64_t rs = 0;
   void* kept = nullptr;  // h in the result's type, rows hs apart
   uint64_t hs = 0;
-  // y and h go past the caches, which keep the operands (with h kept 138 us, 127:
-  // 8192 rows in 8 groups, 1024 -> 4096; what reads results as large finds them
-  // in no L2 either way)
+  // y and h go past the caches, which keep the operands (8192 rows in 8 uneven
+  // groups, 1024 -> 4096, h kept: 96 us, 104 through the caches, with GELU 126, 136;
+  // what reads results as large finds them in no L2 either way)
   bool once = false;
 };
 
@@ -1087,7 +1087,8 @@ constexpr Tile TILES[3] = {{256, 256, 6, 1.15, 0.45}, {128, 512, 4, 0.7, 0.35}, 
 constexpr Tile PACKED_TILES[3] = {{256, 256, 6, 0.6, 0.25}, {128, 512, 4, 0.95, 0.45}, {64, 1024, 3, 0.6, 0.4}};
 // What an epilogue adds to a tile of each size, in us: 128 and 64 share a CU with
 // others, whose products go on meanwhile. With GELU and h kept, 8192 rows in 8
-// uneven groups, 1024 -> 4096: 125 us with 256, 115 with 128 (88, 94 without).
+// uneven groups, 1024 -> 4096: 124 us with 256, 120 with 128 (85, 98 without either;
+// 112, 113 with GELU alone).
 struct Epilogue {
   double us[3] = {0, 0, 0};
   void add(double a, double b, double c) {
@@ -1231,7 +1232,8 @@ void launch_product(P p, uint64_t room, hipStream_t s) {
     const bool few = g_kernel ? g_kernel == 16 : few_cost(B, IS_PACKED, p) <= tiled_cost(tiled, IS_PACKED, p);
     if (copied && reaches && few) return launch_few<T, O, B, IS_PACKED>(p, s);
     // rows that are not whole 16-byte pieces: their tiles take half as long again as estimated (us by this kernel and
-    // by tiles: 1 row, 4100 -> 4097 14, 55; 100 rows, 1001 -> 1501 10, 17; 64 in 8 groups, 2001 -> 513 12, 26)
+    // by tiles: 1 row, 4100 -> 4097 14, 55; 100 rows, 1001 -> 1501 10, 17; 64 in 8 groups, 2001 -> 513 12, 26). Layers
+    // only: a plain product keeps the kernel, and with it the order of its sums, that its results have had.
     if constexpr (FORM == FORWARD && !IS_PACKED && is_linear<P>)
       if (!copied && (g_kernel ? g_kernel == 16 : few_cost(B, false, p) <= 1.5 * tiled)) return launch_few<T, O, B, false, true>(p, s);
   }

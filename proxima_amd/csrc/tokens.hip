@@ -3,7 +3,7 @@
 //   y_t = r_t + sum over picks j of g_tj (W2_e f(W1_e x_t + b1_e) [* W3_e x_t] + b2_e),   e = experts_tj
 //
 // For a few tokens the time is that of reading the matrices of the experts in
-// use, once, so nothing else may wait for memory. Two kernels:
+// use, once, so nothing else may wait for memory. Two kernels, or three:
 //
 //   tokens_hidden  a workgroup takes an expert in use and 16 rows of its W1 (and
 //                  W3), finds the expert's tokens from the ids, and leaves
@@ -11,14 +11,22 @@
 //   tokens_out     a workgroup takes 16 rows of every W2. A token's row of the
 //                  matrix instruction is the same for all experts (zeros where it
 //                  did not pick one), so that the sum over experts and hidden
-//                  columns is one sum in registers and nothing is joined but the
-//                  wavefronts' shares at the end.
+//                  columns is one sum in registers, the wavefronts' shares joined
+//                  at the end. Where such workgroups do not fill the chip it takes
+//                  8 rows (up to 8 tokens; the instruction's other half is another
+//                  piece of the sum), or a slice of the sum;
+//   tokens_join    adds the slices, where there are any. tokens_plan chooses.
 //
 // Tokens go in blocks of 64 (a bit mask of them is one scalar register pair).
-// Sums are held in f32. a is kept as planes of bf16 whose sum it is: two for
-// 16-bit results (2^-17 of it is lost), three (all of f32's 24 bits) for f32.
-// Matrices in f16 are taken apart into two bf16 for the second product, which
-// is exact but for 2^-40 (rest() says why), so that a's range is f32's.
+// Sums are held in f32. a is kept as planes of bf16 whose sum it is: three (all
+// of f32's 24 bits) for f32 results, two for 16-bit ones. There the second keeps 8
+// bits of what is below the first's last, so that up to 2^-16 of a is lost, beside a
+// rounding of the result of 2^-8 (bf16) or 2^-11 (f16); a third would cost 4 to 14%
+// (us with two, and of the same into f32: 8 x 2 of 16 gated experts, 2048 -> 4096 ->
+// 2048 89, 94; 32 x 4 of 64 packed ones, 2048 -> 1024 -> 2048 56, 64; 64 x 8 of 64,
+// 1024 -> 512 -> 1024 56, 61). Matrices in f16 are taken apart into two bf16 for the
+// second product, which is exact but for 2^-40 (rest() says why), so that a's range
+// is f32's.
 #include "activation.hpp"
 #include "block8.hpp"
 #include "common.hpp"

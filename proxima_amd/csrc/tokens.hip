@@ -137,7 +137,8 @@ struct MatrixTile {
 __device__ __forceinline__ float cut(float v) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u); }
 __device__ __forceinline__ uint32_t high_half(float v) { return __builtin_bit_cast(uint32_t, v) >> 16; }
 // What is left of v; of what 16 bits hold exactly 2^-40 of it rather than nothing, as zero times an infinity of the other
-// factor is not a number. (f16 matrices, 8 x 2 of 16 gated experts: 84.9 us, 84.3 without.)
+// factor is not a number. (From |v| = 2^-86 on, where there are three planes 2^-46: below, that is less than bf16's
+// smallest normal value. f16 matrices, 8 x 2 of 16 gated experts: 84.9 us, 84.3 without.)
 __device__ __forceinline__ float rest(float v, float c) {
   return fabsf(v) < __builtin_inff() ? __builtin_fmaf(c, 0x1p-40f, v - c) : v;
 }

@@ -686,5 +686,6 @@ def distill_loss_grad(weight, logits, ids, scores, counts, temperature=1.0, out=
     """(loss, dx): distill_loss and the logits' gradient, weight[t] / temperature (q - p), of the logits' type and
     rounded once; weight [rows] f32 is the loss' own gradient (1 / rows for the mean). Rows without a teacher have zeros.
     `out` may be the logits themselves. Of 16-bit logits the exponentials in dx are off by at most 2^-16 of themselves,
-    2^-8 of what dx' rounding costs in bf16 and 2^-5 in f16. The time grows with the square of `top`, from some 100 entries on."""
+    2^-8 of what dx' rounding costs in bf16 and 2^-5 in f16. The time grows with the square of `top`, from some 100
+    entries on."""
     return _distill(_lib.pxg_distill_loss_grad_device, weight, logits, ids, scores, counts, temperature, True, out)
